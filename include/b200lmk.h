@@ -483,6 +483,61 @@ int lmk_cached_rows(const void* q, const void* k, const void* v, const int64_t q
                     float* prefix_probs, void* out, int B, int H, int T, int P, int D, int max_groups, float sm_scale, int dtype,
                     void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------------------
+ * Attention without landmarks: a sliding window with sinks, and a paged key-value cache.  (No counterparts in the reference.)
+ *
+ * lmk_window_fwd / lmk_window_bwd: query row i stands at position p = Lk - Lq + i and sees key j if j <= p and
+ * (p - j < window or j < sinks), and, with lengths [B] (int32, nullable), p < lengths[b]: a right-padded batch, whose rows behind a
+ * sequence's end give zeros and take no part in any gradient, whatever they hold.
+ *   q [B,H,Lq,D], k, v [B,Hkv,Lk,D] with H a multiple of Hkv (head h reads key head h / (H / Hkv)), strided; o [B,H,Lq,D] dense; lse
+ *   [B*H, Lq] fp32: log2 of the row's normaliser (+inf where a row sees nothing).  D a multiple of 8 up to 128, Lk >= Lq, sm_scale > 0.
+ *   Backward: o, dQ [B,H,Lq,D], dK, dV [B,Hkv,Lk,D] dense, dO strided; workspace of lmk_window_bwd_workspace(...) bytes, 256-byte
+ *   aligned, contents irrelevant.  dK and dV are sums over the heads that share them; no atomics, bit-reproducible.
+ */
+int lmk_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* lengths, int B, int H, int Hkv,
+                   int Lq, int Lk, int D, const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
+                   int window, int sinks, float sm_scale, int dtype, void* stream);
+size_t lmk_window_bwd_workspace(int B, int H, int Hkv, int Lq, int Lk, int D, int window, int sinks, int dtype);
+int lmk_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dO, const float* lse, const int32_t* lengths,
+                   void* dQ, void* dK, void* dV, void* workspace, size_t workspace_bytes, int B, int H, int Hkv, int Lq, int Lk, int D,
+                   const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3], const int64_t do_strides[3],
+                   int window, int sinks, float sm_scale, int dtype, void* stream);
+
+/*
+ * Paged key-value cache.  k_pages, v_pages [n_pages, Hkv, page, D] with element strides {page, head, row} (multiples of 16 bytes; page a
+ * power of two from 16 to 1024); table [B, max_pages] int32 names a sequence's pages in order, lengths [B] int32 its tokens.  Both are
+ * read on the device: lengths are held between 0 and max_pages * page; a table entry outside of 0 .. n_pages - 1 is not followed, its
+ * keys count as hidden, and lmk_device_status says 601.  Sequences may share pages for reading.
+ *
+ * lmk_paged_append: rows 0 .. n_b - 1 of k_new, v_new [B,Hkv,T,D] (strided) behind the tokens of sequence b, whose length moves on by n_b
+ * = counts[b] (int32, nullable: T).  weights (nullable) [B, Hkv, max_pages * page] fp32 are set to 0 for them.  Rows that do not
+ * fit are left out (status 602).
+ *
+ * lmk_paged_attend: query t of q [B,H,T,D] (strided) stands at position p = lengths[b] - T + t and sees key j if j <= p and (window == 0
+ * or p - j < window or j < sinks); o [B,H,T,D] dense, zeros where nothing is visible.  weights (nullable) [B, Hkv, max_pages *
+ * page] fp32: weights = decay * weights + the sum of the key's attention weights over the T queries of the heads that share it, for
+ * every j < lengths[b]; decay 0 does not read what stood there.
+ *
+ * lmk_paged_evict: sequences of more than `budget` tokens keep the first `sinks`, the last `recent` and the budget - sinks - recent of
+ * the rest with the largest weights (the lower index first where they are equal; NaN is the largest), per key head, in order, copied to
+ * the pages fresh [B, n_fresh] names, which must be nobody's; the others stay as they are.  Writes table_out [B, max_pages] (-1: no page),
+ * lengths_out [B], weights_out [B, Hkv, max_pages * page] (0 behind the tokens) and kept [B, Hkv, budget] int32 (the survivors'
+ * former positions, -1 behind them).  The pages of `table` are not written.
+ */
+int lmk_paged_append(const void* k_new, const void* v_new, const int64_t k_new_strides[3], const int64_t v_new_strides[3], void* k_pages,
+                     void* v_pages, const int64_t k_strides[3], const int64_t v_strides[3], const int32_t* table, int32_t* lengths,
+                     const int32_t* counts, float* weights, int B, int Hkv, int T, int D, int page, int n_pages, int max_pages, int dtype,
+                     void* stream);
+size_t lmk_paged_attend_workspace(int B, int H, int Hkv, int T, int D, int page, int max_pages, int weights, int dtype);
+int lmk_paged_attend(const void* q, const int64_t q_strides[3], const void* k_pages, const void* v_pages, const int64_t k_strides[3],
+                     const int64_t v_strides[3], const int32_t* table, const int32_t* lengths, void* o, float* weights, float decay,
+                     void* workspace, size_t workspace_bytes, int B, int H, int Hkv, int T, int D, int page, int n_pages, int max_pages,
+                     int window, int sinks, float sm_scale, int dtype, void* stream);
+int lmk_paged_evict(void* k_pages, void* v_pages, const int64_t k_strides[3], const int64_t v_strides[3], const int32_t* table,
+                    const int32_t* lengths, const float* weights, const int32_t* fresh, int n_fresh, int32_t* table_out,
+                    int32_t* lengths_out, float* weights_out, int32_t* kept, int B, int Hkv, int D, int page, int n_pages, int max_pages,
+                    int budget, int recent, int sinks, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

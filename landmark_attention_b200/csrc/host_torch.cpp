@@ -20,6 +20,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -43,7 +44,9 @@ using torch::autograd::variable_list;
   X(lmk_decode_supported) X(lmk_decode_attend) X(lmk_block_select) X(lmk_block_select_supported)                  \
   X(lmk_prefix_gather) X(lmk_prefix_gather_supported) X(lmk_prefix_pv) X(lmk_landmark_scores)                     \
   X(lmk_landmark_scores_workspace) X(lmk_topk_sorted) X(lmk_chunk_rotate) X(lmk_attn_fwd_lse)                     \
-  X(lmk_selected_attend) X(lmk_gather_kv_to) X(lmk_cached_rows) X(lmk_cached_rows_supported)
+  X(lmk_selected_attend) X(lmk_gather_kv_to) X(lmk_cached_rows) X(lmk_cached_rows_supported) \
+  X(lmk_window_fwd) X(lmk_window_bwd_workspace) X(lmk_window_bwd) X(lmk_paged_append) X(lmk_paged_attend_workspace)                \
+  X(lmk_paged_attend) X(lmk_paged_evict)
 struct Lib {
 #define X(name) decltype(&::name) name = nullptr;
   LMK_FUNCS(X)
@@ -892,6 +895,212 @@ Tensor per_head_attend(const Tensor& q_, const Tensor& k_, const Tensor& v_, con
   return out;
 }
 
+// ------------------------------------------------------------------------------------------------ window attention
+void same_device(const Tensor& t, const Tensor& as, const char* name) {
+  LMK_ASSERT(t.device() == as.device(), std::string(name) + " must be on the same CUDA device as the other tensors");
+}
+// int32 per-sequence numbers on the device, dense
+Tensor counts_i32(const Tensor& t, const Tensor& as, int64_t B, const char* name) {
+  LMK_ASSERT(t.dim() == 1 && t.size(0) == B, std::string(name) + " must hold one number per sequence");
+  LMK_ASSERT(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong, std::string(name) + " must be int32 or int64");
+  same_device(t, as, name);
+  return t.to(at::kInt).contiguous();
+}
+int32_t* i32_ptr(const Tensor& t) { return t.defined() ? t.data_ptr<int32_t>() : nullptr; }
+// what the kernels read in place: TMA's rules in 16 bits, 16-byte vectors in fp32
+bool window_rows(const Tensor& t) {
+  if (t.stride(3) != 1) return false;
+  if (t.scalar_type() != at::kFloat) return tma_rows(t);
+  return t.stride(0) % 4 == 0 && t.stride(1) % 4 == 0 && t.stride(2) % 4 == 0 && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+}
+
+Tensor window_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths, int64_t window, int64_t sinks, double scale,
+                  Tensor* lse) {
+  const auto B = q.size(0), H = q.size(1), Lq = q.size(2), D = q.size(3), Hkv = k.size(1), Lk = k.size(2);
+  Tensor o = empty_like_dtype({B, H, Lq, D}, q);
+  *lse = empty_f32({B * H, Lq}, q);
+  check(lib.lmk_window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse->data_ptr<float>(), i32_ptr(lengths), B, H, Hkv, Lq,
+                           Lk, D, S3(q).v, S3(k).v, S3(v).v, window, sinks, (float)scale, dtype_code(q), stream_of(q)),
+        "lmk_window_fwd");
+  return o;
+}
+
+struct WindowAttention : public torch::autograd::Function<WindowAttention> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const std::optional<Tensor>& lengths_,
+                        int64_t window, int64_t sinks, double scale) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    const Tensor lengths = lengths_.value_or(Tensor());
+    Tensor lse, o = window_fwd(q, k, v, lengths, window, sinks, scale, &lse);
+    ctx->save_for_backward({q, k, v, o, lse, lengths});
+    ctx->saved_data["window"] = window;
+    ctx->saved_data["sinks"] = sinks;
+    ctx->saved_data["scale"] = scale;
+    return o;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (at::GradMode::is_enabled())
+      C10_THROW_ERROR(NotImplementedError, "window_attention has first derivatives only (create_graph is not supported)");
+    auto saved = ctx->get_saved_variables();
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &lse = saved[4], &lengths = saved[5];
+    const int64_t window = ctx->saved_data["window"].toInt(), sinks = ctx->saved_data["sinks"].toInt();
+    const auto B = q.size(0), H = q.size(1), Lq = q.size(2), D = q.size(3), Hkv = k.size(1), Lk = k.size(2);
+    c10::cuda::OptionalCUDAGuard guard(q.device());
+    const Tensor dO = grad_rows(grads[0], q);
+    Tensor dq = empty_like_dtype({B, H, Lq, D}, q), dk = empty_like_dtype({B, Hkv, Lk, D}, q), dv = empty_like_dtype({B, Hkv, Lk, D}, q);
+    const int code = dtype_code(q);
+    const size_t need = std::max<size_t>(lib.lmk_window_bwd_workspace(B, H, Hkv, Lq, Lk, D, window, sinks, code), 256);
+    Tensor ws = at::empty({(int64_t)need}, q.options().requires_grad(false).dtype(at::kByte));
+    check(lib.lmk_window_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dO.data_ptr(), lse.data_ptr<float>(), i32_ptr(lengths),
+                             dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), need, B, H, Hkv, Lq, Lk, D, S3(q).v, S3(k).v,
+                             S3(v).v, S3(dO).v, window, sinks, (float)ctx->saved_data["scale"].toDouble(), code, stream_of(q)),
+          "lmk_window_bwd");
+    return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+// A leaf's gradient belongs to the stream on which a graph of it was built first, for as long as that graph lives.  A captured backward
+// pass would make that stream wait for the capturing one, which breaks the capture: refused here, in front of it.
+void check_capture(const Tensor& t) {
+  if (!t.requires_grad() || !t.is_leaf()) return;
+  const auto acc = torch::autograd::impl::try_get_grad_accumulator(t);
+  if (!acc) return;
+  const auto owner = acc->stream();
+  const c10::Stream now = c10::cuda::getCurrentCUDAStream(t.get_device());
+  TORCH_CHECK(!owner || *owner == now, "window_attention: an autograd graph of the same leaf, built on another stream, is alive; drop it "
+              "before the step is captured, or capture on detached leaves");
+}
+
+Tensor window_attention(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& lengths_, int64_t window, int64_t sinks,
+                        double scale) {
+  require_cuda(q_); require_cuda(k_); require_cuda(v_);
+  LMK_ASSERT(q_.dim() == 4 && k_.dim() == 4 && v_.dim() == 4, "expected q [B, H, Lq, D] and k, v [B, Hkv, Lk, D]");
+  LMK_ASSERT(k_.size(0) == q_.size(0) && k_.size(3) == q_.size(3) && k_.sizes() == v_.sizes(),
+             "k and v must be [B, Hkv, Lk, D] with q's batch and head dim");
+  LMK_ASSERT(q_.scalar_type() == k_.scalar_type() && q_.scalar_type() == v_.scalar_type(), "All tensors must have the same type");
+  dtype_code(q_);
+  same_device(k_, q_, "k");
+  same_device(v_, q_, "v");
+  LMK_ASSERT(window >= 1 && sinks >= 0, "window must be at least 1, sinks at least 0");
+  LMK_ASSERT(q_.numel() > 0 && k_.numel() > 0, "window attention of an empty tensor");
+  window = std::min<int64_t>(window, k_.size(2));        // beyond the sequence both mean all of it
+  sinks = std::min<int64_t>(sinks, k_.size(2));
+  c10::cuda::OptionalCUDAGuard guard(q_.device());
+  const Tensor lengths = lengths_.defined() ? counts_i32(lengths_, q_, q_.size(0), "lengths") : Tensor();
+  Tensor q = q_, k = k_, v = v_;
+  for (Tensor* t : {&q, &k, &v})
+    if (!window_rows(*t)) *t = t->clone(at::MemoryFormat::Contiguous);        // part of the graph where a gradient is wanted
+  if (!needs_grad({q, k, v})) {
+    Tensor lse;
+    return window_fwd(q, k, v, lengths, window, sinks, scale, &lse);
+  }
+  if (at::GradMode::is_enabled() && c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
+    for (const Tensor* t : {&q_, &k_, &v_}) check_capture(*t);
+  return WindowAttention::apply(q, k, v, lengths.defined() ? std::optional<Tensor>(lengths) : std::nullopt, window, sinks, scale);
+}
+
+// ------------------------------------------------------------------------------------------------ paged cache
+struct PagesView {
+  int64_t B, Hkv, D, page, n_pages, max_pages;
+  int code;
+  S3 ks, vs;
+};
+PagesView pages_of(const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& lengths) {
+  require_cuda(k); require_cuda(v); require_cuda(table); require_cuda(lengths);
+  LMK_ASSERT(k.dim() == 4 && v.dim() == 4 && k.sizes() == v.sizes(), "k_pages and v_pages must be [n_pages, Hkv, page, D]");
+  LMK_ASSERT(k.scalar_type() == v.scalar_type(), "All tensors must have the same type");
+  LMK_ASSERT(k.stride(3) == 1 && v.stride(3) == 1, "pages need contiguous features");
+  LMK_ASSERT(table.dim() == 2 && table.scalar_type() == at::kInt && table.is_contiguous(), "table must be a dense int32 [B, max_pages]");
+  LMK_ASSERT(lengths.dim() == 1 && lengths.size(0) == table.size(0) && lengths.scalar_type() == at::kInt && lengths.is_contiguous(),
+             "lengths must be a dense int32 [B]");
+  for (const auto& [t, name] : {std::pair(&v, "v_pages"), std::pair(&table, "table"), std::pair(&lengths, "lengths")}) same_device(*t, k, name);
+  return {table.size(0), k.size(1), k.size(3), k.size(2), k.size(0), table.size(1), dtype_code(k), S3(k), S3(v)};
+}
+float* cache_weights(const Tensor& w, const Tensor& k, const PagesView& p) {
+  if (!w.defined()) return nullptr;
+  LMK_ASSERT(w.is_cuda() && w.scalar_type() == at::kFloat && w.is_contiguous() && w.dim() == 3 && w.size(0) == p.B && w.size(1) == p.Hkv &&
+             w.size(2) == p.max_pages * p.page, "weights must be a dense fp32 [B, Hkv, max_pages * page]");
+  same_device(w, k, "weights");
+  return w.data_ptr<float>();
+}
+int fits_int(int64_t n, const char* name) {
+  LMK_ASSERT(n >= INT32_MIN && n <= INT32_MAX, std::string(name) + " is out of range");
+  return (int)n;
+}
+
+Tensor paged_attention(const Tensor& q_, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& lengths, int64_t window,
+                       int64_t sinks, double scale, const Tensor& weights, double decay) {
+  require_cuda(q_);
+  const PagesView p = pages_of(k, v, table, lengths);
+  LMK_ASSERT(q_.dim() == 4 && q_.size(0) == p.B && q_.size(3) == p.D && q_.numel() > 0, "q must be [B, H, T, D] with the cache's batch and head dim");
+  LMK_ASSERT(q_.scalar_type() == k.scalar_type(), "All tensors must have the same type");
+  same_device(q_, k, "q");
+  LMK_ASSERT(!needs_grad({q_, k, v}), "paged_attention has no gradients: call it under torch.no_grad()");
+  float* w = cache_weights(weights, k, p);
+  c10::cuda::OptionalCUDAGuard guard(q_.device());
+  // 32-bit pieces of rows
+  const bool ok = q_.stride(3) == 1 && (reinterpret_cast<uintptr_t>(q_.data_ptr()) & 3) == 0 &&
+                  (q_.element_size() == 4 || (q_.stride(0) % 2 == 0 && q_.stride(1) % 2 == 0 && q_.stride(2) % 2 == 0));
+  const Tensor q = ok ? q_ : q_.clone(at::MemoryFormat::Contiguous);
+  const auto H = q.size(1), T = q.size(2);
+  LMK_ASSERT(p.Hkv > 0 && H % p.Hkv == 0, "query heads must be a multiple of the cache's heads");
+  Tensor o = empty_like_dtype({p.B, H, T, p.D}, q);
+  const size_t need = std::max<size_t>(lib.lmk_paged_attend_workspace(p.B, H, p.Hkv, fits_int(T, "T"), p.D, p.page, p.max_pages, w != nullptr, p.code), 256);
+  Tensor ws = at::empty({(int64_t)need}, q.options().requires_grad(false).dtype(at::kByte));
+  check(lib.lmk_paged_attend(q.data_ptr(), S3(q).v, k.data_ptr(), v.data_ptr(), p.ks.v, p.vs.v, i32_ptr(table), i32_ptr(lengths), o.data_ptr(),
+                             w, (float)decay, ws.data_ptr(), need, p.B, H, p.Hkv, T, p.D, p.page, p.n_pages, p.max_pages,
+                             fits_int(window, "window"), fits_int(sinks, "sinks"), (float)scale, p.code, stream_of(q)),
+        "lmk_paged_attend");
+  return o;
+}
+
+void paged_append(const Tensor& k_, const Tensor& v_, const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& lengths,
+                  const Tensor& counts_, const Tensor& weights) {
+  require_cuda(k_); require_cuda(v_);
+  const PagesView p = pages_of(kp, vp, table, lengths);
+  LMK_ASSERT(k_.dim() == 4 && k_.sizes() == v_.sizes() && k_.size(0) == p.B && k_.size(1) == p.Hkv && k_.size(3) == p.D,
+             "k and v must be [B, Hkv, T, D] with the cache's batch, heads and head dim");
+  LMK_ASSERT(k_.scalar_type() == kp.scalar_type() && v_.scalar_type() == kp.scalar_type(), "All tensors must have the same type");
+  same_device(k_, kp, "k");
+  same_device(v_, kp, "v");
+  LMK_ASSERT(!needs_grad({kp, vp}), "the cache's pages take no gradients");
+  float* w = cache_weights(weights, kp, p);
+  if (k_.size(2) == 0) return;
+  c10::cuda::OptionalCUDAGuard guard(kp.device());
+  const Tensor counts = counts_.defined() ? counts_i32(counts_, kp, p.B, "counts") : Tensor();
+  const int64_t vec = 16 / kp.element_size();
+  Tensor k = k_, v = v_;
+  for (Tensor* t : {&k, &v})
+    if (t->stride(3) != 1 || t->stride(0) % vec != 0 || t->stride(1) % vec != 0 || t->stride(2) % vec != 0 ||
+        (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) != 0)
+      *t = t->detach().clone(at::MemoryFormat::Contiguous);
+  check(lib.lmk_paged_append(k.data_ptr(), v.data_ptr(), S3(k).v, S3(v).v, kp.data_ptr(), vp.data_ptr(), p.ks.v, p.vs.v, i32_ptr(table),
+                             i32_ptr(lengths), i32_ptr(counts), w, p.B, p.Hkv, fits_int(k.size(2), "T"), p.D, p.page, p.n_pages, p.max_pages,
+                             p.code, stream_of(kp)),
+        "lmk_paged_append");
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> paged_evict(const Tensor& kp, const Tensor& vp, const Tensor& table, const Tensor& lengths,
+                                                       const Tensor& weights, const Tensor& fresh, int64_t budget, int64_t recent,
+                                                       int64_t sinks) {
+  const PagesView p = pages_of(kp, vp, table, lengths);
+  LMK_ASSERT(weights.defined(), "paged_evict needs the cache's weights");
+  const float* w = cache_weights(weights, kp, p);
+  LMK_ASSERT(fresh.is_cuda() && fresh.dim() == 2 && fresh.size(0) == p.B && fresh.scalar_type() == at::kInt && fresh.is_contiguous(),
+             "fresh must be a dense int32 [B, pages]");
+  same_device(fresh, kp, "fresh");
+  LMK_ASSERT(budget >= 1 && budget <= p.max_pages * p.page, "budget must lie between 1 and the table's capacity");
+  LMK_ASSERT(!needs_grad({kp, vp}), "the cache's pages take no gradients");
+  c10::cuda::OptionalCUDAGuard guard(kp.device());
+  Tensor table_out = at::empty_like(table), lengths_out = at::empty_like(lengths), weights_out = at::empty_like(weights);
+  Tensor kept = at::empty({p.B, p.Hkv, budget}, table.options());
+  check(lib.lmk_paged_evict(kp.data_ptr(), vp.data_ptr(), p.ks.v, p.vs.v, i32_ptr(table), i32_ptr(lengths), w, i32_ptr(fresh),
+                            fits_int(fresh.size(1), "fresh"), i32_ptr(table_out), i32_ptr(lengths_out), weights_out.data_ptr<float>(),
+                            i32_ptr(kept), p.B, p.Hkv, p.D, p.page, p.n_pages, p.max_pages, budget, fits_int(recent, "recent"),
+                            fits_int(sinks, "sinks"), p.code, stream_of(kp)),
+        "lmk_paged_evict");
+  return {table_out, lengths_out, weights_out, kept};
+}
+
 // ------------------------------------------------------------------------------------------------ Python entry points
 const Tensor& tensor_arg(PyObject* o, const char* name) {
   if (!THPVariable_Check(o)) {
@@ -910,6 +1119,9 @@ double float_arg(PyObject* o) {
   const double v = PyFloat_AsDouble(o);
   if (v == -1.0 && PyErr_Occurred()) throw python_error();
   return v;
+}
+double scale_arg(PyObject* o, const Tensor& q) {      // None: 1 / sqrt(head dim)
+  return o == Py_None ? (q.dim() > 0 && q.size(-1) > 0 ? 1.0 / std::sqrt((double)q.size(-1)) : 1.0) : float_arg(o);
 }
 void need_args(Py_ssize_t n, Py_ssize_t want) {
   if (n != want) {
@@ -1087,6 +1299,49 @@ PyObject* py_per_head_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// window_attention(q, k, v, lengths | None, window, sinks, scale | None)
+PyObject* py_window_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  need_args(n, 7);
+  const Tensor& q = tensor_arg(a[0], "q");
+  return THPVariable_Wrap(window_attention(q, tensor_arg(a[1], "k"), tensor_arg(a[2], "v"), opt_tensor_arg(a[3], "lengths"), int_arg(a[4]),
+                                           int_arg(a[5]), scale_arg(a[6], q)));
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_attention(q, k_pages, v_pages, table, lengths, window | None, sinks, scale | None, weights | None, decay)
+PyObject* py_paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  need_args(n, 10);
+  const Tensor& q = tensor_arg(a[0], "q");
+  const int64_t window = a[5] == Py_None ? 0 : int_arg(a[5]), sinks = int_arg(a[6]);
+  LMK_ASSERT((a[5] == Py_None || window >= 1) && sinks >= 0, "window must be at least 1 (or None), sinks at least 0");
+  return THPVariable_Wrap(paged_attention(q, tensor_arg(a[1], "k_pages"), tensor_arg(a[2], "v_pages"), tensor_arg(a[3], "table"),
+                                          tensor_arg(a[4], "lengths"), window, sinks, scale_arg(a[7], q), opt_tensor_arg(a[8], "weights"),
+                                          float_arg(a[9])));
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_append(k, v, k_pages, v_pages, table, lengths, counts | None, weights | None)
+PyObject* py_paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  need_args(n, 8);
+  paged_append(tensor_arg(a[0], "k"), tensor_arg(a[1], "v"), tensor_arg(a[2], "k_pages"), tensor_arg(a[3], "v_pages"), tensor_arg(a[4], "table"),
+               tensor_arg(a[5], "lengths"), opt_tensor_arg(a[6], "counts"), opt_tensor_arg(a[7], "weights"));
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
+// paged_evict(k_pages, v_pages, table, lengths, weights, fresh, budget, recent, sinks) -> (table, lengths, weights, kept)
+PyObject* py_paged_evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  need_args(n, 9);
+  auto [t, l, w, k] = paged_evict(tensor_arg(a[0], "k_pages"), tensor_arg(a[1], "v_pages"), tensor_arg(a[2], "table"), tensor_arg(a[3], "lengths"),
+                                  tensor_arg(a[4], "weights"), tensor_arg(a[5], "fresh"), int_arg(a[6]), int_arg(a[7]), int_arg(a[8]));
+  return wrap_tuple(t, l, w, k);
+  END_HANDLE_TH_ERRORS
+}
+
 #define FAST(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fn)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {{"init", py_init, METH_O, nullptr},
                          FAST("fused_attention", py_fused_attention),
@@ -1101,6 +1356,10 @@ PyMethodDef methods[] = {{"init", py_init, METH_O, nullptr},
                          FAST("per_head_attend", py_per_head_attend),
                          FAST("cache_retrieve", py_cache_retrieve),
                          FAST("prefix_pv", py_prefix_pv),
+                         FAST("window_attention", py_window_attention),
+                         FAST("paged_attention", py_paged_attention),
+                         FAST("paged_append", py_paged_append),
+                         FAST("paged_evict", py_paged_evict),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_lmk_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
