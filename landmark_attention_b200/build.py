@@ -20,7 +20,7 @@ HOST_SOURCE = os.path.join(CSRC, "host_torch.cpp")
 HOST_PATH = os.path.join(LIB_DIR, "_lmk_host.so")
 SOURCES = ["api.cu", "attn_general.cu", "attn_f32.cu", "attn_sm100.cu", "attn_mask_sm100.cu", "grouped_softmax.cu", "retrieval.cu",
            "scores_sm100.cu", "cache_store.cu", "decode.cu",
-           "block_cache.cu", "window_general.cu", "window.cu", "paged.cu"]
+           "block_cache.cu", "window.cu", "window_f32.cu", "window_sm100.cu", "paged.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC"]
 

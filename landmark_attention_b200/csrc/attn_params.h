@@ -33,6 +33,7 @@ bool attn_sm100_takes(int B, int H, int Lq, int Lk, int D, int block, int dtype)
 // pointers and strides of q, k, v (and o, dO for the backward pass) are addressable by TMA
 bool attn_sm100_operands_ok(const AttnParams& p, bool backward);
 void attn_sm100_set_max_ctas(int n);
+int attn_sm100_max_ctas();
 int attn_sm100_fwd(const AttnParams& p, int dtype, cudaStream_t st);
 int attn_sm100_bwd(const AttnParams& p, int dtype, cudaStream_t st);
 size_t attn_sm100_bwd_workspace(int B, int H, int Lq, int Lk, int D);
@@ -53,6 +54,8 @@ int* device_status_word();
 // TMA descriptor of a [B, H, L, 128] 16-bit tensor with element strides {batch, head, row}: box = 64 features x
 // `box_rows` rows, 128-byte swizzle (cached by pointer, shape and strides).  Binds the device's primary context first.
 int tensor_map_4d(CUtensorMap* m, const void* ptr, int dtype, int B, int H, int L, const int64_t st[3], int box_rows);
+// the same for D features, encoded at every call
+int tensor_map_4d_now(CUtensorMap* m, const void* ptr, int dtype, int B, int H, int L, int D, const int64_t st[3], int box_rows);
 bool tensor_map_operand_ok(const void* p, const int64_t st[3]);
 
 // Fused attention with arbitrary landmark positions (attn_mask_sm100.cu).  R [B*H, Lq], A [B*H, G, Lq] fp32.

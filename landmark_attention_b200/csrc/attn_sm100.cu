@@ -35,6 +35,7 @@
 #include "common.cuh"
 #include "attn_params.h"
 #include "sm100_ptx.cuh"
+#include "sm100_tiles.cuh"
 
 namespace lmk {
 
@@ -50,29 +51,6 @@ constexpr int kQTile = 128;
 constexpr uint32_t kTileBytes = 16384;   // one [128 x 64] or two [64 x 64] 16-bit tiles
 constexpr uint32_t kHalfTile = 8192;
 constexpr float kLog2e = 1.4426950408889634f;
-
-template <bool kBf16>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-  if (kBf16) {
-    __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&t);
-  } else {
-    __half2 t = __floats2half2_rn(a, b);
-    return *reinterpret_cast<uint32_t*>(&t);
-  }
-}
-
-// write one row (64 16-bit values, given as 32 packed words) of a [128 x 64] K-major 128B-swizzled tile
-__device__ __forceinline__ void store_row_sw128(uint32_t tile_base, int row, const uint32_t (&w)[32]) {
-  const uint32_t row_addr = tile_base + row * 128;
-#pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    uint32_t addr = row_addr + ((c ^ (row & 7)) << 4);
-    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(w[4 * c]), "r"(w[4 * c + 1]),
-                 "r"(w[4 * c + 2]), "r"(w[4 * c + 3])
-                 : "memory");
-  }
-}
 
 // Row reductions with four independent chains: one softmax thread has little other work in flight, so a single
 // 63-deep dependent chain of max / add would expose the ALU latency on every step.
@@ -646,13 +624,6 @@ sm100_fwd2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
 // 4 -> 90.3, 64 -> 91.3; B1 H32 L8192 D128 2 -> 2590, 3 -> 2577, 4 -> 2566)
 constexpr int kBwdPolyEvery = 4;
 
-template <bool kBf16>
-__device__ __forceinline__ uint32_t pack2p(uint64_t v) {
-  float lo, hi;
-  upk2(v, lo, hi);
-  return pack2<kBf16>(lo, hi);
-}
-
 // With kIrr the rows of a warp can be of different kinds (groups end anywhere).  The TMEM accesses have to be executed by all lanes
 // of a warp together, so nothing branches on `kind` there: mixed warps take one masked pass with per-row limits and shifts.
 // M2L = (row max + log(row sum)) * log2(e): exp2(s * c - M2L) is the outer-softmax probability.
@@ -832,54 +803,6 @@ template <int kStages> struct DkvSmem {
   uint64_t acc_full[2], acc_empty[2];               // [0] dV, [1] dK
   uint32_t tmem_base;
 };
-
-// Stores 32 accumulator columns of one TMEM lane per thread as 16-bit values.  Four neighbouring lanes exchange 16-byte
-// chunks first, so that a warp's store covers 64 contiguous bytes of eight rows and not 16 bytes of thirty-two.
-// row_off[j]: element offset of row j of the lane's four rows, or -1 for a row that is not stored.  An output of the C interface
-// may start at any word: one off a 16-byte boundary is stored word by word.
-template <bool kBf16>
-__device__ __forceinline__ void store_acc_cols(void* out, const int64_t (&row_off)[4], const uint32_t (&r)[32], int col0, int D,
-                                               int lane) {
-  uint4 v[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    v[e].x = pack2<kBf16>(__uint_as_float(r[8 * e + 0]), __uint_as_float(r[8 * e + 1]));
-    v[e].y = pack2<kBf16>(__uint_as_float(r[8 * e + 2]), __uint_as_float(r[8 * e + 3]));
-    v[e].z = pack2<kBf16>(__uint_as_float(r[8 * e + 4]), __uint_as_float(r[8 * e + 5]));
-    v[e].w = pack2<kBf16>(__uint_as_float(r[8 * e + 6]), __uint_as_float(r[8 * e + 7]));
-  }
-  // transpose of the 4 x 4 matrix (lane of the four, chunk): swap the off-diagonal chunks of 2 x 2 blocks, then the blocks
-  auto swap = [&](uint4& a, uint4& b, int step) {      // lower lane: b <-> partner's a
-    const bool up = (lane & step) != 0;
-    uint4 x = up ? a : b;
-    x.x = __shfl_xor_sync(0xffffffffu, x.x, step);
-    x.y = __shfl_xor_sync(0xffffffffu, x.y, step);
-    x.z = __shfl_xor_sync(0xffffffffu, x.z, step);
-    x.w = __shfl_xor_sync(0xffffffffu, x.w, step);
-    a = up ? x : a;
-    b = up ? b : x;
-  };
-  swap(v[0], v[1], 1);
-  swap(v[2], v[3], 1);
-  swap(v[0], v[2], 2);
-  swap(v[1], v[3], 2);
-  const int col = col0 + 8 * (lane & 3);
-  if (col >= D) return;
-  const bool wide = ((uintptr_t)out & 15) == 0;       // rows and columns are multiples of 16 bytes
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (row_off[j] < 0) continue;
-    uint32_t* to = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(out) + row_off[j] + col);
-    if (wide) {
-      *reinterpret_cast<uint4*>(to) = v[j];
-    } else {
-      to[0] = v[j].x;
-      to[1] = v[j].y;
-      to[2] = v[j].z;
-      to[3] = v[j].w;
-    }
-  }
-}
 
 // Persistent; a work unit is a PAIR of adjacent 64-key blocks (a = 2c, b = 2c+1) of one (batch, head).  Both blocks
 // stay in shared memory while the unit streams the query tiles that see them, so each Q/dO tile is fetched from
@@ -1674,21 +1597,22 @@ int cached_map(CUtensorMap* m, const MapKey& key, EncodeFn encode) {
 
 // [B, H, L, D] tensor with element strides {b, h, row}; box = 64 features x `box_rows` rows, 128-byte swizzle; what lies
 // outside the tensor (rows past L, features past D) reads as zeros
+int encode_map_4d(CUtensorMap* m, const void* ptr, int dtype, int B, int H, int L, int D, const int64_t st[3], int box_rows) {
+  EncodeTiledFn enc = get_encode();
+  if (!enc) return fail(LMK_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)L, (cuuint64_t)H, (cuuint64_t)B};
+  cuuint64_t strides[3] = {(cuuint64_t)st[2] * 2, (cuuint64_t)st[1] * 2, (cuuint64_t)st[0] * 2};
+  cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  CUresult r = enc(m, dtype == LMK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                   const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(LMK_ERR_CUDA, "cuTensorMapEncodeTiled (4-D) failed with %d", (int)r);
+  return LMK_OK;
+}
 int make_map_4d(CUtensorMap* m, const void* ptr, int dtype, int B, int H, int L, int D, const int64_t st[3], int box_rows) {
   const MapKey key{ptr, 4, dtype, B, H, L, box_rows, D, {st[0], st[1], st[2]}};
-  return cached_map(m, key, [&](CUtensorMap* out) {
-    EncodeTiledFn enc = get_encode();
-    if (!enc) return fail(LMK_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-    cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)L, (cuuint64_t)H, (cuuint64_t)B};
-    cuuint64_t strides[3] = {(cuuint64_t)st[2] * 2, (cuuint64_t)st[1] * 2, (cuuint64_t)st[0] * 2};
-    cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
-    cuuint32_t estr[4] = {1, 1, 1, 1};
-    CUresult r = enc(out, dtype == LMK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
-                     const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(LMK_ERR_CUDA, "cuTensorMapEncodeTiled (4-D) failed with %d", (int)r);
-    return (int)LMK_OK;
-  });
+  return cached_map(m, key, [&](CUtensorMap* out) { return encode_map_4d(out, ptr, dtype, B, H, L, D, st, box_rows); });
 }
 
 // landmark keys: k viewed as [B, H, L/64, 64, D]; box = 64 features x 1 row-in-block x 64 blocks
@@ -1794,6 +1718,12 @@ bool attn_sm100_operands_ok(const AttnParams& p, bool backward) {
 
 void attn_sm100_set_max_ctas(int n) { g_max_ctas.store(n > 0 ? n : 0); }
 
+int attn_sm100_max_ctas() { return g_max_ctas.load(); }
+
+int tensor_map_4d_now(CUtensorMap* m, const void* ptr, int dtype, int B, int H, int L, int D, const int64_t st[3], int box_rows) {
+  bind_context();
+  return encode_map_4d(m, ptr, dtype, B, H, L, D, st, box_rows);
+}
 int tensor_map_4d(CUtensorMap* m, const void* ptr, int dtype, int B, int H, int L, const int64_t st[3], int box_rows) {
   bind_context();
   return make_map_4d(m, ptr, dtype, B, H, L, 128, st, box_rows);

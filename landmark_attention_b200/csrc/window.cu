@@ -1,6 +1,7 @@
 // extern "C" entry points of sliding-window attention: argument checks, the division of the sinks' gradient, the choice of kernels.
 #include "common.cuh"
 #include "window_params.h"
+#include "sm100_ptx.cuh"
 
 namespace lmk {
 namespace {
@@ -15,7 +16,7 @@ int check_window(const void* q, const void* k, const void* v, const float* lse, 
   LMK_CHECK_ARG(H % Hkv == 0, "window attention: %d query heads are not a multiple of %d key heads", H, Hkv);
   LMK_CHECK_ARG((int64_t)B * H <= 65535, "window attention: B*H = %lld exceeds 65535", (long long)B * H);
   LMK_CHECK_ARG(Lk >= Lq, "window attention: %d queries are more than %d keys", Lq, Lk);
-  LMK_CHECK_ARG(Lk <= (1 << 28), "window attention: %d keys exceed 2^28", Lk);
+  LMK_CHECK_ARG(Lk <= (1 << 22), "window attention: %d keys exceed 2^22", Lk);
   LMK_CHECK_ARG(D >= 8 && D <= 128 && D % 8 == 0, "window attention: head dim %d must be a multiple of 8 up to 128", D);
   LMK_CHECK_ARG(dtype == LMK_F32 || dtype == LMK_F16 || dtype == LMK_BF16, "window attention: bad dtype %d", dtype);
   LMK_CHECK_ARG(window >= 1, "window attention: window %d must be at least 1", window);
@@ -32,9 +33,10 @@ void fill(WindowParams& p, const void* q, const void* k, const void* v, const in
   p.sinks = sinks < Lk ? sinks : Lk;
   for (int i = 0; i < 3; ++i) { p.qs[i] = qs[i]; p.ks[i] = ks[i]; p.vs[i] = vs[i]; }
 }
-// fp32 rows are read as 16-byte vectors
-bool rows_ok(const void* p, const int64_t* st, int dtype) {
-  return dtype != LMK_F32 || (((uintptr_t)p & 15) == 0 && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0);
+// fp32 rows are read as 16-byte vectors, 16-bit tensors by TMA
+bool rows_ok(const void* p, const int64_t* st, int D, int dtype) {
+  if (dtype != LMK_F32) return window_sm100_operand_ok(p, st, D);
+  return ((uintptr_t)p & 15) == 0 && st[0] % 4 == 0 && st[1] % 4 == 0 && st[2] % 4 == 0;
 }
 
 // How the query tiles of the sinks' key tiles are dealt out (SinkSplit): runs as long as the window's share of an ordinary key tile, or
@@ -57,13 +59,47 @@ int plan_split(SinkSplit* s, int B, int Hkv, int Lq, int Lk, int window, int sin
 size_t part_bytes(const SinkSplit& s, int B, int Hkv, int D, int kk) {
   return sizeof(float) * (size_t)B * Hkv * s.tiles * (1 + s.runs) * 2 * kk * D;
 }
-void tile_sizes(int dtype, int* qt, int* kk) {
-  (void)dtype;
-  *qt = 64;
-  *kk = 64;
+void tile_sizes(int dtype, int* qt, int* kk) { *qt = *kk = dtype == LMK_F32 ? 64 : 128; }      // of the dK/dV kernels
+
+// The parts of the split key tiles, added up in the order of their runs.
+template <typename T>
+__global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ WindowParams p, int qt, int kk) {
+  ptx::grid_dep_wait();
+  ptx::grid_dep_launch();
+  const int tile = blockIdx.y % p.split.tiles, bk = blockIdx.y / p.split.tiles, b = bk / p.Hkv;
+  const int len = p.lengths == nullptr ? p.Lk : min(max(ptx::ld_behind_wait(p.lengths + b), 0), p.Lk);
+  const QueryTiles qts = queries_of_keys(tile, qt, kk, p.Lq, p.Lk - p.Lq, len, p.window, p.sinks);
+  const int runs = (qts.end - qts.last + p.split.run - 1) / p.split.run;
+  const int e = (blockIdx.x * 256 + threadIdx.x) * 4, key = e / p.D, f = e - key * p.D;
+  if (key >= kk || tile * kk + key >= p.Lk) return;
+  const int64_t slot = 2ll * kk * p.D;
+  const float* part = p.split.part + ((int64_t)bk * p.split.tiles + tile) * (1 + p.split.runs) * slot + e;
+  const int64_t at = ((int64_t)bk * p.Lk + tile * kk + key) * p.D + f;
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {                     // dK, dV
+    float4 sum = *reinterpret_cast<const float4*>(part + g * (slot / 2));
+    for (int r = 1; r <= runs; ++r) {
+      const float4 x = *reinterpret_cast<const float4*>(part + r * slot + g * (slot / 2));
+      sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
+    }
+    T* const to = (T*)(g == 0 ? p.dk : p.dv) + at;
+    to[0] = from_f32<T>(sum.x);
+    to[1] = from_f32<T>(sum.y);
+    to[2] = from_f32<T>(sum.z);
+    to[3] = from_f32<T>(sum.w);
+  }
 }
 
 }  // namespace
+
+int window_join_parts(const WindowParams& p, int qt, int kk, int dtype, cudaStream_t st) {
+  const dim3 grid((kk * p.D / 4 + 255) / 256, p.B * p.Hkv * p.split.tiles);
+  if (dtype == LMK_F32) LMK_CUDA(launch_overlapped(window_join_kernel<float>, grid, dim3(256), 0, st, p, qt, kk));
+  else if (dtype == LMK_F16) LMK_CUDA(launch_overlapped(window_join_kernel<__half>, grid, dim3(256), 0, st, p, qt, kk));
+  else LMK_CUDA(launch_overlapped(window_join_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p, qt, kk));
+  return LMK_OK;
+}
+
 }  // namespace lmk
 
 using namespace lmk;
@@ -78,9 +114,10 @@ extern "C" int lmk_window_fwd(const void* q, const void* k, const void* v, void*
   fill(p, q, k, v, lengths, B, H, Hkv, Lq, Lk, D, q_strides, k_strides, v_strides, window, sinks, sm_scale);
   p.o = o;
   p.lse = lse;
-  LMK_CHECK_ARG(rows_ok(q, q_strides, dtype) && rows_ok(k, k_strides, dtype) && rows_ok(v, v_strides, dtype),
-                "window attention: fp32 rows must start on 16-byte boundaries");
-  return window_general_fwd(p, dtype, static_cast<cudaStream_t>(stream));
+  LMK_CHECK_ARG(rows_ok(q, q_strides, D, dtype) && rows_ok(k, k_strides, D, dtype) && rows_ok(v, v_strides, D, dtype),
+                "window attention: tensors must start on 16-byte boundaries, strides be multiples of 16 bytes (16-bit types: positive, rows not overlapping)");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == LMK_F32 ? window_f32_fwd(p, st) : window_sm100_fwd(p, dtype, st);
 }
 
 extern "C" size_t lmk_window_bwd_workspace(int B, int H, int Hkv, int Lq, int Lk, int D, int window, int sinks, int dtype) {
@@ -107,8 +144,8 @@ extern "C" int lmk_window_bwd(const void* q, const void* k, const void* v, const
   p.lse = const_cast<float*>(lse);
   p.dq = dQ; p.dk = dK; p.dv = dV;
   for (int i = 0; i < 3; ++i) p.dos[i] = do_strides[i];
-  LMK_CHECK_ARG(rows_ok(q, q_strides, dtype) && rows_ok(k, k_strides, dtype) && rows_ok(v, v_strides, dtype) && rows_ok(dO, do_strides, dtype),
-                "window attention: fp32 rows must start on 16-byte boundaries");
+  LMK_CHECK_ARG(rows_ok(q, q_strides, D, dtype) && rows_ok(k, k_strides, D, dtype) && rows_ok(v, v_strides, D, dtype) && rows_ok(dO, do_strides, D, dtype),
+                "window attention: tensors must start on 16-byte boundaries, strides be multiples of 16 bytes (16-bit types: positive, rows not overlapping)");
   int qt, kk;
   tile_sizes(dtype, &qt, &kk);
   if ((rc = plan_split(&p.split, B, Hkv, Lq, Lk, p.window, p.sinks, qt, kk)) != LMK_OK) return rc;
@@ -119,5 +156,6 @@ extern "C" int lmk_window_bwd(const void* q, const void* k, const void* v, const
     return fail(LMK_ERR_WORKSPACE, "window attention backward: workspace of %zu bytes on a 256-byte boundary needed", need);
   p.delta = static_cast<float*>(workspace);
   p.split.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes);
-  return window_general_bwd(p, dtype, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == LMK_F32 ? window_f32_bwd(p, st) : window_sm100_bwd(p, dtype, st);
 }

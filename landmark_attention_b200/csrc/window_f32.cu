@@ -1,4 +1,4 @@
-// Sliding-window attention with sinks on the CUDA cores, fp32 accumulation: 64 x 64 tiles of scores, 4 x 4 results a thread.
+// Sliding-window attention with sinks in fp32, on the CUDA cores: 64 x 64 tiles of scores, 4 x 4 results a thread.
 //
 //   S = scale Q K^T over the visible keys, P = e^{S - lse}, O = P V (running maximum and sum, one pass over the keys)
 //   dV = P^T dO,  dP = dO V^T,  delta = rowsum(O dO),  dS = scale P (dP - delta),  dQ = dS K,  dK = dS^T Q
@@ -18,35 +18,25 @@ using namespace ptx;
 constexpr int kTile = 64, kPad = 68, kThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 
-template <typename T> __device__ __forceinline__ float4 load4(const T* p);
-template <> __device__ __forceinline__ float4 load4<float>(const float* p) { return *reinterpret_cast<const float4*>(p); }
-template <typename T> __device__ __forceinline__ float4 load4(const T* p) {
-  return make_float4(to_f32(p[0]), to_f32(p[1]), to_f32(p[2]), to_f32(p[3]));
-}
-template <typename T> __device__ __forceinline__ void store4(T* p, float4 x) {
-  p[0] = from_f32<T>(x.x);
-  p[1] = from_f32<T>(x.y);
-  p[2] = from_f32<T>(x.z);
-  p[3] = from_f32<T>(x.w);
-}
+__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
 // 64 rows of D features -> [kD][kPad], rows from `valid` on and features from D on as zeros
-template <typename T, int kD>
-__device__ __forceinline__ void load_transposed(float* to, const T* from, int64_t stride, int valid, int D) {
+template <int kD>
+__device__ __forceinline__ void load_transposed(float* to, const float* from, int64_t stride, int valid, int D) {
   for (int e = threadIdx.x; e < kTile * kD / 4; e += kThreads) {
     const int r = e / (kD / 4), c = (e % (kD / 4)) * 4;
-    const float4 x = r < valid && c < D ? load4<T>(from + r * stride + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 x = r < valid && c < D ? load4(from + r * stride + c) : make_float4(0.f, 0.f, 0.f, 0.f);
     to[c * kPad + r] = x.x;
     to[(c + 1) * kPad + r] = x.y;
     to[(c + 2) * kPad + r] = x.z;
     to[(c + 3) * kPad + r] = x.w;
   }
 }
-template <typename T, int kD>
-__device__ __forceinline__ void load_rows(float* to, const T* from, int64_t stride, int valid, int D) {      // -> [64][kD]
+template <int kD>
+__device__ __forceinline__ void load_rows(float* to, const float* from, int64_t stride, int valid, int D) {      // -> [64][kD]
   for (int e = threadIdx.x; e < kTile * kD / 4; e += kThreads) {
     const int r = e / (kD / 4), c = (e % (kD / 4)) * 4;
-    *reinterpret_cast<float4*>(to + r * kD + c) = r < valid && c < D ? load4<T>(from + r * stride + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+    *reinterpret_cast<float4*>(to + r * kD + c) = r < valid && c < D ? load4(from + r * stride + c) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
 }
 // d[4][4] = sum over n of a[n][row ..] b[n][col ..]
@@ -71,8 +61,8 @@ __device__ __forceinline__ int length_of(const WindowParams& p, int b) {
   return p.lengths == nullptr ? p.Lk : min(max(ld_behind_wait(p.lengths + b), 0), p.Lk);
 }
 
-template <typename T, int kD>
-__global__ void __launch_bounds__(kThreads) window_fwd_kernel(const __grid_constant__ WindowParams p, float scale_log2) {
+template <int kD>
+__global__ void __launch_bounds__(kThreads) window_fwd_f32_kernel(const __grid_constant__ WindowParams p, float scale_log2) {
   extern __shared__ float smem[];
   float *qt = smem, *kt = qt + kD * kPad, *vr = kt + kD * kPad, *pt = vr + kTile * kD;      // pt [key][row]
   grid_dep_wait();
@@ -81,10 +71,10 @@ __global__ void __launch_bounds__(kThreads) window_fwd_kernel(const __grid_const
   const int tiles = gridDim.x, tile = tiles - 1 - (int)blockIdx.x, bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H;
   const int hk = h / (p.H / p.Hkv), off = p.Lk - p.Lq, len = length_of(p, b);
   const int rows = min(kTile, p.Lq - tile * kTile), p0 = off + tile * kTile;
-  const T* q = (const T*)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)tile * kTile * p.qs[2];
-  const T* k = (const T*)p.k + b * p.ks[0] + hk * p.ks[1];
-  const T* v = (const T*)p.v + b * p.vs[0] + hk * p.vs[1];
-  load_transposed<T, kD>(qt, q, p.qs[2], min(rows, len - p0), p.D);
+  const float* q = (const float*)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)tile * kTile * p.qs[2];
+  const float* k = (const float*)p.k + b * p.ks[0] + hk * p.ks[1];
+  const float* v = (const float*)p.v + b * p.vs[0] + hk * p.vs[1];
+  load_transposed<kD>(qt, q, p.qs[2], min(rows, len - p0), p.D);
   float m[4], l[4], o[4][kD / 16];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -97,8 +87,8 @@ __global__ void __launch_bounds__(kThreads) window_fwd_kernel(const __grid_const
   for (int i = 0, n = kts.sink_tiles + kts.last - kts.first + 1; i < n; ++i) {
     const int key0 = (i < kts.sink_tiles ? i : kts.first + i - kts.sink_tiles) * kTile;
     __syncthreads();
-    load_transposed<T, kD>(kt, k + key0 * p.ks[2], p.ks[2], len - key0, p.D);
-    load_rows<T, kD>(vr, v + key0 * p.vs[2], p.vs[2], len - key0, p.D);
+    load_transposed<kD>(kt, k + key0 * p.ks[2], p.ks[2], len - key0, p.D);
+    load_rows<kD>(vr, v + key0 * p.vs[2], p.vs[2], len - key0, p.D);
     __syncthreads();
     float s[4][4];
     product<kD>(s, qt, kt, ty, tx);
@@ -157,15 +147,15 @@ __global__ void __launch_bounds__(kThreads) window_fwd_kernel(const __grid_const
 #pragma unroll
     for (int c = 0; c < kD / 64; ++c)
       if (c * 64 + tx * 4 < p.D)
-        store4<T>((T*)p.o + at * p.D + c * 64 + tx * 4,
-                  make_float4(o[r][4 * c] * inv, o[r][4 * c + 1] * inv, o[r][4 * c + 2] * inv, o[r][4 * c + 3] * inv));
+        *reinterpret_cast<float4*>((float*)p.o + at * p.D + c * 64 + tx * 4) =
+            make_float4(o[r][4 * c] * inv, o[r][4 * c + 1] * inv, o[r][4 * c + 2] * inv, o[r][4 * c + 3] * inv);
     if (tx == 0) p.lse[at] = l[r] == 0.f ? INFINITY : m[r] + log2f(l[r]);
   }
 }
 
 // dQ of a tile of 64 query rows, and delta for the dK/dV kernel
-template <typename T, int kD>
-__global__ void __launch_bounds__(kThreads) window_dq_kernel(const __grid_constant__ WindowParams p, float scale_log2) {
+template <int kD>
+__global__ void __launch_bounds__(kThreads) window_dq_f32_kernel(const __grid_constant__ WindowParams p, float scale_log2) {
   extern __shared__ float smem[];
   float *qt = smem, *gt = qt + kD * kPad, *kt = gt + kD * kPad, *vt = kt + kD * kPad, *dst = vt + kD * kPad;      // dst [key][row]
   grid_dep_wait();
@@ -175,10 +165,10 @@ __global__ void __launch_bounds__(kThreads) window_dq_kernel(const __grid_consta
   const int hk = h / (p.H / p.Hkv), off = p.Lk - p.Lq, len = length_of(p, b);
   const int rows = min(kTile, p.Lq - tile * kTile), p0 = off + tile * kTile, valid = min(rows, len - p0);
   const int64_t row0 = (int64_t)bh * p.Lq + tile * kTile;
-  const T* k = (const T*)p.k + b * p.ks[0] + hk * p.ks[1];
-  const T* v = (const T*)p.v + b * p.vs[0] + hk * p.vs[1];
-  load_transposed<T, kD>(qt, (const T*)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)tile * kTile * p.qs[2], p.qs[2], valid, p.D);
-  load_transposed<T, kD>(gt, (const T*)p.dO + b * p.dos[0] + h * p.dos[1] + (int64_t)tile * kTile * p.dos[2], p.dos[2], valid, p.D);
+  const float* k = (const float*)p.k + b * p.ks[0] + hk * p.ks[1];
+  const float* v = (const float*)p.v + b * p.vs[0] + hk * p.vs[1];
+  load_transposed<kD>(qt, (const float*)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)tile * kTile * p.qs[2], p.qs[2], valid, p.D);
+  load_transposed<kD>(gt, (const float*)p.dO + b * p.dos[0] + h * p.dos[1] + (int64_t)tile * kTile * p.dos[2], p.dos[2], valid, p.D);
   __syncthreads();
   float delta[4], lse[4], dq[4][kD / 16];
 #pragma unroll
@@ -186,7 +176,7 @@ __global__ void __launch_bounds__(kThreads) window_dq_kernel(const __grid_consta
     const int row = ty * 4 + r;
     float sum = 0.f;
     if (row < valid)
-      for (int c = tx; c < p.D; c += 16) sum = fmaf(to_f32(((const T*)p.o)[(row0 + row) * p.D + c]), gt[c * kPad + row], sum);
+      for (int c = tx; c < p.D; c += 16) sum = fmaf(((const float*)p.o)[(row0 + row) * p.D + c], gt[c * kPad + row], sum);
 #pragma unroll
     for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
     delta[r] = sum;
@@ -199,8 +189,8 @@ __global__ void __launch_bounds__(kThreads) window_dq_kernel(const __grid_consta
   for (int i = 0, n = kts.sink_tiles + kts.last - kts.first + 1; i < n; ++i) {
     const int key0 = (i < kts.sink_tiles ? i : kts.first + i - kts.sink_tiles) * kTile;
     __syncthreads();
-    load_transposed<T, kD>(kt, k + key0 * p.ks[2], p.ks[2], len - key0, p.D);
-    load_transposed<T, kD>(vt, v + key0 * p.vs[2], p.vs[2], len - key0, p.D);
+    load_transposed<kD>(kt, k + key0 * p.ks[2], p.ks[2], len - key0, p.D);
+    load_transposed<kD>(vt, v + key0 * p.vs[2], p.vs[2], len - key0, p.D);
     __syncthreads();
     float s[4][4], dp[4][4];
     product<kD>(s, qt, kt, ty, tx);
@@ -234,13 +224,13 @@ __global__ void __launch_bounds__(kThreads) window_dq_kernel(const __grid_consta
     if (row >= rows) continue;
 #pragma unroll
     for (int c = 0; c < kD / 16; ++c)
-      if (c * 16 + tx < p.D) ((T*)p.dq)[(row0 + row) * p.D + c * 16 + tx] = from_f32<T>(row < valid ? dq[r][c] : 0.f);
+      if (c * 16 + tx < p.D) ((float*)p.dq)[(row0 + row) * p.D + c * 16 + tx] = row < valid ? dq[r][c] : 0.f;
   }
 }
 
 // dK and dV of a tile of 64 keys of one key head from a run of query tiles of all heads that share it
-template <typename T, int kD>
-__global__ void __launch_bounds__(kThreads) window_dkv_kernel(const __grid_constant__ WindowParams p, float scale_log2) {
+template <int kD>
+__global__ void __launch_bounds__(kThreads) window_dkv_f32_kernel(const __grid_constant__ WindowParams p, float scale_log2) {
   extern __shared__ float smem[];
   float *kt = smem, *vt = kt + kD * kPad, *qt = vt + kD * kPad, *gt = qt + kD * kPad;
   float *pr = gt + kD * kPad, *dsr = pr + kTile * kPad;                  // [query][key]
@@ -260,8 +250,8 @@ __global__ void __launch_bounds__(kThreads) window_dkv_kernel(const __grid_const
     if (first > last) return;
   }
   const int key0 = tile * kTile, valid_k = min(kTile, len - key0);
-  load_transposed<T, kD>(kt, (const T*)p.k + b * p.ks[0] + hk * p.ks[1] + key0 * p.ks[2], p.ks[2], valid_k, p.D);
-  load_transposed<T, kD>(vt, (const T*)p.v + b * p.vs[0] + hk * p.vs[1] + key0 * p.vs[2], p.vs[2], valid_k, p.D);
+  load_transposed<kD>(kt, (const float*)p.k + b * p.ks[0] + hk * p.ks[1] + key0 * p.ks[2], p.ks[2], valid_k, p.D);
+  load_transposed<kD>(vt, (const float*)p.v + b * p.vs[0] + hk * p.vs[1] + key0 * p.vs[2], p.vs[2], valid_k, p.D);
   float dk[4][kD / 16], dv[4][kD / 16];                                  // keys 4 ty .., features tx + 16 c
 #pragma unroll
   for (int r = 0; r < 4; ++r)
@@ -273,8 +263,8 @@ __global__ void __launch_bounds__(kThreads) window_dkv_kernel(const __grid_const
       const int valid_q = min(min(kTile, p.Lq - t * kTile), len - off - t * kTile);
       const int64_t row0 = ((int64_t)b * p.H + h) * p.Lq + t * kTile;
       __syncthreads();
-      load_transposed<T, kD>(qt, (const T*)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)t * kTile * p.qs[2], p.qs[2], valid_q, p.D);
-      load_transposed<T, kD>(gt, (const T*)p.dO + b * p.dos[0] + h * p.dos[1] + (int64_t)t * kTile * p.dos[2], p.dos[2], valid_q, p.D);
+      load_transposed<kD>(qt, (const float*)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)t * kTile * p.qs[2], p.qs[2], valid_q, p.D);
+      load_transposed<kD>(gt, (const float*)p.dO + b * p.dos[0] + h * p.dos[1] + (int64_t)t * kTile * p.dos[2], p.dos[2], valid_q, p.D);
       __syncthreads();
       float s[4][4], dp[4][4];
       product<kD>(s, qt, kt, ty, tx);
@@ -324,34 +314,10 @@ __global__ void __launch_bounds__(kThreads) window_dkv_kernel(const __grid_const
         part[key * p.D + f] = dk[r][c];
         part[(kTile + key) * p.D + f] = dv[r][c];
       } else {
-        ((T*)p.dk)[at + f] = from_f32<T>(dk[r][c]);
-        ((T*)p.dv)[at + f] = from_f32<T>(dv[r][c]);
+        ((float*)p.dk)[at + f] = dk[r][c];
+        ((float*)p.dv)[at + f] = dv[r][c];
       }
     }
-  }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ WindowParams p, int qt, int kk) {
-  grid_dep_wait();
-  grid_dep_launch();
-  const int tile = blockIdx.y % p.split.tiles, bk = blockIdx.y / p.split.tiles, b = bk / p.Hkv;
-  const int len = length_of(p, b);
-  const QueryTiles qts = queries_of_keys(tile, qt, kk, p.Lq, p.Lk - p.Lq, len, p.window, p.sinks);
-  const int runs = (qts.end - qts.last + p.split.run - 1) / p.split.run;
-  const int e = (blockIdx.x * 256 + threadIdx.x) * 4, key = e / p.D, f = e - key * p.D;
-  if (key >= kk || tile * kk + key >= p.Lk) return;
-  const int64_t slot = 2ll * kk * p.D;
-  const float* part = p.split.part + ((int64_t)bk * p.split.tiles + tile) * (1 + p.split.runs) * slot + e;
-  const int64_t at = ((int64_t)bk * p.Lk + tile * kk + key) * p.D + f;
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {                     // dK, dV
-    float4 sum = *reinterpret_cast<const float4*>(part + g * (slot / 2));
-    for (int r = 1; r <= runs; ++r) {
-      const float4 x = *reinterpret_cast<const float4*>(part + r * slot + g * (slot / 2));
-      sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
-    }
-    store4<T>((T*)(g == 0 ? p.dk : p.dv) + at, sum);
   }
 }
 
@@ -363,41 +329,27 @@ template <typename F> int allow(F* kernel, size_t smem) {
   LMK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   return LMK_OK;
 }
-template <typename T, int kD> int fwd(const WindowParams& p, cudaStream_t st) {
-  int rc = allow(window_fwd_kernel<T, kD>, kSmemFwd<kD>);
+template <int kD> int fwd(const WindowParams& p, cudaStream_t st) {
+  int rc = allow(window_fwd_f32_kernel<kD>, kSmemFwd<kD>);
   if (rc != LMK_OK) return rc;
   const dim3 grid((p.Lq + kTile - 1) / kTile, p.B * p.H);
-  LMK_CUDA(launch_overlapped(window_fwd_kernel<T, kD>, grid, dim3(kThreads), kSmemFwd<kD>, st, p, p.scale * kLog2e));
+  LMK_CUDA(launch_overlapped(window_fwd_f32_kernel<kD>, grid, dim3(kThreads), kSmemFwd<kD>, st, p, p.scale * kLog2e));
   return LMK_OK;
 }
-template <typename T, int kD> int bwd(const WindowParams& p, cudaStream_t st) {
-  int rc = allow(window_dq_kernel<T, kD>, kSmemDq<kD>);
-  if (rc == LMK_OK) rc = allow(window_dkv_kernel<T, kD>, kSmemDkv<kD>);
+template <int kD> int bwd(const WindowParams& p, cudaStream_t st) {
+  int rc = allow(window_dq_f32_kernel<kD>, kSmemDq<kD>);
+  if (rc == LMK_OK) rc = allow(window_dkv_f32_kernel<kD>, kSmemDkv<kD>);
   if (rc != LMK_OK) return rc;
   const dim3 grid_q((p.Lq + kTile - 1) / kTile, p.B * p.H);
   const dim3 grid_k((p.Lk + kTile - 1) / kTile + p.split.tiles * p.split.runs, p.B * p.Hkv);
-  LMK_CUDA(launch_overlapped(window_dq_kernel<T, kD>, grid_q, dim3(kThreads), kSmemDq<kD>, st, p, p.scale * kLog2e));
-  LMK_CUDA(launch_overlapped(window_dkv_kernel<T, kD>, grid_k, dim3(kThreads), kSmemDkv<kD>, st, p, p.scale * kLog2e));
-  return p.split.tiles > 0 ? window_join_parts(p, kTile, kTile, std::is_same<T, float>::value ? LMK_F32 : std::is_same<T, __half>::value ? LMK_F16 : LMK_BF16, st)
-                           : LMK_OK;
+  LMK_CUDA(launch_overlapped(window_dq_f32_kernel<kD>, grid_q, dim3(kThreads), kSmemDq<kD>, st, p, p.scale * kLog2e));
+  LMK_CUDA(launch_overlapped(window_dkv_f32_kernel<kD>, grid_k, dim3(kThreads), kSmemDkv<kD>, st, p, p.scale * kLog2e));
+  return p.split.tiles > 0 ? window_join_parts(p, kTile, kTile, LMK_F32, st) : LMK_OK;
 }
 
 }  // namespace
 
-#define LMK_GENERAL(FN) \
-  if (dtype == LMK_F32) return p.D <= 64 ? FN<float, 64>(p, st) : FN<float, 128>(p, st); \
-  if (dtype == LMK_F16) return p.D <= 64 ? FN<__half, 64>(p, st) : FN<__half, 128>(p, st); \
-  return p.D <= 64 ? FN<__nv_bfloat16, 64>(p, st) : FN<__nv_bfloat16, 128>(p, st)
-int window_general_fwd(const WindowParams& p, int dtype, cudaStream_t st) { LMK_GENERAL(fwd); }
-int window_general_bwd(const WindowParams& p, int dtype, cudaStream_t st) { LMK_GENERAL(bwd); }
-#undef LMK_GENERAL
-
-int window_join_parts(const WindowParams& p, int qt, int kk, int dtype, cudaStream_t st) {
-  const dim3 grid((kk * p.D / 4 + 255) / 256, p.B * p.Hkv * p.split.tiles);
-  if (dtype == LMK_F32) LMK_CUDA(launch_overlapped(window_join_kernel<float>, grid, dim3(256), 0, st, p, qt, kk));
-  else if (dtype == LMK_F16) LMK_CUDA(launch_overlapped(window_join_kernel<__half>, grid, dim3(256), 0, st, p, qt, kk));
-  else LMK_CUDA(launch_overlapped(window_join_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p, qt, kk));
-  return LMK_OK;
-}
+int window_f32_fwd(const WindowParams& p, cudaStream_t st) { return p.D <= 64 ? fwd<64>(p, st) : fwd<128>(p, st); }
+int window_f32_bwd(const WindowParams& p, cudaStream_t st) { return p.D <= 64 ? bwd<64>(p, st) : bwd<128>(p, st); }
 
 }  // namespace lmk

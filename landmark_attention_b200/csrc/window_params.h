@@ -75,8 +75,13 @@ __host__ __device__ inline bool window_sees(int pos, int key, int window, int si
   return key <= pos && (pos - key < window || key < sinks);
 }
 
-int window_general_fwd(const WindowParams& p, int dtype, cudaStream_t st);
-int window_general_bwd(const WindowParams& p, int dtype, cudaStream_t st);
+// fp32, tiles of 64 query rows and 64 keys
+int window_f32_fwd(const WindowParams& p, cudaStream_t st);
+int window_f32_bwd(const WindowParams& p, cudaStream_t st);
+// 16-bit types, tiles of 128 query rows; dK and dV in tiles of 128 keys
+int window_sm100_fwd(const WindowParams& p, int dtype, cudaStream_t st);
+int window_sm100_bwd(const WindowParams& p, int dtype, cudaStream_t st);
+bool window_sm100_operand_ok(const void* p, const int64_t st[3], int D);
 // adds up the parts of the split key tiles (kk keys each) into dk and dv
 int window_join_parts(const WindowParams& p, int qt, int kk, int dtype, cudaStream_t st);
 

@@ -1,0 +1,1243 @@
+// Sliding-window attention with sinks on the tensor cores (sm_100a): bf16 / fp16, head dims up to 128, TMA-fed tcgen05 products with
+// accumulators in TMEM.  Query tiles of 128 rows meet key tiles of 64 (forward, dQ) or pairs of them (dK, dV); only the tiles that
+// the window or the sinks make visible are visited (window_params.h), and only those on an edge are masked.
+//
+// Forward: one or two query tiles a CTA that share one stream of key tiles, newest first, the sinks' last.
+//   S = Q K^T -> a softmax thread owns one row (= one TMEM lane): p = 2^(s c - m), l += sum p, P written in 16 bits over the TMEM
+//   columns its S came from -> O += P V with A = P from TMEM.  m is the running maximum, but is only moved when a tile exceeds it by more
+//   than 2^8: O then has to be read, scaled and written back (TMEM), which with the first tile's maximum as m happens to a few rows of
+//   a long sequence.  p <= 2^8 costs no precision: p, l and O are floating point, and O / l does not depend on m.
+// Backward: recomputed from lse = m + log2 l, in two launches.
+//   dQ: unit = (query tile, head), persistent.  Q and dO rows go to TMEM as A operands; per key tile S, dP -> dS over the V tile -> dQ += dS K.
+//   dK/dV: unit = (pair of key tiles, key head, run of query tiles), persistent; Q and dO tiles of all heads that share the keys
+//   stream through.  P^T dO and dS^T Q take P and dS from shared memory as MN-major operands.  The accumulators are the sums over the
+//   group's heads.  The query tiles of a pair with sinks are dealt out to several units (SinkSplit): one unit would be as long as the
+//   sequence.
+// Rows behind a sequence's end (lengths) are hidden by selects and, where a product would multiply them with a zero, overwritten with zeros in
+// shared memory by the loading thread, so that NaN there stays there.
+// All waits are bounded (sm100_ptx.cuh).
+#include <mutex>
+#include "common.cuh"
+#include "attn_params.h"
+#include "window_params.h"
+#include "sm100_ptx.cuh"
+#include "sm100_tiles.cuh"
+
+namespace lmk {
+namespace {
+
+using namespace ptx;
+
+constexpr int kBlk = 64;
+constexpr int kQTile = 128;
+constexpr uint32_t kTileBytes = 16384;   // one [128 x 64] or two [64 x 64] 16-bit tiles
+constexpr uint32_t kHalfTile = 8192;
+constexpr float kLog2e = 1.4426950408889634f;
+enum { kErrFwdProducer = 711, kErrFwdMma = 712, kErrFwdSoftmax = 713, kErrFwdEpilogue = 714, kErrDkvProducer = 721, kErrDkvMma = 722,
+       kErrDkvSoftmax = 723, kErrDkvEpilogue = 724, kErrDqProducer = 731, kErrDqMma = 732, kErrDqSoftmax = 733, kErrDqEpilogue = 734 };
+
+__device__ __forceinline__ int length_of(const int* lengths, int b, int Lk) {
+  return lengths == nullptr ? Lk : min(max(ld_behind_wait(lengths + b), 0), Lk);
+}
+// rows [from, rows) of a tile of 64-feature sub-tiles become zeros; one thread, ahead of products that read the tile
+__device__ __forceinline__ void zero_rows(uint32_t tile, uint32_t subtile_bytes, int subtiles, int from, int rows) {
+  for (int c = 0; c < subtiles; ++c)
+    for (uint32_t a = tile + c * subtile_bytes + from * 128u; a < tile + c * subtile_bytes + rows * 128u; a += 16)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(a), "r"(0) : "memory");
+  fence_proxy_async_smem();
+}
+
+// A row's visible columns of the key tile that starts at key0: j <= last and (j >= first or j < sink)
+struct Columns {
+  int last, first, sink;
+  __device__ Columns(int pos, int key0, int window, int sinks) : last(pos - key0), first(pos - window + 1 - key0), sink(sinks - key0) {}
+  __device__ bool sees(int j) const { return j <= last && (j >= first || j < sink); }
+};
+// every row at positions p0 .. p1 sees every key of the tile / no row sees one
+__device__ __forceinline__ bool tile_full(int p0, int p1, int key0, int window, int sinks) {
+  return key0 + kBlk - 1 <= p0 && (p1 - key0 < window || key0 + kBlk <= sinks);
+}
+__device__ __forceinline__ bool tile_empty(int p0, int p1, int key0, int window, int sinks) {
+  return key0 > p1 || (p0 - (key0 + kBlk - 1) >= window && key0 >= sinks);
+}
+
+struct WindowTensors {
+  void* o;                  // forward: output
+  float* lse;
+  const int* lengths;
+  int H, G, Lq, Lk, D, window, sinks;
+  float scale, scale_log2;
+};
+
+// ---------------------------------------------------------------------------------------------- forward
+template <int kTiles> constexpr int kFwdStages = kTiles == 2 ? 5 : 2;
+template <int kTiles> constexpr int kFwdThreads = (4 * kTiles + 3) * 32;
+constexpr int kFwdPolyEvery = 8;         // one pair of exponentials in this many is a polynomial on the FMA pipe
+constexpr float kLazy = 8.f;             // the maximum moves when it is exceeded by this much (log2)
+
+template <int kStages> struct FwdSmem {
+  uint64_t q_full, patch;
+  uint64_t full[kStages], empty[kStages];
+  uint64_t s_full[2][2], s_free[2][2], p_ready[2][2];      // [tile][S / P buffer]
+  uint64_t o_full;
+  uint32_t tmem_base;
+};
+
+__device__ __forceinline__ float max_of_64(const float (&v)[64]) {      // NaN where one is
+  float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int j = 0; j < 64; j += 2) m[j / 2 % 4] = max3_nan(m[j / 2 % 4], v[j], v[j + 1]);
+  return max3_nan(max3_nan(m[0], m[1], m[2]), m[3], m[3]);
+}
+
+template <bool kBf16, int kD, int kTiles>
+__global__ void __launch_bounds__(kFwdThreads<kTiles>, 3 - kTiles)
+window_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                        const __grid_constant__ CUtensorMap tm_v, const WindowTensors p, int* status) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  constexpr int kStages = kFwdStages<kTiles>, kSw = 4 * kTiles;        // softmax warps; the three roles follow them
+  auto q_tile = [&](int w) { return base + (uint32_t)w * 32768u; };
+  auto k_slot = [&](int s) { return base + kTiles * 32768u + (uint32_t)s * 32768u; };
+  auto v_slot = [&](int s) { return base + kTiles * 32768u + (uint32_t)s * 32768u + 16384u; };
+  FwdSmem<kStages>* sm = reinterpret_cast<FwdSmem<kStages>*>(smem_raw + (base - raw) + (kTiles + kStages) * 32768u);
+
+  const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
+  const int t_a = ((int)gridDim.y - 1 - (int)blockIdx.y) * kTiles;      // longest tiles first, across all heads
+  const int bh = blockIdx.x, b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
+  const int off = p.Lk - p.Lq;
+  grid_dep_wait();
+  grid_dep_launch();
+  const int len = warp_uniform(length_of(p.lengths, b, p.Lk));
+  const int pos_a = off + t_a * kQTile;                 // key position of tile A's first row
+  if (pos_a >= len) {                                   // nothing but padding
+    const int rows = min(kTiles * kQTile, p.Lq - t_a * kQTile);
+    uint4* const o = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.o) + ((int64_t)bh * p.Lq + t_a * kQTile) * p.D);
+    for (int e = tid; e < rows * p.D / 8; e += kFwdThreads<kTiles>) o[e] = make_uint4(0u, 0u, 0u, 0u);
+    for (int r = tid; r < rows; r += kFwdThreads<kTiles>) p.lse[(int64_t)bh * p.Lq + t_a * kQTile + r] = INFINITY;
+    return;
+  }
+  const bool has_b = kTiles == 2 && (t_a + 1) * kQTile < p.Lq && pos_a + kQTile < len;
+  const KeyTiles ka = keys_of_queries(t_a, kQTile, kBlk, p.Lq, off, len, p.window, p.sinks);
+  const KeyTiles kb = has_b ? keys_of_queries(t_a + 1, kQTile, kBlk, p.Lq, off, len, p.window, p.sinks) : ka;
+  const int st = (p.sinks + kBlk - 1) / kBlk;
+  const int newest = kb.last, n_win = newest - ka.first + 1, total = n_win + ka.sink_tiles;
+  auto tile_of = [&](int i) { return i < n_win ? newest - i : ka.sink_tiles - 1 - (i - n_win); };
+  auto active = [&](int w, int i) {
+    const int n = tile_of(i);
+    return w == 1 ? has_b && (n < st || n >= kb.first) : n <= ka.last;
+  };
+
+  if (tid == 0) {
+    mbar_init(smem_u32(&sm->q_full), 1);
+    mbar_init(smem_u32(&sm->patch), 1);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(smem_u32(&sm->full[s]), 1);
+      mbar_init(smem_u32(&sm->empty[s]), 1);
+    }
+    for (int w = 0; w < 2; ++w)
+      for (int s = 0; s < 2; ++s) {
+        mbar_init(smem_u32(&sm->s_full[w][s]), 1);
+        mbar_init(smem_u32(&sm->s_free[w][s]), 1);
+        mbar_init(smem_u32(&sm->p_ready[w][s]), 128);
+      }
+    mbar_init(smem_u32(&sm->o_full), 1);
+    mbar_init_fence();
+  }
+  if (warp == kSw + 1) tmem_alloc(smem_u32(&sm->tmem_base), kTiles * 256);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = (uint32_t)warp_uniform((int)sm->tmem_base);
+  auto tmem_s = [&](int w, int sb) { return tmem + (uint32_t)(w * 128 + sb * 64); };
+  auto tmem_o = [&](int w) { return tmem + kTiles * 128u + (uint32_t)w * 128u; };
+
+  if (warp == kSw) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      const uint32_t qb = smem_u32(&sm->q_full);
+      mbar_arrive_expect_tx(qb, (has_b ? 2 : 1) * (kD / 64) * kTileBytes);
+      for (int w = 0; w < (has_b ? 2 : 1); ++w)
+        for (int c = 0; c < kD / 64; ++c) tma_load_4d(q_tile(w) + c * kTileBytes, &tm_q, qb, 64 * c, (t_a + w) * kQTile, h, b);
+      for (int i = 0; i < total; ++i) {
+        const int s = i % kStages, key0 = tile_of(i) * kBlk;
+        mbar_wait(smem_u32(&sm->empty[s]), ((i / kStages) & 1) ^ 1, status, kErrFwdProducer);
+        const bool ends = key0 + kBlk > len && len < p.Lk;      // the tile the sequence ends in, once at most (the newest)
+        const uint32_t fb = smem_u32(ends ? &sm->patch : &sm->full[s]);
+        mbar_arrive_expect_tx(fb, 2 * (kD / 64) * kHalfTile);
+        for (int c = 0; c < kD / 64; ++c) {
+          tma_load_4d(k_slot(s) + c * kHalfTile, &tm_k, fb, 64 * c, key0, hk, b);
+          tma_load_4d(v_slot(s) + c * kHalfTile, &tm_v, fb, 64 * c, key0, hk, b);
+        }
+        if (ends) {
+          mbar_wait(fb, 0, status, kErrFwdProducer);
+          zero_rows(v_slot(s), kHalfTile, kD / 64, len - key0, kBlk);
+          mbar_arrive(smem_u32(&sm->full[s]));
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == kSw + 1) {
+    // ------------------------------------------------------------------ MMA issuer 1: S = Q K^T
+    constexpr uint32_t fmt = kBf16 ? 1u : 0u;
+    constexpr uint32_t idesc_s = instr_desc_f16(fmt, 128, 64, 0, 0);
+    mbar_wait(smem_u32(&sm->q_full), 0, status, kErrFwdMma);
+    const uint64_t dq0 = smem_desc_sw128(q_tile(0), 16, 1024);
+    const uint64_t dk0 = smem_desc_sw128(k_slot(0), 16, 1024);
+    int ks[2] = {0, 0};
+    int s = 0;
+    uint32_t ph = 0;
+    for (int j = 0; j < total; ++j) {
+      mbar_wait(smem_u32(&sm->full[s]), ph, status, kErrFwdMma);
+      const uint64_t dk = desc_advance(dk0, (uint32_t)s * 32768u);
+#pragma unroll
+      for (int w = 0; w < kTiles; ++w) {
+        if (!active(w, j)) continue;
+        const int k = ks[w]++, sb = k & 1;
+        if (k >= 2) mbar_wait(smem_u32(&sm->s_free[w][sb]), ((k >> 1) & 1) ^ 1, status, kErrFwdMma);
+        tc_fence_after();
+        const uint64_t dq = desc_advance(dq0, (uint32_t)w * 32768u);
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < kD / 16; ++kk)
+            mma_f16_ss(tmem_s(w, sb), desc_advance(dq, kmajor_step(kk, kTileBytes)), desc_advance(dk, kmajor_step(kk, kHalfTile)), idesc_s, kk > 0);
+          mma_commit(smem_u32(&sm->s_full[w][sb]));
+        }
+      }
+      if (++s == kStages) { s = 0; ph ^= 1; }
+    }
+    __syncwarp();
+  } else if (warp == kSw + 2) {
+    // ------------------------------------------------------------------ MMA issuer 2: O += P V
+    constexpr uint32_t fmt = kBf16 ? 1u : 0u;
+    constexpr uint32_t idesc_o = instr_desc_f16(fmt, 128, kD, 0, 1);
+    const uint64_t dv0 = smem_desc_sw128(v_slot(0), kHalfTile, 1024);
+    int kp[2] = {0, 0};
+    int s = 0;
+    for (int i = 0; i < total; ++i) {
+      const uint64_t dv = desc_advance(dv0, (uint32_t)s * 32768u);
+#pragma unroll
+      for (int w = 0; w < kTiles; ++w) {
+        if (!active(w, i)) continue;
+        const int k = kp[w]++;
+        mbar_wait(smem_u32(&sm->p_ready[w][k & 1]), (k >> 1) & 1, status, kErrFwdMma);
+        tc_fence_after();
+        const uint32_t tp = tmem_s(w, k & 1);      // P: 8 columns = 16 keys per K-step
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < kBlk / 16; ++kk)
+            mma_f16_ts(tmem_o(w), tp + kk * 8, desc_advance(dv, kk * 2048), idesc_o, (k > 0 || kk > 0) ? 1u : 0u);
+          mma_commit(smem_u32(&sm->s_free[w][k & 1]));
+        }
+      }
+      // the stage is free once both P V products are done; each of them waited for its S product to be read
+      if (elect_one()) mma_commit(smem_u32(&sm->empty[s]));
+      if (++s == kStages) s = 0;
+    }
+    if (elect_one()) mma_commit(smem_u32(&sm->o_full));
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ softmax warpgroups
+    const int w = warp >> 2;                       // 0: tile A, 1: tile B
+    const int row = tid & 127;
+    const int pos = pos_a + w * kQTile + row;
+    const int warp_p0 = warp_uniform(pos_a + w * kQTile + (warp & 3) * 32), warp_p1 = warp_p0 + 31;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const float c = p.scale_log2;
+    float m2 = -INFINITY, l = 0.f;
+    int k = 0;
+    for (int i = 0; i < total; ++i) {
+      if (!active(w, i)) continue;
+      const int sb = k & 1, key0 = tile_of(i) * kBlk;
+      mbar_wait(smem_u32(&sm->s_full[w][sb]), (k / 2) & 1, status, kErrFwdSoftmax);
+      tc_fence_after();
+      uint32_t wgt[32];
+      if (tile_empty(warp_p0, warp_p1, key0, p.window, p.sinks)) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) wgt[j] = 0u;
+      } else {
+        float sv[64];
+        {
+          uint32_t ra[32], rb[32];
+          tmem_ld_32x32b_x32(tmem_s(w, sb) + lane_base, ra);
+          tmem_ld_32x32b_x32(tmem_s(w, sb) + 32 + lane_base, rb);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            sv[j] = __uint_as_float(ra[j]);
+            sv[32 + j] = __uint_as_float(rb[j]);
+          }
+        }
+        const bool full = tile_full(warp_p0, warp_p1, key0, p.window, p.sinks);
+        if (!full) {
+          const Columns col(pos, key0, p.window, p.sinks);
+#pragma unroll
+          for (int j = 0; j < 64; ++j) sv[j] = col.sees(j) ? sv[j] : -INFINITY;
+        }
+        const float mx = max_of_64(sv);
+        const float mc = mx * c;                                     // -inf: nothing visible
+        const bool move = mc > m2 + kLazy;                           // from -inf on too
+        if (__any_sync(0xffffffffu, move && m2 != -INFINITY)) {
+          // O is rescaled behind the product of the item before, whose end s_free of its buffer tells (this thread sees every
+          // second phase of it at the latest: S of this item was only issued behind the product two items back)
+          mbar_wait(smem_u32(&sm->s_free[w][sb ^ 1]), ((k - 1) >> 1) & 1, status, kErrFwdSoftmax);
+          tc_fence_after();
+          const float f = move ? ex2(m2 - mc) : 1.f;                 // from -inf: 0, where O is 0
+          l *= f;
+          for (int cc = 0; cc < kD / 16; ++cc) {                      // 16 columns at a time: the row's scores stay in registers
+            uint32_t r[16];
+            tmem_ld_32x32b_x16(tmem_o(w) + cc * 16 + lane_base, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * f);
+            tmem_st_32x32b_x16(tmem_o(w) + cc * 16 + lane_base, r);
+          }
+          tmem_st_wait();
+        }
+        if (move) m2 = mc;
+        uint64_t sp[32];
+        if (!full) {
+          const float shift = m2 == -INFINITY ? 0.f : m2;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) sp[j] = pk2(ex2(fmaf(sv[2 * j], c, -shift)), ex2(fmaf(sv[2 * j + 1], c, -shift)));
+        } else {
+          // polynomials make finite numbers of NaN and infinities: a maximum that is one makes NaN of the shift of all
+          const float n = fmaf(mx, 0.f, -m2);
+          const uint64_t c2 = pk2(c, c), n2 = pk2(n, n);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const uint64_t x = fma2(pk2(sv[2 * j], sv[2 * j + 1]), c2, n2);
+            if (j % kFwdPolyEvery == 1) {
+              sp[j] = ex2_poly2<4>(x);
+            } else {
+              float x0, x1;
+              upk2(x, x0, x1);
+              sp[j] = pk2(ex2(x0), ex2(x1));
+            }
+          }
+        }
+        uint64_t s0 = sp[0], s1 = sp[1], s2 = sp[2], s3 = sp[3];
+#pragma unroll
+        for (int j = 4; j < 32; j += 4) {
+          s0 = add2(s0, sp[j]);
+          s1 = add2(s1, sp[j + 1]);
+          s2 = add2(s2, sp[j + 2]);
+          s3 = add2(s3, sp[j + 3]);
+        }
+        float dl, dh;
+        upk2(add2(add2(s0, s1), add2(s2, s3)), dl, dh);
+        l += dl + dh;
+        // P enters the product in 16 bits: half a step of relative error a weight; l sums the unrounded ones
+#pragma unroll
+        for (int j = 0; j < 32; ++j) wgt[j] = pack2p<kBf16>(sp[j]);
+      }
+      tmem_st_32x32b_x32(tmem_s(w, sb) + lane_base, wgt);     // P replaces S in place; the P V product reads it there
+      tmem_st_wait();
+      tc_fence_before();
+      mbar_arrive(smem_u32(&sm->p_ready[w][sb]));
+      ++k;
+    }
+    // ------------------------------------------------------------------ epilogue
+    const int t = t_a + w;
+    if (w == 0 || has_b) {
+      mbar_wait(smem_u32(&sm->o_full), 0, status, kErrFwdEpilogue);
+      tc_fence_after();
+    }
+    const int grow = t * kQTile + row;
+    const bool stored = grow < p.Lq, valid = pos < len && l != 0.f;
+    const float inv = valid ? 1.f / l : 0.f;
+    uint4* orow = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.o) + ((int64_t)bh * p.Lq + grow) * p.D);
+#pragma unroll
+    for (int cc = 0; cc < kD / 32; ++cc) {
+      uint32_t r[32];
+      if (w == 0 || has_b) {
+        tmem_ld_32x32b_x32(tmem_o(w) + cc * 32 + lane_base, r);
+        tmem_ld_wait();
+      }
+#pragma unroll
+      for (int v4 = 0; v4 < 4; ++v4) {
+        uint4 pk;
+        pk.x = pack2<kBf16>(__uint_as_float(r[8 * v4 + 0]) * inv, __uint_as_float(r[8 * v4 + 1]) * inv);
+        pk.y = pack2<kBf16>(__uint_as_float(r[8 * v4 + 2]) * inv, __uint_as_float(r[8 * v4 + 3]) * inv);
+        pk.z = pack2<kBf16>(__uint_as_float(r[8 * v4 + 4]) * inv, __uint_as_float(r[8 * v4 + 5]) * inv);
+        pk.w = pack2<kBf16>(__uint_as_float(r[8 * v4 + 6]) * inv, __uint_as_float(r[8 * v4 + 7]) * inv);
+        if (!valid) pk = make_uint4(0u, 0u, 0u, 0u);          // (not 0 * whatever padding left in the accumulator)
+        if (stored && cc * 32 + v4 * 8 < p.D) orow[cc * 4 + v4] = pk;
+      }
+    }
+    if (stored) p.lse[(int64_t)bh * p.Lq + grow] = valid ? m2 + __log2f(l) : INFINITY;
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == kSw + 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTiles * 256);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- backward
+// one pair of exponentials in this many is a cubic (7.5e-5, below half a step of either type); full tiles only
+constexpr int kBwdPolyEvery = 4;
+
+// Reads 64 columns of S from TMEM and leaves the row's weights p = 2^(s c - lse) in sp, hidden columns 0.
+// kind 0: nothing visible, 1: masked, 2: full (the same for all rows of a warp).
+template <typename AfterFn>
+__device__ __forceinline__ void bwd_weights(uint64_t (&sp)[32], uint32_t ts, int kind, const Columns& col, float c, float lse, AfterFn after_s) {
+  if (kind == 0) {
+    after_s();
+#pragma unroll
+    for (int j = 0; j < 32; ++j) sp[j] = 0ull;
+    return;
+  }
+  {
+    uint32_t ra[32], rb[32];
+    tmem_ld_32x32b_x32(ts, ra);
+    tmem_ld_32x32b_x32(ts + 32, rb);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      sp[j] = pk2u(ra[2 * j], ra[2 * j + 1]);
+      sp[16 + j] = pk2u(rb[2 * j], rb[2 * j + 1]);
+    }
+  }
+  after_s();      // S is in registers: its buffer may take the next product
+  const uint64_t c2 = pk2(c, c), m2 = pk2(-lse, -lse);
+  if (kind == 1) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      float a, b;
+      upk2(fma2(sp[j], c2, m2), a, b);
+      sp[j] = pk2(col.sees(2 * j) ? ex2(a) : 0.f, col.sees(2 * j + 1) ? ex2(b) : 0.f);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j) {
+      const uint64_t x = fma2(sp[j], c2, m2);
+      if (j % kBwdPolyEvery == 1) {
+        sp[j] = ex2_poly2<3>(x);
+      } else {
+        float a, b;
+        upk2(x, a, b);
+        sp[j] = pk2(ex2(a), ex2(b));
+      }
+    }
+  }
+}
+
+// Reads dP from TMEM, arrives on free_bar, and leaves the row of dS = p (dP - delta) scale, packed to 16 bits, in wd.
+template <bool kBf16>
+__device__ __forceinline__ void bwd_dscores(uint32_t (&wd)[32], const uint64_t (&sp)[32], uint32_t tdp, uint32_t free_bar, int kind,
+                                            const Columns& col, float scale, float delta) {
+  if (kind == 0) {
+    tc_fence_before();
+    mbar_arrive(free_bar);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) wd[j] = 0u;
+    return;
+  }
+  uint64_t dp[32];
+  {
+    uint32_t ra[32], rb[32];
+    tmem_ld_32x32b_x32(tdp, ra);
+    tmem_ld_32x32b_x32(tdp + 32, rb);
+    tmem_ld_wait();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      dp[j] = pk2u(ra[2 * j], ra[2 * j + 1]);
+      dp[16 + j] = pk2u(rb[2 * j], rb[2 * j + 1]);
+    }
+  }
+  tc_fence_before();
+  mbar_arrive(free_bar);
+  const uint64_t sc2 = pk2(scale, scale);
+  const float ns = -delta * scale;
+  const uint64_t ns2 = pk2(ns, ns);
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    float d0, d1;
+    upk2(mul2(sp[j], fma2(dp[j], sc2, ns2)), d0, d1);
+    if (kind == 1) {                          // what a hidden value or a padded row brought along is dropped, not multiplied by 0
+      d0 = col.sees(2 * j) ? d0 : 0.f;
+      d1 = col.sees(2 * j + 1) ? d1 : 0.f;
+    }
+    wd[j] = pack2<kBf16>(d0, d1);
+  }
+}
+
+constexpr int kBwdGroups = 2;                       // softmax warpgroups
+constexpr int kBwdThreads = (kBwdGroups * 4 + 3) * 32;
+constexpr int kPair = 128;                          // keys of a dK/dV unit
+template <int kD> constexpr int kDkvStages = kD == 128 ? 2 : 4;
+
+template <int kStages> struct DkvSmem {
+  uint64_t k_full, k_empty, v_full, v_empty, patch;
+  uint64_t q_full[kStages], q_empty[kStages];       // Q: until dK has read it
+  uint64_t do_full[kStages], do_empty[kStages];     // dO: until dP and dV have read it
+  uint64_t s_full, s_free, dp_full, dp_free;        // S, dP of both blocks (N = 128 products)
+  uint64_t p_ready, p_free, ds_ready, ds_free;      // the P rows are in the weight tiles / dV has read them; likewise dS in their place
+  uint64_t acc_full[2], acc_empty[2];               // [0] dV, [1] dK
+  uint32_t tmem_base;
+};
+
+struct DkvArgs {
+  const float *lse, *delta;
+  void *dk, *dv;
+  const int* lengths;
+  int H, Hkv, G, B, Lq, Lk, D, window, sinks, n_pairs;
+  float scale, scale_log2;
+  SinkSplit split;
+};
+// a unit: query tiles first .. last of every head of the group against a pair of key tiles
+struct DkvUnit {
+  int b, hk, pair, first, n_q, len;      // n_q: query tiles of one head
+  int run;                               // -1: the window's share, else the run of the sinks' share
+  __device__ bool base() const { return run < 0; }
+};
+
+template <bool kBf16, int kD>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
+                        const __grid_constant__ DkvArgs p, int* status) {
+  constexpr int kStages = kDkvStages<kD>;
+  constexpr uint32_t kOperand = (kD / 64) * kTileBytes;     // [128 rows x kD] as 64-feature sub-tiles of 16 KB
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  const uint32_t k_pair = base, v_pair = base + kOperand;
+  auto q_slot = [&](int s) { return base + 2 * kOperand + (uint32_t)s * 2 * kOperand; };
+  auto do_slot = [&](int s) { return base + 3 * kOperand + (uint32_t)s * 2 * kOperand; };
+  const uint32_t w_tile = base + (2 + 2 * kStages) * kOperand;         // P, then dS: [128 q x 64 keys] of block a, then of b
+  DkvSmem<kStages>* sm =
+      reinterpret_cast<DkvSmem<kStages>*>(smem_raw + (base - raw) + (2 + 2 * kStages) * kOperand + 2 * kTileBytes);
+
+  const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
+  const int off = p.Lk - p.Lq, heads = p.B * p.Hkv;
+  const int n_runs = p.split.tiles * p.split.runs * heads, n_units = n_runs + p.n_pairs * heads;
+  auto unit_at = [&](int r) { return r * (int)gridDim.x + ((r & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x); };
+  // the runs first: they are as long as the longest of the others
+  auto unit_of = [&](int w) {
+    DkvUnit u;
+    int bk;
+    if (w < n_runs) {
+      const int x = w / heads;
+      bk = w - x * heads;
+      u.pair = x / p.split.runs;
+      u.run = x - u.pair * p.split.runs;
+    } else {
+      u.pair = (w - n_runs) / heads;
+      bk = (w - n_runs) - u.pair * heads;
+      u.run = -1;
+    }
+    u.b = bk / p.Hkv;
+    u.hk = bk - u.b * p.Hkv;
+    u.len = length_of(p.lengths, u.b, p.Lk);
+    const QueryTiles q = queries_of_keys(u.pair, kQTile, kPair, p.Lq, off, u.len, p.window, p.sinks);
+    u.first = q.first;
+    int last = u.pair < p.split.tiles ? q.last : q.end;
+    if (u.run >= 0) {
+      u.first = q.last + 1 + u.run * p.split.run;
+      last = min(q.end, u.first + p.split.run - 1);
+    }
+    u.n_q = max(last - u.first + 1, 0);
+    return u;
+  };
+
+  if (tid == 0) {
+    for (uint64_t* bar : {&sm->k_full, &sm->k_empty, &sm->v_full, &sm->v_empty, &sm->patch, &sm->s_full, &sm->dp_full, &sm->p_free, &sm->ds_free})
+      mbar_init(smem_u32(bar), 1);
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(smem_u32(&sm->q_full[s]), 1);
+      mbar_init(smem_u32(&sm->q_empty[s]), 1);
+      mbar_init(smem_u32(&sm->do_full[s]), 1);
+      mbar_init(smem_u32(&sm->do_empty[s]), 2);       // dP and dV, issued by different warps
+    }
+    for (uint64_t* bar : {&sm->s_free, &sm->dp_free, &sm->p_ready, &sm->ds_ready}) mbar_init(smem_u32(bar), 256);
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(smem_u32(&sm->acc_full[g]), 1);
+      mbar_init(smem_u32(&sm->acc_empty[g]), 128);
+    }
+    mbar_init_fence();
+  }
+  if (warp == kBwdGroups * 4 + 1) tmem_alloc(smem_u32(&sm->tmem_base), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = (uint32_t)warp_uniform((int)sm->tmem_base);
+  const uint32_t tmem_s = tmem, tmem_dp = tmem + 128u, tmem_dv = tmem + 256u, tmem_dk = tmem + 256u + kD;
+
+  if (warp == kBwdGroups * 4) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int it = 0, u = 0, patches = 0;
+      for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
+        const DkvUnit un = unit_of(w);
+        const int n_items = un.n_q * p.G;
+        if (n_items == 0) continue;
+        auto load_pair = [&](uint32_t dst, const CUtensorMap* tm, uint64_t* full, uint64_t* empty) {
+          const uint32_t fb = smem_u32(full);
+          mbar_wait(smem_u32(empty), (u & 1) ^ 1, status, kErrDkvProducer);
+          mbar_arrive_expect_tx(fb, kOperand);
+          for (int g = 0; g < 2; ++g)
+            for (int c = 0; c < kD / 64; ++c)
+              tma_load_4d(dst + c * kTileBytes + g * kHalfTile, tm, fb, 64 * c, un.pair * kPair + g * kBlk, un.hk, un.b);
+        };
+        auto load_rows = [&](uint32_t dst, const CUtensorMap* tm, uint64_t* full, uint64_t* empty, int h, int tile) {
+          mbar_wait(smem_u32(empty), ((it / kStages) & 1) ^ 1, status, kErrDkvProducer);
+          const int rows = un.len - off - tile * kQTile;            // rows of the tile that the sequence has
+          const bool ends = rows < kQTile && un.len < p.Lk;
+          const uint32_t fb = smem_u32(ends ? &sm->patch : full);
+          mbar_arrive_expect_tx(fb, kOperand);
+          for (int c = 0; c < kD / 64; ++c) tma_load_4d(dst + c * kTileBytes, tm, fb, 64 * c, tile * kQTile, h, un.b);
+          if (ends) {
+            mbar_wait(fb, patches++ & 1, status, kErrDkvProducer);
+            zero_rows(dst, kTileBytes, kD / 64, rows, kQTile);
+            mbar_arrive(smem_u32(full));
+          }
+        };
+        load_pair(k_pair, &tm_k, &sm->k_full, &sm->k_empty);
+        for (int i = 0; i < n_items; ++i, ++it) {
+          const int s = it % kStages, g = i / un.n_q, h = un.hk * p.G + g, tile = un.first + i - g * un.n_q;
+          load_rows(q_slot(s), &tm_q, &sm->q_full[s], &sm->q_empty[s], h, tile);
+          if (i == 0) load_pair(v_pair, &tm_v, &sm->v_full, &sm->v_empty);
+          load_rows(do_slot(s), &tm_do, &sm->do_full[s], &sm->do_empty[s], h, tile);
+        }
+        ++u;
+      }
+    }
+    __syncwarp();
+  } else if (warp == kBwdGroups * 4 + 1) {
+    // ------------------------------------------------------------------ S = Q K^T and dP = dO V^T of both blocks at once
+    constexpr uint32_t fmt = kBf16 ? 1u : 0u;
+    constexpr uint32_t idesc_s = instr_desc_f16(fmt, 128, 128, 0, 0);
+    const uint64_t dk0 = smem_desc_sw128(k_pair, 16, 1024), dv0 = smem_desc_sw128(v_pair, 16, 1024);
+    const uint64_t dq0 = smem_desc_sw128(q_slot(0), 16, 1024), ddo0 = smem_desc_sw128(do_slot(0), 16, 1024);
+    int it = 0, u = 0;
+    for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
+      const int n_items = warp_uniform(unit_of(w).n_q) * p.G;
+      if (n_items == 0) continue;
+      mbar_wait(smem_u32(&sm->k_full), u & 1, status, kErrDkvMma);
+      for (int i = 0; i < n_items; ++i, ++it) {
+        const int s = it % kStages;
+        const uint64_t dq = desc_advance(dq0, (uint32_t)s * 2 * kOperand), ddo = desc_advance(ddo0, (uint32_t)s * 2 * kOperand);
+        mbar_wait(smem_u32(&sm->q_full[s]), (it / kStages) & 1, status, kErrDkvMma);
+        if (it >= 1) mbar_wait(smem_u32(&sm->s_free), (it & 1) ^ 1, status, kErrDkvMma);
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < kD / 16; ++kk)
+            mma_f16_ss(tmem_s, desc_advance(dq, kmajor_step(kk, kTileBytes)), desc_advance(dk0, kmajor_step(kk, kTileBytes)), idesc_s, kk > 0);
+          mma_commit(smem_u32(&sm->s_full));
+          if (i == n_items - 1) mma_commit(smem_u32(&sm->k_empty));
+        }
+        if (i == 0) mbar_wait(smem_u32(&sm->v_full), u & 1, status, kErrDkvMma);
+        mbar_wait(smem_u32(&sm->do_full[s]), (it / kStages) & 1, status, kErrDkvMma);
+        if (it >= 1) mbar_wait(smem_u32(&sm->dp_free), (it & 1) ^ 1, status, kErrDkvMma);
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < kD / 16; ++kk)
+            mma_f16_ss(tmem_dp, desc_advance(ddo, kmajor_step(kk, kTileBytes)), desc_advance(dv0, kmajor_step(kk, kTileBytes)), idesc_s, kk > 0);
+          mma_commit(smem_u32(&sm->dp_full));
+          mma_commit(smem_u32(&sm->do_empty[s]));
+          if (i == n_items - 1) mma_commit(smem_u32(&sm->v_empty));
+        }
+      }
+      ++u;
+    }
+  } else if (warp == kBwdGroups * 4 + 2) {
+    // ------------------------------------------------------------------ dV += P^T dO and dK += dS^T Q
+    constexpr uint32_t fmt = kBf16 ? 1u : 0u;
+    constexpr uint32_t idesc_t = instr_desc_f16(fmt, 128, kD, 1, 1);
+    const uint64_t dq0t = smem_desc_sw128(q_slot(0), kTileBytes, 1024);
+    const uint64_t ddo0t = smem_desc_sw128(do_slot(0), kTileBytes, 1024);
+    const uint64_t dwt = smem_desc_sw128(w_tile, kTileBytes, 1024);
+    int it = 0, u = 0;
+    for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
+      const int n_items = warp_uniform(unit_of(w).n_q) * p.G;
+      if (n_items == 0) continue;
+      for (int i = 0; i < n_items; ++i, ++it) {
+        const int s = it % kStages;
+        const uint64_t ddot = desc_advance(ddo0t, (uint32_t)s * 2 * kOperand), dqt = desc_advance(dq0t, (uint32_t)s * 2 * kOperand);
+        mbar_wait(smem_u32(&sm->do_full[s]), (it / kStages) & 1, status, kErrDkvMma);
+        if (i == 0) mbar_wait(smem_u32(&sm->acc_empty[0]), (u & 1) ^ 1, status, kErrDkvMma);
+        mbar_wait(smem_u32(&sm->p_ready), it & 1, status, kErrDkvMma);
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < kQTile / 16; ++kk)
+            mma_f16_ss(tmem_dv, desc_advance(dwt, kk * 2048), desc_advance(ddot, kk * 2048), idesc_t, (i > 0 || kk > 0) ? 1u : 0u);
+          mma_commit(smem_u32(&sm->p_free));
+          mma_commit(smem_u32(&sm->do_empty[s]));
+          if (i == n_items - 1) mma_commit(smem_u32(&sm->acc_full[0]));
+        }
+        if (i == 0) mbar_wait(smem_u32(&sm->acc_empty[1]), (u & 1) ^ 1, status, kErrDkvMma);
+        mbar_wait(smem_u32(&sm->ds_ready), it & 1, status, kErrDkvMma);
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < kQTile / 16; ++kk)
+            mma_f16_ss(tmem_dk, desc_advance(dwt, kk * 2048), desc_advance(dqt, kk * 2048), idesc_t, (i > 0 || kk > 0) ? 1u : 0u);
+          mma_commit(smem_u32(&sm->ds_free));
+          mma_commit(smem_u32(&sm->q_empty[s]));
+          if (i == n_items - 1) mma_commit(smem_u32(&sm->acc_full[1]));
+        }
+      }
+      ++u;
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax: warpgroup g owns block g of the pair and drains dV (0) or dK (1)
+    const int g = warp >> 2;
+    const int row = tid & 127;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t my_tile = w_tile + (uint32_t)g * kTileBytes;
+    int it = 0, u = 0;
+    grid_dep_wait();                               // delta comes from the dQ kernel, which may still be running (see the launch)
+    for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
+      const DkvUnit un = unit_of(w);
+      const int n_items = un.n_q * p.G, bk = un.b * p.Hkv + un.hk, key0 = un.pair * kPair + g * kBlk;
+      const bool split = un.pair < p.split.tiles;
+      float* const part = split ? p.split.part + (((int64_t)bk * p.split.tiles + un.pair) * (1 + p.split.runs) + 1 + un.run) * 2 * kPair * p.D : nullptr;
+      const int out_key = un.pair * kPair + row;   // TMEM lane = key of the pair
+      if (n_items == 0) {                          // keys that nobody sees
+        if (un.base() && out_key < p.Lk) {
+          if (split) {
+            float4* to = reinterpret_cast<float4*>(part + ((g == 0 ? kPair : 0) + row) * p.D);
+            for (int e = 0; e < p.D / 4; ++e) to[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+          } else {
+            uint32_t* to = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(g == 0 ? p.dv : p.dk) + ((int64_t)bk * p.Lk + out_key) * p.D);
+            for (int e = 0; e < p.D / 2; ++e) to[e] = 0u;
+          }
+        }
+        __syncwarp();
+        continue;
+      }
+      float n_lse = 0.f, n_delta = 0.f;
+      auto fetch = [&](int i) {                    // one item ahead, so that the latency is never exposed
+        const int head = un.hk * p.G + i / un.n_q, rr = min((un.first + i % un.n_q) * kQTile + row, p.Lq - 1);
+        const int64_t at = ((int64_t)un.b * p.H + head) * p.Lq + rr;
+        n_lse = ld_behind_wait(p.lse + at);
+        n_delta = ld_behind_wait(p.delta + at);
+      };
+      fetch(0);
+      for (int i = 0, tq = un.first; i < n_items; ++i, ++it) {
+        const int pos = off + tq * kQTile + row;
+        const int warp_p0 = warp_uniform(off + tq * kQTile + (warp & 3) * 32), warp_p1 = warp_p0 + 31;
+        const bool row_valid = tq * kQTile + row < p.Lq && pos < un.len;
+        const float lse = n_lse, delta = n_delta;
+        if (i + 1 < n_items) fetch(i + 1);
+        // a warp with a row that is none masks (its position becomes -1: it sees nothing)
+        const bool all_rows = warp_p1 < un.len && (tq * kQTile + (warp & 3) * 32 + 31) < p.Lq;
+        const Columns col(row_valid ? pos : -1, key0, p.window, p.sinks);
+        const int kind = warp_uniform(tile_empty(warp_p0, warp_p1, key0, p.window, p.sinks) ? 0
+                                      : all_rows && tile_full(warp_p0, warp_p1, key0, p.window, p.sinks) ? 2 : 1);
+        if (++tq == un.first + un.n_q) tq = un.first;
+        mbar_wait(smem_u32(&sm->s_full), it & 1, status, kErrDkvSoftmax);
+        tc_fence_after();
+        uint64_t sp[32];
+        bwd_weights(sp, tmem_s + (uint32_t)g * 64u + lane_base, kind, col, p.scale_log2, lse, [&]() {
+          tc_fence_before();
+          mbar_arrive(smem_u32(&sm->s_free));
+        });
+        uint32_t wd[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) wd[j] = pack2p<kBf16>(sp[j]);
+        if (it >= 1) mbar_wait(smem_u32(&sm->ds_free), (it & 1) ^ 1, status, kErrDkvSoftmax);
+        store_row_sw128(my_tile, row, wd);
+        fence_proxy_async_smem();
+        mbar_arrive(smem_u32(&sm->p_ready));
+        mbar_wait(smem_u32(&sm->dp_full), it & 1, status, kErrDkvSoftmax);
+        tc_fence_after();
+        bwd_dscores<kBf16>(wd, sp, tmem_dp + (uint32_t)g * 64u + lane_base, smem_u32(&sm->dp_free), kind, col, p.scale, delta);
+        mbar_wait(smem_u32(&sm->p_free), it & 1, status, kErrDkvSoftmax);
+        store_row_sw128(my_tile, row, wd);
+        fence_proxy_async_smem();
+        mbar_arrive(smem_u32(&sm->ds_ready));
+      }
+      // epilogue: dV by warpgroup 0, dK by warpgroup 1
+      const int64_t off_r = out_key < p.Lk ? ((int64_t)bk * p.Lk + out_key) * p.D : -1;
+      int64_t row_off[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) row_off[j] = __shfl_sync(0xffffffffu, off_r, (lane & ~3) + j);
+      mbar_wait(smem_u32(&sm->acc_full[g]), u & 1, status, kErrDkvEpilogue);
+      tc_fence_after();
+      const uint32_t t_acc = (g == 0 ? tmem_dv : tmem_dk) + lane_base;
+      void* const out = g == 0 ? p.dv : p.dk;
+      float* const prow = split ? part + ((g == 0 ? kPair : 0) + row) * p.D : nullptr;
+#pragma unroll
+      for (int c = 0; c < kD / 32; ++c) {
+        uint32_t ra[32];
+        tmem_ld_32x32b_x32(t_acc + c * 32, ra);
+        tmem_ld_wait();
+        if (c == kD / 32 - 1) {
+          tc_fence_before();
+          mbar_arrive(smem_u32(&sm->acc_empty[g]));     // the next unit may start accumulating
+        }
+        if (split) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (c * 32 + e * 4 < p.D)
+              *reinterpret_cast<uint4*>(prow + c * 32 + e * 4) = make_uint4(ra[4 * e], ra[4 * e + 1], ra[4 * e + 2], ra[4 * e + 3]);
+        } else {
+          store_acc_cols<kBf16>(out, row_off, ra, c * 32, p.D, lane);
+        }
+      }
+      ++u;
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == kBwdGroups * 4 + 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- backward: dQ
+constexpr int kDqStages = 4;
+constexpr int kSdpBufs = 2;                         // S / dP buffers in TMEM
+constexpr int kDqThreads = kBwdThreads + 32;        // S and dP are issued by warps of their own
+
+struct DqSmem {
+  uint64_t qdo_full, patch;
+  uint64_t ops_ready;       // the unit's Q and dO rows sit in TMEM (written by the softmax warpgroups)
+  uint64_t ops_free;        // the S / dP products of the unit have read them
+  uint64_t delta_read;      // both softmax warpgroups are done with the Q, dO and O tiles in shared memory
+  uint64_t full[kDqStages], empty[kDqStages], ds_ready[kDqStages];
+  uint64_t s_full[kSdpBufs], s_free[kSdpBufs], dp_full[kSdpBufs], dp_free[kSdpBufs];
+  uint64_t acc_full[2];     // per draining warpgroup (the one that took the unit's last item)
+  uint64_t acc_empty;
+  uint32_t tmem_base;
+};
+struct DqArgs {
+  const float* lse;
+  float* delta;
+  void* dq;
+  const int* lengths;
+  int H, Hkv, G, BH, Lq, Lk, D, window, sinks;
+  float scale, scale_log2;
+};
+struct DqUnit {
+  int t, bh, b, h, len, total, n_win;
+  KeyTiles k;
+  __device__ int tile_of(int i) const { return i < n_win ? k.last - i : k.sink_tiles - 1 - (i - n_win); }
+};
+
+template <bool kBf16, int kD>
+__global__ void __launch_bounds__(kDqThreads, 1)
+window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
+                       const __grid_constant__ CUtensorMap tm_o, const DqArgs p, int* status) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  const uint32_t q_tile = base, do_tile = base + 32768u;
+  auto k_slot = [&](int s) { return base + 65536u + (uint32_t)s * 32768u; };
+  auto v_slot = [&](int s) { return base + 65536u + (uint32_t)s * 32768u + 16384u; };   // V tile, later dS
+  const uint32_t o_tile = base + 65536u + kDqStages * 32768u;                           // forward output tile, only for delta
+  DqSmem* sm = reinterpret_cast<DqSmem*>(smem_raw + (base - raw) + 65536u + kDqStages * 32768u + 32768u);
+
+  const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
+  const int n_tiles = (p.Lq + kQTile - 1) / kQTile, off = p.Lk - p.Lq, n_units = n_tiles * p.BH;
+  auto unit_at = [&](int r) { return r * (int)gridDim.x + ((r & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x); };
+  auto unit_of = [&](int w) {
+    DqUnit u;
+    u.t = n_tiles - 1 - w / p.BH;
+    u.bh = w % p.BH;
+    u.b = u.bh / p.H;
+    u.h = u.bh - u.b * p.H;
+    u.len = length_of(p.lengths, u.b, p.Lk);
+    u.k = keys_of_queries(u.t, kQTile, kBlk, p.Lq, off, u.len, p.window, p.sinks);
+    u.n_win = u.k.last - u.k.first + 1;
+    u.total = u.n_win + u.k.sink_tiles;
+    return u;
+  };
+
+  if (tid == 0) {
+    for (uint64_t* bar : {&sm->qdo_full, &sm->patch}) mbar_init(smem_u32(bar), 1);
+    mbar_init(smem_u32(&sm->ops_ready), 256);
+    mbar_init(smem_u32(&sm->ops_free), 2);          // the S issuer and the dP issuer
+    mbar_init(smem_u32(&sm->delta_read), 256);
+    for (int s = 0; s < kDqStages; ++s) {
+      mbar_init(smem_u32(&sm->full[s]), 1);
+      mbar_init(smem_u32(&sm->empty[s]), 1);
+      mbar_init(smem_u32(&sm->ds_ready[s]), 128);
+    }
+    for (int s = 0; s < kSdpBufs; ++s) {
+      mbar_init(smem_u32(&sm->s_full[s]), 1);
+      mbar_init(smem_u32(&sm->s_free[s]), 128);
+      mbar_init(smem_u32(&sm->dp_full[s]), 1);
+      mbar_init(smem_u32(&sm->dp_free[s]), 128);
+    }
+    mbar_init(smem_u32(&sm->acc_full[0]), 1);
+    mbar_init(smem_u32(&sm->acc_full[1]), 1);
+    mbar_init(smem_u32(&sm->acc_empty), 128);
+    mbar_init_fence();
+  }
+  if (warp == kBwdGroups * 4 + 1) tmem_alloc(smem_u32(&sm->tmem_base), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = (uint32_t)warp_uniform((int)sm->tmem_base);
+  // TMEM: S buffers [0,128), dP buffers [128,256), dQ [256,384), Q rows [384,448), dO rows [448,512)
+  const uint32_t tmem_s = tmem, tmem_dp = tmem + 128, tmem_dq = tmem + 256, tmem_q = tmem + 384, tmem_do = tmem + 448;
+  grid_dep_wait();
+  grid_dep_launch();
+
+  if (warp == kBwdGroups * 4) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int it = 0, u = 0, patches = 0;
+      for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
+        const DqUnit un = unit_of(w);
+        if (un.total == 0) continue;
+        const int hk = un.h / p.G;
+        const uint32_t qb = smem_u32(&sm->qdo_full);
+        mbar_wait(smem_u32(&sm->delta_read), (u & 1) ^ 1, status, kErrDqProducer);
+        mbar_arrive_expect_tx(qb, 3 * (kD / 64) * kTileBytes);
+        for (int c = 0; c < kD / 64; ++c) {
+          tma_load_4d(o_tile + c * kTileBytes, &tm_o, qb, 64 * c, un.t * kQTile, un.h, un.b);
+          tma_load_4d(q_tile + c * kTileBytes, &tm_q, qb, 64 * c, un.t * kQTile, un.h, un.b);
+          tma_load_4d(do_tile + c * kTileBytes, &tm_do, qb, 64 * c, un.t * kQTile, un.h, un.b);
+        }
+        for (int i = 0; i < un.total; ++i, ++it) {
+          const int s = it % kDqStages, key0 = un.tile_of(i) * kBlk;
+          mbar_wait(smem_u32(&sm->empty[s]), ((it / kDqStages) & 1) ^ 1, status, kErrDqProducer);
+          const bool ends = key0 + kBlk > un.len && un.len < p.Lk;
+          const uint32_t fb = smem_u32(ends ? &sm->patch : &sm->full[s]);
+          mbar_arrive_expect_tx(fb, 2 * (kD / 64) * kHalfTile);
+          for (int c = 0; c < kD / 64; ++c) {
+            tma_load_4d(k_slot(s) + c * kHalfTile, &tm_k, fb, 64 * c, key0, hk, un.b);
+            tma_load_4d(v_slot(s) + c * kHalfTile, &tm_v, fb, 64 * c, key0, hk, un.b);
+          }
+          if (ends) {                              // dS is 0 there, and dQ += dS K
+            mbar_wait(fb, patches++ & 1, status, kErrDqProducer);
+            zero_rows(k_slot(s), kHalfTile, kD / 64, un.len - key0, kBlk);
+            mbar_arrive(smem_u32(&sm->full[s]));
+          }
+        }
+        ++u;
+      }
+    }
+    __syncwarp();
+  } else if (warp == kBwdGroups * 4 + 1 || warp == kBwdGroups * 4 + 3) {
+    // ------------------------------------------------------------------ S = Q K^T (warp +1), dP = dO V^T (warp +3)
+    constexpr uint32_t fmt = kBf16 ? 1u : 0u;
+    constexpr uint32_t idesc_s = instr_desc_f16(fmt, 128, 64, 0, 0);
+    const bool is_s = warp == kBwdGroups * 4 + 1;
+    const uint64_t db0 = smem_desc_sw128(is_s ? k_slot(0) : v_slot(0), 16, 1024);
+    const uint32_t t_out = is_s ? tmem_s : tmem_dp, t_a = is_s ? tmem_q : tmem_do;
+    int it = 0, u = 0;
+    for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
+      const int total = warp_uniform(unit_of(w).total);
+      if (total == 0) continue;
+      for (int i = 0; i < total; ++i, ++it) {
+        const int s = it % kDqStages, sb = it % kSdpBufs;
+        mbar_wait(smem_u32(&sm->full[s]), (it / kDqStages) & 1, status, kErrDqMma);
+        if (it >= kSdpBufs) mbar_wait(smem_u32(is_s ? &sm->s_free[sb] : &sm->dp_free[sb]), ((it / kSdpBufs) & 1) ^ 1, status, kErrDqMma);
+        if (i == 0) mbar_wait(smem_u32(&sm->ops_ready), u & 1, status, kErrDqMma);
+        tc_fence_after();
+        const uint64_t db = desc_advance(db0, (uint32_t)s * 32768u);
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < kD / 16; ++kk)      // A from TMEM: 8 columns = 16 features per K-step
+            mma_f16_ts(t_out + sb * 64, t_a + kk * 8, desc_advance(db, kmajor_step(kk, kHalfTile)), idesc_s, kk > 0);
+          mma_commit(smem_u32(is_s ? &sm->s_full[sb] : &sm->dp_full[sb]));
+        }
+      }
+      if (elect_one()) mma_commit(smem_u32(&sm->ops_free));        // the next unit's Q / dO rows may be written
+      ++u;
+    }
+    __syncwarp();
+  } else if (warp == kBwdGroups * 4 + 2) {
+    // ------------------------------------------------------------------ dQ += dS K
+    constexpr uint32_t fmt = kBf16 ? 1u : 0u;
+    constexpr uint32_t idesc_q = instr_desc_f16(fmt, 128, kD, 0, 1);
+    const uint64_t dv0 = smem_desc_sw128(v_slot(0), 16, 1024);
+    const uint64_t dk0t = smem_desc_sw128(k_slot(0), kHalfTile, 1024);
+    int it = 0, u = 0;
+    for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
+      const int total = warp_uniform(unit_of(w).total);
+      if (total == 0) continue;
+      for (int i = 0; i < total; ++i, ++it) {
+        const int s = it % kDqStages;
+        if (i == 0) mbar_wait(smem_u32(&sm->acc_empty), (u & 1) ^ 1, status, kErrDqMma);
+        mbar_wait(smem_u32(&sm->ds_ready[s]), (it / kDqStages) & 1, status, kErrDqMma);
+        tc_fence_after();
+        const uint64_t dds = desc_advance(dv0, (uint32_t)s * 32768u), dkt = desc_advance(dk0t, (uint32_t)s * 32768u);
+        if (elect_one()) {
+#pragma unroll
+          for (int kk = 0; kk < kBlk / 16; ++kk)
+            mma_f16_ss(tmem_dq, desc_advance(dds, kk * 32), desc_advance(dkt, kk * 2048), idesc_q, (i > 0 || kk > 0) ? 1u : 0u);
+          mma_commit(smem_u32(&sm->empty[s]));
+        }
+      }
+      if (elect_one()) mma_commit(smem_u32(&sm->acc_full[(it - 1) & 1]));     // drained by the warpgroup that took the last item
+      ++u;
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ softmax: warpgroup g takes the items with (running count) % 2 == g
+    const int g = warp >> 2;
+    const int row = tid & 127;
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    int it0 = 0, u = 0, drains = 0;
+    // dQ of a unit is drained by the warpgroup that took its last item, but only behind the prologue of the next unit: its last product
+    // queues behind that unit's first S / dP products
+    int64_t drain_row = -1;
+    bool drain_stored = false, drain_valid = false;
+    auto drain = [&]() {
+      mbar_wait(smem_u32(&sm->acc_full[g]), drains & 1, status, kErrDqEpilogue);
+      ++drains;
+      tc_fence_after();
+      uint4* orow = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.dq) + drain_row * p.D);
+#pragma unroll
+      for (int c = 0; c < kD / 32; ++c) {
+        uint32_t r[32];
+        tmem_ld_32x32b_x32(tmem_dq + c * 32 + lane_base, r);
+        tmem_ld_wait();
+        if (c == kD / 32 - 1) {
+          tc_fence_before();
+          mbar_arrive(smem_u32(&sm->acc_empty));     // the next unit may start accumulating
+        }
+#pragma unroll
+        for (int v4 = 0; v4 < 4; ++v4) {
+          uint4 pk;
+          pk.x = pack2<kBf16>(__uint_as_float(r[8 * v4 + 0]), __uint_as_float(r[8 * v4 + 1]));
+          pk.y = pack2<kBf16>(__uint_as_float(r[8 * v4 + 2]), __uint_as_float(r[8 * v4 + 3]));
+          pk.z = pack2<kBf16>(__uint_as_float(r[8 * v4 + 4]), __uint_as_float(r[8 * v4 + 5]));
+          pk.w = pack2<kBf16>(__uint_as_float(r[8 * v4 + 6]), __uint_as_float(r[8 * v4 + 7]));
+          if (!drain_valid) pk = make_uint4(0u, 0u, 0u, 0u);
+          if (drain_stored && c * 32 + v4 * 8 < p.D) orow[c * 4 + v4] = pk;
+        }
+      }
+      drain_row = -1;
+    };
+    // row statistics of the next unit are asked for while the current one runs
+    float n_lse = 0.f;
+    auto fetch_rows = [&](int w) {
+      if (w >= n_units) return;
+      const int rr = min((n_tiles - 1 - w / p.BH) * kQTile + row, p.Lq - 1);
+      n_lse = ld_behind_wait(p.lse + (int64_t)(w % p.BH) * p.Lq + rr);
+    };
+    fetch_rows(unit_at(0));
+    for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
+      const DqUnit un = unit_of(w);
+      const int64_t grow = (int64_t)un.bh * p.Lq + un.t * kQTile + row;
+      const int pos = off + un.t * kQTile + row;
+      const bool stored = un.t * kQTile + row < p.Lq, valid = stored && pos < un.len;
+      const float lse = n_lse;
+      fetch_rows(unit_at(r + 1));
+      if (un.total == 0) {                         // nothing but padding
+        if (g == 0 && stored) {
+          uint4* orow = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.dq) + grow * p.D);
+          for (int e = 0; e < p.D / 8; ++e) orow[e] = make_uint4(0u, 0u, 0u, 0u);
+          p.delta[grow] = 0.f;
+        }
+        __syncwarp();
+        continue;
+      }
+      const int warp_p0 = warp_uniform(off + un.t * kQTile + (warp & 3) * 32), warp_p1 = warp_p0 + 31;
+      // delta = rowsum(O * dO), straight from the swizzled tiles; warpgroup 0 also publishes it for the dK/dV kernel
+      mbar_wait(smem_u32(&sm->qdo_full), u & 1, status, kErrDqSoftmax);
+      float delta = 0.f;
+      uint32_t opw[kD / 64][32];      // this thread's row of the operand its warpgroup moves to TMEM (0: Q, 1: dO)
+#pragma unroll
+      for (int sub = 0; sub < kD / 64; ++sub)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const uint32_t at = (uint32_t)sub * kTileBytes + (uint32_t)row * 128u + (uint32_t)((c ^ (row & 7)) << 4);
+          uint32_t ov[4], gv[4];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(ov[0]), "=r"(ov[1]), "=r"(ov[2]), "=r"(ov[3]) : "r"(o_tile + at));
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(gv[0]), "=r"(gv[1]), "=r"(gv[2]), "=r"(gv[3]) : "r"(do_tile + at));
+          if (g == 1) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) opw[sub][4 * c + e] = gv[e];
+          } else {
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(opw[sub][4 * c]), "=r"(opw[sub][4 * c + 1]), "=r"(opw[sub][4 * c + 2]), "=r"(opw[sub][4 * c + 3])
+                         : "r"(q_tile + at));
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float2 fo, fg;
+            if (kBf16) {
+              fo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&ov[e]));
+              fg = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&gv[e]));
+            } else {
+              fo = __half22float2(*reinterpret_cast<const __half2*>(&ov[e]));
+              fg = __half22float2(*reinterpret_cast<const __half2*>(&gv[e]));
+            }
+            delta = fmaf(fo.x, fg.x, delta);
+            delta = fmaf(fo.y, fg.y, delta);
+          }
+        }
+      // TMA writes the next unit's rows through another proxy than these loads went through
+      fence_proxy_async_smem();
+      mbar_arrive(smem_u32(&sm->delta_read));
+      // row -> TMEM lane, 32-bit word j (two features) -> column j: the layout of a K-major A operand
+      mbar_wait(smem_u32(&sm->ops_free), (u & 1) ^ 1, status, kErrDqSoftmax);
+      tc_fence_after();
+      {
+        const uint32_t dst = (g == 0 ? tmem_q : tmem_do) + lane_base;
+        tmem_st_32x32b_x32(dst, opw[0]);
+        if constexpr (kD == 128) tmem_st_32x32b_x32(dst + 32, opw[1]);
+        tmem_st_wait();
+      }
+      tc_fence_before();
+      mbar_arrive(smem_u32(&sm->ops_ready));
+      if (g == 0 && stored) p.delta[grow] = valid ? delta : 0.f;
+      if (warp_uniform(drain_row >= 0)) drain();
+      for (int i = (it0 + g) & 1; i < un.total; i += kBwdGroups) {
+        const int it = it0 + i, s = it % kDqStages, sb = it % kSdpBufs, key0 = un.tile_of(i) * kBlk;
+        const Columns col(pos, key0, p.window, p.sinks);
+        // a row of padding spoils its own row of dQ alone, which is not stored
+        const int kind = warp_uniform(tile_empty(warp_p0, warp_p1, key0, p.window, p.sinks) ? 0
+                                      : tile_full(warp_p0, warp_p1, key0, p.window, p.sinks) ? 2 : 1);
+        mbar_wait(smem_u32(&sm->s_full[sb]), (it / kSdpBufs) & 1, status, kErrDqSoftmax);
+        tc_fence_after();
+        uint64_t sp[32];
+        bwd_weights(sp, tmem_s + sb * 64 + lane_base, kind, col, p.scale_log2, lse, [&]() {
+          tc_fence_before();
+          mbar_arrive(smem_u32(&sm->s_free[sb]));
+        });
+        mbar_wait(smem_u32(&sm->dp_full[sb]), (it / kSdpBufs) & 1, status, kErrDqSoftmax);
+        tc_fence_after();
+        uint32_t wd[32];
+        bwd_dscores<kBf16>(wd, sp, tmem_dp + sb * 64 + lane_base, smem_u32(&sm->dp_free[sb]), kind, col, p.scale, delta);
+        store_row_sw128(v_slot(s), row, wd);      // dS replaces the V tile of this stage, which dP has finished reading
+        fence_proxy_async_smem();
+        mbar_arrive(smem_u32(&sm->ds_ready[s]));
+      }
+      it0 += un.total;
+      if (g == ((it0 - 1) & 1)) {
+        drain_row = grow;
+        drain_stored = stored;
+        drain_valid = valid;
+      }
+      ++u;
+    }
+    if (warp_uniform(drain_row >= 0)) drain();
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == kBwdGroups * 4 + 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- host side
+template <int kTiles> constexpr size_t kSmemFwd = 1024 + (kTiles + kFwdStages<kTiles>) * 32768 + sizeof(FwdSmem<kFwdStages<kTiles>>);
+template <int kD> constexpr size_t kSmemDkv =
+    1024 + (2 + 2 * kDkvStages<kD>) * (kD / 64) * kTileBytes + 2 * kTileBytes + sizeof(DkvSmem<kDkvStages<kD>>);
+constexpr size_t kSmemDq = 1024 + 65536 + kDqStages * 32768 + 32768 + sizeof(DqSmem);
+static_assert(kSmemFwd<2> <= 232448 && kSmemFwd<1> <= 232448 / 2 - 1024 && kSmemDkv<128> <= 232448 && kSmemDkv<64> <= 232448 && kSmemDq <= 232448,
+              "shared memory of one SM");
+
+struct Facts {
+  bool ready = false;
+  int n_sm = 0;
+  int* status = nullptr;
+};
+// SM count, status word and the opt-in to large shared memory, once per device
+int facts_of(const Facts** out) {
+  static std::mutex mu;
+  static Facts facts[64];
+  int dev = 0, rc;
+  LMK_CUDA(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return fail(LMK_ERR_UNSUPPORTED, "device index %d out of range", dev);
+  std::lock_guard<std::mutex> lock(mu);
+  Facts& f = facts[dev];
+  if (!f.ready) {
+    if ((rc = sm_count(&f.n_sm)) != LMK_OK) return rc;
+    f.status = device_status_word();
+    if (f.status == nullptr) return fail(LMK_ERR_CUDA, "no device status word");
+    const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
+#define LMK_ATTRS(BF, DIM)                                                                         \
+    LMK_CUDA(cudaFuncSetAttribute(window_fwd_sm100_kernel<BF, DIM, 1>, attr, (int)kSmemFwd<1>));   \
+    LMK_CUDA(cudaFuncSetAttribute(window_fwd_sm100_kernel<BF, DIM, 2>, attr, (int)kSmemFwd<2>));   \
+    LMK_CUDA(cudaFuncSetAttribute(window_dq_sm100_kernel<BF, DIM>, attr, (int)kSmemDq));           \
+    LMK_CUDA(cudaFuncSetAttribute(window_dkv_sm100_kernel<BF, DIM>, attr, (int)kSmemDkv<DIM>));
+    LMK_ATTRS(true, 128) LMK_ATTRS(true, 64) LMK_ATTRS(false, 128) LMK_ATTRS(false, 64)
+#undef LMK_ATTRS
+    f.ready = true;
+  }
+  *out = &f;
+  return LMK_OK;
+}
+
+int maps(const WindowParams& p, int dtype, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v) {
+  int rc = tensor_map_4d_now(q, p.q, dtype, p.B, p.H, p.Lq, p.D, p.qs, kQTile);
+  if (rc == LMK_OK) rc = tensor_map_4d_now(k, p.k, dtype, p.B, p.Hkv, p.Lk, p.D, p.ks, kBlk);
+  if (rc == LMK_OK) rc = tensor_map_4d_now(v, p.v, dtype, p.B, p.Hkv, p.Lk, p.D, p.vs, kBlk);
+  return rc;
+}
+
+}  // namespace
+
+bool window_sm100_operand_ok(const void* p, const int64_t st[3], int D) {
+  return ((uintptr_t)p & 15) == 0 && st[0] > 0 && st[1] > 0 && st[0] % 8 == 0 && st[1] % 8 == 0 && st[2] % 8 == 0 && st[2] >= D;
+}
+
+int window_sm100_fwd(const WindowParams& p, int dtype, cudaStream_t st) {
+  const Facts* f;
+  CUtensorMap tq, tk, tv;
+  int rc = facts_of(&f);
+  if (rc != LMK_OK || (rc = maps(p, dtype, &tq, &tk, &tv)) != LMK_OK) return rc;
+  WindowTensors a = {p.o, p.lse, p.lengths, p.H, p.H / p.Hkv, p.Lq, p.Lk, p.D, p.window, p.sinks, p.scale, p.scale * kLog2e};
+  const int n_tiles = (p.Lq + kQTile - 1) / kQTile;
+  const int per_cta = n_tiles == 1 ? 2 : 1;
+  const dim3 grid(p.B * p.H, (n_tiles + per_cta - 1) / per_cta);
+#define LMK_FWD(BF, DIM)                                                                                                                \
+  do {                                                                                                                                  \
+    if (per_cta == 1)                                                                                                                   \
+      LMK_CUDA(launch_overlapped(window_fwd_sm100_kernel<BF, DIM, 1>, grid, dim3(kFwdThreads<1>), kSmemFwd<1>, st, tq, tk, tv, a, f->status)); \
+    else                                                                                                                                \
+      LMK_CUDA(launch_overlapped(window_fwd_sm100_kernel<BF, DIM, 2>, grid, dim3(kFwdThreads<2>), kSmemFwd<2>, st, tq, tk, tv, a, f->status)); \
+  } while (0)
+  if (dtype == LMK_BF16) {
+    if (p.D <= 64) LMK_FWD(true, 64); else LMK_FWD(true, 128);
+  } else {
+    if (p.D <= 64) LMK_FWD(false, 64); else LMK_FWD(false, 128);
+  }
+#undef LMK_FWD
+  return LMK_OK;
+}
+
+int window_sm100_bwd(const WindowParams& p, int dtype, cudaStream_t st) {
+  const Facts* f;
+  CUtensorMap tq, tk, tv, tdo, to;
+  const int64_t dense[3] = {(int64_t)p.H * p.Lq * p.D, (int64_t)p.Lq * p.D, (int64_t)p.D};
+  int rc = facts_of(&f);
+  if (rc != LMK_OK || (rc = maps(p, dtype, &tq, &tk, &tv)) != LMK_OK) return rc;
+  if ((rc = tensor_map_4d_now(&tdo, p.dO, dtype, p.B, p.H, p.Lq, p.D, p.dos, kQTile)) != LMK_OK) return rc;
+  if ((rc = tensor_map_4d_now(&to, p.o, dtype, p.B, p.H, p.Lq, p.D, dense, kQTile)) != LMK_OK) return rc;
+  int n_sm = f->n_sm;
+  const int cap = attn_sm100_max_ctas();
+  if (cap >= 1 && cap < n_sm) n_sm = cap;
+  const int n_pairs = (p.Lk + kPair - 1) / kPair, G = p.H / p.Hkv;
+  const int64_t dq_units = (int64_t)((p.Lq + kQTile - 1) / kQTile) * p.B * p.H;
+  const int64_t dkv_units = ((int64_t)n_pairs + (int64_t)p.split.tiles * p.split.runs) * p.B * p.Hkv;
+  const DqArgs aq = {p.lse, p.delta, p.dq, p.lengths, p.H, p.Hkv, G, p.B * p.H, p.Lq, p.Lk, p.D, p.window, p.sinks, p.scale, p.scale * kLog2e};
+  const DkvArgs ak = {p.lse, p.delta, p.dk, p.dv, p.lengths, p.H, p.Hkv, G, p.B, p.Lq, p.Lk, p.D, p.window, p.sinks, n_pairs, p.scale, p.scale * kLog2e,
+                      p.split};
+  const dim3 grid_q((unsigned)(dq_units < n_sm ? dq_units : n_sm)), grid_k((unsigned)(dkv_units < n_sm ? dkv_units : n_sm));
+  // The dK/dV kernel may start on every SM that the dQ kernel has left: it reads q, k, v, dO, lse and lengths, which were complete before
+  // any CTA of the dQ kernel was behind its wait, and delta, for which its softmax threads wait.
+#define LMK_BWD(BF, DIM)                                                                                                                    \
+  do {                                                                                                                                      \
+    LMK_CUDA(launch_overlapped(window_dq_sm100_kernel<BF, DIM>, grid_q, dim3(kDqThreads), kSmemDq, st, tq, tk, tv, tdo, to, aq, f->status)); \
+    LMK_CUDA(launch_overlapped(window_dkv_sm100_kernel<BF, DIM>, grid_k, dim3(kBwdThreads), kSmemDkv<DIM>, st, tq, tk, tv, tdo, ak, f->status)); \
+  } while (0)
+  if (dtype == LMK_BF16) {
+    if (p.D <= 64) LMK_BWD(true, 64); else LMK_BWD(true, 128);
+  } else {
+    if (p.D <= 64) LMK_BWD(false, 64); else LMK_BWD(false, 128);
+  }
+#undef LMK_BWD
+  return p.split.tiles > 0 ? window_join_parts(p, kQTile, kPair, dtype, st) : LMK_OK;
+}
+
+}  // namespace lmk
