@@ -8,7 +8,8 @@
 //   than 2^8: O then has to be read, scaled and written back (TMEM), which with the first tile's maximum as m happens to a few rows of
 //   a long sequence.  p <= 2^8 costs no precision: p, l and O are floating point, and O / l does not depend on m.
 // Backward: recomputed from lse = m + log2 l, in two launches.
-//   dQ: unit = (query tile, head), persistent.  Q and dO rows go to TMEM as A operands; per key tile S, dP -> dS over the V tile -> dQ += dS K.
+//   dQ: unit = (query tile, head), persistent.  Q and dO rows go to TMEM as A operands; per key tile S, dP -> dS in 16 bits over
+//   the TMEM columns of dP -> dQ += dS K with A = dS from TMEM.
 //   dK/dV: unit = (pair of key tiles, key head, run of query tiles), persistent; Q and dO tiles of all heads that share the keys
 //   stream through.  P^T dO and dS^T Q take P and dS from shared memory as MN-major operands.  The accumulators are the sums over the
 //   group's heads.  The query tiles of a pair with sinks are dealt out to several units (SinkSplit): one unit would be as long as the
@@ -425,13 +426,12 @@ __device__ __forceinline__ void bwd_weights(uint64_t (&sp)[32], uint32_t ts, int
   }
 }
 
-// Reads dP from TMEM, arrives on free_bar, and leaves the row of dS = p (dP - delta) scale, packed to 16 bits, in wd.
-template <bool kBf16>
-__device__ __forceinline__ void bwd_dscores(uint32_t (&wd)[32], const uint64_t (&sp)[32], uint32_t tdp, uint32_t free_bar, int kind,
-                                            const Columns& col, float scale, float delta) {
+// Reads dP from TMEM and leaves the row of dS = p (dP - delta) scale, packed to 16 bits, in wd.
+template <bool kBf16, typename AfterFn>
+__device__ __forceinline__ void bwd_dscores(uint32_t (&wd)[32], const uint64_t (&sp)[32], uint32_t tdp, int kind, const Columns& col, float scale,
+                                            float delta, AfterFn after_dp) {
   if (kind == 0) {
-    tc_fence_before();
-    mbar_arrive(free_bar);
+    after_dp();
 #pragma unroll
     for (int j = 0; j < 32; ++j) wd[j] = 0u;
     return;
@@ -448,8 +448,7 @@ __device__ __forceinline__ void bwd_dscores(uint32_t (&wd)[32], const uint64_t (
       dp[16 + j] = pk2u(rb[2 * j], rb[2 * j + 1]);
     }
   }
-  tc_fence_before();
-  mbar_arrive(free_bar);
+  after_dp();
   const uint64_t sc2 = pk2(scale, scale);
   const float ns = -delta * scale;
   const uint64_t ns2 = pk2(ns, ns);
@@ -749,7 +748,10 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         mbar_arrive(smem_u32(&sm->p_ready));
         mbar_wait(smem_u32(&sm->dp_full), it & 1, status, kErrDkvSoftmax);
         tc_fence_after();
-        bwd_dscores<kBf16>(wd, sp, tmem_dp + (uint32_t)g * 64u + lane_base, smem_u32(&sm->dp_free), kind, col, p.scale, delta);
+        bwd_dscores<kBf16>(wd, sp, tmem_dp + (uint32_t)g * 64u + lane_base, kind, col, p.scale, delta, [&]() {
+          tc_fence_before();
+          mbar_arrive(smem_u32(&sm->dp_free));
+        });
         mbar_wait(smem_u32(&sm->p_free), it & 1, status, kErrDkvSoftmax);
         store_row_sw128(my_tile, row, wd);
         fence_proxy_async_smem();
@@ -804,8 +806,9 @@ struct DqSmem {
   uint64_t ops_ready;       // the unit's Q and dO rows sit in TMEM (written by the softmax warpgroups)
   uint64_t ops_free;        // the S / dP products of the unit have read them
   uint64_t delta_read;      // both softmax warpgroups are done with the Q, dO and O tiles in shared memory
-  uint64_t full[kDqStages], empty[kDqStages], ds_ready[kDqStages];
-  uint64_t s_full[kSdpBufs], s_free[kSdpBufs], dp_full[kSdpBufs], dp_free[kSdpBufs];
+  uint64_t full[kDqStages], empty[kDqStages];
+  uint64_t s_full[kSdpBufs], s_free[kSdpBufs], dp_full[kSdpBufs];
+  uint64_t ds_ready[kSdpBufs], dp_free[kSdpBufs];      // dS has taken dP's place / dQ has read it
   uint64_t acc_full[2];     // per draining warpgroup (the one that took the unit's last item)
   uint64_t acc_empty;
   uint32_t tmem_base;
@@ -834,7 +837,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   const uint32_t base = (raw + 1023u) & ~1023u;
   const uint32_t q_tile = base, do_tile = base + 32768u;
   auto k_slot = [&](int s) { return base + 65536u + (uint32_t)s * 32768u; };
-  auto v_slot = [&](int s) { return base + 65536u + (uint32_t)s * 32768u + 16384u; };   // V tile, later dS
+  auto v_slot = [&](int s) { return base + 65536u + (uint32_t)s * 32768u + 16384u; };
   const uint32_t o_tile = base + 65536u + kDqStages * 32768u;                           // forward output tile, only for delta
   DqSmem* sm = reinterpret_cast<DqSmem*>(smem_raw + (base - raw) + 65536u + kDqStages * 32768u + 32768u);
 
@@ -862,13 +865,13 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     for (int s = 0; s < kDqStages; ++s) {
       mbar_init(smem_u32(&sm->full[s]), 1);
       mbar_init(smem_u32(&sm->empty[s]), 1);
-      mbar_init(smem_u32(&sm->ds_ready[s]), 128);
     }
     for (int s = 0; s < kSdpBufs; ++s) {
+      mbar_init(smem_u32(&sm->ds_ready[s]), 128);
       mbar_init(smem_u32(&sm->s_full[s]), 1);
       mbar_init(smem_u32(&sm->s_free[s]), 128);
       mbar_init(smem_u32(&sm->dp_full[s]), 1);
-      mbar_init(smem_u32(&sm->dp_free[s]), 128);
+      mbar_init(smem_u32(&sm->dp_free[s]), 1);
     }
     mbar_init(smem_u32(&sm->acc_full[0]), 1);
     mbar_init(smem_u32(&sm->acc_full[1]), 1);
@@ -954,22 +957,22 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     // ------------------------------------------------------------------ dQ += dS K
     constexpr uint32_t fmt = kBf16 ? 1u : 0u;
     constexpr uint32_t idesc_q = instr_desc_f16(fmt, 128, kD, 0, 1);
-    const uint64_t dv0 = smem_desc_sw128(v_slot(0), 16, 1024);
     const uint64_t dk0t = smem_desc_sw128(k_slot(0), kHalfTile, 1024);
     int it = 0, u = 0;
     for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
       const int total = warp_uniform(unit_of(w).total);
       if (total == 0) continue;
       for (int i = 0; i < total; ++i, ++it) {
-        const int s = it % kDqStages;
+        const int s = it % kDqStages, sb = it % kSdpBufs;
         if (i == 0) mbar_wait(smem_u32(&sm->acc_empty), (u & 1) ^ 1, status, kErrDqMma);
-        mbar_wait(smem_u32(&sm->ds_ready[s]), (it / kDqStages) & 1, status, kErrDqMma);
+        mbar_wait(smem_u32(&sm->ds_ready[sb]), (it / kSdpBufs) & 1, status, kErrDqMma);
         tc_fence_after();
-        const uint64_t dds = desc_advance(dv0, (uint32_t)s * 32768u), dkt = desc_advance(dk0t, (uint32_t)s * 32768u);
+        const uint64_t dkt = desc_advance(dk0t, (uint32_t)s * 32768u);
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kBlk / 16; ++kk)
-            mma_f16_ss(tmem_dq, desc_advance(dds, kk * 32), desc_advance(dkt, kk * 2048), idesc_q, (i > 0 || kk > 0) ? 1u : 0u);
+            mma_f16_ts(tmem_dq, tmem_dp + sb * 64 + kk * 8, desc_advance(dkt, kk * 2048), idesc_q, (i > 0 || kk > 0) ? 1u : 0u);
+          mma_commit(smem_u32(&sm->dp_free[sb]));                  // dS has been read: the buffer may take the next dP
           mma_commit(smem_u32(&sm->empty[s]));
         }
       }
@@ -1090,7 +1093,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       if (g == 0 && stored) p.delta[grow] = valid ? delta : 0.f;
       if (warp_uniform(drain_row >= 0)) drain();
       for (int i = (it0 + g) & 1; i < un.total; i += kBwdGroups) {
-        const int it = it0 + i, s = it % kDqStages, sb = it % kSdpBufs, key0 = un.tile_of(i) * kBlk;
+        const int it = it0 + i, sb = it % kSdpBufs, key0 = un.tile_of(i) * kBlk;
         const Columns col(pos, key0, p.window, p.sinks);
         // a row of padding spoils its own row of dQ alone, which is not stored
         const int kind = warp_uniform(tile_empty(warp_p0, warp_p1, key0, p.window, p.sinks) ? 0
@@ -1105,10 +1108,11 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         mbar_wait(smem_u32(&sm->dp_full[sb]), (it / kSdpBufs) & 1, status, kErrDqSoftmax);
         tc_fence_after();
         uint32_t wd[32];
-        bwd_dscores<kBf16>(wd, sp, tmem_dp + sb * 64 + lane_base, smem_u32(&sm->dp_free[sb]), kind, col, p.scale, delta);
-        store_row_sw128(v_slot(s), row, wd);      // dS replaces the V tile of this stage, which dP has finished reading
-        fence_proxy_async_smem();
-        mbar_arrive(smem_u32(&sm->ds_ready[s]));
+        bwd_dscores<kBf16>(wd, sp, tmem_dp + sb * 64 + lane_base, kind, col, p.scale, delta, []() {});
+        tmem_st_32x32b_x32(tmem_dp + sb * 64 + lane_base, wd);      // dS replaces dP in place; dQ takes it from there as its A operand
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&sm->ds_ready[sb]));
       }
       it0 += un.total;
       if (g == ((it0 - 1) & 1)) {
