@@ -11,8 +11,7 @@
 //   dQ: unit = (query tile, head), persistent.  Q and dO rows go to TMEM as A operands; per key tile S, dP -> dS in 16 bits over
 //   the TMEM columns of dP -> dQ += dS K with A = dS from TMEM.
 //   dK/dV: unit = (pair of key tiles, key head, run of query tiles), persistent; Q and dO tiles of all heads that share the keys
-//   stream through.  P^T dO and dS^T Q take P and dS from shared memory as MN-major operands.  The accumulators are the sums over the
-//   group's heads.  The query tiles of a pair with sinks are dealt out to several units (SinkSplit): one unit would be as long as the
+//   stream through, and their contributions are summed in the accumulators.  The query tiles of a pair with sinks are dealt out to several units (SinkSplit): one unit would be as long as the
 //   sequence.
 // Rows behind a sequence's end (lengths) are hidden by selects and, where a product would multiply them with a zero, overwritten with zeros in
 // shared memory by the loading thread, so that NaN there stays there.
@@ -54,12 +53,12 @@ struct Columns {
   __device__ Columns(int pos, int key0, int window, int sinks) : last(pos - key0), first(pos - window + 1 - key0), sink(sinks - key0) {}
   __device__ bool sees(int j) const { return j <= last && (j >= first || j < sink); }
 };
-// every row at positions p0 .. p1 sees every key of the tile / no row sees one
-__device__ __forceinline__ bool tile_full(int p0, int p1, int key0, int window, int sinks) {
-  return key0 + kBlk - 1 <= p0 && (p1 - key0 < window || key0 + kBlk <= sinks);
+// Every one of the rows at positions p0 .. p1 sees every one of the keys k0 .. k1 / none sees one.
+__device__ __forceinline__ bool all_seen(int p0, int p1, int k0, int k1, int window, int sinks) {
+  return k1 <= p0 && (p1 - k0 < window || k1 < sinks);
 }
-__device__ __forceinline__ bool tile_empty(int p0, int p1, int key0, int window, int sinks) {
-  return key0 > p1 || (p0 - (key0 + kBlk - 1) >= window && key0 >= sinks);
+__device__ __forceinline__ bool none_seen(int p0, int p1, int k0, int k1, int window, int sinks) {
+  return k0 > p1 || (p0 - k1 >= window && k0 >= sinks);
 }
 
 struct WindowTensors {
@@ -254,7 +253,7 @@ window_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       mbar_wait(smem_u32(&sm->s_full[w][sb]), (k / 2) & 1, status, kErrFwdSoftmax);
       tc_fence_after();
       uint32_t wgt[32];
-      if (tile_empty(warp_p0, warp_p1, key0, p.window, p.sinks)) {
+      if (none_seen(warp_p0, warp_p1, key0, key0 + kBlk - 1, p.window, p.sinks)) {
 #pragma unroll
         for (int j = 0; j < 32; ++j) wgt[j] = 0u;
       } else {
@@ -270,7 +269,7 @@ window_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             sv[32 + j] = __uint_as_float(rb[j]);
           }
         }
-        const bool full = tile_full(warp_p0, warp_p1, key0, p.window, p.sinks);
+        const bool full = all_seen(warp_p0, warp_p1, key0, key0 + kBlk - 1, p.window, p.sinks);
         if (!full) {
           const Columns col(pos, key0, p.window, p.sinks);
 #pragma unroll
@@ -378,105 +377,82 @@ window_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
 }
 
 // ---------------------------------------------------------------------------------------------- backward
+// Four softmax warpgroups in both kernels: with the normaliser known there are no sums over a row, so a row's columns can belong to
+// several threads, and 32 columns a thread fit 96 registers.  (Two warpgroups of 64 columns: see the figures at the kernels.)
+constexpr int kBwdWarps = 16;
+constexpr int kCols = 32;                           // columns of a score tile that one thread holds
 // one pair of exponentials in this many is a cubic (7.5e-5, below half a step of either type); full tiles only
 constexpr int kBwdPolyEvery = 4;
 
-// Reads 64 columns of S from TMEM and leaves the row's weights p = 2^(s c - lse) in sp, hidden columns 0.
-// kind 0: nothing visible, 1: masked, 2: full (the same for all rows of a warp).
-template <typename AfterFn>
-__device__ __forceinline__ void bwd_weights(uint64_t (&sp)[32], uint32_t ts, int kind, const Columns& col, float c, float lse, AfterFn after_s) {
-  if (kind == 0) {
-    after_s();
+// TMEM columns -> 16 packed pairs
+__device__ __forceinline__ void load_pairs(uint64_t (&x)[kCols / 2], uint32_t taddr) {
+  uint32_t r[kCols];
+  tmem_ld_32x32b_x32(taddr, r);
+  tmem_ld_wait();
 #pragma unroll
-    for (int j = 0; j < 32; ++j) sp[j] = 0ull;
-    return;
-  }
-  {
-    uint32_t ra[32], rb[32];
-    tmem_ld_32x32b_x32(ts, ra);
-    tmem_ld_32x32b_x32(ts + 32, rb);
-    tmem_ld_wait();
+  for (int j = 0; j < kCols / 2; ++j) x[j] = pk2u(r[2 * j], r[2 * j + 1]);
+}
+// x: scores -> weights 2^(s c + nl), nl = -lse, of pair j given by nl(j); hidden columns become 0 (kind 1)
+template <typename NegLse, typename Sees>
+__device__ __forceinline__ void weights_of(uint64_t (&x)[kCols / 2], int kind, float c, NegLse nl, Sees sees) {
+  const uint64_t c2 = pk2(c, c);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      sp[j] = pk2u(ra[2 * j], ra[2 * j + 1]);
-      sp[16 + j] = pk2u(rb[2 * j], rb[2 * j + 1]);
-    }
-  }
-  after_s();      // S is in registers: its buffer may take the next product
-  const uint64_t c2 = pk2(c, c), m2 = pk2(-lse, -lse);
-  if (kind == 1) {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
+  for (int j = 0; j < kCols / 2; ++j) {
+    const uint64_t e = fma2(x[j], c2, nl(j));
+    if (kind == 1) {
       float a, b;
-      upk2(fma2(sp[j], c2, m2), a, b);
-      sp[j] = pk2(col.sees(2 * j) ? ex2(a) : 0.f, col.sees(2 * j + 1) ? ex2(b) : 0.f);
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      const uint64_t x = fma2(sp[j], c2, m2);
-      if (j % kBwdPolyEvery == 1) {
-        sp[j] = ex2_poly2<3>(x);
-      } else {
-        float a, b;
-        upk2(x, a, b);
-        sp[j] = pk2(ex2(a), ex2(b));
-      }
+      upk2(e, a, b);
+      x[j] = pk2(sees(2 * j) ? ex2(a) : 0.f, sees(2 * j + 1) ? ex2(b) : 0.f);
+    } else if (j % kBwdPolyEvery == 1) {
+      x[j] = ex2_poly2<3>(e);
+    } else {
+      float a, b;
+      upk2(e, a, b);
+      x[j] = pk2(ex2(a), ex2(b));
     }
   }
 }
-
-// Reads dP from TMEM and leaves the row of dS = p (dP - delta) scale, packed to 16 bits, in wd.
-template <bool kBf16, typename AfterFn>
-__device__ __forceinline__ void bwd_dscores(uint32_t (&wd)[32], const uint64_t (&sp)[32], uint32_t tdp, int kind, const Columns& col, float scale,
-                                            float delta, AfterFn after_dp) {
-  if (kind == 0) {
-    after_dp();
+// dS = p (dP - delta) scale in 16 bits; nd(j): -delta scale of pair j.  What a hidden value or a padded row brought along is dropped by
+// a select, not multiplied by 0 (kind 1).
+template <bool kBf16, typename NegDelta, typename Sees>
+__device__ __forceinline__ void dscores_of(uint32_t (&w)[kCols / 2], const uint64_t (&p)[kCols / 2], const uint64_t (&dp)[kCols / 2], int kind,
+                                           float scale, NegDelta nd, Sees sees) {
+  const uint64_t s2 = pk2(scale, scale);
 #pragma unroll
-    for (int j = 0; j < 32; ++j) wd[j] = 0u;
-    return;
-  }
-  uint64_t dp[32];
-  {
-    uint32_t ra[32], rb[32];
-    tmem_ld_32x32b_x32(tdp, ra);
-    tmem_ld_32x32b_x32(tdp + 32, rb);
-    tmem_ld_wait();
-#pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      dp[j] = pk2u(ra[2 * j], ra[2 * j + 1]);
-      dp[16 + j] = pk2u(rb[2 * j], rb[2 * j + 1]);
+  for (int j = 0; j < kCols / 2; ++j) {
+    float a, b;
+    upk2(mul2(p[j], fma2(dp[j], s2, nd(j))), a, b);
+    if (kind == 1) {
+      a = sees(2 * j) ? a : 0.f;
+      b = sees(2 * j + 1) ? b : 0.f;
     }
-  }
-  after_dp();
-  const uint64_t sc2 = pk2(scale, scale);
-  const float ns = -delta * scale;
-  const uint64_t ns2 = pk2(ns, ns);
-#pragma unroll
-  for (int j = 0; j < 32; ++j) {
-    float d0, d1;
-    upk2(mul2(sp[j], fma2(dp[j], sc2, ns2)), d0, d1);
-    if (kind == 1) {                          // what a hidden value or a padded row brought along is dropped, not multiplied by 0
-      d0 = col.sees(2 * j) ? d0 : 0.f;
-      d1 = col.sees(2 * j + 1) ? d1 : 0.f;
-    }
-    wd[j] = pack2<kBf16>(d0, d1);
+    w[j] = pack2<kBf16>(a, b);
   }
 }
 
-constexpr int kBwdGroups = 2;                       // softmax warpgroups
-constexpr int kBwdThreads = (kBwdGroups * 4 + 3) * 32;
-constexpr int kPair = 128;                          // keys of a dK/dV unit
-template <int kD> constexpr int kDkvStages = kD == 128 ? 2 : 4;
+// ---------------------------------------------------------------------------------------------- backward: dK, dV
+// Transposed scores: S^T = K Q^T and dP^T = V dO^T, 128 keys on the TMEM lanes and 128 queries on the columns, so that P^T and dS^T, written
+// in 16 bits over the columns they came from, are the A operands of dV += P^T dO and dK += dS^T Q straight from TMEM: no
+// shared-memory tiles for them, and all four products run at the tensor cores' rate.  Shared memory still moves 256 KB an
+// item (K and V as A operands, Q and dO twice as B, their loads), as long as the products take: 2048 clk each.
+// TMEM: 128 S + 128 dP + kD dV + kD dK columns.  The softmax threads and the products take turns: while P^T of an item is made, dK of the
+// item before and dP of this one run; while dS^T is made, dV and the next S.  Row statistics are per column here: the loading
+// warp lays them out in shared memory, and a warp reads four at a time by broadcast.
+constexpr int kPair = 128;                          // keys of a unit
+constexpr int kDkvThreads = (kBwdWarps + 3) * 32;
+constexpr int kDkvStages = 2;
 
-template <int kStages> struct DkvSmem {
+struct DkvSmem {
   uint64_t k_full, k_empty, v_full, v_empty, patch;
-  uint64_t q_full[kStages], q_empty[kStages];       // Q: until dK has read it
-  uint64_t do_full[kStages], do_empty[kStages];     // dO: until dP and dV have read it
-  uint64_t s_full, s_free, dp_full, dp_free;        // S, dP of both blocks (N = 128 products)
-  uint64_t p_ready, p_free, ds_ready, ds_free;      // the P rows are in the weight tiles / dV has read them; likewise dS in their place
-  uint64_t acc_full[2], acc_empty[2];               // [0] dV, [1] dK
+  uint64_t q_full[kDkvStages], q_empty[kDkvStages];       // Q and the statistics: until dK has been formed
+  uint64_t do_full[kDkvStages], do_empty[kDkvStages];     // dO: until dP and dV have read it
+  uint64_t stat_full[kDkvStages];
+  uint64_t s_full, s_free, dp_full, dp_free;              // the products' results are there / P and dS in their places have been read
+  uint64_t p_ready, ds_ready;
+  uint64_t acc_full[2], acc_empty[2];                     // [0] dV, [1] dK
   uint32_t tmem_base;
+  alignas(16) float nlse[kDkvStages][kQTile];             // -lse
+  alignas(16) float ndelta[kDkvStages][kQTile];           // -delta scale
 };
 
 struct DkvArgs {
@@ -495,11 +471,11 @@ struct DkvUnit {
 };
 
 template <bool kBf16, int kD>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+__global__ void __launch_bounds__(kDkvThreads, 1)
 window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                         const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
                         const __grid_constant__ DkvArgs p, int* status) {
-  constexpr int kStages = kDkvStages<kD>;
+  constexpr int kStages = kDkvStages;
   constexpr uint32_t kOperand = (kD / 64) * kTileBytes;     // [128 rows x kD] as 64-feature sub-tiles of 16 KB
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -507,9 +483,7 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   const uint32_t k_pair = base, v_pair = base + kOperand;
   auto q_slot = [&](int s) { return base + 2 * kOperand + (uint32_t)s * 2 * kOperand; };
   auto do_slot = [&](int s) { return base + 3 * kOperand + (uint32_t)s * 2 * kOperand; };
-  const uint32_t w_tile = base + (2 + 2 * kStages) * kOperand;         // P, then dS: [128 q x 64 keys] of block a, then of b
-  DkvSmem<kStages>* sm =
-      reinterpret_cast<DkvSmem<kStages>*>(smem_raw + (base - raw) + (2 + 2 * kStages) * kOperand + 2 * kTileBytes);
+  DkvSmem* sm = reinterpret_cast<DkvSmem*>(smem_raw + (base - raw) + (2 + 2 * kStages) * kOperand);
 
   const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
   const int off = p.Lk - p.Lq, heads = p.B * p.Hkv;
@@ -544,70 +518,102 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   };
 
   if (tid == 0) {
-    for (uint64_t* bar : {&sm->k_full, &sm->k_empty, &sm->v_full, &sm->v_empty, &sm->patch, &sm->s_full, &sm->dp_full, &sm->p_free, &sm->ds_free})
+    for (uint64_t* bar : {&sm->k_full, &sm->k_empty, &sm->v_full, &sm->v_empty, &sm->patch, &sm->s_full, &sm->s_free, &sm->dp_full, &sm->dp_free})
       mbar_init(smem_u32(bar), 1);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(smem_u32(&sm->q_full[s]), 1);
       mbar_init(smem_u32(&sm->q_empty[s]), 1);
       mbar_init(smem_u32(&sm->do_full[s]), 1);
       mbar_init(smem_u32(&sm->do_empty[s]), 2);       // dP and dV, issued by different warps
+      mbar_init(smem_u32(&sm->stat_full[s]), 32);
     }
-    for (uint64_t* bar : {&sm->s_free, &sm->dp_free, &sm->p_ready, &sm->ds_ready}) mbar_init(smem_u32(bar), 256);
+    for (uint64_t* bar : {&sm->p_ready, &sm->ds_ready}) mbar_init(smem_u32(bar), kBwdWarps * 32);
     for (int g = 0; g < 2; ++g) {
       mbar_init(smem_u32(&sm->acc_full[g]), 1);
-      mbar_init(smem_u32(&sm->acc_empty[g]), 128);
+      mbar_init(smem_u32(&sm->acc_empty[g]), kBwdWarps * 16);
     }
     mbar_init_fence();
   }
-  if (warp == kBwdGroups * 4 + 1) tmem_alloc(smem_u32(&sm->tmem_base), 512);
+  if (warp == kBwdWarps + 1) tmem_alloc(smem_u32(&sm->tmem_base), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = (uint32_t)warp_uniform((int)sm->tmem_base);
   const uint32_t tmem_s = tmem, tmem_dp = tmem + 128u, tmem_dv = tmem + 256u, tmem_dk = tmem + 256u + kD;
+  // A operand of K-step kk (16 queries) of P^T / dS^T: a warpgroup's 32 queries sit in the first 16 of their 32 columns
+  auto a_step = [](int kk) { return (uint32_t)((kk >> 1) * kCols + (kk & 1) * 8); };
 
-  if (warp == kBwdGroups * 4) {
-    // ------------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      int it = 0, u = 0, patches = 0;
-      for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
-        const DkvUnit un = unit_of(w);
-        const int n_items = un.n_q * p.G;
-        if (n_items == 0) continue;
-        auto load_pair = [&](uint32_t dst, const CUtensorMap* tm, uint64_t* full, uint64_t* empty) {
-          const uint32_t fb = smem_u32(full);
-          mbar_wait(smem_u32(empty), (u & 1) ^ 1, status, kErrDkvProducer);
+  if (warp == kBwdWarps) {
+    // ------------------------------------------------------------------ loads: lane 0 issues TMA, all lanes bring the statistics
+    int it = 0, u = 0, patches = 0;
+    bool behind = false;                           // behind the dQ kernel, which writes delta
+    for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
+      const DkvUnit un = unit_of(w);
+      const int n_items = un.n_q * p.G;
+      if (n_items == 0) continue;
+      auto load_pair = [&](uint32_t dst, const CUtensorMap* tm, uint64_t* full, uint64_t* empty) {
+        const uint32_t fb = smem_u32(full);
+        mbar_wait(smem_u32(empty), (u & 1) ^ 1, status, kErrDkvProducer);
+        if (lane == 0) {
           mbar_arrive_expect_tx(fb, kOperand);
           for (int g = 0; g < 2; ++g)
             for (int c = 0; c < kD / 64; ++c)
               tma_load_4d(dst + c * kTileBytes + g * kHalfTile, tm, fb, 64 * c, un.pair * kPair + g * kBlk, un.hk, un.b);
-        };
-        auto load_rows = [&](uint32_t dst, const CUtensorMap* tm, uint64_t* full, uint64_t* empty, int h, int tile) {
-          mbar_wait(smem_u32(empty), ((it / kStages) & 1) ^ 1, status, kErrDkvProducer);
-          const int rows = un.len - off - tile * kQTile;            // rows of the tile that the sequence has
-          const bool ends = rows < kQTile && un.len < p.Lk;
-          const uint32_t fb = smem_u32(ends ? &sm->patch : full);
+        }
+        __syncwarp();
+      };
+      auto load_rows = [&](uint32_t dst, const CUtensorMap* tm, uint64_t* full, uint64_t* empty, int h, int tile) {
+        mbar_wait(smem_u32(empty), ((it / kStages) & 1) ^ 1, status, kErrDkvProducer);
+        const int rows = un.len - off - tile * kQTile;            // rows of the tile that the sequence has
+        const bool ends = rows < kQTile && un.len < p.Lk;
+        const uint32_t fb = smem_u32(ends ? &sm->patch : full);
+        if (lane == 0) {
           mbar_arrive_expect_tx(fb, kOperand);
           for (int c = 0; c < kD / 64; ++c) tma_load_4d(dst + c * kTileBytes, tm, fb, 64 * c, tile * kQTile, h, un.b);
           if (ends) {
-            mbar_wait(fb, patches++ & 1, status, kErrDkvProducer);
+            mbar_wait(fb, patches & 1, status, kErrDkvProducer);
             zero_rows(dst, kTileBytes, kD / 64, rows, kQTile);
             mbar_arrive(smem_u32(full));
           }
-        };
-        load_pair(k_pair, &tm_k, &sm->k_full, &sm->k_empty);
-        for (int i = 0; i < n_items; ++i, ++it) {
-          const int s = it % kStages, g = i / un.n_q, h = un.hk * p.G + g, tile = un.first + i - g * un.n_q;
-          load_rows(q_slot(s), &tm_q, &sm->q_full[s], &sm->q_empty[s], h, tile);
-          if (i == 0) load_pair(v_pair, &tm_v, &sm->v_full, &sm->v_empty);
-          load_rows(do_slot(s), &tm_do, &sm->do_full[s], &sm->do_empty[s], h, tile);
         }
-        ++u;
+        if (ends) ++patches;
+        __syncwarp();
+      };
+      float4 nl, nd;
+      auto ask = [&](int i) {                      // statistics of an item's rows 4 lane .. 4 lane + 3, one item ahead
+        const int g = i / un.n_q, tile = un.first + i - g * un.n_q, row = tile * kQTile + lane * 4;
+        const int64_t at = ((int64_t)un.b * p.H + un.hk * p.G + g) * p.Lq + row;
+        float l[4], d[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool valid = off + row + e < un.len;
+          l[e] = valid ? -ld_behind_wait(p.lse + at + e) : -INFINITY;
+          d[e] = valid ? -p.scale * ld_behind_wait(p.delta + at + e) : 0.f;
+        }
+        nl = make_float4(l[0], l[1], l[2], l[3]);
+        nd = make_float4(d[0], d[1], d[2], d[3]);
+      };
+      load_pair(k_pair, &tm_k, &sm->k_full, &sm->k_empty);
+      for (int i = 0; i < n_items; ++i, ++it) {
+        const int s = it % kStages, g = i / un.n_q, h = un.hk * p.G + g, tile = un.first + i - g * un.n_q;
+        load_rows(q_slot(s), &tm_q, &sm->q_full[s], &sm->q_empty[s], h, tile);
+        if (i == 0) load_pair(v_pair, &tm_v, &sm->v_full, &sm->v_empty);
+        if (!behind) {
+          grid_dep_wait();
+          behind = true;
+        }
+        if (i == 0) ask(0);
+        *reinterpret_cast<float4*>(&sm->nlse[s][lane * 4]) = nl;
+        *reinterpret_cast<float4*>(&sm->ndelta[s][lane * 4]) = nd;
+        mbar_arrive(smem_u32(&sm->stat_full[s]));
+        if (i + 1 < n_items) ask(i + 1);
+        load_rows(do_slot(s), &tm_do, &sm->do_full[s], &sm->do_empty[s], h, tile);
       }
+      ++u;
     }
     __syncwarp();
-  } else if (warp == kBwdGroups * 4 + 1) {
-    // ------------------------------------------------------------------ S = Q K^T and dP = dO V^T of both blocks at once
+  } else if (warp == kBwdWarps + 1) {
+    // ------------------------------------------------------------------ S^T = K Q^T and dP^T = V dO^T
     constexpr uint32_t fmt = kBf16 ? 1u : 0u;
     constexpr uint32_t idesc_s = instr_desc_f16(fmt, 128, 128, 0, 0);
     const uint64_t dk0 = smem_desc_sw128(k_pair, 16, 1024), dv0 = smem_desc_sw128(v_pair, 16, 1024);
@@ -626,7 +632,7 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kD / 16; ++kk)
-            mma_f16_ss(tmem_s, desc_advance(dq, kmajor_step(kk, kTileBytes)), desc_advance(dk0, kmajor_step(kk, kTileBytes)), idesc_s, kk > 0);
+            mma_f16_ss(tmem_s, desc_advance(dk0, kmajor_step(kk, kTileBytes)), desc_advance(dq, kmajor_step(kk, kTileBytes)), idesc_s, kk > 0);
           mma_commit(smem_u32(&sm->s_full));
           if (i == n_items - 1) mma_commit(smem_u32(&sm->k_empty));
         }
@@ -637,7 +643,7 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kD / 16; ++kk)
-            mma_f16_ss(tmem_dp, desc_advance(ddo, kmajor_step(kk, kTileBytes)), desc_advance(dv0, kmajor_step(kk, kTileBytes)), idesc_s, kk > 0);
+            mma_f16_ss(tmem_dp, desc_advance(dv0, kmajor_step(kk, kTileBytes)), desc_advance(ddo, kmajor_step(kk, kTileBytes)), idesc_s, kk > 0);
           mma_commit(smem_u32(&sm->dp_full));
           mma_commit(smem_u32(&sm->do_empty[s]));
           if (i == n_items - 1) mma_commit(smem_u32(&sm->v_empty));
@@ -645,13 +651,13 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       }
       ++u;
     }
-  } else if (warp == kBwdGroups * 4 + 2) {
-    // ------------------------------------------------------------------ dV += P^T dO and dK += dS^T Q
+    __syncwarp();
+  } else if (warp == kBwdWarps + 2) {
+    // ------------------------------------------------------------------ dV += P^T dO and dK += dS^T Q, A from TMEM
     constexpr uint32_t fmt = kBf16 ? 1u : 0u;
-    constexpr uint32_t idesc_t = instr_desc_f16(fmt, 128, kD, 1, 1);
+    constexpr uint32_t idesc_t = instr_desc_f16(fmt, 128, kD, 0, 1);
     const uint64_t dq0t = smem_desc_sw128(q_slot(0), kTileBytes, 1024);
     const uint64_t ddo0t = smem_desc_sw128(do_slot(0), kTileBytes, 1024);
-    const uint64_t dwt = smem_desc_sw128(w_tile, kTileBytes, 1024);
     int it = 0, u = 0;
     for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
       const int n_items = warp_uniform(unit_of(w).n_q) * p.G;
@@ -659,15 +665,15 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       for (int i = 0; i < n_items; ++i, ++it) {
         const int s = it % kStages;
         const uint64_t ddot = desc_advance(ddo0t, (uint32_t)s * 2 * kOperand), dqt = desc_advance(dq0t, (uint32_t)s * 2 * kOperand);
-        mbar_wait(smem_u32(&sm->do_full[s]), (it / kStages) & 1, status, kErrDkvMma);
+        mbar_wait(smem_u32(&sm->do_full[s]), (it / kStages) & 1, status, kErrDkvMma);      // P may be there first
         if (i == 0) mbar_wait(smem_u32(&sm->acc_empty[0]), (u & 1) ^ 1, status, kErrDkvMma);
         mbar_wait(smem_u32(&sm->p_ready), it & 1, status, kErrDkvMma);
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kQTile / 16; ++kk)
-            mma_f16_ss(tmem_dv, desc_advance(dwt, kk * 2048), desc_advance(ddot, kk * 2048), idesc_t, (i > 0 || kk > 0) ? 1u : 0u);
-          mma_commit(smem_u32(&sm->p_free));
+            mma_f16_ts(tmem_dv, tmem_s + a_step(kk), desc_advance(ddot, kk * 2048), idesc_t, (i > 0 || kk > 0) ? 1u : 0u);
+          mma_commit(smem_u32(&sm->s_free));
           mma_commit(smem_u32(&sm->do_empty[s]));
           if (i == n_items - 1) mma_commit(smem_u32(&sm->acc_full[0]));
         }
@@ -677,120 +683,122 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kQTile / 16; ++kk)
-            mma_f16_ss(tmem_dk, desc_advance(dwt, kk * 2048), desc_advance(dqt, kk * 2048), idesc_t, (i > 0 || kk > 0) ? 1u : 0u);
-          mma_commit(smem_u32(&sm->ds_free));
+            mma_f16_ts(tmem_dk, tmem_dp + a_step(kk), desc_advance(dqt, kk * 2048), idesc_t, (i > 0 || kk > 0) ? 1u : 0u);
+          mma_commit(smem_u32(&sm->dp_free));
           mma_commit(smem_u32(&sm->q_empty[s]));
           if (i == n_items - 1) mma_commit(smem_u32(&sm->acc_full[1]));
         }
       }
       ++u;
     }
+    __syncwarp();
   } else {
-    // ------------------------------------------------------------------ softmax: warpgroup g owns block g of the pair and drains dV (0) or dK (1)
+    // ------------------------------------------------------------------ softmax: lane = key of the pair, warpgroup = 32 queries of the tile
     const int g = warp >> 2;
     const int row = tid & 127;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t my_tile = w_tile + (uint32_t)g * kTileBytes;
+    const uint32_t ts = tmem_s + (uint32_t)g * kCols + lane_base, tdp = tmem_dp + (uint32_t)g * kCols + lane_base;
     int it = 0, u = 0;
-    grid_dep_wait();                               // delta comes from the dQ kernel, which may still be running (see the launch)
     for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
       const DkvUnit un = unit_of(w);
-      const int n_items = un.n_q * p.G, bk = un.b * p.Hkv + un.hk, key0 = un.pair * kPair + g * kBlk;
+      const int n_items = un.n_q * p.G, bk = un.b * p.Hkv + un.hk, key = un.pair * kPair + row;
       const bool split = un.pair < p.split.tiles;
       float* const part = split ? p.split.part + (((int64_t)bk * p.split.tiles + un.pair) * (1 + p.split.runs) + 1 + un.run) * 2 * kPair * p.D : nullptr;
-      const int out_key = un.pair * kPair + row;   // TMEM lane = key of the pair
+      // this thread's part of the results: warpgroups 0, 1 the halves of dV's features, 2, 3 of dK's
+      constexpr int kOut = kD / 2;
+      const bool is_dv = g < 2;
+      const int col0 = (g & 1) * kOut;
       if (n_items == 0) {                          // keys that nobody sees
-        if (un.base() && out_key < p.Lk) {
+        if (un.base() && key < p.Lk) {
           if (split) {
-            float4* to = reinterpret_cast<float4*>(part + ((g == 0 ? kPair : 0) + row) * p.D);
-            for (int e = 0; e < p.D / 4; ++e) to[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+            float* to = part + ((is_dv ? kPair : 0) + row) * p.D;
+            for (int e = col0; e < min(col0 + kOut, p.D); e += 4) *reinterpret_cast<float4*>(to + e) = make_float4(0.f, 0.f, 0.f, 0.f);
           } else {
-            uint32_t* to = reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(g == 0 ? p.dv : p.dk) + ((int64_t)bk * p.Lk + out_key) * p.D);
-            for (int e = 0; e < p.D / 2; ++e) to[e] = 0u;
+            uint16_t* to = reinterpret_cast<uint16_t*>(is_dv ? p.dv : p.dk) + ((int64_t)bk * p.Lk + key) * p.D;
+            for (int e = col0; e < min(col0 + kOut, p.D); e += 2) *reinterpret_cast<uint32_t*>(to + e) = 0u;
           }
         }
         __syncwarp();
         continue;
       }
-      float n_lse = 0.f, n_delta = 0.f;
-      auto fetch = [&](int i) {                    // one item ahead, so that the latency is never exposed
-        const int head = un.hk * p.G + i / un.n_q, rr = min((un.first + i % un.n_q) * kQTile + row, p.Lq - 1);
-        const int64_t at = ((int64_t)un.b * p.H + head) * p.Lq + rr;
-        n_lse = ld_behind_wait(p.lse + at);
-        n_delta = ld_behind_wait(p.delta + at);
-      };
-      fetch(0);
+      const int kmin = warp_uniform(un.pair * kPair + (warp & 3) * 32), kmax = kmin + 31;
+      const int last = key < p.sinks ? INT32_MAX / 2 : key + p.window;      // the key is seen from positions key .. last - 1
       for (int i = 0, tq = un.first; i < n_items; ++i, ++it) {
-        const int pos = off + tq * kQTile + row;
-        const int warp_p0 = warp_uniform(off + tq * kQTile + (warp & 3) * 32), warp_p1 = warp_p0 + 31;
-        const bool row_valid = tq * kQTile + row < p.Lq && pos < un.len;
-        const float lse = n_lse, delta = n_delta;
-        if (i + 1 < n_items) fetch(i + 1);
-        // a warp with a row that is none masks (its position becomes -1: it sees nothing)
-        const bool all_rows = warp_p1 < un.len && (tq * kQTile + (warp & 3) * 32 + 31) < p.Lq;
-        const Columns col(row_valid ? pos : -1, key0, p.window, p.sinks);
-        const int kind = warp_uniform(tile_empty(warp_p0, warp_p1, key0, p.window, p.sinks) ? 0
-                                      : all_rows && tile_full(warp_p0, warp_p1, key0, p.window, p.sinks) ? 2 : 1);
+        const int s = it % kStages, p0 = off + tq * kQTile + g * kCols;      // position of column 0
         if (++tq == un.first + un.n_q) tq = un.first;
+        const int first = key - p0, end = min(last, un.len) - p0;
+        auto sees = [&](int j) { return j >= first && j < end; };
+        const int p1 = p0 + kCols - 1;
+        const int kind = warp_uniform(p0 >= un.len || none_seen(p0, p1, kmin, kmax, p.window, p.sinks) ? 0
+                                      : p1 < un.len && all_seen(p0, p1, kmin, kmax, p.window, p.sinks) ? 2 : 1);
+        const ulonglong2* const nl = reinterpret_cast<const ulonglong2*>(&sm->nlse[s][g * kCols]);
+        const ulonglong2* const nd = reinterpret_cast<const ulonglong2*>(&sm->ndelta[s][g * kCols]);
+        mbar_wait(smem_u32(&sm->stat_full[s]), (it / kStages) & 1, status, kErrDkvSoftmax);
         mbar_wait(smem_u32(&sm->s_full), it & 1, status, kErrDkvSoftmax);
         tc_fence_after();
-        uint64_t sp[32];
-        bwd_weights(sp, tmem_s + (uint32_t)g * 64u + lane_base, kind, col, p.scale_log2, lse, [&]() {
-          tc_fence_before();
-          mbar_arrive(smem_u32(&sm->s_free));
-        });
-        uint32_t wd[32];
+        uint64_t sp[kCols / 2];
+        uint32_t wd[kCols / 2];
+        if (kind != 0) {
+          load_pairs(sp, ts);
+          weights_of(sp, kind, p.scale_log2, [&](int j) { const ulonglong2 x = nl[j >> 1]; return (uint64_t)(j & 1 ? x.y : x.x); }, sees);
 #pragma unroll
-        for (int j = 0; j < 32; ++j) wd[j] = pack2p<kBf16>(sp[j]);
-        if (it >= 1) mbar_wait(smem_u32(&sm->ds_free), (it & 1) ^ 1, status, kErrDkvSoftmax);
-        store_row_sw128(my_tile, row, wd);
-        fence_proxy_async_smem();
+          for (int j = 0; j < kCols / 2; ++j) wd[j] = pack2p<kBf16>(sp[j]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kCols / 2; ++j) wd[j] = 0u;
+        }
+        tmem_st_32x32b_x16(ts, wd);
+        tmem_st_wait();
+        tc_fence_before();
         mbar_arrive(smem_u32(&sm->p_ready));
         mbar_wait(smem_u32(&sm->dp_full), it & 1, status, kErrDkvSoftmax);
         tc_fence_after();
-        bwd_dscores<kBf16>(wd, sp, tmem_dp + (uint32_t)g * 64u + lane_base, kind, col, p.scale, delta, [&]() {
-          tc_fence_before();
-          mbar_arrive(smem_u32(&sm->dp_free));
-        });
-        mbar_wait(smem_u32(&sm->p_free), it & 1, status, kErrDkvSoftmax);
-        store_row_sw128(my_tile, row, wd);
-        fence_proxy_async_smem();
+        if (kind != 0) {
+          uint64_t dp[kCols / 2];
+          load_pairs(dp, tdp);
+          dscores_of<kBf16>(wd, sp, dp, kind, p.scale, [&](int j) { const ulonglong2 x = nd[j >> 1]; return (uint64_t)(j & 1 ? x.y : x.x); }, sees);
+        }
+        tmem_st_32x32b_x16(tdp, wd);               // (kind 0: still zeros)
+        tmem_st_wait();
+        tc_fence_before();
         mbar_arrive(smem_u32(&sm->ds_ready));
       }
-      // epilogue: dV by warpgroup 0, dK by warpgroup 1
-      const int64_t off_r = out_key < p.Lk ? ((int64_t)bk * p.Lk + out_key) * p.D : -1;
+      // epilogue
+      const int64_t off_r = key < p.Lk ? ((int64_t)bk * p.Lk + key) * p.D : -1;
       int64_t row_off[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) row_off[j] = __shfl_sync(0xffffffffu, off_r, (lane & ~3) + j);
-      mbar_wait(smem_u32(&sm->acc_full[g]), u & 1, status, kErrDkvEpilogue);
+      const int acc = is_dv ? 0 : 1;
+      mbar_wait(smem_u32(&sm->acc_full[acc]), u & 1, status, kErrDkvEpilogue);
       tc_fence_after();
-      const uint32_t t_acc = (g == 0 ? tmem_dv : tmem_dk) + lane_base;
-      void* const out = g == 0 ? p.dv : p.dk;
-      float* const prow = split ? part + ((g == 0 ? kPair : 0) + row) * p.D : nullptr;
+      const uint32_t t_acc = (is_dv ? tmem_dv : tmem_dk) + col0 + lane_base;
+      float* const prow = split ? part + ((is_dv ? kPair : 0) + row) * p.D : nullptr;
 #pragma unroll
-      for (int c = 0; c < kD / 32; ++c) {
+      for (int c = 0; c < kOut / 32; ++c) {
         uint32_t ra[32];
         tmem_ld_32x32b_x32(t_acc + c * 32, ra);
         tmem_ld_wait();
-        if (c == kD / 32 - 1) {
+        if (c == kOut / 32 - 1) {
           tc_fence_before();
-          mbar_arrive(smem_u32(&sm->acc_empty[g]));     // the next unit may start accumulating
+          mbar_arrive(smem_u32(&sm->acc_empty[acc]));     // the next unit may start accumulating
         }
         if (split) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (c * 32 + e * 4 < p.D)
-              *reinterpret_cast<uint4*>(prow + c * 32 + e * 4) = make_uint4(ra[4 * e], ra[4 * e + 1], ra[4 * e + 2], ra[4 * e + 3]);
+            if (col0 + c * 32 + e * 4 < p.D)
+              *reinterpret_cast<uint4*>(prow + col0 + c * 32 + e * 4) = make_uint4(ra[4 * e], ra[4 * e + 1], ra[4 * e + 2], ra[4 * e + 3]);
         } else {
-          store_acc_cols<kBf16>(out, row_off, ra, c * 32, p.D, lane);
+          store_acc_cols<kBf16>(is_dv ? p.dv : p.dk, row_off, ra, col0 + c * 32, p.D, lane);
         }
+        __syncwarp();
       }
       ++u;
     }
+    grid_dep_wait();                               // a CTA without units, too, ends behind the kernel in front
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == kBwdGroups * 4 + 1) {
+  if (warp == kBwdWarps + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -799,17 +807,17 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
 // ---------------------------------------------------------------------------------------------- backward: dQ
 constexpr int kDqStages = 4;
 constexpr int kSdpBufs = 2;                         // S / dP buffers in TMEM
-constexpr int kDqThreads = kBwdThreads + 32;        // S and dP are issued by warps of their own
+constexpr int kDqThreads = (kBwdWarps + 4) * 32;    // S and dP are issued by warps of their own
 
 struct DqSmem {
   uint64_t qdo_full, patch;
   uint64_t ops_ready;       // the unit's Q and dO rows sit in TMEM (written by the softmax warpgroups)
   uint64_t ops_free;        // the S / dP products of the unit have read them
-  uint64_t delta_read;      // both softmax warpgroups are done with the Q, dO and O tiles in shared memory
+  uint64_t delta_read;      // the softmax warpgroups are done with the Q, dO and O tiles in shared memory
   uint64_t full[kDqStages], empty[kDqStages];
   uint64_t s_full[kSdpBufs], s_free[kSdpBufs], dp_full[kSdpBufs];
   uint64_t ds_ready[kSdpBufs], dp_free[kSdpBufs];      // dS has taken dP's place / dQ has read it
-  uint64_t acc_full[2];     // per draining warpgroup (the one that took the unit's last item)
+  uint64_t acc_full[2];     // per draining pair of warpgroups (the one that took the unit's last item)
   uint64_t acc_empty;
   uint32_t tmem_base;
 };
@@ -859,26 +867,26 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 
   if (tid == 0) {
     for (uint64_t* bar : {&sm->qdo_full, &sm->patch}) mbar_init(smem_u32(bar), 1);
-    mbar_init(smem_u32(&sm->ops_ready), 256);
+    mbar_init(smem_u32(&sm->ops_ready), kBwdWarps * 32);
     mbar_init(smem_u32(&sm->ops_free), 2);          // the S issuer and the dP issuer
-    mbar_init(smem_u32(&sm->delta_read), 256);
+    mbar_init(smem_u32(&sm->delta_read), kBwdWarps * 32);
     for (int s = 0; s < kDqStages; ++s) {
       mbar_init(smem_u32(&sm->full[s]), 1);
       mbar_init(smem_u32(&sm->empty[s]), 1);
     }
     for (int s = 0; s < kSdpBufs; ++s) {
-      mbar_init(smem_u32(&sm->ds_ready[s]), 128);
+      mbar_init(smem_u32(&sm->ds_ready[s]), 256);
       mbar_init(smem_u32(&sm->s_full[s]), 1);
-      mbar_init(smem_u32(&sm->s_free[s]), 128);
+      mbar_init(smem_u32(&sm->s_free[s]), 256);
       mbar_init(smem_u32(&sm->dp_full[s]), 1);
       mbar_init(smem_u32(&sm->dp_free[s]), 1);
     }
     mbar_init(smem_u32(&sm->acc_full[0]), 1);
     mbar_init(smem_u32(&sm->acc_full[1]), 1);
-    mbar_init(smem_u32(&sm->acc_empty), 128);
+    mbar_init(smem_u32(&sm->acc_empty), 256);
     mbar_init_fence();
   }
-  if (warp == kBwdGroups * 4 + 1) tmem_alloc(smem_u32(&sm->tmem_base), 512);
+  if (warp == kBwdWarps + 1) tmem_alloc(smem_u32(&sm->tmem_base), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -888,7 +896,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   grid_dep_wait();
   grid_dep_launch();
 
-  if (warp == kBwdGroups * 4) {
+  if (warp == kBwdWarps) {
     // ------------------------------------------------------------------ TMA producer
     if (lane == 0) {
       int it = 0, u = 0, patches = 0;
@@ -924,11 +932,11 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       }
     }
     __syncwarp();
-  } else if (warp == kBwdGroups * 4 + 1 || warp == kBwdGroups * 4 + 3) {
+  } else if (warp == kBwdWarps + 1 || warp == kBwdWarps + 3) {
     // ------------------------------------------------------------------ S = Q K^T (warp +1), dP = dO V^T (warp +3)
     constexpr uint32_t fmt = kBf16 ? 1u : 0u;
     constexpr uint32_t idesc_s = instr_desc_f16(fmt, 128, 64, 0, 0);
-    const bool is_s = warp == kBwdGroups * 4 + 1;
+    const bool is_s = warp == kBwdWarps + 1;
     const uint64_t db0 = smem_desc_sw128(is_s ? k_slot(0) : v_slot(0), 16, 1024);
     const uint32_t t_out = is_s ? tmem_s : tmem_dp, t_a = is_s ? tmem_q : tmem_do;
     int it = 0, u = 0;
@@ -953,7 +961,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       ++u;
     }
     __syncwarp();
-  } else if (warp == kBwdGroups * 4 + 2) {
+  } else if (warp == kBwdWarps + 2) {
     // ------------------------------------------------------------------ dQ += dS K
     constexpr uint32_t fmt = kBf16 ? 1u : 0u;
     constexpr uint32_t idesc_q = instr_desc_f16(fmt, 128, kD, 0, 1);
@@ -971,7 +979,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kBlk / 16; ++kk)
-            mma_f16_ts(tmem_dq, tmem_dp + sb * 64 + kk * 8, desc_advance(dkt, kk * 2048), idesc_q, (i > 0 || kk > 0) ? 1u : 0u);
+            mma_f16_ts(tmem_dq, tmem_dp + sb * 64 + (kk >> 1) * kCols + (kk & 1) * 8, desc_advance(dkt, kk * 2048), idesc_q, (i > 0 || kk > 0) ? 1u : 0u);
           mma_commit(smem_u32(&sm->dp_free[sb]));                  // dS has been read: the buffer may take the next dP
           mma_commit(smem_u32(&sm->empty[s]));
         }
@@ -981,26 +989,29 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     }
     __syncwarp();
   } else {
-    // ------------------------------------------------------------------ softmax: warpgroup g takes the items with (running count) % 2 == g
-    const int g = warp >> 2;
+    // ------------------------------------------------------------------ softmax: warpgroups 2 e, 2 e + 1 take the items with (running count) % 2 == e,
+    // 32 columns each
+    const int g = warp >> 2, pair = g >> 1, half = g & 1;
     const int row = tid & 127;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     int it0 = 0, u = 0, drains = 0;
-    // dQ of a unit is drained by the warpgroup that took its last item, but only behind the prologue of the next unit: its last product
-    // queues behind that unit's first S / dP products
+    // dQ of a unit is drained by the pair that took its last item, half of the features each, but only behind the prologue of the next
+    // unit: its last product queues behind that unit's first S / dP products
+    constexpr int kOut = kD / 2;
     int64_t drain_row = -1;
     bool drain_stored = false, drain_valid = false;
     auto drain = [&]() {
-      mbar_wait(smem_u32(&sm->acc_full[g]), drains & 1, status, kErrDqEpilogue);
+      mbar_wait(smem_u32(&sm->acc_full[pair]), drains & 1, status, kErrDqEpilogue);
       ++drains;
       tc_fence_after();
       uint4* orow = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.dq) + drain_row * p.D);
 #pragma unroll
-      for (int c = 0; c < kD / 32; ++c) {
+      for (int c = 0; c < kOut / 32; ++c) {
+        const int col = half * kOut + c * 32;
         uint32_t r[32];
-        tmem_ld_32x32b_x32(tmem_dq + c * 32 + lane_base, r);
+        tmem_ld_32x32b_x32(tmem_dq + col + lane_base, r);
         tmem_ld_wait();
-        if (c == kD / 32 - 1) {
+        if (c == kOut / 32 - 1) {
           tc_fence_before();
           mbar_arrive(smem_u32(&sm->acc_empty));     // the next unit may start accumulating
         }
@@ -1012,8 +1023,9 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           pk.z = pack2<kBf16>(__uint_as_float(r[8 * v4 + 4]), __uint_as_float(r[8 * v4 + 5]));
           pk.w = pack2<kBf16>(__uint_as_float(r[8 * v4 + 6]), __uint_as_float(r[8 * v4 + 7]));
           if (!drain_valid) pk = make_uint4(0u, 0u, 0u, 0u);
-          if (drain_stored && c * 32 + v4 * 8 < p.D) orow[c * 4 + v4] = pk;
+          if (drain_stored && col + v4 * 8 < p.D) orow[col / 8 + v4] = pk;
         }
+        __syncwarp();
       }
       drain_row = -1;
     };
@@ -1042,80 +1054,99 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         continue;
       }
       const int warp_p0 = warp_uniform(off + un.t * kQTile + (warp & 3) * 32), warp_p1 = warp_p0 + 31;
-      // delta = rowsum(O * dO), straight from the swizzled tiles; warpgroup 0 also publishes it for the dK/dV kernel
+      // The unit's rows: a warpgroup moves half of the features of Q (pair 0) or dO (pair 1) to TMEM and sums O * dO over a quarter of
+      // them, straight from the swizzled tiles.
       mbar_wait(smem_u32(&sm->qdo_full), u & 1, status, kErrDqSoftmax);
-      float delta = 0.f;
-      uint32_t opw[kD / 64][32];      // this thread's row of the operand its warpgroup moves to TMEM (0: Q, 1: dO)
+      constexpr int kChunks = kD / 16;             // 16-byte chunks of half a row
+      uint32_t opw[4 * kChunks];
+      auto chunk_at = [&](int c) { return (uint32_t)(c >> 3) * kTileBytes + (uint32_t)row * 128u + (uint32_t)(((c & 7) ^ (row & 7)) << 4); };
 #pragma unroll
-      for (int sub = 0; sub < kD / 64; ++sub)
+      for (int c = 0; c < kChunks; ++c)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(opw[4 * c]), "=r"(opw[4 * c + 1]), "=r"(opw[4 * c + 2]), "=r"(opw[4 * c + 3])
+                     : "r"((pair == 0 ? q_tile : do_tile) + chunk_at(half * kChunks + c)));
+      float sum = 0.f;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const uint32_t at = (uint32_t)sub * kTileBytes + (uint32_t)row * 128u + (uint32_t)((c ^ (row & 7)) << 4);
-          uint32_t ov[4], gv[4];
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(ov[0]), "=r"(ov[1]), "=r"(ov[2]), "=r"(ov[3]) : "r"(o_tile + at));
-          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(gv[0]), "=r"(gv[1]), "=r"(gv[2]), "=r"(gv[3]) : "r"(do_tile + at));
-          if (g == 1) {
+      for (int c = 0; c < kChunks / 2; ++c) {
+        uint32_t ov[4], gv[4];
+        const uint32_t at = chunk_at(g * (kChunks / 2) + c);
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(ov[0]), "=r"(ov[1]), "=r"(ov[2]), "=r"(ov[3]) : "r"(o_tile + at));
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(gv[0]), "=r"(gv[1]), "=r"(gv[2]), "=r"(gv[3]) : "r"(do_tile + at));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) opw[sub][4 * c + e] = gv[e];
+        for (int e = 0; e < 4; ++e) {
+          float2 fo, fg;
+          if (kBf16) {
+            fo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&ov[e]));
+            fg = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&gv[e]));
           } else {
-            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                         : "=r"(opw[sub][4 * c]), "=r"(opw[sub][4 * c + 1]), "=r"(opw[sub][4 * c + 2]), "=r"(opw[sub][4 * c + 3])
-                         : "r"(q_tile + at));
+            fo = __half22float2(*reinterpret_cast<const __half2*>(&ov[e]));
+            fg = __half22float2(*reinterpret_cast<const __half2*>(&gv[e]));
           }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float2 fo, fg;
-            if (kBf16) {
-              fo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&ov[e]));
-              fg = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&gv[e]));
-            } else {
-              fo = __half22float2(*reinterpret_cast<const __half2*>(&ov[e]));
-              fg = __half22float2(*reinterpret_cast<const __half2*>(&gv[e]));
-            }
-            delta = fmaf(fo.x, fg.x, delta);
-            delta = fmaf(fo.y, fg.y, delta);
-          }
+          sum = fmaf(fo.x, fg.x, sum);
+          sum = fmaf(fo.y, fg.y, sum);
         }
-      // TMA writes the next unit's rows through another proxy than these loads went through
-      fence_proxy_async_smem();
-      mbar_arrive(smem_u32(&sm->delta_read));
+      }
+      // the shares of the sum change hands in the O tile, which everybody has read by then
+      asm volatile("bar.sync 1, %0;" ::"n"(kBwdWarps * 32) : "memory");
+      auto share = [&](int k) { return o_tile + (uint32_t)(k * kQTile + row) * 4u; };
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(share(g)), "f"(sum) : "memory");
       // row -> TMEM lane, 32-bit word j (two features) -> column j: the layout of a K-major A operand
       mbar_wait(smem_u32(&sm->ops_free), (u & 1) ^ 1, status, kErrDqSoftmax);
       tc_fence_after();
       {
-        const uint32_t dst = (g == 0 ? tmem_q : tmem_do) + lane_base;
-        tmem_st_32x32b_x32(dst, opw[0]);
-        if constexpr (kD == 128) tmem_st_32x32b_x32(dst + 32, opw[1]);
+        const uint32_t dst = (pair == 0 ? tmem_q : tmem_do) + half * (kD / 4) + lane_base;
+        if constexpr (kD == 128) tmem_st_32x32b_x32(dst, opw);
+        else tmem_st_32x32b_x16(dst, opw);
         tmem_st_wait();
       }
       tc_fence_before();
       mbar_arrive(smem_u32(&sm->ops_ready));
+      asm volatile("bar.sync 1, %0;" ::"n"(kBwdWarps * 32) : "memory");
+      float part[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(part[k]) : "r"(share(k)) : "memory");
+      const float delta = (part[0] + part[1]) + (part[2] + part[3]);
+      // TMA writes the next unit's rows through another proxy than these accesses went through
+      fence_proxy_async_smem();
+      mbar_arrive(smem_u32(&sm->delta_read));
       if (g == 0 && stored) p.delta[grow] = valid ? delta : 0.f;
       if (warp_uniform(drain_row >= 0)) drain();
-      for (int i = (it0 + g) & 1; i < un.total; i += kBwdGroups) {
-        const int it = it0 + i, sb = it % kSdpBufs, key0 = un.tile_of(i) * kBlk;
+      const uint64_t nl = pk2(-lse, -lse);
+      const float nds = -delta * p.scale;
+      const uint64_t nd = pk2(nds, nds);
+      for (int i = (it0 + pair) & 1; i < un.total; i += 2) {
+        const int it = it0 + i, sb = it % kSdpBufs, key0 = un.tile_of(i) * kBlk + half * kCols;
         const Columns col(pos, key0, p.window, p.sinks);
+        auto sees = [&](int j) { return col.sees(j); };
         // a row of padding spoils its own row of dQ alone, which is not stored
-        const int kind = warp_uniform(tile_empty(warp_p0, warp_p1, key0, p.window, p.sinks) ? 0
-                                      : tile_full(warp_p0, warp_p1, key0, p.window, p.sinks) ? 2 : 1);
+        const int kind = warp_uniform(none_seen(warp_p0, warp_p1, key0, key0 + kCols - 1, p.window, p.sinks) ? 0
+                                      : all_seen(warp_p0, warp_p1, key0, key0 + kCols - 1, p.window, p.sinks) ? 2 : 1);
+        const uint32_t ts = tmem_s + sb * 64 + half * kCols + lane_base, tdp = tmem_dp + sb * 64 + half * kCols + lane_base;
         mbar_wait(smem_u32(&sm->s_full[sb]), (it / kSdpBufs) & 1, status, kErrDqSoftmax);
         tc_fence_after();
-        uint64_t sp[32];
-        bwd_weights(sp, tmem_s + sb * 64 + lane_base, kind, col, p.scale_log2, lse, [&]() {
-          tc_fence_before();
-          mbar_arrive(smem_u32(&sm->s_free[sb]));
-        });
+        uint64_t sp[kCols / 2];
+        if (kind != 0) load_pairs(sp, ts);
+        tc_fence_before();
+        mbar_arrive(smem_u32(&sm->s_free[sb]));      // S is in registers: its buffer may take the next product
+        if (kind != 0) weights_of(sp, kind, p.scale_log2, [&](int) { return nl; }, sees);
         mbar_wait(smem_u32(&sm->dp_full[sb]), (it / kSdpBufs) & 1, status, kErrDqSoftmax);
         tc_fence_after();
-        uint32_t wd[32];
-        bwd_dscores<kBf16>(wd, sp, tmem_dp + sb * 64 + lane_base, kind, col, p.scale, delta, []() {});
-        tmem_st_32x32b_x32(tmem_dp + sb * 64 + lane_base, wd);      // dS replaces dP in place; dQ takes it from there as its A operand
+        uint32_t wd[kCols / 2];
+        if (kind != 0) {
+          uint64_t dp[kCols / 2];
+          load_pairs(dp, tdp);
+          dscores_of<kBf16>(wd, sp, dp, kind, p.scale, [&](int) { return nd; }, sees);
+        } else {
+#pragma unroll
+          for (int j = 0; j < kCols / 2; ++j) wd[j] = 0u;
+        }
+        tmem_st_32x32b_x16(tdp, wd);      // dS takes the place of dP; dQ takes it from there as its A operand
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(smem_u32(&sm->ds_ready[sb]));
       }
       it0 += un.total;
-      if (g == ((it0 - 1) & 1)) {
+      if (pair == ((it0 - 1) & 1)) {
         drain_row = grow;
         drain_stored = stored;
         drain_valid = valid;
@@ -1126,7 +1157,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == kBwdGroups * 4 + 1) {
+  if (warp == kBwdWarps + 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -1134,8 +1165,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 
 // ---------------------------------------------------------------------------------------------- host side
 template <int kTiles> constexpr size_t kSmemFwd = 1024 + (kTiles + kFwdStages<kTiles>) * 32768 + sizeof(FwdSmem<kFwdStages<kTiles>>);
-template <int kD> constexpr size_t kSmemDkv =
-    1024 + (2 + 2 * kDkvStages<kD>) * (kD / 64) * kTileBytes + 2 * kTileBytes + sizeof(DkvSmem<kDkvStages<kD>>);
+template <int kD> constexpr size_t kSmemDkv = 1024 + (2 + 2 * kDkvStages) * (kD / 64) * kTileBytes + sizeof(DkvSmem);
 constexpr size_t kSmemDq = 1024 + 65536 + kDqStages * 32768 + 32768 + sizeof(DqSmem);
 static_assert(kSmemFwd<2> <= 232448 && kSmemFwd<1> <= 232448 / 2 - 1024 && kSmemDkv<128> <= 232448 && kSmemDkv<64> <= 232448 && kSmemDq <= 232448,
               "shared memory of one SM");
@@ -1229,11 +1259,11 @@ int window_sm100_bwd(const WindowParams& p, int dtype, cudaStream_t st) {
                       p.split};
   const dim3 grid_q((unsigned)(dq_units < n_sm ? dq_units : n_sm)), grid_k((unsigned)(dkv_units < n_sm ? dkv_units : n_sm));
   // The dK/dV kernel may start on every SM that the dQ kernel has left: it reads q, k, v, dO, lse and lengths, which were complete before
-  // any CTA of the dQ kernel was behind its wait, and delta, for which its softmax threads wait.
+  // any CTA of the dQ kernel was behind its wait, and delta, for which its loading warp waits.
 #define LMK_BWD(BF, DIM)                                                                                                                    \
   do {                                                                                                                                      \
     LMK_CUDA(launch_overlapped(window_dq_sm100_kernel<BF, DIM>, grid_q, dim3(kDqThreads), kSmemDq, st, tq, tk, tv, tdo, to, aq, f->status)); \
-    LMK_CUDA(launch_overlapped(window_dkv_sm100_kernel<BF, DIM>, grid_k, dim3(kBwdThreads), kSmemDkv<DIM>, st, tq, tk, tv, tdo, ak, f->status)); \
+    LMK_CUDA(launch_overlapped(window_dkv_sm100_kernel<BF, DIM>, grid_k, dim3(kDkvThreads), kSmemDkv<DIM>, st, tq, tk, tv, tdo, ak, f->status)); \
   } while (0)
   if (dtype == LMK_BF16) {
     if (p.D <= 64) LMK_BWD(true, 64); else LMK_BWD(true, 128);
