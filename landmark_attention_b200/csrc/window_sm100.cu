@@ -439,16 +439,16 @@ __device__ __forceinline__ void dscores_of(uint32_t (&w)[kCols / 2], const uint6
 // item before and dP of this one run; while dS^T is made, dV and the next S.  Row statistics are per column here: the loading
 // warp lays them out in shared memory, and a warp reads four at a time by broadcast.
 constexpr int kPair = 128;                          // keys of a unit
-constexpr int kDkvThreads = (kBwdWarps + 3) * 32;
+constexpr int kDkvThreads = (kBwdWarps + 2) * 32;
 constexpr int kDkvStages = 2;
 
 struct DkvSmem {
   uint64_t k_full, k_empty, v_full, v_empty, patch;
   uint64_t q_full[kDkvStages], q_empty[kDkvStages];       // Q and the statistics: until dK has been formed
-  uint64_t do_full[kDkvStages], do_empty[kDkvStages];     // dO: until dP and dV have read it
+  uint64_t do_full[kDkvStages], do_empty[kDkvStages];     // dO: until dV has been formed
   uint64_t stat_full[kDkvStages];
-  uint64_t s_full, s_free, dp_full, dp_free;              // the products' results are there / P and dS in their places have been read
-  uint64_t p_ready, ds_ready;
+  uint64_t s_full, dp_full;                               // the products' results are there
+  uint64_t p_ready, ds_ready;                             // P and dS have taken their places
   uint64_t acc_full[2], acc_empty[2];                     // [0] dV, [1] dK
   uint32_t tmem_base;
   alignas(16) float nlse[kDkvStages][kQTile];             // -lse
@@ -518,13 +518,13 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   };
 
   if (tid == 0) {
-    for (uint64_t* bar : {&sm->k_full, &sm->k_empty, &sm->v_full, &sm->v_empty, &sm->patch, &sm->s_full, &sm->s_free, &sm->dp_full, &sm->dp_free})
+    for (uint64_t* bar : {&sm->k_full, &sm->k_empty, &sm->v_full, &sm->v_empty, &sm->patch, &sm->s_full, &sm->dp_full})
       mbar_init(smem_u32(bar), 1);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(smem_u32(&sm->q_full[s]), 1);
       mbar_init(smem_u32(&sm->q_empty[s]), 1);
       mbar_init(smem_u32(&sm->do_full[s]), 1);
-      mbar_init(smem_u32(&sm->do_empty[s]), 2);       // dP and dV, issued by different warps
+      mbar_init(smem_u32(&sm->do_empty[s]), 1);
       mbar_init(smem_u32(&sm->stat_full[s]), 32);
     }
     for (uint64_t* bar : {&sm->p_ready, &sm->ds_ready}) mbar_init(smem_u32(bar), kBwdWarps * 32);
@@ -613,83 +613,89 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     }
     __syncwarp();
   } else if (warp == kBwdWarps + 1) {
-    // ------------------------------------------------------------------ S^T = K Q^T and dP^T = V dO^T
+    // ------------------------------------------------------------------ all four products, A of dV and dK from TMEM
+    // One warp issues them: S of the next item right behind dV, which reads the P that stands in its place, and dP right behind dK.
+    // The tensor core works through what one thread issues in order, so neither waits for the other's end; with two issuing
+    // warps and barriers between them an item took 3400 clk instead of KKKK, most of it the way from a product's end to the next one's start.
     constexpr uint32_t fmt = kBf16 ? 1u : 0u;
-    constexpr uint32_t idesc_s = instr_desc_f16(fmt, 128, 128, 0, 0);
+    constexpr uint32_t idesc_s = instr_desc_f16(fmt, 128, 128, 0, 0), idesc_t = instr_desc_f16(fmt, 128, kD, 0, 1);
     const uint64_t dk0 = smem_desc_sw128(k_pair, 16, 1024), dv0 = smem_desc_sw128(v_pair, 16, 1024);
     const uint64_t dq0 = smem_desc_sw128(q_slot(0), 16, 1024), ddo0 = smem_desc_sw128(do_slot(0), 16, 1024);
-    int it = 0, u = 0;
-    for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
-      const int n_items = warp_uniform(unit_of(w).n_q) * p.G;
-      if (n_items == 0) continue;
-      mbar_wait(smem_u32(&sm->k_full), u & 1, status, kErrDkvMma);
-      for (int i = 0; i < n_items; ++i, ++it) {
-        const int s = it % kStages;
-        const uint64_t dq = desc_advance(dq0, (uint32_t)s * 2 * kOperand), ddo = desc_advance(ddo0, (uint32_t)s * 2 * kOperand);
-        mbar_wait(smem_u32(&sm->q_full[s]), (it / kStages) & 1, status, kErrDkvMma);
-        if (it >= 1) mbar_wait(smem_u32(&sm->s_free), (it & 1) ^ 1, status, kErrDkvMma);
-        tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < kD / 16; ++kk)
-            mma_f16_ss(tmem_s, desc_advance(dk0, kmajor_step(kk, kTileBytes)), desc_advance(dq, kmajor_step(kk, kTileBytes)), idesc_s, kk > 0);
-          mma_commit(smem_u32(&sm->s_full));
-          if (i == n_items - 1) mma_commit(smem_u32(&sm->k_empty));
-        }
-        if (i == 0) mbar_wait(smem_u32(&sm->v_full), u & 1, status, kErrDkvMma);
-        mbar_wait(smem_u32(&sm->do_full[s]), (it / kStages) & 1, status, kErrDkvMma);
-        if (it >= 1) mbar_wait(smem_u32(&sm->dp_free), (it & 1) ^ 1, status, kErrDkvMma);
-        tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < kD / 16; ++kk)
-            mma_f16_ss(tmem_dp, desc_advance(dv0, kmajor_step(kk, kTileBytes)), desc_advance(ddo, kmajor_step(kk, kTileBytes)), idesc_s, kk > 0);
-          mma_commit(smem_u32(&sm->dp_full));
-          mma_commit(smem_u32(&sm->do_empty[s]));
-          if (i == n_items - 1) mma_commit(smem_u32(&sm->v_empty));
-        }
+    const uint64_t dq0t = smem_desc_sw128(q_slot(0), kTileBytes, 1024), ddo0t = smem_desc_sw128(do_slot(0), kTileBytes, 1024);
+    struct Cursor { int r, i, n, u; };             // item i of n in the u-th unit that has any; n = 0: no more
+    auto advance = [&](Cursor& c) {
+      if (++c.i < c.n) return;
+      c.i = 0;
+      c.n = 0;
+      ++c.u;
+      for (;;) {
+        const int w = unit_at(++c.r);
+        if (w >= n_units) return;
+        c.n = warp_uniform(unit_of(w).n_q) * p.G;
+        if (c.n > 0) return;
       }
-      ++u;
+    };
+    auto slot = [&](uint64_t d, int it) { return desc_advance(d, (uint32_t)(it % kStages) * 2 * kOperand); };
+    auto issue_s = [&](const Cursor& c, int it) {
+      if (c.i == 0) mbar_wait(smem_u32(&sm->k_full), c.u & 1, status, kErrDkvMma);
+      mbar_wait(smem_u32(&sm->q_full[it % kStages]), (it / kStages) & 1, status, kErrDkvMma);
+      tc_fence_after();
+      const uint64_t dq = slot(dq0, it);
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < kD / 16; ++kk)
+          mma_f16_ss(tmem_s, desc_advance(dk0, kmajor_step(kk, kTileBytes)), desc_advance(dq, kmajor_step(kk, kTileBytes)), idesc_s, kk > 0);
+        mma_commit(smem_u32(&sm->s_full));
+        if (c.i == c.n - 1) mma_commit(smem_u32(&sm->k_empty));
+      }
+    };
+    auto issue_dp = [&](const Cursor& c, int it) {
+      if (c.i == 0) mbar_wait(smem_u32(&sm->v_full), c.u & 1, status, kErrDkvMma);
+      mbar_wait(smem_u32(&sm->do_full[it % kStages]), (it / kStages) & 1, status, kErrDkvMma);
+      tc_fence_after();
+      const uint64_t ddo = slot(ddo0, it);
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < kD / 16; ++kk)
+          mma_f16_ss(tmem_dp, desc_advance(dv0, kmajor_step(kk, kTileBytes)), desc_advance(ddo, kmajor_step(kk, kTileBytes)), idesc_s, kk > 0);
+        mma_commit(smem_u32(&sm->dp_full));
+        if (c.i == c.n - 1) mma_commit(smem_u32(&sm->v_empty));
+      }
+    };
+    Cursor now = {-1, 0, 0, -1};
+    advance(now);
+    if (now.n > 0) {
+      issue_s(now, 0);
+      issue_dp(now, 0);
     }
-    __syncwarp();
-  } else if (warp == kBwdWarps + 2) {
-    // ------------------------------------------------------------------ dV += P^T dO and dK += dS^T Q, A from TMEM
-    constexpr uint32_t fmt = kBf16 ? 1u : 0u;
-    constexpr uint32_t idesc_t = instr_desc_f16(fmt, 128, kD, 0, 1);
-    const uint64_t dq0t = smem_desc_sw128(q_slot(0), kTileBytes, 1024);
-    const uint64_t ddo0t = smem_desc_sw128(do_slot(0), kTileBytes, 1024);
-    int it = 0, u = 0;
-    for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
-      const int n_items = warp_uniform(unit_of(w).n_q) * p.G;
-      if (n_items == 0) continue;
-      for (int i = 0; i < n_items; ++i, ++it) {
-        const int s = it % kStages;
-        const uint64_t ddot = desc_advance(ddo0t, (uint32_t)s * 2 * kOperand), dqt = desc_advance(dq0t, (uint32_t)s * 2 * kOperand);
-        mbar_wait(smem_u32(&sm->do_full[s]), (it / kStages) & 1, status, kErrDkvMma);      // P may be there first
-        if (i == 0) mbar_wait(smem_u32(&sm->acc_empty[0]), (u & 1) ^ 1, status, kErrDkvMma);
-        mbar_wait(smem_u32(&sm->p_ready), it & 1, status, kErrDkvMma);
-        tc_fence_after();
-        if (elect_one()) {
+    for (int it = 0; now.n > 0; ++it) {
+      const int s = it % kStages;
+      Cursor next = now;
+      advance(next);
+      if (now.i == 0) mbar_wait(smem_u32(&sm->acc_empty[0]), (now.u & 1) ^ 1, status, kErrDkvMma);
+      mbar_wait(smem_u32(&sm->p_ready), it & 1, status, kErrDkvMma);
+      tc_fence_after();
+      const uint64_t ddot = slot(ddo0t, it), dqt = slot(dq0t, it);
+      if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kQTile / 16; ++kk)
-            mma_f16_ts(tmem_dv, tmem_s + a_step(kk), desc_advance(ddot, kk * 2048), idesc_t, (i > 0 || kk > 0) ? 1u : 0u);
-          mma_commit(smem_u32(&sm->s_free));
-          mma_commit(smem_u32(&sm->do_empty[s]));
-          if (i == n_items - 1) mma_commit(smem_u32(&sm->acc_full[0]));
-        }
-        if (i == 0) mbar_wait(smem_u32(&sm->acc_empty[1]), (u & 1) ^ 1, status, kErrDkvMma);
-        mbar_wait(smem_u32(&sm->ds_ready), it & 1, status, kErrDkvMma);
-        tc_fence_after();
-        if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < kQTile / 16; ++kk)
-            mma_f16_ts(tmem_dk, tmem_dp + a_step(kk), desc_advance(dqt, kk * 2048), idesc_t, (i > 0 || kk > 0) ? 1u : 0u);
-          mma_commit(smem_u32(&sm->dp_free));
-          mma_commit(smem_u32(&sm->q_empty[s]));
-          if (i == n_items - 1) mma_commit(smem_u32(&sm->acc_full[1]));
-        }
+        for (int kk = 0; kk < kQTile / 16; ++kk)
+          mma_f16_ts(tmem_dv, tmem_s + a_step(kk), desc_advance(ddot, kk * 2048), idesc_t, (now.i > 0 || kk > 0) ? 1u : 0u);
+        mma_commit(smem_u32(&sm->do_empty[s]));
+        if (now.i == now.n - 1) mma_commit(smem_u32(&sm->acc_full[0]));
       }
-      ++u;
+      if (next.n > 0) issue_s(next, it + 1);
+      if (now.i == 0) mbar_wait(smem_u32(&sm->acc_empty[1]), (now.u & 1) ^ 1, status, kErrDkvMma);
+      mbar_wait(smem_u32(&sm->ds_ready), it & 1, status, kErrDkvMma);
+      tc_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < kQTile / 16; ++kk)
+          mma_f16_ts(tmem_dk, tmem_dp + a_step(kk), desc_advance(dqt, kk * 2048), idesc_t, (now.i > 0 || kk > 0) ? 1u : 0u);
+        mma_commit(smem_u32(&sm->q_empty[s]));
+        if (now.i == now.n - 1) mma_commit(smem_u32(&sm->acc_full[1]));
+      }
+      if (next.n > 0) issue_dp(next, it + 1);
+      now = next;
     }
     __syncwarp();
   } else {
@@ -807,7 +813,7 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
 // ---------------------------------------------------------------------------------------------- backward: dQ
 constexpr int kDqStages = 4;
 constexpr int kSdpBufs = 2;                         // S / dP buffers in TMEM
-constexpr int kDqThreads = (kBwdWarps + 4) * 32;    // S and dP are issued by warps of their own
+constexpr int kDqThreads = (kBwdWarps + 2) * 32;
 
 struct DqSmem {
   uint64_t qdo_full, patch;
@@ -816,7 +822,7 @@ struct DqSmem {
   uint64_t delta_read;      // the softmax warpgroups are done with the Q, dO and O tiles in shared memory
   uint64_t full[kDqStages], empty[kDqStages];
   uint64_t s_full[kSdpBufs], s_free[kSdpBufs], dp_full[kSdpBufs];
-  uint64_t ds_ready[kSdpBufs], dp_free[kSdpBufs];      // dS has taken dP's place / dQ has read it
+  uint64_t ds_ready[kSdpBufs];                         // dS has taken dP's place
   uint64_t acc_full[2];     // per draining pair of warpgroups (the one that took the unit's last item)
   uint64_t acc_empty;
   uint32_t tmem_base;
@@ -868,7 +874,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   if (tid == 0) {
     for (uint64_t* bar : {&sm->qdo_full, &sm->patch}) mbar_init(smem_u32(bar), 1);
     mbar_init(smem_u32(&sm->ops_ready), kBwdWarps * 32);
-    mbar_init(smem_u32(&sm->ops_free), 2);          // the S issuer and the dP issuer
+    mbar_init(smem_u32(&sm->ops_free), 1);
     mbar_init(smem_u32(&sm->delta_read), kBwdWarps * 32);
     for (int s = 0; s < kDqStages; ++s) {
       mbar_init(smem_u32(&sm->full[s]), 1);
@@ -879,7 +885,6 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       mbar_init(smem_u32(&sm->s_full[s]), 1);
       mbar_init(smem_u32(&sm->s_free[s]), 256);
       mbar_init(smem_u32(&sm->dp_full[s]), 1);
-      mbar_init(smem_u32(&sm->dp_free[s]), 1);
     }
     mbar_init(smem_u32(&sm->acc_full[0]), 1);
     mbar_init(smem_u32(&sm->acc_full[1]), 1);
@@ -932,60 +937,78 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       }
     }
     __syncwarp();
-  } else if (warp == kBwdWarps + 1 || warp == kBwdWarps + 3) {
-    // ------------------------------------------------------------------ S = Q K^T (warp +1), dP = dO V^T (warp +3)
+  } else if (warp == kBwdWarps + 1) {
+    // ------------------------------------------------------------------ all three products, two items ahead with S and dP
+    // One warp issues them: dP of item i + 2 right behind dQ of item i, which reads the dS that stands in its place (see the dK/dV kernel).
     constexpr uint32_t fmt = kBf16 ? 1u : 0u;
-    constexpr uint32_t idesc_s = instr_desc_f16(fmt, 128, 64, 0, 0);
-    const bool is_s = warp == kBwdWarps + 1;
-    const uint64_t db0 = smem_desc_sw128(is_s ? k_slot(0) : v_slot(0), 16, 1024);
-    const uint32_t t_out = is_s ? tmem_s : tmem_dp, t_a = is_s ? tmem_q : tmem_do;
-    int it = 0, u = 0;
-    for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
-      const int total = warp_uniform(unit_of(w).total);
-      if (total == 0) continue;
-      for (int i = 0; i < total; ++i, ++it) {
-        const int s = it % kDqStages, sb = it % kSdpBufs;
-        mbar_wait(smem_u32(&sm->full[s]), (it / kDqStages) & 1, status, kErrDqMma);
-        if (it >= kSdpBufs) mbar_wait(smem_u32(is_s ? &sm->s_free[sb] : &sm->dp_free[sb]), ((it / kSdpBufs) & 1) ^ 1, status, kErrDqMma);
-        if (i == 0) mbar_wait(smem_u32(&sm->ops_ready), u & 1, status, kErrDqMma);
-        tc_fence_after();
-        const uint64_t db = desc_advance(db0, (uint32_t)s * 32768u);
-        if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < kD / 16; ++kk)      // A from TMEM: 8 columns = 16 features per K-step
-            mma_f16_ts(t_out + sb * 64, t_a + kk * 8, desc_advance(db, kmajor_step(kk, kHalfTile)), idesc_s, kk > 0);
-          mma_commit(smem_u32(is_s ? &sm->s_full[sb] : &sm->dp_full[sb]));
+    constexpr uint32_t idesc_s = instr_desc_f16(fmt, 128, 64, 0, 0), idesc_q = instr_desc_f16(fmt, 128, kD, 0, 1);
+    const uint64_t dk0 = smem_desc_sw128(k_slot(0), 16, 1024), dv0 = smem_desc_sw128(v_slot(0), 16, 1024);
+    const uint64_t dk0t = smem_desc_sw128(k_slot(0), kHalfTile, 1024);
+    int r = -1, u = -1;
+    auto next_unit = [&]() {                       // items of the next unit that has any, 0: no more
+      for (;;) {
+        const int w = unit_at(++r);
+        if (w >= n_units) return 0;
+        const int n = warp_uniform(unit_of(w).total);
+        if (n > 0) {
+          ++u;
+          return n;
         }
       }
-      if (elect_one()) mma_commit(smem_u32(&sm->ops_free));        // the next unit's Q / dO rows may be written
-      ++u;
-    }
-    __syncwarp();
-  } else if (warp == kBwdWarps + 2) {
-    // ------------------------------------------------------------------ dQ += dS K
-    constexpr uint32_t fmt = kBf16 ? 1u : 0u;
-    constexpr uint32_t idesc_q = instr_desc_f16(fmt, 128, kD, 0, 1);
-    const uint64_t dk0t = smem_desc_sw128(k_slot(0), kHalfTile, 1024);
-    int it = 0, u = 0;
-    for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
-      const int total = warp_uniform(unit_of(w).total);
-      if (total == 0) continue;
-      for (int i = 0; i < total; ++i, ++it) {
-        const int s = it % kDqStages, sb = it % kSdpBufs;
+    };
+    auto slot = [&](uint64_t d, int it) { return desc_advance(d, (uint32_t)(it % kDqStages) * 32768u); };
+    auto issue_s = [&](bool first, int it) {
+      const int sb = it % kSdpBufs;
+      mbar_wait(smem_u32(&sm->full[it % kDqStages]), (it / kDqStages) & 1, status, kErrDqMma);
+      if (it >= kSdpBufs) mbar_wait(smem_u32(&sm->s_free[sb]), ((it / kSdpBufs) & 1) ^ 1, status, kErrDqMma);
+      if (first) mbar_wait(smem_u32(&sm->ops_ready), u & 1, status, kErrDqMma);
+      tc_fence_after();
+      const uint64_t db = slot(dk0, it);
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < kD / 16; ++kk)      // A from TMEM: 8 columns = 16 features per K-step
+          mma_f16_ts(tmem_s + sb * 64, tmem_q + kk * 8, desc_advance(db, kmajor_step(kk, kHalfTile)), idesc_s, kk > 0);
+        mma_commit(smem_u32(&sm->s_full[sb]));
+      }
+    };
+    auto issue_dp = [&](bool last, int it) {
+      const int sb = it % kSdpBufs;
+      const uint64_t db = slot(dv0, it);
+      if (elect_one()) {
+#pragma unroll
+        for (int kk = 0; kk < kD / 16; ++kk)
+          mma_f16_ts(tmem_dp + sb * 64, tmem_do + kk * 8, desc_advance(db, kmajor_step(kk, kHalfTile)), idesc_s, kk > 0);
+        mma_commit(smem_u32(&sm->dp_full[sb]));
+        if (last) mma_commit(smem_u32(&sm->ops_free));        // the next unit's Q / dO rows may be written
+      }
+    };
+    // A unit's first two items are issued behind the last dQ of the unit before: its rows come to TMEM only when the softmax warps are
+    // through with that one's items.
+    int it = 0;
+    for (int n = next_unit(); n > 0;) {
+      for (int i = 0; i < min(n, kSdpBufs); ++i) {
+        issue_s(i == 0, it + i);
+        issue_dp(i == n - 1, it + i);
+      }
+      for (int i = 0; i < n; ++i, ++it) {
+        const int sb = it % kSdpBufs;
+        const bool more = i + kSdpBufs < n;
+        if (more) issue_s(false, it + kSdpBufs);
         if (i == 0) mbar_wait(smem_u32(&sm->acc_empty), (u & 1) ^ 1, status, kErrDqMma);
         mbar_wait(smem_u32(&sm->ds_ready[sb]), (it / kSdpBufs) & 1, status, kErrDqMma);
         tc_fence_after();
-        const uint64_t dkt = desc_advance(dk0t, (uint32_t)s * 32768u);
+        const uint64_t dkt = slot(dk0t, it);
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < kBlk / 16; ++kk)
-            mma_f16_ts(tmem_dq, tmem_dp + sb * 64 + (kk >> 1) * kCols + (kk & 1) * 8, desc_advance(dkt, kk * 2048), idesc_q, (i > 0 || kk > 0) ? 1u : 0u);
-          mma_commit(smem_u32(&sm->dp_free[sb]));                  // dS has been read: the buffer may take the next dP
-          mma_commit(smem_u32(&sm->empty[s]));
+            mma_f16_ts(tmem_dq, tmem_dp + sb * 64 + (kk >> 1) * kCols + (kk & 1) * 8, desc_advance(dkt, kk * 2048), idesc_q,
+                       (i > 0 || kk > 0) ? 1u : 0u);
+          mma_commit(smem_u32(&sm->empty[it % kDqStages]));
+          if (i == n - 1) mma_commit(smem_u32(&sm->acc_full[it & 1]));     // drained by the pair that took the last item
         }
+        if (more) issue_dp(i + kSdpBufs == n - 1, it + kSdpBufs);
       }
-      if (elect_one()) mma_commit(smem_u32(&sm->acc_full[(it - 1) & 1]));     // drained by the warpgroup that took the last item
-      ++u;
+      n = next_unit();
     }
     __syncwarp();
   } else {
