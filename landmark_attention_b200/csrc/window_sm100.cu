@@ -384,13 +384,35 @@ constexpr int kCols = 32;                           // columns of a score tile t
 // one pair of exponentials in this many is a cubic (7.5e-5, below half a step of either type); full tiles only
 constexpr int kBwdPolyEvery = 4;
 
-// TMEM columns -> 16 packed pairs
+// 32 TMEM columns of the thread's lane -> 16 packed pairs
 __device__ __forceinline__ void load_pairs(uint64_t (&x)[kCols / 2], uint32_t taddr) {
   uint32_t r[kCols];
   tmem_ld_32x32b_x32(taddr, r);
   tmem_ld_wait();
 #pragma unroll
   for (int j = 0; j < kCols / 2; ++j) x[j] = pk2u(r[2 * j], r[2 * j + 1]);
+}
+// The same 32 x 32 part of a score tile as fragments: x[h][2 j + e] is row 16 h + 8 e + lane / 4, columns 8 j + 2 (lane % 4) and the next.
+__device__ __forceinline__ void load_fragments(uint64_t (&x)[2][8], uint32_t taddr) {
+  uint32_t a[16], b[16];
+  tmem_ld_16x256b_x4(taddr, a);
+  tmem_ld_16x256b_x4(taddr + (16u << 16), b);
+  tmem_ld_wait();
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    x[0][k] = pk2u(a[2 * k], a[2 * k + 1]);
+    x[1][k] = pk2u(b[2 * k], b[2 * k + 1]);
+  }
+}
+__device__ __forceinline__ void store_fragments(const uint32_t (&w)[2][8], uint32_t taddr) {
+  tmem_st_16x128b_x4(taddr, w[0]);
+  tmem_st_16x128b_x4(taddr + (16u << 16), w[1]);
+  tmem_st_wait();
+}
+__device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
+  float a, b;
+  upk2(x, a, b);
+  return pk2(ex2(a), ex2(b));
 }
 // x: scores -> weights 2^(s c + nl), nl = -lse, of pair j given by nl(j); hidden columns become 0 (kind 1)
 template <typename NegLse, typename Sees>
@@ -437,7 +459,8 @@ __device__ __forceinline__ void dscores_of(uint32_t (&w)[kCols / 2], const uint6
 // item (K and V as A operands, Q and dO twice as B, their loads), as long as the products take: 2048 clk each.
 // TMEM: 128 S + 128 dP + kD dV + kD dK columns.  The softmax threads and the products take turns: while P^T of an item is made, dK of the
 // item before and dP of this one run; while dS^T is made, dV and the next S.  Row statistics are per column here: the loading
-// warp lays them out in shared memory, and a warp reads four at a time by broadcast.
+// warp lays them out in shared memory, and the score tiles are read as fragments, whose threads need eight columns' values and not 32: with a
+// column a register 128 KB of broadcasts an item competed with the operands (3550 -> 3300 us at B1 H32 Hkv8 L32768, window 4096).
 constexpr int kPair = 128;                          // keys of a unit
 constexpr int kDkvThreads = (kBwdWarps + 2) * 32;
 constexpr int kDkvStages = 2;
@@ -616,7 +639,7 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     // ------------------------------------------------------------------ all four products, A of dV and dK from TMEM
     // One warp issues them: S of the next item right behind dV, which reads the P that stands in its place, and dP right behind dK.
     // The tensor core works through what one thread issues in order, so neither waits for the other's end; with two issuing
-    // warps and barriers between them an item took 3400 clk instead of KKKK, most of it the way from a product's end to the next one's start.
+  XX
     constexpr uint32_t fmt = kBf16 ? 1u : 0u;
     constexpr uint32_t idesc_s = instr_desc_f16(fmt, 128, 128, 0, 0), idesc_t = instr_desc_f16(fmt, 128, kD, 0, 1);
     const uint64_t dk0 = smem_desc_sw128(k_pair, 16, 1024), dv0 = smem_desc_sw128(v_pair, 16, 1024);
@@ -728,44 +751,84 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         continue;
       }
       const int kmin = warp_uniform(un.pair * kPair + (warp & 3) * 32), kmax = kmin + 31;
-      const int last = key < p.sinks ? INT32_MAX / 2 : key + p.window;      // the key is seen from positions key .. last - 1
+      const int frow = kmin + (lane >> 2), fcol = 2 * (lane & 3);      // fragments: keys frow + 8 e, queries fcol + 8 j and the next
       for (int i = 0, tq = un.first; i < n_items; ++i, ++it) {
-        const int s = it % kStages, p0 = off + tq * kQTile + g * kCols;      // position of column 0
+        const int s = it % kStages, p0 = off + tq * kQTile + g * kCols, p1 = p0 + kCols - 1;      // positions of the columns
         if (++tq == un.first + un.n_q) tq = un.first;
-        const int first = key - p0, end = min(last, un.len) - p0;
-        auto sees = [&](int j) { return j >= first && j < end; };
-        const int p1 = p0 + kCols - 1;
-        const int kind = warp_uniform(p0 >= un.len || none_seen(p0, p1, kmin, kmax, p.window, p.sinks) ? 0
-                                      : p1 < un.len && all_seen(p0, p1, kmin, kmax, p.window, p.sinks) ? 2 : 1);
-        const ulonglong2* const nl = reinterpret_cast<const ulonglong2*>(&sm->nlse[s][g * kCols]);
-        const ulonglong2* const nd = reinterpret_cast<const ulonglong2*>(&sm->ndelta[s][g * kCols]);
+        const int kind = p0 >= un.len || none_seen(p0, p1, kmin, kmax, p.window, p.sinks) ? 0
+                         : p1 < un.len && all_seen(p0, p1, kmin, kmax, p.window, p.sinks) ? 2 : 1;
+        const uint64_t* const nl = reinterpret_cast<const uint64_t*>(&sm->nlse[s][g * kCols + fcol]);
+        const uint64_t* const nd = reinterpret_cast<const uint64_t*>(&sm->ndelta[s][g * kCols + fcol]);
         mbar_wait(smem_u32(&sm->stat_full[s]), (it / kStages) & 1, status, kErrDkvSoftmax);
         mbar_wait(smem_u32(&sm->s_full), it & 1, status, kErrDkvSoftmax);
         tc_fence_after();
-        uint64_t sp[kCols / 2];
-        uint32_t wd[kCols / 2];
+        uint64_t sp[2][8];                         // [16 lanes][pair 2 j + e]
+        uint32_t wd[2][8];
         if (kind != 0) {
-          load_pairs(sp, ts);
-          weights_of(sp, kind, p.scale_log2, [&](int j) { const ulonglong2 x = nl[j >> 1]; return (uint64_t)(j & 1 ? x.y : x.x); }, sees);
+          load_fragments(sp, ts);
+          uint64_t l2[4];
 #pragma unroll
-          for (int j = 0; j < kCols / 2; ++j) wd[j] = pack2p<kBf16>(sp[j]);
+          for (int j = 0; j < 4; ++j) l2[j] = nl[4 * j];
+          const uint64_t c2 = pk2(p.scale_log2, p.scale_log2);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sp[h][k] = fma2(sp[h][k], c2, l2[k >> 1]);
+          if (kind == 2) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int k = 0; k < 8; ++k) sp[h][k] = k % kBwdPolyEvery == 1 ? ex2_poly2<3>(sp[h][k]) : ex2_pair(sp[h][k]);
+          } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int key_r = frow + 16 * h + 8 * e, first = key_r - p0 - fcol;       // the key is seen from columns first .. end - 1
+                const int end = min(key_r < p.sinks ? INT32_MAX / 2 : key_r + p.window, un.len) - p0 - fcol;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  float x, y;
+                  upk2(sp[h][2 * j + e], x, y);
+                  sp[h][2 * j + e] = pk2(8 * j >= first && 8 * j < end ? ex2(x) : 0.f, 8 * j + 1 >= first && 8 * j + 1 < end ? ex2(y) : 0.f);
+                }
+              }
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) wd[h][k] = pack2p<kBf16>(sp[h][k]);
         } else {
 #pragma unroll
-          for (int j = 0; j < kCols / 2; ++j) wd[j] = 0u;
+          for (int k = 0; k < 8; ++k) wd[0][k] = wd[1][k] = 0u;
         }
-        tmem_st_32x32b_x16(ts, wd);
-        tmem_st_wait();
+        store_fragments(wd, ts);
         tc_fence_before();
         mbar_arrive(smem_u32(&sm->p_ready));
         mbar_wait(smem_u32(&sm->dp_full), it & 1, status, kErrDkvSoftmax);
         tc_fence_after();
         if (kind != 0) {
-          uint64_t dp[kCols / 2];
-          load_pairs(dp, tdp);
-          dscores_of<kBf16>(wd, sp, dp, kind, p.scale, [&](int j) { const ulonglong2 x = nd[j >> 1]; return (uint64_t)(j & 1 ? x.y : x.x); }, sees);
+          uint64_t dp[2][8];
+          load_fragments(dp, tdp);
+          uint64_t d2[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) d2[j] = nd[4 * j];
+          const uint64_t s2 = pk2(p.scale, p.scale);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              uint64_t x = mul2(sp[h][k], fma2(dp[h][k], s2, d2[k >> 1]));
+              if (kind == 1) {                     // a key behind the end may hold anything: dropped, not multiplied by 0
+                float x0, x1, w0, w1;
+                upk2(x, x0, x1);
+                upk2(sp[h][k], w0, w1);
+                x = pk2(w0 == 0.f ? 0.f : x0, w1 == 0.f ? 0.f : x1);
+              }
+              wd[h][k] = pack2p<kBf16>(x);
+            }
         }
-        tmem_st_32x32b_x16(tdp, wd);               // (kind 0: still zeros)
-        tmem_st_wait();
+        store_fragments(wd, tdp);                  // (kind 0: still zeros)
         tc_fence_before();
         mbar_arrive(smem_u32(&sm->ds_ready));
       }
