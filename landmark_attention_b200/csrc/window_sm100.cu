@@ -639,7 +639,7 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     // ------------------------------------------------------------------ all four products, A of dV and dK from TMEM
     // One warp issues them: S of the next item right behind dV, which reads the P that stands in its place, and dP right behind dK.
     // The tensor core works through what one thread issues in order, so neither waits for the other's end; with two issuing
-  XX
+    // warps and barriers between them an item's time was mostly the way from a product's end to the next one's start.
     constexpr uint32_t fmt = kBf16 ? 1u : 0u;
     constexpr uint32_t idesc_s = instr_desc_f16(fmt, 128, 128, 0, 0), idesc_t = instr_desc_f16(fmt, 128, kD, 0, 1);
     const uint64_t dk0 = smem_desc_sw128(k_pair, 16, 1024), dv0 = smem_desc_sw128(v_pair, 16, 1024);
