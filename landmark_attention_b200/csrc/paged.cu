@@ -78,30 +78,24 @@ struct AttendArgs {
   float2* whole;                       // [items][16] of items in one piece (weights only)
   float* scores;                       // [B, Hkv, rows, capacity] in units of log2 (weights only)
   int H, T, G, rows, tiles, window, sinks, grid, least;
+  bool one_piece;                      // every row is one CTA's: CTAs take items instead of lengths of the line
   float scale_log2;
 };
 
-// Where a piece of work lies: all sequences' steps in one line.
-struct Line {
-  int64_t total;                       // steps of all items
-  int64_t piece;                       // steps a CTA takes
-};
-// Sum of f(b) over all sequences, and over those before `b` or up to the one that holds step `at`.  Whole warp.
-struct Found { int b; int64_t before; };
-
+// All sequences' steps lie in one line; a CTA takes `piece` of them.  The sums over the sequences are worked out by whole warps.
 template <typename F>
-__device__ __forceinline__ int64_t warp_total(int B, F f) {
+__device__ __forceinline__ int64_t warp_total(int B, F f) {      // sum of f(b) over b < B
   int64_t sum = 0;
   for (int b = threadIdx.x & 31; b < B; b += 32) sum += f(b);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return sum;
 }
+struct Found { int b; int64_t before; };
 template <typename F>
-__device__ __forceinline__ Found warp_find(int B, int64_t at, F f) {      // the last b whose steps begin at or before `at`
+__device__ __forceinline__ Found warp_find(int B, int64_t at, F f) {      // the sequence that holds step `at`, and the steps in front of it
   const int lane = threadIdx.x & 31;
   int64_t before = 0;
-  Found r{B, 0};
   for (int b0 = 0; b0 < B; b0 += 32) {
     const int64_t n = b0 + lane < B ? f(b0 + lane) : 0;
     int64_t inc = n;
@@ -113,26 +107,13 @@ __device__ __forceinline__ Found warp_find(int B, int64_t at, F f) {      // the
     const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && before + inc > at);
     if (hit) {
       const int src = __ffs((int)hit) - 1;
-      r.b = b0 + src;
-      r.before = __shfl_sync(0xffffffffu, before + inc - n, src);
-      return r;
+      return {b0 + src, __shfl_sync(0xffffffffu, before + inc - n, src)};
     }
     before += __shfl_sync(0xffffffffu, inc, 31);
   }
-  r.before = before;
-  return r;
+  return {B, before};
 }
-template <typename F>
-__device__ __forceinline__ int64_t warp_before(int B, int b, F f) {
-  return warp_total(b < B ? b : B, f);
-}
-
-__device__ __forceinline__ Line line_of(const AttendArgs& a, int64_t total) {
-  Line l;
-  l.total = total;
-  l.piece = max((total + a.grid - 1) / a.grid, (int64_t)a.least);
-  return l;
-}
+__device__ __forceinline__ int64_t piece_of(const AttendArgs& a, int64_t total) { return max((total + a.grid - 1) / a.grid, (int64_t)a.least); }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
   const int bytes = take ? 16 : 0;     // 0: filled with zeros, src is not read
@@ -263,19 +244,15 @@ __device__ __forceinline__ void take_step(Rows16<T, kD>& w, const uint8_t* stage
   }
 }
 
-// A warp's result of a piece in its own part of shared memory: [16][kD] floats, then 16 maxima and 16 sums
-template <int kD> constexpr int kResultFloats = kRowTile * kD + 2 * kRowTile;
+// A warp's unnormalised outputs as [16][kD] floats, and its maxima and sums
 template <typename T, int kD>
-__device__ __forceinline__ void leave_result(Rows16<T, kD>& w, float* to) {
+__device__ __forceinline__ void leave_result(Rows16<T, kD>& w, float* to, float2* stat) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     w.l[e] += __shfl_xor_sync(0xffffffffu, w.l[e], 1);
     w.l[e] += __shfl_xor_sync(0xffffffffu, w.l[e], 2);
-    if (t4 == 0) {
-      to[kRowTile * kD + g + 8 * e] = w.m[e];
-      to[kRowTile * kD + kRowTile + g + 8 * e] = w.l[e];
-    }
+    if (t4 == 0) stat[g + 8 * e] = make_float2(w.m[e], w.l[e]);
 #pragma unroll
     for (int n = 0; n < kD / 8; ++n)
       *reinterpret_cast<float2*>(to + (g + 8 * e) * kD + n * 8 + 2 * t4) = make_float2(w.o[n][2 * e], w.o[n][2 * e + 1]);
@@ -291,69 +268,82 @@ template <int kD> struct Rows32 {
 template <typename T, int kD>
 __global__ void __launch_bounds__(kWarps * 32) paged_attend_kernel(const __grid_constant__ AttendArgs a) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  __shared__ int64_t s_total;
-  __shared__ Found s_found;
+  __shared__ float2 s_stat[kWarps][kRowTile];
   constexpr bool kF32 = std::is_same<T, float>::value;
   grid_dep_wait();
   grid_dep_launch();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Pages& pg = a.pg;
   const int per_seq = pg.Hkv * a.tiles;
-  auto steps_of = [&](int b) { return (int64_t)per_seq * span_of(pg.length(b), a.T, a.window, a.sinks).steps; };
-  if (warp == 0) {
-    const int64_t total = warp_total(pg.B, steps_of);
-    const Line line = line_of(a, total);
-    const Found f = warp_find(pg.B, blockIdx.x * line.piece, steps_of);
-    if (lane == 0) {
-      s_total = total;
-      s_found = f;
-    }
-  }
+  const int len_lane = lane < pg.B ? pg.length(lane) : 0;      // the first 32 lengths stay at hand
+  auto length = [&](int b) { return b < 32 ? __shfl_sync(0xffffffffu, len_lane, b) : pg.length(b); };      // (the same b in all lanes)
+  auto steps_of = [&](int b) { return (int64_t)per_seq * span_of(b < 32 ? len_lane : pg.length(b), a.T, a.window, a.sinks).steps; };
   // sequences without keys: their outputs are zeros (a share of the sequences for every CTA)
-  for (int b = blockIdx.x; b < pg.B; b += a.grid)
-    if (pg.length(b) == 0)
+  for (int b = blockIdx.x; b < pg.B; b += gridDim.x)
+    if (length(b) == 0)
       for (int64_t i = tid; i < (int64_t)a.H * a.T * pg.D; i += kWarps * 32) reinterpret_cast<T*>(a.o)[b * (int64_t)a.H * a.T * pg.D + i] = from_f32<T>(0.f);
-  __syncthreads();
-  const Line line = line_of(a, s_total);
-  const int64_t begin = blockIdx.x * line.piece, end = min(begin + line.piece, line.total);
-  if (begin >= end) return;
-  int b = s_found.b;
-  int64_t before = s_found.before;
-  Span sp = span_of(pg.length(b), a.T, a.window, a.sinks);
   uint8_t* ring = smem + warp * kStages * kStageBytes<T, kD>;
   const uint32_t ring_at = smem_u32(ring);
-  float* const result = reinterpret_cast<float*>(ring);
-  static_assert(kResultFloats<kD> * 4 <= kStages * kStageBytes<T, kD>, "a warp's result fits its ring");
+  static_assert(kRowTile * kD * 4 <= kStageBytes<T, kD>, "a warp's outputs fit a stage");
 
-  for (int64_t at = begin; at < end;) {
-    while (at >= before + (int64_t)per_seq * sp.steps) {      // the next sequence that has keys
-      before += (int64_t)per_seq * sp.steps;
-      ++b;
-      sp = span_of(pg.length(b), a.T, a.window, a.sinks);
+  // A place in the line, moved on by whole warps.
+  struct Place {
+    int b, item, step;
+    Span sp;
+  };
+  auto settle = [&](Place& p) {                      // `step` may lie behind the item's end
+    while (p.step >= p.sp.steps) {
+      p.step -= p.sp.steps;
+      if (++p.item < per_seq) continue;
+      p.item = 0;
+      do {                                           // the next sequence that has keys
+        if (++p.b >= pg.B) return;                   // behind the last one: nothing is taken from there
+        p.sp = span_of(length(p.b), a.T, a.window, a.sinks);
+      } while (p.sp.steps == 0);
     }
-    const int item = (int)((at - before) / sp.steps), step0 = (int)((at - before) - (int64_t)item * sp.steps);
-    const int h = item / a.tiles, row0 = (item - h * a.tiles) * kRowTile;
-    const int count = (int)min((int64_t)(sp.steps - step0), end - at);
-    const int mine = (count - warp + kWarps - 1) / kWarps;     // steps step0 + warp, + kWarps, ...
-    const int p0 = sp.len - a.T;                               // position of the first token's queries
-    const int lo_seen = a.window > 0 && p0 >= a.window ? p0 - a.window + 1 : 0;
+  };
+  auto lo_seen = [&](int len) {                      // the first key that the first token's window holds
+    const int p0 = len - a.T;
+    return a.window > 0 && p0 >= a.window ? p0 - a.window + 1 : 0;
+  };
 
-    auto page_id = [&](int i) { return i < mine ? pg.id(b, sp.key(step0 + warp + i * kWarps) >> pg.shift) : 0; };
-    auto issue = [&](int i, int id) {
+  const int64_t cap = (int64_t)pg.max_pages << pg.shift;
+
+  // The steps begin .. end - 1 of the line, of which `now` is the first.
+  auto take = [&](int64_t begin, int64_t end, Place now) {
+    // Loads run ahead of the steps that use them, also into the next item: first the page's number, a step later its rows.
+    const int mine = (int)((end - begin - warp + kWarps - 1) / kWarps);      // this warp's steps: begin + warp, + kWarps, ...
+    Place ask = now;
+    ask.step += warp;
+    settle(ask);
+    struct Asked { int b, h, key0, len, id; } next;
+    unsigned bad = 0;                                  // bit i % kStages: the step in that stage has no page
+    auto ask_page = [&](int i) {
+      if (i >= mine) return;
+      next.b = ask.b;
+      next.h = ask.item / a.tiles;
+      next.key0 = ask.sp.key(ask.step);
+      next.len = ask.sp.len;
+      next.id = pg.id(next.b, next.key0 >> pg.shift);
+      ask.step += kWarps;
+      settle(ask);
+    };
+    auto issue = [&](int i) {
       if (i < mine) {
-        const int key0 = sp.key(step0 + warp + i * kWarps);
-        const bool ok = id >= 0 && id < pg.n_pages;
+        const bool ok = next.id >= 0 && next.id < pg.n_pages;
         if (!ok && lane == 0) note(pg.status, kBadPage);
-        const int row = key0 & (pg.page - 1);
-        const T* kp = reinterpret_cast<const T*>(pg.k) + (ok ? (int64_t)id * pg.ks[0] + h * pg.ks[1] + (int64_t)row * pg.ks[2] : 0);
-        const T* vp = reinterpret_cast<const T*>(pg.v) + (ok ? (int64_t)id * pg.vs[0] + h * pg.vs[1] + (int64_t)row * pg.vs[2] : 0);
+        const unsigned bit = 1u << (i % kStages);
+        bad = ok ? bad & ~bit : bad | bit;
+        const int row = next.key0 & (pg.page - 1), lo = lo_seen(next.len);
+        const T* kp = reinterpret_cast<const T*>(pg.k) + (ok ? (int64_t)next.id * pg.ks[0] + next.h * pg.ks[1] + (int64_t)row * pg.ks[2] : 0);
+        const T* vp = reinterpret_cast<const T*>(pg.v) + (ok ? (int64_t)next.id * pg.vs[0] + next.h * pg.vs[1] + (int64_t)row * pg.vs[2] : 0);
         const uint32_t to = ring_at + (uint32_t)(i % kStages) * kStageBytes<T, kD>;
         constexpr int kChunks = kRowBytes<T, kD> / 16, kVec = 16 / (int)sizeof(T);
 #pragma unroll
         for (int e = 0; e < kStep * kChunks / 32; ++e) {
           const int r = (e * 32 + lane) / kChunks, c = (e * 32 + lane) % kChunks;
-          const int key = key0 + r;
-          const bool take = ok && key < sp.len && (key >= lo_seen || key < a.sinks) && c * kVec < pg.D;
+          const int key = next.key0 + r;
+          const bool take = ok && key < next.len && (key >= lo || key < a.sinks) && c * kVec < pg.D;
           const int64_t off_k = take ? (int64_t)r * pg.ks[2] + c * kVec : 0, off_v = take ? (int64_t)r * pg.vs[2] + c * kVec : 0;
           cp_async16(to + chunk_at<T, kD>(r, c), kp + off_k, take);
           cp_async16(to + kStep * kRowBytes<T, kD> + chunk_at<T, kD>(r, c), vp + off_v, take);
@@ -361,348 +351,350 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attend_kernel(const __grid_
       }
       cp_async_commit();
     };
-
-    // ids run ahead of the loads that need them
-    int ids[kStages];
-#pragma unroll
-    for (int i = 0; i < kStages; ++i) ids[i] = page_id(i);
-    unsigned bad = 0;                                          // bit i % kStages: the step in that stage has no page
-    auto mark = [&](int i, int id) {
-      const unsigned bit = 1u << (i % kStages);
-      bad = (id >= 0 && id < pg.n_pages) ? bad & ~bit : bad | bit;
-    };
-    __syncwarp();
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) {
-      issue(i, ids[i]);
-      mark(i, ids[i]);
+      ask_page(i);
+      issue(i);
     }
-    int next = ids[kStages - 1];
-    const int64_t score_row = ((int64_t)b * pg.Hkv + h) * a.rows;
-    const int64_t cap = (int64_t)pg.max_pages << pg.shift;
+    ask_page(kStages - 1);
 
-    if constexpr (!kF32) {
-      Rows16<T, kD> w;
-      load_queries<T, kD>(w, a, b, h, row0);
-      int pos[2];
+    int i = 0;                                         // this warp's steps that are done; stage (i + kStages - 1) % kStages is free
+    for (int64_t at = begin; at < end;) {
+      const Span sp = now.sp;
+      const int b = now.b, step0 = now.step, h = now.item / a.tiles, row0 = (now.item - h * a.tiles) * kRowTile;
+      const int count = (int)min((int64_t)(sp.steps - step0), end - at);
+      const int p0 = sp.len - a.T;                               // position of the first token's queries
+      const int first = (int)((warp - (at - begin)) & (kWarps - 1));
+      const int64_t score_row = ((int64_t)b * pg.Hkv + h) * a.rows;
+      // every row that exists sees all 16 keys (the last token's window is the one that has moved on furthest)
+      auto all_see = [&](int key0, bool no_page) {
+        return !no_page && p0 >= 0 && key0 + kStep - 1 <= p0 && (a.window == 0 || p0 + a.T - 1 - key0 < a.window);
+      };
+
+      if constexpr (!kF32) {
+        Rows16<T, kD> w;
+        load_queries<T, kD>(w, a, b, h, row0);
+        int pos[2];
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = row0 + (lane >> 2) + 8 * e;
-        pos[e] = r < a.rows ? p0 + r % a.T : -1;
-      }
-      for (int i = 0; i < mine; ++i) {
-        cp_async_wait<kStages - 2>();
-        __syncwarp();
-        issue(i + kStages - 1, next);
-        const int id = next;
-        next = page_id(i + kStages);
-        const int key0 = sp.key(step0 + warp + i * kWarps);
-        const bool no_page = bad >> (i % kStages) & 1u;
-        mark(i + kStages - 1, id);
-        // every row that exists sees all 16 keys (the last row of the window is the one that has gone furthest)
-        const bool all = !no_page && p0 >= 0 && key0 + kStep - 1 <= p0 && (a.window == 0 || p0 + a.T - 1 - key0 < a.window);
-        take_step<T, kD>(w, ring + (i % kStages) * kStageBytes<T, kD>, a.scale_log2, all,
-            [&](int e, int j) {
-              const int key = key0 + j;
-              return !no_page && key <= pos[e] && (a.window == 0 || pos[e] - key < a.window || key < a.sinks);
-            },
-            [&](const float (&s)[2][4]) {
-              if (a.weights == nullptr) return;
-#pragma unroll
-              for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const int r = row0 + (lane >> 2) + 8 * e;
-                  if (r < a.rows)
-                    *reinterpret_cast<float2*>(a.scores + (score_row + r) * cap + key0 + 8 * n + 2 * (lane & 3)) =
-                        make_float2(s[n][2 * e], s[n][2 * e + 1]);
-                }
-            });
-      }
-      cp_async_wait<0>();
-      __syncwarp();
-      leave_result<T, kD>(w, result);
-    } else {
-      // fp32 on the FMA units.  Scores: lane = (key, half of the features); outputs: lane = kD / 32 features of every row.
-      Rows32<kD> w;
-      const int n_rows = min(kRowTile, a.rows - row0);
-      float* const qs = reinterpret_cast<float*>(smem + kAttendSmem<T, kD>);         // [16][kD], the CTA's query rows
-      float* const ps = qs + kRowTile * kD + warp * kRowTile * kStep;                // [16][16], the warp's weights
-      __syncthreads();                                                               // the piece before is done with the queries
-      for (int e = tid; e < kRowTile * kD; e += kWarps * 32) {
-        const int r = row0 + e / kD, c = e % kD;
-        qs[e] = r < a.rows && c < pg.D ? *(reinterpret_cast<const float*>(a.q) + b * a.qs[0] + (int64_t)(h * a.G + r / a.T) * a.qs[1] +
-                                           (int64_t)(r % a.T) * a.qs[2] + c) : 0.f;
-      }
-      __syncthreads();
-#pragma unroll
-      for (int r = 0; r < kRowTile; ++r) {
-        w.m[r] = -INFINITY;
-        w.l[r] = 0.f;
-#pragma unroll
-        for (int c = 0; c < kD / 32; ++c) w.o[r][c] = 0.f;
-      }
-      for (int i = 0; i < mine; ++i) {
-        cp_async_wait<kStages - 2>();
-        __syncwarp();
-        issue(i + kStages - 1, next);
-        const int id = next;
-        next = page_id(i + kStages);
-        const int key0 = sp.key(step0 + warp + i * kWarps);
-        const bool no_page = bad >> (i % kStages) & 1u;
-        mark(i + kStages - 1, id);
-        const uint8_t* stage = ring + (i % kStages) * kStageBytes<T, kD>;
-        const int j = lane & 15, half = lane >> 4;
-        float s[kRowTile];
-#pragma unroll
-        for (int r = 0; r < kRowTile; ++r) s[r] = 0.f;
-        for (int c = 0; c < kD / 8; ++c) {                   // the half's 16-byte chunks
-          const int chunk = half * (kD / 8) + c;
-          const float4 x = *reinterpret_cast<const float4*>(stage + chunk_at<T, kD>(j, chunk));
-#pragma unroll
-          for (int r = 0; r < kRowTile; ++r) {
-            if (r >= n_rows) break;
-            const float4 y = *reinterpret_cast<const float4*>(qs + r * kD + chunk * 4);
-            s[r] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s[r]))));
-          }
+        for (int e = 0; e < 2; ++e) {
+          const int r = row0 + (lane >> 2) + 8 * e;
+          pos[e] = r < a.rows ? p0 + r % a.T : -1;
         }
+        for (int k = first; k < count; k += kWarps, ++i) {
+          cp_async_wait<kStages - 2>();
+          __syncwarp();
+          const bool no_page = bad >> (i % kStages) & 1u;
+          issue(i + kStages - 1);
+          ask_page(i + kStages);
+          const int key0 = sp.key(step0 + k);
+          take_step<T, kD>(w, ring + (i % kStages) * kStageBytes<T, kD>, a.scale_log2, all_see(key0, no_page),
+              [&](int e, int j) {
+                const int key = key0 + j;
+                return !no_page && key <= pos[e] && (a.window == 0 || pos[e] - key < a.window || key < a.sinks);
+              },
+              [&](const float (&s)[2][4]) {
+                if (a.weights == nullptr) return;
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+#pragma unroll
+                  for (int e = 0; e < 2; ++e) {
+                    const int r = row0 + (lane >> 2) + 8 * e;
+                    if (r < a.rows)
+                      *reinterpret_cast<float2*>(a.scores + (score_row + r) * cap + key0 + 8 * n + 2 * (lane & 3)) =
+                          make_float2(s[n][2 * e], s[n][2 * e + 1]);
+                  }
+              });
+          __syncwarp();
+        }
+        leave_result<T, kD>(w, reinterpret_cast<float*>(ring + ((i + kStages - 1) % kStages) * kStageBytes<T, kD>), s_stat[warp]);
+      } else {
+        // fp32 on the FMA units.  Scores: lane = (key, half of the features); outputs: lane = kD / 32 features of every row.
+        Rows32<kD> w;
+        const int n_rows = min(kRowTile, a.rows - row0);
+        float* const qs = reinterpret_cast<float*>(smem + kAttendSmem<T, kD>);         // [16][kD], the CTA's query rows
+        float* const ps = qs + kRowTile * kD + warp * kRowTile * kStep;                // [16][16], the warp's weights
+        for (int e = tid; e < kRowTile * kD; e += kWarps * 32) {
+          const int r = row0 + e / kD, c = e % kD;
+          qs[e] = r < a.rows && c < pg.D ? *(reinterpret_cast<const float*>(a.q) + b * a.qs[0] + (int64_t)(h * a.G + r / a.T) * a.qs[1] +
+                                             (int64_t)(r % a.T) * a.qs[2] + c) : 0.f;
+        }
+        __syncthreads();
 #pragma unroll
         for (int r = 0; r < kRowTile; ++r) {
-          if (r >= n_rows) break;
-          float x = (s[r] + __shfl_xor_sync(0xffffffffu, s[r], 16)) * a.scale_log2;
-          const int pos = p0 + (row0 + r) % a.T, key = key0 + j;
-          if (no_page || key > pos || !(a.window == 0 || pos - key < a.window || key < a.sinks)) x = -INFINITY;
-          if (a.weights != nullptr && half == 0) a.scores[(score_row + row0 + r) * cap + key] = x;
-          float mx = x;
+          w.m[r] = -INFINITY;
+          w.l[r] = 0.f;
 #pragma unroll
-          for (int o = 8; o > 0; o >>= 1) {
-            const float y = __shfl_xor_sync(0xffffffffu, mx, o);
-            mx = max3_nan(mx, y, y);
-          }
-          mx = max3_nan(mx, w.m[r], w.m[r]);
-          const float shift = mx == -INFINITY ? 0.f : mx;
-          const float f = ex2(w.m[r] - shift);
-          w.m[r] = mx;
-          const float p = exp2f(x - shift);
-          w.l[r] = w.l[r] * f + (half == 0 ? p : 0.f);
-#pragma unroll
-          for (int c = 0; c < kD / 32; ++c) w.o[r][c] *= f;
-          if (half == 0) ps[r * kStep + j] = p;
+          for (int c = 0; c < kD / 32; ++c) w.o[r][c] = 0.f;
         }
-        __syncwarp();
-        const uint8_t* vs = stage + kStep * kRowBytes<T, kD>;
-        for (int k = 0; k < kStep; ++k) {
-          float v[kD / 32];
+        for (int k = first; k < count; k += kWarps, ++i) {
+          cp_async_wait<kStages - 2>();
+          __syncwarp();
+          const bool no_page = bad >> (i % kStages) & 1u;
+          issue(i + kStages - 1);
+          ask_page(i + kStages);
+          const int key0 = sp.key(step0 + k);
+          const uint8_t* stage = ring + (i % kStages) * kStageBytes<T, kD>;
+          const int j = lane & 15, half = lane >> 4;
+          float s[kRowTile];
 #pragma unroll
-          for (int c = 0; c < kD / 32; ++c) {
-            const int f = lane * (kD / 32) + c;
-            v[c] = *reinterpret_cast<const float*>(vs + chunk_at<T, kD>(k, f / 4) + (f % 4) * 4);
+          for (int r = 0; r < kRowTile; ++r) s[r] = 0.f;
+          for (int c = 0; c < kD / 8; ++c) {                   // the half's 16-byte chunks
+            const int chunk = half * (kD / 8) + c;
+            const float4 x = *reinterpret_cast<const float4*>(stage + chunk_at<T, kD>(j, chunk));
+#pragma unroll
+            for (int r = 0; r < kRowTile; ++r) {
+              if (r >= n_rows) break;
+              const float4 y = *reinterpret_cast<const float4*>(qs + r * kD + chunk * 4);
+              s[r] = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, s[r]))));
+            }
           }
 #pragma unroll
           for (int r = 0; r < kRowTile; ++r) {
             if (r >= n_rows) break;
-            const float p = ps[r * kStep + k];
+            float x = (s[r] + __shfl_xor_sync(0xffffffffu, s[r], 16)) * a.scale_log2;
+            const int pos = p0 + (row0 + r) % a.T, key = key0 + j;
+            if (no_page || key > pos || !(a.window == 0 || pos - key < a.window || key < a.sinks)) x = -INFINITY;
+            if (a.weights != nullptr && half == 0) a.scores[(score_row + row0 + r) * cap + key] = x;
+            float mx = x;
 #pragma unroll
-            for (int c = 0; c < kD / 32; ++c) w.o[r][c] = fmaf(p, v[c], w.o[r][c]);
+            for (int o = 8; o > 0; o >>= 1) {
+              const float y = __shfl_xor_sync(0xffffffffu, mx, o);
+              mx = max3_nan(mx, y, y);
+            }
+            mx = max3_nan(mx, w.m[r], w.m[r]);
+            const float shift = mx == -INFINITY ? 0.f : mx;
+            const float f = ex2(w.m[r] - shift);
+            w.m[r] = mx;
+            const float p = exp2f(x - shift);
+            w.l[r] = w.l[r] * f + (half == 0 ? p : 0.f);
+#pragma unroll
+            for (int c = 0; c < kD / 32; ++c) w.o[r][c] *= f;
+            if (half == 0) ps[r * kStep + j] = p;
           }
-        }
-        __syncwarp();
-      }
-      cp_async_wait<0>();
-      __syncwarp();
+          __syncwarp();
+          const uint8_t* vs = stage + kStep * kRowBytes<T, kD>;
+          for (int key = 0; key < kStep; ++key) {
+            float v[kD / 32];
 #pragma unroll
-      for (int r = 0; r < kRowTile; ++r) {
-        const float l = warp_sum(w.l[r]);
-        if (lane == 0) {
-          result[kRowTile * kD + r] = w.m[r];
-          result[kRowTile * kD + kRowTile + r] = l;
-        }
+            for (int c = 0; c < kD / 32; ++c) {
+              const int f = lane * (kD / 32) + c;
+              v[c] = *reinterpret_cast<const float*>(vs + chunk_at<T, kD>(key, f / 4) + (f % 4) * 4);
+            }
 #pragma unroll
-        for (int c = 0; c < kD / 32; ++c) result[r * kD + lane * (kD / 32) + c] = w.o[r][c];
+            for (int r = 0; r < kRowTile; ++r) {
+              if (r >= n_rows) break;
+              const float p = ps[r * kStep + key];
+#pragma unroll
+              for (int c = 0; c < kD / 32; ++c) w.o[r][c] = fmaf(p, v[c], w.o[r][c]);
+            }
+          }
+          __syncwarp();
+        }
+        float* const result = reinterpret_cast<float*>(ring + ((i + kStages - 1) % kStages) * kStageBytes<T, kD>);
+#pragma unroll
+        for (int r = 0; r < kRowTile; ++r) {
+          const float l = warp_sum(w.l[r]);
+          if (lane == 0) s_stat[warp][r] = make_float2(w.m[r], l);
+#pragma unroll
+          for (int c = 0; c < kD / 32; ++c) result[r * kD + lane * (kD / 32) + c] = w.o[r][c];
+        }
       }
-    }
 
-    // the four warps' results, joined: 8 threads a row
-    __syncthreads();
-    {
-      const int r = tid >> 3, part = tid & 7;
-      const float* res[kWarps];
-      float mx = -INFINITY, l = 0.f, f[kWarps];
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) {
-        res[k] = reinterpret_cast<const float*>(smem + k * kStages * kStageBytes<T, kD>);
-        const float mk = res[k][kRowTile * kD + r];
-        mx = max3_nan(mx, mk, mk);
-      }
-      const float shift = mx == -INFINITY ? 0.f : mx;
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) {
-        f[k] = ex2(res[k][kRowTile * kD + r] - shift);
-        l += f[k] * res[k][kRowTile * kD + kRowTile + r];
-      }
-      const bool exists = row0 + r < a.rows, all = count == sp.steps;
-      const int64_t slot = 2 * (int64_t)blockIdx.x + (step0 > 0 ? 0 : 1);
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      T* const orow = reinterpret_cast<T*>(a.o) + (((int64_t)b * a.H + h * a.G + (row0 + r) / a.T) * a.T + (row0 + r) % a.T) * pg.D;
-      float* const arow = a.acc + (slot * kRowTile + r) * kD;
-#pragma unroll
-      for (int c = 0; c < kD / 32; ++c) {
-        const int col = c * 32 + part * 4;
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      // the four warps' results, joined, 8 threads a row, while the next item's rows are on their way
+      const int free_stage = (i + kStages - 1) % kStages;
+      __shared__ int s_free[kWarps];
+      if (lane == 0) s_free[warp] = free_stage;
+      __syncthreads();
+      {
+        const int r = tid >> 3, part = tid & 7;
+        const float* res[kWarps];
+        float mx = -INFINITY, l = 0.f, f[kWarps];
 #pragma unroll
         for (int k = 0; k < kWarps; ++k) {
-          const float4 x = *reinterpret_cast<const float4*>(res[k] + r * kD + col);
-          sum.x = fmaf(f[k], x.x, sum.x);
-          sum.y = fmaf(f[k], x.y, sum.y);
-          sum.z = fmaf(f[k], x.z, sum.z);
-          sum.w = fmaf(f[k], x.w, sum.w);
+          res[k] = reinterpret_cast<const float*>(smem + (k * kStages + s_free[k]) * kStageBytes<T, kD>);
+          mx = max3_nan(mx, s_stat[k][r].x, s_stat[k][r].x);
         }
-        if (!exists || col >= pg.D) continue;
-        if (!all) {
-          *reinterpret_cast<float4*>(arow + col) = sum;
-        } else if constexpr (kF32) {
-          *reinterpret_cast<float4*>(orow + col) = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
-        } else {
-          uint2 x = make_uint2(pack16<T>(sum.x * inv, sum.y * inv), pack16<T>(sum.z * inv, sum.w * inv));
-          *reinterpret_cast<uint2*>(orow + col) = x;
+        const float shift = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) {
+          f[k] = ex2(s_stat[k][r].x - shift);
+          l += f[k] * s_stat[k][r].y;
+        }
+        const bool exists = row0 + r < a.rows, all = count == sp.steps;
+        const int64_t slot = 2 * (int64_t)blockIdx.x + (step0 > 0 ? 0 : 1);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        T* const orow = reinterpret_cast<T*>(a.o) + (((int64_t)b * a.H + h * a.G + (row0 + r) / a.T) * a.T + (row0 + r) % a.T) * pg.D;
+        float* const arow = a.acc + (slot * kRowTile + r) * kD;
+#pragma unroll
+        for (int c = 0; c < kD / 32; ++c) {
+          const int col = c * 32 + part * 4;
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int k = 0; k < kWarps; ++k) {
+            const float4 x = *reinterpret_cast<const float4*>(res[k] + r * kD + col);
+            sum.x = fmaf(f[k], x.x, sum.x);
+            sum.y = fmaf(f[k], x.y, sum.y);
+            sum.z = fmaf(f[k], x.z, sum.z);
+            sum.w = fmaf(f[k], x.w, sum.w);
+          }
+          if (!exists || col >= pg.D) continue;
+          if (!all) {
+            *reinterpret_cast<float4*>(arow + col) = sum;
+          } else if constexpr (kF32) {
+            *reinterpret_cast<float4*>(orow + col) = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+          } else {
+            *reinterpret_cast<uint2*>(orow + col) = make_uint2(pack16<T>(sum.x * inv, sum.y * inv), pack16<T>(sum.z * inv, sum.w * inv));
+          }
+        }
+        if (exists && part == 0) {
+          if (!all) a.stat[slot * kRowTile + r] = make_float2(mx, l);
+          else if (a.weights != nullptr) a.whole[(((int64_t)b * pg.Hkv + h) * a.tiles + row0 / kRowTile) * kRowTile + r] = make_float2(mx, l);
         }
       }
-      if (exists && part == 0) {
-        if (!all) a.stat[slot * kRowTile + r] = make_float2(mx, l);
-        else if (a.weights != nullptr) a.whole[(((int64_t)b * pg.Hkv + h) * a.tiles + row0 / kRowTile) * kRowTile + r] = make_float2(mx, l);
-      }
+      __syncthreads();
+      at += count;
+      now.step += count;
+      settle(now);
     }
-    __syncthreads();
-    at += count;
+  };
+
+  for (int x = blockIdx.x;; x += gridDim.x) {
+    int b, item, step = 0;
+    int64_t begin = 0, end;
+    Span sp;
+    if (a.one_piece) {
+      if (x >= pg.B * per_seq) break;
+      b = x / per_seq;
+      item = x - b * per_seq;
+      sp = span_of(length(b), a.T, a.window, a.sinks);
+      end = sp.steps;
+    } else {
+      const int64_t total = warp_total(pg.B, steps_of), piece = piece_of(a, total);
+      begin = blockIdx.x * piece;
+      end = min(begin + piece, total);
+      if (begin >= end) break;
+      const Found f = warp_find(pg.B, begin, steps_of);
+      b = f.b;
+      sp = span_of(length(b), a.T, a.window, a.sinks);
+      item = (int)((begin - f.before) / sp.steps);
+      step = (int)(begin - f.before - (int64_t)item * sp.steps);
+    }
+    if (begin < end) take(begin, end, {b, item, step, sp});
+    if (!a.one_piece) break;
   }
 }
 
-// Joins the pieces of rows that several CTAs worked on; with weights: adds every key's share of its group's rows.
-// Grid (items, slices): slice s joins the features [32 s, 32 s + 32) and takes every gridDim.y-th run of 1024 keys.
-constexpr int kJoinThreads = 256;
+// Behind the pieces: blocks 0 .. joins - 1 join the rows that several CTAs worked on, one (item, slice of 32 features) each; the others add
+// every key's share of its group's rows to its weight, 1024 keys of a (sequence, key head) each.  Lengths are read ahead of the wait:
+// they were complete before the attention kernel was behind its own.
+constexpr int kJoinThreads = 256, kRunKeys = 4 * kJoinThreads;
 template <typename T, int kD>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ AttendArgs a) {
-  __shared__ int64_t s_total, s_before;
-  __shared__ float2 s_stat[kRowTile];
-  grid_dep_wait();
-  grid_dep_launch();
+__global__ void __launch_bounds__(kJoinThreads) paged_finish_kernel(const __grid_constant__ AttendArgs a, int joins) {
+  extern __shared__ float2 s_rows[];                 // (maximum, 1 / sum) of the group's rows
   const Pages& pg = a.pg;
   const int tid = threadIdx.x;
   const int per_seq = pg.Hkv * a.tiles;
-  const int b = blockIdx.x / per_seq, item = blockIdx.x - b * per_seq;
   auto steps_of = [&](int i) { return (int64_t)per_seq * span_of(pg.length(i), a.T, a.window, a.sinks).steps; };
-  if (tid < 32) {
-    const int64_t total = warp_total(pg.B, steps_of), before = warp_before(pg.B, b, steps_of);
-    if (tid == 0) {
-      s_total = total;
-      s_before = before;
-    }
-  }
-  __syncthreads();
-  const Span sp = span_of(pg.length(b), a.T, a.window, a.sinks);
+  const bool join = (int)blockIdx.x < joins;
+  const int x = join ? blockIdx.x / (kD / 32) : blockIdx.x - joins, slice = blockIdx.x % (kD / 32);
+  const int64_t cap = (int64_t)pg.max_pages << pg.shift;
+  const int runs = (int)((cap + kRunKeys - 1) / kRunKeys);
+  const int b = join ? x / per_seq : x / runs / pg.Hkv;
+  const int64_t piece = piece_of(a, warp_total(pg.B, steps_of)), before = warp_total(b, steps_of);
+  const int len = pg.length(b);
+  const Span sp = span_of(len, a.T, a.window, a.sinks);
+  grid_dep_wait();
+  grid_dep_launch();
   if (sp.steps == 0) return;
-  const Line line = line_of(a, s_total);
-  const int64_t start = s_before + (int64_t)item * sp.steps;
-  const int c0 = (int)(start / line.piece), c1 = (int)((start + sp.steps - 1) / line.piece);
-  const int h = item / a.tiles, row0 = (item - h * a.tiles) * kRowTile;
-  const int n_rows = min(kRowTile, a.rows - row0);
-  auto slot_of = [&](int c) { return 2 * (int64_t)c + (c == c0 ? 1 : 0); };
-  if (c1 > c0) {
+  auto first_cta = [&](int item) { return (int)((before + (int64_t)item * sp.steps) / piece); };
+  auto last_cta = [&](int item) { return (int)((before + (int64_t)item * sp.steps + sp.steps - 1) / piece); };
+
+  if (join) {
+    const int item = x - b * per_seq, c0 = first_cta(item), c1 = last_cta(item);
+    if (c0 == c1) return;
+    const int h = item / a.tiles, row0 = (item - h * a.tiles) * kRowTile;
+    const int n_rows = min(kRowTile, a.rows - row0);
+    auto slot_of = [&](int c) { return 2 * (int64_t)c + (c == c0 ? 1 : 0); };
     const int r = tid >> 4, part = tid & 15;         // 16 threads a row
     float mx = -INFINITY, l = 0.f;
-    if (r < n_rows) {
+    if (r < n_rows)
       for (int c = c0 + part; c <= c1; c += 16) {
         const float m = a.stat[slot_of(c) * kRowTile + r].x;
         mx = max3_nan(mx, m, m);
       }
-    }
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) {
       const float m = __shfl_xor_sync(0xffffffffu, mx, o);
       mx = max3_nan(mx, m, m);
     }
     const float shift = mx == -INFINITY ? 0.f : mx;
-    if (r < n_rows)
-      for (int c = c0 + part; c <= c1; c += 16) {
-        const float2 x = a.stat[slot_of(c) * kRowTile + r];
-        l += ex2(x.x - shift) * x.y;
-      }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if (part == 0) s_stat[r] = make_float2(mx, l);
-    const int col = blockIdx.y * 32 + part * 2;
-    if (r < n_rows && blockIdx.y < kD / 32 && col < pg.D) {
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      float2 sum = make_float2(0.f, 0.f);
-      for (int c = c0; c <= c1; ++c) {
-        const float f = ex2(a.stat[slot_of(c) * kRowTile + r].x - shift);
-        const float2 x = *reinterpret_cast<const float2*>(a.acc + (slot_of(c) * kRowTile + r) * kD + col);
-        sum.x = fmaf(f, x.x, sum.x);
-        sum.y = fmaf(f, x.y, sum.y);
-      }
-      T* const to = reinterpret_cast<T*>(a.o) + (((int64_t)b * a.H + h * a.G + (row0 + r) / a.T) * a.T + (row0 + r) % a.T) * pg.D + col;
-      to[0] = from_f32<T>(sum.x * inv);
-      to[1] = from_f32<T>(sum.y * inv);
+    const int col = slice * 32 + part * 2;
+    if (r >= n_rows || col >= pg.D) return;
+    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {
+      const float2 st = a.stat[slot_of(c) * kRowTile + r];
+      const float2 v = *reinterpret_cast<const float2*>(a.acc + (slot_of(c) * kRowTile + r) * kD + col);
+      const float f = ex2(st.x - shift);
+      l = fmaf(f, st.y, l);
+      sum.x = fmaf(f, v.x, sum.x);
+      sum.y = fmaf(f, v.y, sum.y);
     }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    T* const to = reinterpret_cast<T*>(a.o) + (((int64_t)b * a.H + h * a.G + (row0 + r) / a.T) * a.T + (row0 + r) % a.T) * pg.D + col;
+    to[0] = from_f32<T>(sum.x * inv);
+    to[1] = from_f32<T>(sum.y * inv);
+    return;
   }
-}
 
-// weights[b, h, j] = decay weights[b, h, j] + sum over the rows of the group of e^{s_j - m} / l, for all j < length
-template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) paged_weights_kernel(const __grid_constant__ AttendArgs a) {
-  extern __shared__ float2 s_rows[];                 // (maximum, 1 / sum) of the group's rows
-  __shared__ int64_t s_total, s_before;
-  grid_dep_wait();
-  grid_dep_launch();
-  const Pages& pg = a.pg;
-  const int tid = threadIdx.x;
-  const int b = blockIdx.y / pg.Hkv, h = blockIdx.y - b * pg.Hkv;
-  const int per_seq = pg.Hkv * a.tiles;
-  auto steps_of = [&](int i) { return (int64_t)per_seq * span_of(pg.length(i), a.T, a.window, a.sinks).steps; };
-  const int len = pg.length(b);
-  if ((int64_t)blockIdx.x * kJoinThreads * 4 >= len) return;
-  if (tid < 32) {
-    const int64_t total = warp_total(pg.B, steps_of), before = warp_before(pg.B, b, steps_of);
-    if (tid == 0) {
-      s_total = total;
-      s_before = before;
-    }
-  }
-  __syncthreads();
-  const Span sp = span_of(len, a.T, a.window, a.sinks);
-  const Line line = line_of(a, s_total);
+  // weights[b, h, j] = decay weights[b, h, j] + sum over the rows of the group of e^{s_j - m} / l, for all j < length
+  const int h = x / runs - b * pg.Hkv, j0 = (x % runs) * kRunKeys;
+  if (j0 >= len) return;
   for (int r = tid; r < a.rows; r += kJoinThreads) {
-    const int tile = r / kRowTile, rr = r - tile * kRowTile;
-    const int64_t start = s_before + (int64_t)(h * a.tiles + tile) * sp.steps;
-    const int c0 = (int)(start / line.piece), c1 = (int)((start + sp.steps - 1) / line.piece);
-    float2 x;
-    if (c0 == c1) {
-      x = a.whole[(((int64_t)b * pg.Hkv + h) * a.tiles + tile) * kRowTile + rr];
+    const int tile = r / kRowTile, rr = r - tile * kRowTile, item = h * a.tiles + tile, c0 = first_cta(item), c1 = last_cta(item);
+    float2 y;
+    if (a.one_piece || c0 == c1) {
+      y = a.whole[((int64_t)b * per_seq + item) * kRowTile + rr];
     } else {
-      x = make_float2(-INFINITY, 0.f);
+      y = make_float2(-INFINITY, 0.f);
       for (int c = c0; c <= c1; ++c) {
-        const float2 y = a.stat[(2 * (int64_t)c + (c == c0 ? 1 : 0)) * kRowTile + rr];
-        const float m = max3_nan(x.x, y.x, y.x), shift = m == -INFINITY ? 0.f : m;
-        x.y = x.y * ex2(x.x - shift) + y.y * ex2(y.x - shift);
-        x.x = m;
+        const float2 z = a.stat[(2 * (int64_t)c + (c == c0 ? 1 : 0)) * kRowTile + rr];
+        const float m = max3_nan(y.x, z.x, z.x), shift = m == -INFINITY ? 0.f : m;
+        y.y = y.y * ex2(y.x - shift) + z.y * ex2(z.x - shift);
+        y.x = m;
       }
     }
-    s_rows[r] = make_float2(x.x == -INFINITY ? 0.f : x.x, x.y == 0.f ? 0.f : 1.f / x.y);
+    s_rows[r] = make_float2(y.x == -INFINITY ? 0.f : y.x, y.y == 0.f ? 0.f : 1.f / y.y);
   }
   __syncthreads();
-  const int64_t cap = (int64_t)pg.max_pages << pg.shift;
-  const float* const scores = a.scores + ((int64_t)b * pg.Hkv + h) * a.rows * cap;
-  float* const weights = a.weights + ((int64_t)b * pg.Hkv + h) * cap;
-  for (int e = 0; e < 4; ++e) {
-    const int j = (blockIdx.x * 4 + e) * kJoinThreads + tid;
-    if (j >= len) break;
-    float w = a.decay == 0.f ? 0.f : a.decay * weights[j];         // decay 0: whatever stood there is not read
-    if (j < sp.first * kStep || j >= sp.lo) {
-      float sum = 0.f;
-      for (int r = 0; r < a.rows; ++r) sum += ex2(scores[r * cap + j] - s_rows[r].x) * s_rows[r].y;
-      w += sum;
+  const int j = j0 + tid * 4;                          // four keys a thread; whole steps are seen or not
+  if (j >= len) return;
+  float* const to = a.weights + ((int64_t)b * pg.Hkv + h) * cap + j;
+  float4 w = make_float4(0.f, 0.f, 0.f, 0.f);          // decay 0: whatever stood there is not read
+  if (a.decay != 0.f) {
+    w = *reinterpret_cast<const float4*>(to);
+    w = make_float4(a.decay * w.x, a.decay * w.y, a.decay * w.z, a.decay * w.w);
+  }
+  if (j < sp.first * kStep || j >= sp.lo) {
+    const float* s = a.scores + ((int64_t)b * pg.Hkv + h) * a.rows * cap + j;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int r = 0; r < a.rows; ++r, s += cap) {
+      const float4 v = *reinterpret_cast<const float4*>(s);
+      const float2 st = s_rows[r];
+      sum.x = fmaf(ex2(v.x - st.x), st.y, sum.x);
+      sum.y = fmaf(ex2(v.y - st.x), st.y, sum.y);
+      sum.z = fmaf(ex2(v.z - st.x), st.y, sum.z);
+      sum.w = fmaf(ex2(v.w - st.x), st.y, sum.w);
     }
-    weights[j] = w;
+    w = make_float4(w.x + sum.x, w.y + sum.y, w.z + sum.z, w.w + sum.w);
+  }
+  if (j + 3 < len) {
+    *reinterpret_cast<float4*>(to) = w;
+  } else {
+    to[0] = w.x;
+    if (j + 1 < len) to[1] = w.y;
+    if (j + 2 < len) to[2] = w.z;
   }
 }
 
@@ -782,17 +774,20 @@ struct EvictArgs {
   int *table_out, *lengths_out, *kept;
   float* weights_out;
 };
-constexpr int kSelectThreads = 1024;
+constexpr int kSelectThreads = 1024, kSelectWarps = kSelectThreads / 32;
+constexpr int kHists = 8;                                      // copies of the histogram, a warp in eight has one to itself
+constexpr int kCachedKeys = 48 * 1024;                         // longer rows of weights are read from memory in every pass
 // ascending as unsigned; the two zeros are equal, NaN counts as the largest.  On the bits alone: arithmetic may drop a NaN's sign.
-__device__ __forceinline__ uint32_t order_bits(float w) {
-  const uint32_t u = __float_as_uint(w);
+__device__ __forceinline__ uint32_t order_bits(uint32_t u) {
   if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
   if ((u & 0x7fffffffu) == 0) return 0x80000000u;
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
+template <bool kCached>
 __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __grid_constant__ EvictArgs a) {
-  __shared__ int hist[256];
-  __shared__ int warp_sums[33];
+  extern __shared__ uint32_t s_w[];                            // kCached: the row's weights
+  __shared__ int hist[kHists][256];
+  __shared__ int s_stay[kSelectWarps], s_tie[kSelectWarps];
   __shared__ uint32_t s_prefix;
   __shared__ int s_left;
   grid_dep_wait();
@@ -801,8 +796,8 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int b = blockIdx.x / pg.Hkv, h = blockIdx.x - b * pg.Hkv;
   const int64_t cap = (int64_t)pg.max_pages << pg.shift, at = ((int64_t)b * pg.Hkv + h) * cap;
-  const float* const w = a.weights + at;
-  float* const wo = a.weights_out + at;
+  const uint32_t* const w = reinterpret_cast<const uint32_t*>(a.weights) + at;
+  uint32_t* const wo = reinterpret_cast<uint32_t*>(a.weights_out) + at;
   int* const kept = a.kept + ((int64_t)b * pg.Hkv + h) * a.budget;
   const int len = pg.length(b);
   const bool over = len > a.budget;
@@ -813,21 +808,27 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
     if (tid == 0) a.lengths_out[b] = over ? a.budget : len;
   }
   if (!over) {
-    for (int64_t j = tid; j < cap; j += kSelectThreads) wo[j] = j < len ? ld_behind_wait(w + j) : 0.f;
+    for (int64_t j = tid; j < cap; j += kSelectThreads) wo[j] = j < len ? w[j] : 0u;
     for (int j = tid; j < a.budget; j += kSelectThreads) kept[j] = j < len ? j : -1;
     return;
   }
+  if constexpr (kCached) {
+    const uint4* const from = reinterpret_cast<const uint4*>(w);            // rows are whole pages, so whole vectors
+    for (int j = tid; j < (len + 3) / 4; j += kSelectThreads) reinterpret_cast<uint4*>(s_w)[j] = from[j];
+  }
+  auto bits = [&](int j) { return kCached ? s_w[j] : w[j]; };
   const int from = a.sinks, to = len - a.recent;               // the candidates
   const int want = a.budget - a.sinks - a.recent;              // < to - from
   uint32_t prefix = 0;
   int left = want;                                             // to be found among the keys that share the prefix
   if (want > 0) {
     for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += kSelectThreads) hist[i] = 0;
+      for (int i = tid; i < kHists * 256; i += kSelectThreads) hist[i >> 8][i & 255] = 0;
       __syncthreads();
+      int* const mine = hist[warp % kHists];
       for (int j = from + tid; j < to; j += kSelectThreads) {
-        const uint32_t u = order_bits(ld_behind_wait(w + j));
-        if (shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(u >> shift) & 255u], 1);
+        const uint32_t u = order_bits(bits(j));
+        if (shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&mine[(u >> shift) & 255u], 1);
       }
       __syncthreads();
       if (warp == 0) {
@@ -835,7 +836,9 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
         int c[8], sum = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          c[e] = hist[255 - 8 * lane - e];
+          c[e] = 0;
+#pragma unroll
+          for (int k = 0; k < kHists; ++k) c[e] += hist[k][255 - 8 * lane - e];
           sum += c[e];
         }
         int inc = sum;
@@ -860,84 +863,90 @@ __global__ void __launch_bounds__(kSelectThreads) paged_select_kernel(const __gr
       prefix = s_prefix;
       left = s_left;
     }
+  } else if (kCached) {
+    __syncthreads();
   }
-  // ordered: a key stays if it is a sink or recent, above the border, or among the first `left` on it
-  int out = 0, ties = 0;                                       // survivors and border keys in front of this round
-  for (int j0 = 0; j0 < len; j0 += kSelectThreads) {
-    const int j = j0 + tid;
-    float x = 0.f;
-    bool stay = false, tie = false;
-    if (j < len) {
-      x = ld_behind_wait(w + j);
-      const uint32_t u = order_bits(x);
-      const bool ends = j < from || j >= to;
-      stay = ends || (want > 0 && u > prefix);
-      tie = !ends && want > 0 && u == prefix;
-    }
-    const unsigned tb = __ballot_sync(0xffffffffu, tie), sb = __ballot_sync(0xffffffffu, stay);
-    // border keys in front of this one, to know whether it stays
-    if (lane == 0) warp_sums[warp] = __popc(tb) | __popc(sb) << 16;
-    __syncthreads();
-    int my_ties = ties, round_ties = 0;
-    for (int k = 0; k < kSelectThreads / 32; ++k) {
-      const int x2 = warp_sums[k] & 0xffff;
-      if (k < warp) my_ties += x2;
-      round_ties += x2;
-    }
-    __syncthreads();
-    my_ties += __popc(tb & ((1u << lane) - 1u));
-    stay |= tie && my_ties < left;
+  // Ordered: a key stays if it is a sink or recent, above the border, or among the first `left` on it.  A warp owns a run of keys: it
+  // counts them, learns how many stay in front of its run, and writes them.
+  const int rows = (len + kSelectThreads - 1) / kSelectThreads, j0 = warp * rows * 32;
+  auto look = [&](int j, bool* stay, bool* tie) {
+    const uint32_t x = j < len ? bits(j) : 0u, u = order_bits(x);
+    const bool ends = j < from || j >= to;
+    *stay = j < len && (ends || (want > 0 && u > prefix));
+    *tie = j < len && !ends && want > 0 && u == prefix;
+    return x;
+  };
+  int n_stay = 0, n_tie = 0;
+  for (int r = 0; r < rows; ++r) {
+    bool stay, tie;
+    look(j0 + r * 32 + lane, &stay, &tie);
+    n_stay += __popc(__ballot_sync(0xffffffffu, stay));
+    n_tie += __popc(__ballot_sync(0xffffffffu, tie));
+  }
+  if (lane == 0) {
+    s_stay[warp] = n_stay;
+    s_tie[warp] = n_tie;
+  }
+  __syncthreads();
+  int ties = __reduce_add_sync(0xffffffffu, lane < warp ? s_tie[lane] : 0);
+  int out = __reduce_add_sync(0xffffffffu, lane < warp ? s_stay[lane] : 0) + min(ties, left);
+  const unsigned below = (1u << lane) - 1u;
+  for (int r = 0; r < rows; ++r) {
+    const int j = j0 + r * 32 + lane;
+    bool stay, tie;
+    const uint32_t x = look(j, &stay, &tie);
+    const unsigned tb = __ballot_sync(0xffffffffu, tie);
+    stay |= tie && ties + __popc(tb & below) < left;
     const unsigned kb = __ballot_sync(0xffffffffu, stay);
-    if (lane == 0) warp_sums[warp] = __popc(kb);
-    __syncthreads();
-    int my_out = out, round_out = 0;
-    for (int k = 0; k < kSelectThreads / 32; ++k) {
-      const int x2 = warp_sums[k];
-      if (k < warp) my_out += x2;
-      round_out += x2;
-    }
-    __syncthreads();
-    my_out += __popc(kb & ((1u << lane) - 1u));
     if (stay) {
-      kept[my_out] = j;
-      wo[my_out] = x;
+      kept[out + __popc(kb & below)] = j;
+      wo[out + __popc(kb & below)] = x;
     }
-    out += round_out;
-    ties += round_ties;
+    ties += __popc(tb);
+    out += __popc(kb);
   }
-  for (int64_t j = a.budget + tid; j < cap; j += kSelectThreads) wo[j] = 0.f;
+  for (int64_t j = a.budget + tid; j < cap; j += kSelectThreads) wo[j] = 0u;
 }
 
-__global__ void __launch_bounds__(256) paged_move_kernel(const __grid_constant__ EvictArgs a, int vecs, int size) {
-  grid_dep_wait();
-  grid_dep_launch();
+constexpr int kMoveThreads = 256, kMoveRounds = 4;
+__global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const __grid_constant__ EvictArgs a, int vecs, int size) {
   const Pages& pg = a.pg;
   const int b = blockIdx.y / pg.Hkv, h = blockIdx.y - b * pg.Hkv;
-  if (pg.length(b) <= a.budget) return;
-  const int* const kept = a.kept + ((int64_t)b * pg.Hkv + h) * a.budget;
-  const int per = 256 / vecs > 0 ? 256 / vecs : 1;             // rows a round
+  const int per = kMoveThreads / vecs;                         // rows a round
   const int c = threadIdx.x % vecs, lr = threadIdx.x / vecs;
-  if (lr >= per) return;
-  constexpr int kRounds = 8;
-  const int base = blockIdx.x * per * kRounds;
+  const int base = blockIdx.x * per * kMoveRounds + lr;
+  grid_dep_wait();
+  grid_dep_launch();
+  if (lr >= per || pg.length(b) <= a.budget) return;
+  const int* const kept = a.kept + ((int64_t)b * pg.Hkv + h) * a.budget;
+  auto at = [&](const int64_t (&s)[3], int64_t id, int64_t row) { return (id * s[0] + h * s[1] + row * s[2]) * size + c * 16ll; };
+  int j[kMoveRounds], src[kMoveRounds], dst[kMoveRounds];
+  // the rounds' loads one kind after the other: survivors, page numbers, rows
 #pragma unroll
-  for (int e = 0; e < kRounds; ++e) {
-    const int r = base + e * per + lr;
-    if (r >= a.budget) break;
-    const int j = ld_behind_wait(kept + r);
-    const int src = pg.id(b, j >> pg.shift);
-    const int page_no = r >> pg.shift;
-    const int dst = page_no < a.n_fresh ? ld_behind_wait(a.fresh + (int64_t)b * a.n_fresh + page_no) : -1;
-    if (src < 0 || src >= pg.n_pages || dst < 0 || dst >= pg.n_pages) {
-      note(pg.status, kBadPage);
-      continue;
-    }
-    const int64_t from = j & (pg.page - 1), to = r & (pg.page - 1);
-    auto at = [&](const int64_t (&s)[3], int64_t id, int64_t row) { return (id * s[0] + h * s[1] + row * s[2]) * size + c * 16ll; };
-    const uint4 xk = *reinterpret_cast<const uint4*>((const char*)a.k + at(pg.ks, src, from));
-    const uint4 xv = *reinterpret_cast<const uint4*>((const char*)a.v + at(pg.vs, src, from));
-    *reinterpret_cast<uint4*>((char*)a.k + at(pg.ks, dst, to)) = xk;
-    *reinterpret_cast<uint4*>((char*)a.v + at(pg.vs, dst, to)) = xv;
+  for (int e = 0; e < kMoveRounds; ++e) {
+    const int r = base + e * per, page_no = r >> pg.shift;
+    j[e] = r < a.budget ? ld_behind_wait(kept + r) : -1;
+    dst[e] = r < a.budget && page_no < a.n_fresh ? ld_behind_wait(a.fresh + (int64_t)b * a.n_fresh + page_no) : -1;
+  }
+#pragma unroll
+  for (int e = 0; e < kMoveRounds; ++e) src[e] = j[e] >= 0 ? pg.id(b, j[e] >> pg.shift) : -1;
+  uint4 xk[kMoveRounds], xv[kMoveRounds];
+#pragma unroll
+  for (int e = 0; e < kMoveRounds; ++e) {
+    const bool ok = src[e] >= 0 && src[e] < pg.n_pages && dst[e] >= 0 && dst[e] < pg.n_pages;
+    if (j[e] >= 0 && !ok) note(pg.status, kBadPage);
+    if (!ok) j[e] = -1;
+    if (j[e] < 0) continue;
+    const int64_t from = j[e] & (pg.page - 1);
+    xk[e] = *reinterpret_cast<const uint4*>((const char*)a.k + at(pg.ks, src[e], from));
+    xv[e] = *reinterpret_cast<const uint4*>((const char*)a.v + at(pg.vs, src[e], from));
+  }
+#pragma unroll
+  for (int e = 0; e < kMoveRounds; ++e) {
+    if (j[e] < 0) continue;
+    const int64_t to = (base + e * per) & (pg.page - 1);
+    *reinterpret_cast<uint4*>((char*)a.k + at(pg.ks, dst[e], to)) = xk[e];
+    *reinterpret_cast<uint4*>((char*)a.v + at(pg.vs, dst[e], to)) = xv[e];
   }
 }
 
@@ -980,6 +989,7 @@ template <typename T, int kD> constexpr int attend_smem() {
 // CTAs of the attention kernel an SM holds (by shared memory: 192 KB in 16 bits at D = 128 are two CTAs)
 int attend_per_sm(int dtype, int D) { return dtype == LMK_F32 ? (D <= 64 ? 2 : 1) : (D <= 64 ? 4 : 2); }
 constexpr int kLeastSteps = 8;         // of a CTA: two a warp
+constexpr int kWholeSteps = 32;        // tables of up to this many steps a sequence: every row is one CTA's, and nothing is to be joined
 
 struct AttendPlan {
   int grid, rows, tiles, kD;
@@ -1014,14 +1024,15 @@ int launch_attend(const AttendArgs& a, cudaStream_t st) {
     LMK_CUDA(cudaFuncSetAttribute(paged_attend_kernel<T, kD>, cudaFuncAttributeMaxDynamicSharedMemorySize, attend_smem<T, kD>()));
     ready[dev].store(true, std::memory_order_release);
   }
-  LMK_CUDA(launch_overlapped(paged_attend_kernel<T, kD>, dim3(a.grid), dim3(kWarps * 32), attend_smem<T, kD>(), st, a));
+  const int64_t items = (int64_t)a.pg.B * a.pg.Hkv * a.tiles;
+  const unsigned grid = a.one_piece && items < a.grid ? (unsigned)items : (unsigned)a.grid;
+  LMK_CUDA(launch_overlapped(paged_attend_kernel<T, kD>, dim3(grid), dim3(kWarps * 32), attend_smem<T, kD>(), st, a));
   const int64_t cap = (int64_t)a.pg.max_pages << a.pg.shift;
-  // a row is in several pieces only where its steps can exceed the least piece
-  if (cap / kStep > 1) LMK_CUDA(launch_overlapped(paged_join_kernel<T, kD>, dim3(a.pg.B * a.pg.Hkv * a.tiles, kD / 32), dim3(kJoinThreads), 0, st, a));
-  if (a.weights != nullptr) {
-    const int runs = (int)((cap + kJoinThreads * 4 - 1) / (kJoinThreads * 4));
-    LMK_CUDA(launch_overlapped(paged_weights_kernel<T>, dim3(runs, a.pg.B * a.pg.Hkv), dim3(kJoinThreads), sizeof(float2) * a.rows, st, a));
-  }
+  const int64_t joins = !a.one_piece ? items * (kD / 32) : 0;
+  const int64_t runs = a.weights != nullptr ? (cap + kRunKeys - 1) / kRunKeys * a.pg.B * a.pg.Hkv : 0;
+  if (joins + runs > INT32_MAX) return fail(LMK_ERR_UNSUPPORTED, "paged attention: too many rows and keys for one call");
+  if (joins + runs > 0)
+    LMK_CUDA(launch_overlapped(paged_finish_kernel<T, kD>, dim3((unsigned)(joins + runs)), dim3(kJoinThreads), sizeof(float2) * a.rows, st, a, (int)joins));
   return LMK_OK;
 }
 
@@ -1048,6 +1059,7 @@ extern "C" int lmk_paged_attend(const void* q, const int64_t q_strides[3], const
   LMK_CHECK_ARG(attend_sizes_ok(B, H, Hkv, T), "paged attention: T=%d tokens of %d heads a key head are too many (up to 1024 tokens, 4096 rows)", T, H / Hkv);
   LMK_CHECK_ARG(window >= 0 && sinks >= 0, "paged attention: window=%d and sinks=%d must not be negative", window, sinks);
   LMK_CHECK_ARG(isfinite(sm_scale) && isfinite(decay), "paged attention: scale and decay must be finite");
+  LMK_CHECK_ARG(((uintptr_t)weights & 15) == 0, "paged attention: weights must start on a 16-byte boundary");
   const int pair = 4 / dtype_size(dtype);
   LMK_CHECK_ARG(((uintptr_t)q & 3) == 0 && q_strides[0] % pair == 0 && q_strides[1] % pair == 0 && q_strides[2] % pair == 0,
                 "paged attention: q must lie on 4-byte boundaries");
@@ -1067,6 +1079,7 @@ extern "C" int lmk_paged_attend(const void* q, const int64_t q_strides[3], const
   a.scores = reinterpret_cast<float*>(ws + p.scores);
   a.H = H; a.T = T; a.G = H / Hkv; a.rows = p.rows; a.tiles = p.tiles; a.window = window; a.sinks = window > 0 ? sinks : 0; a.grid = p.grid;
   a.least = kLeastSteps;
+  a.one_piece = (int64_t)max_pages * page <= kWholeSteps * kStep;
   a.scale_log2 = sm_scale * kLog2e;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define LMK_ATTEND(T) return p.kD == 64 ? launch_attend<T, 64>(a, st) : launch_attend<T, 128>(a, st)
@@ -1110,6 +1123,7 @@ extern "C" int lmk_paged_evict(void* k_pages, void* v_pages, const int64_t k_str
   EvictArgs a = {};
   int rc = check_pages(a.pg, k_pages, v_pages, k_strides, v_strides, table, lengths, B, Hkv, D, page, n_pages, max_pages, dtype);
   if (rc != LMK_OK) return rc;
+  LMK_CHECK_ARG((((uintptr_t)weights | (uintptr_t)weights_out) & 15) == 0, "paged evict: weights must start on a 16-byte boundary");
   LMK_CHECK_ARG(weights && fresh && table_out && lengths_out && weights_out && kept, "paged evict: an array is null");
   LMK_CHECK_ARG(table_out != table && lengths_out != lengths && weights_out != weights, "paged evict: outputs must not be the inputs");
   LMK_CHECK_ARG(budget >= 1 && recent >= 0 && sinks >= 0 && (int64_t)recent + sinks <= budget,
@@ -1121,8 +1135,20 @@ extern "C" int lmk_paged_evict(void* k_pages, void* v_pages, const int64_t k_str
   a.table_out = table_out; a.lengths_out = lengths_out; a.weights_out = weights_out; a.kept = kept;
   const int size = dtype_size(dtype), vecs = D * size / 16;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  LMK_CUDA(launch_overlapped(paged_select_kernel, dim3(B * Hkv), dim3(kSelectThreads), 0, st, a));
-  const int rows = (256 / vecs) * 8;
-  LMK_CUDA(launch_overlapped(paged_move_kernel, dim3((budget + rows - 1) / rows, B * Hkv), dim3(256), 0, st, a, vecs, size));
+  if ((int64_t)max_pages * page <= kCachedKeys) {
+    static std::atomic<bool> ready[64];
+    int dev = 0;
+    LMK_CUDA(cudaGetDevice(&dev));
+    if (dev < 0 || dev >= 64) return fail(LMK_ERR_UNSUPPORTED, "device index %d out of range", dev);
+    if (!ready[dev].load(std::memory_order_acquire)) {
+      LMK_CUDA(cudaFuncSetAttribute(paged_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kCachedKeys * 4));
+      ready[dev].store(true, std::memory_order_release);
+    }
+    LMK_CUDA(launch_overlapped(paged_select_kernel<true>, dim3(B * Hkv), dim3(kSelectThreads), (size_t)max_pages * page * 4, st, a));
+  } else {
+    LMK_CUDA(launch_overlapped(paged_select_kernel<false>, dim3(B * Hkv), dim3(kSelectThreads), 0, st, a));
+  }
+  const int rows = (kMoveThreads / vecs) * kMoveRounds;
+  LMK_CUDA(launch_overlapped(paged_move_kernel, dim3((budget + rows - 1) / rows, B * Hkv), dim3(kMoveThreads), 0, st, a, vecs, size));
   return LMK_OK;
 }
