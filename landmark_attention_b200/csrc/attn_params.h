@@ -56,6 +56,8 @@ int* device_status_word();
 int tensor_map_4d(CUtensorMap* m, const void* ptr, int dtype, int B, int H, int L, const int64_t st[3], int box_rows);
 // the same for D features, encoded at every call
 int tensor_map_4d_now(CUtensorMap* m, const void* ptr, int dtype, int B, int H, int L, int D, const int64_t st[3], int box_rows);
+// pages [n_pages, H, page, D] of a cache, strides {page, head, row}: box = 128 bytes of features x `box_rows` rows of one head
+int tensor_map_pages(CUtensorMap* m, const void* ptr, int dtype, int n_pages, int H, int page, int D, const int64_t st[3], int box_rows);
 bool tensor_map_operand_ok(const void* p, const int64_t st[3]);
 
 // Fused attention with arbitrary landmark positions (attn_mask_sm100.cu).  R [B*H, Lq], A [B*H, G, Lq] fp32.

@@ -1720,6 +1720,23 @@ void attn_sm100_set_max_ctas(int n) { g_max_ctas.store(n > 0 ? n : 0); }
 
 int attn_sm100_max_ctas() { return g_max_ctas.load(); }
 
+int tensor_map_pages(CUtensorMap* m, const void* ptr, int dtype, int n_pages, int H, int page, int D, const int64_t st[3], int box_rows) {
+  bind_context();
+  EncodeTiledFn enc = get_encode();
+  if (!enc) return fail(LMK_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const int size = dtype_size(dtype);
+  const int64_t dense[3] = {(int64_t)H * page * D, (int64_t)page * D, D};      // in place of strides that nothing is reached by
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)page, (cuuint64_t)H, (cuuint64_t)n_pages};
+  cuuint64_t strides[3] = {(cuuint64_t)st[2] * size, (cuuint64_t)(H > 1 ? st[1] : dense[1]) * size, (cuuint64_t)(n_pages > 1 ? st[0] : dense[0]) * size};
+  cuuint32_t box[4] = {128u / size, (cuuint32_t)box_rows, 1, 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType type = dtype == LMK_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dtype == LMK_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUresult r = enc(m, type, 4, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(LMK_ERR_CUDA, "cuTensorMapEncodeTiled (pages) failed with %d", (int)r);
+  return LMK_OK;
+}
 int tensor_map_4d_now(CUtensorMap* m, const void* ptr, int dtype, int B, int H, int L, int D, const int64_t st[3], int box_rows) {
   bind_context();
   return encode_map_4d(m, ptr, dtype, B, H, L, D, st, box_rows);

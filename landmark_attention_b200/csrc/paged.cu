@@ -12,8 +12,10 @@
 //     length of it, so neither short sequences nor a large capacity leave SMs idle, whatever the lengths are; they are read on the
 //     device, so a captured graph serves them as they grow.  A piece that holds all of its keys is written out at once; pieces of a
 //     longer row leave their maximum, sum and unnormalised output, which a second kernel joins.
-//   - A warp streams its own steps (every fourth of the CTA's) through its own ring in shared memory with cp.async: no barrier of the CTA in
-//     the loop.  Rows that nobody sees are filled with zeros instead of loaded, so what they hold does not matter.
+//   - A warp streams its own steps (every fourth of the CTA's) through its own ring in shared memory: no barrier of the CTA in the loop.  One
+//     lane asks TMA for a step's rows (with 16-byte cp.async the addresses alone took 1200 clk a step, as long as the arithmetic, and
+//     the warps could not keep up with the memory).  Rows that nobody sees are overwritten with zeros before the values are used, so
+//     what they hold does not matter.
 //   - The G T query rows of a key head are the 16 rows of an mma.sync tile (fp32: FMAs), so K and V are read once for all of them.
 // Weights (for eviction): the scores are kept, 4 bytes a key and query row, and the second kernel, which knows every row's maximum and
 // sum, adds e^{s - m} / l of a group's rows to the key's weight.  One thread adds up one key: no atomics, bit-reproducible.
@@ -31,10 +33,9 @@ using namespace ptx;
 
 constexpr int kStep = 16;              // keys a warp takes at a time; pages are whole steps
 constexpr int kRowTile = 16;           // query rows of one key head at a time
-constexpr int kWarps = 4;
 constexpr int kStages = 3;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kBadPage = 601, kFull = 602;
+constexpr int kBadPage = 601, kFull = 602, kErrRing = 611;
 
 struct Pages {
   const void *k, *v;
@@ -80,28 +81,29 @@ struct AttendArgs {
   int H, T, G, rows, tiles, window, sinks, grid, least;
   bool one_piece;                      // every row is one CTA's: CTAs take items instead of lengths of the line
   float scale_log2;
+  // query row of a key head -> head of its group, token
+  __device__ int head(int r) const { return T == 1 ? r : r / T; }
+  __device__ int token(int r) const { return T == 1 ? 0 : r % T; }
 };
 
 // All sequences' steps lie in one line; a CTA takes `piece` of them.  The sums over the sequences are worked out by whole warps.
 template <typename F>
-__device__ __forceinline__ int64_t warp_total(int B, F f) {      // sum of f(b) over b < B
-  int64_t sum = 0;
+__device__ __forceinline__ int warp_total(int B, F f) {      // sum of f(b) over b < B
+  int sum = 0;
   for (int b = threadIdx.x & 31; b < B; b += 32) sum += f(b);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  return sum;
+  return __reduce_add_sync(0xffffffffu, sum);
 }
-struct Found { int b; int64_t before; };
+struct Found { int b, before; };
 template <typename F>
-__device__ __forceinline__ Found warp_find(int B, int64_t at, F f) {      // the sequence that holds step `at`, and the steps in front of it
+__device__ __forceinline__ Found warp_find(int B, int at, F f) {      // the sequence that holds step `at`, and the steps in front of it
   const int lane = threadIdx.x & 31;
-  int64_t before = 0;
+  int before = 0;
   for (int b0 = 0; b0 < B; b0 += 32) {
-    const int64_t n = b0 + lane < B ? f(b0 + lane) : 0;
-    int64_t inc = n;
+    const int n = b0 + lane < B ? f(b0 + lane) : 0;
+    int inc = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+      const int v = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += v;
     }
     const unsigned hit = __ballot_sync(0xffffffffu, n > 0 && before + inc > at);
@@ -113,22 +115,15 @@ __device__ __forceinline__ Found warp_find(int B, int64_t at, F f) {      // the
   }
   return {B, before};
 }
-__device__ __forceinline__ int64_t piece_of(const AttendArgs& a, int64_t total) { return max((total + a.grid - 1) / a.grid, (int64_t)a.least); }
+__device__ __forceinline__ int piece_of(const AttendArgs& a, int total) { return max((total + a.grid - 1) / a.grid, a.least); }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool take) {
-  const int bytes = take ? 16 : 0;     // 0: filled with zeros, src is not read
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-template <typename T, int kD> constexpr int kRowBytes = kD * (int)sizeof(T);
-template <typename T, int kD> constexpr int kStageBytes = 2 * kStep * kRowBytes<T, kD>;      // K, then V
-template <typename T, int kD> constexpr int kAttendSmem = kWarps * kStages * kStageBytes<T, kD>;
-
-// byte offset of 16-byte chunk c of row r: chunks change places within a row so that eight rows' equal chunks lie in different banks
-template <typename T, int kD>
-__device__ __forceinline__ uint32_t chunk_at(int r, int c) { return (uint32_t)(r * kRowBytes<T, kD> + ((c ^ (r & 7)) << 4)); }
+// A stage of a warp's ring: the step's keys, then its values, as sub-tiles of 16 rows of 128 bytes in TMA's 128-byte swizzle.
+constexpr int kSubTile = kStep * 128;
+template <typename T, int kD> constexpr int kSubTiles = kD * (int)sizeof(T) / 128;
+template <typename T, int kD> constexpr int kStageBytes = 2 * kSubTiles<T, kD> * kSubTile;
+template <typename T, int kD, int kWarps> constexpr int kAttendSmem = kWarps * kStages * kStageBytes<T, kD>;
+// byte offset of the 16-byte chunk c of row r
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) { return (uint32_t)((c >> 3) * kSubTile + r * 128 + (((c & 7) ^ (r & 7)) << 4)); }
 
 // One warp's state over its steps of a piece: 16 query rows, of which a thread of the mma.sync form holds rows g and g + 8 (g = lane / 4).
 template <typename T, int kD> struct Rows16 {
@@ -144,7 +139,7 @@ __device__ __forceinline__ void load_queries(Rows16<T, kD>& w, const AttendArgs&
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     const int r = row0 + g + 8 * e;
-    base[e] = r < a.rows ? reinterpret_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)(h * a.G + r / a.T) * a.qs[1] + (int64_t)(r % a.T) * a.qs[2]
+    base[e] = r < a.rows ? reinterpret_cast<const T*>(a.q) + b * a.qs[0] + (int64_t)(h * a.G + a.head(r)) * a.qs[1] + (int64_t)a.token(r) * a.qs[2]
                          : nullptr;
   }
 #pragma unroll
@@ -178,14 +173,14 @@ __device__ __forceinline__ uint32_t pack16(float a, float b) {
 template <typename T, int kD, typename Seen, typename Keep>
 __device__ __forceinline__ void take_step(Rows16<T, kD>& w, const uint8_t* stage, float scale_log2, bool all, Seen seen, Keep keep) {
   const int lane = threadIdx.x & 31, t4 = lane & 3;
-  float s[2][4] = {};
+  float s[2][4] = {}, s1[2][4] = {};                 // even and odd features: two shorter chains of products
   const int kr = (lane >> 4) * 8 + (lane & 7), kc = (lane >> 3) & 1;
 #pragma unroll
   for (int kk = 0; kk < kD / 16; ++kk) {
     uint32_t f[4];
-    ldmatrix_x4(f, stage + chunk_at<T, kD>(kr, kk * 2 + kc));
-    mma16<T>(s[0], w.q[kk][0], w.q[kk][1], w.q[kk][2], w.q[kk][3], f[0], f[1]);
-    mma16<T>(s[1], w.q[kk][0], w.q[kk][1], w.q[kk][2], w.q[kk][3], f[2], f[3]);
+    ldmatrix_x4(f, stage + chunk_at(kr, kk * 2 + kc));
+    mma16<T>(kk & 1 ? s1[0] : s[0], w.q[kk][0], w.q[kk][1], w.q[kk][2], w.q[kk][3], f[0], f[1]);
+    mma16<T>(kk & 1 ? s1[1] : s[1], w.q[kk][0], w.q[kk][1], w.q[kk][2], w.q[kk][3], f[2], f[3]);
   }
   // element (n, e): row g + 8 (e / 2), key 8 n + 2 t + e % 2
   float mx[2] = {-INFINITY, -INFINITY};
@@ -193,7 +188,7 @@ __device__ __forceinline__ void take_step(Rows16<T, kD>& w, const uint8_t* stage
   for (int n = 0; n < 2; ++n)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      float x = s[n][e] * scale_log2;
+      float x = (s[n][e] + s1[n][e]) * scale_log2;
       if (!all && !seen(e >> 1, 8 * n + 2 * t4 + (e & 1))) x = -INFINITY;
       s[n][e] = x;
       mx[e >> 1] = max3_nan(mx[e >> 1], x, x);
@@ -233,12 +228,12 @@ __device__ __forceinline__ void take_step(Rows16<T, kD>& w, const uint8_t* stage
   // the weights enter the product in 16 bits (half a step of relative error each, as in every kernel here); their sum l does not
   const uint32_t p0 = pack16<T>(s[0][0], s[0][1]), p1 = pack16<T>(s[0][2], s[0][3]);
   const uint32_t p2 = pack16<T>(s[1][0], s[1][1]), p3 = pack16<T>(s[1][2], s[1][3]);
-  const uint8_t* vs = stage + kStep * kRowBytes<T, kD>;
+  const uint8_t* vs = stage + kSubTiles<T, kD> * kSubTile;
   const int vr = ((lane >> 3) & 1) * 8 + (lane & 7), vc = lane >> 4;
 #pragma unroll
   for (int n = 0; n < kD / 16; ++n) {
     uint32_t f[4];
-    ldmatrix_x4_trans(f, vs + chunk_at<T, kD>(vr, n * 2 + vc));
+    ldmatrix_x4_trans(f, vs + chunk_at(vr, n * 2 + vc));
     mma16<T>(w.o[2 * n], p0, p1, p2, p3, f[0], f[1]);
     mma16<T>(w.o[2 * n + 1], p0, p1, p2, p3, f[2], f[3]);
   }
@@ -265,25 +260,39 @@ template <int kD> struct Rows32 {
   float m[kRowTile], l[kRowTile];
 };
 
-template <typename T, int kD>
-__global__ void __launch_bounds__(kWarps * 32) paged_attend_kernel(const __grid_constant__ AttendArgs a) {
-  extern __shared__ __align__(1024) uint8_t smem[];
+// kWarps: 4, with two CTAs an SM or four for 64 features; 8 on whole rows where there are no more of them than SMs, and the latency of a
+// warp's steps counts (us: 32 rows of 300 keys 10.1 with 4, 8.8 with 8; 512 rows 23.5 / 34.6).
+template <typename T, int kD, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32) paged_attend_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                                                                   const __grid_constant__ AttendArgs a) {
+  extern __shared__ uint8_t smem_raw[];
   __shared__ float2 s_stat[kWarps][kRowTile];
+  __shared__ int s_free[kWarps];
+  __shared__ uint64_t s_full[kWarps][kStages];
   constexpr bool kF32 = std::is_same<T, float>::value;
+  constexpr int kSub = kSubTiles<T, kD>;
+  uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
+  if (lane == 0) {
+    for (int k = 0; k < kStages; ++k) mbar_init(smem_u32(&s_full[warp][k]), 1);
+    mbar_init_fence();
+    prefetch_tensormap(&tm_k);
+    prefetch_tensormap(&tm_v);
+  }
+  __syncwarp();
   grid_dep_wait();
   grid_dep_launch();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Pages& pg = a.pg;
   const int per_seq = pg.Hkv * a.tiles;
   const int len_lane = lane < pg.B ? pg.length(lane) : 0;      // the first 32 lengths stay at hand
   auto length = [&](int b) { return b < 32 ? __shfl_sync(0xffffffffu, len_lane, b) : pg.length(b); };      // (the same b in all lanes)
-  auto steps_of = [&](int b) { return (int64_t)per_seq * span_of(b < 32 ? len_lane : pg.length(b), a.T, a.window, a.sinks).steps; };
+  auto steps_of = [&](int b) { return per_seq * span_of(b < 32 ? len_lane : pg.length(b), a.T, a.window, a.sinks).steps; };
   // sequences without keys: their outputs are zeros (a share of the sequences for every CTA)
   for (int b = blockIdx.x; b < pg.B; b += gridDim.x)
     if (length(b) == 0)
       for (int64_t i = tid; i < (int64_t)a.H * a.T * pg.D; i += kWarps * 32) reinterpret_cast<T*>(a.o)[b * (int64_t)a.H * a.T * pg.D + i] = from_f32<T>(0.f);
-  uint8_t* ring = smem + warp * kStages * kStageBytes<T, kD>;
-  const uint32_t ring_at = smem_u32(ring);
+  uint8_t* const ring = smem + warp * kStages * kStageBytes<T, kD>;
+  const uint32_t ring_at = (uint32_t)warp_uniform((int)smem_u32(ring)), bar_at = (uint32_t)warp_uniform((int)smem_u32(&s_full[warp][0]));
   static_assert(kRowTile * kD * 4 <= kStageBytes<T, kD>, "a warp's outputs fit a stage");
 
   // A place in the line, moved on by whole warps.
@@ -302,70 +311,77 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attend_kernel(const __grid_
       } while (p.sp.steps == 0);
     }
   };
-  auto lo_seen = [&](int len) {                      // the first key that the first token's window holds
-    const int p0 = len - a.T;
-    return a.window > 0 && p0 >= a.window ? p0 - a.window + 1 : 0;
-  };
-
   const int64_t cap = (int64_t)pg.max_pages << pg.shift;
+  int i = 0;                                         // this warp's steps that are done; stage (i + kStages - 1) % kStages is free
 
   // The steps begin .. end - 1 of the line, of which `now` is the first.
-  auto take = [&](int64_t begin, int64_t end, Place now) {
-    // Loads run ahead of the steps that use them, also into the next item: first the page's number, a step later its rows.
-    const int mine = (int)((end - begin - warp + kWarps - 1) / kWarps);      // this warp's steps: begin + warp, + kWarps, ...
+  auto take = [&](int begin, int end, Place now) {
+    // Loads run ahead of the steps that use them, also into the next item: first the page's number, then its rows.
+    const int last = i + (end - begin - warp + kWarps - 1) / kWarps;       // this warp's steps: begin + warp, + kWarps, ...
     Place ask = now;
     ask.step += warp;
     settle(ask);
-    struct Asked { int b, h, key0, len, id; } next;
-    unsigned bad = 0;                                  // bit i % kStages: the step in that stage has no page
-    auto ask_page = [&](int i) {
-      if (i >= mine) return;
-      next.b = ask.b;
-      next.h = ask.item / a.tiles;
-      next.key0 = ask.sp.key(ask.step);
-      next.len = ask.sp.len;
-      next.id = pg.id(next.b, next.key0 >> pg.shift);
+    struct Asked { int h, key0, id; };
+    unsigned bad = 0;                                // bit n % kStages: step n, in that stage, has no page
+    auto ask_page = [&](int n) {
+      Asked x = {0, 0, 0};
+      if (n >= last) return x;
+      x.h = a.tiles == 1 ? ask.item : ask.item / a.tiles;
+      x.key0 = ask.sp.key(ask.step);
+      x.id = pg.id(ask.b, x.key0 >> pg.shift);
       ask.step += kWarps;
       settle(ask);
+      return x;
     };
-    auto issue = [&](int i) {
-      if (i < mine) {
-        const bool ok = next.id >= 0 && next.id < pg.n_pages;
-        if (!ok && lane == 0) note(pg.status, kBadPage);
-        const unsigned bit = 1u << (i % kStages);
-        bad = ok ? bad & ~bit : bad | bit;
-        const int row = next.key0 & (pg.page - 1), lo = lo_seen(next.len);
-        const T* kp = reinterpret_cast<const T*>(pg.k) + (ok ? (int64_t)next.id * pg.ks[0] + next.h * pg.ks[1] + (int64_t)row * pg.ks[2] : 0);
-        const T* vp = reinterpret_cast<const T*>(pg.v) + (ok ? (int64_t)next.id * pg.vs[0] + next.h * pg.vs[1] + (int64_t)row * pg.vs[2] : 0);
-        const uint32_t to = ring_at + (uint32_t)(i % kStages) * kStageBytes<T, kD>;
-        constexpr int kChunks = kRowBytes<T, kD> / 16, kVec = 16 / (int)sizeof(T);
+    auto issue = [&](int n, const Asked& x) {
+      if (n >= last) return;
+      // one elected lane issues; what it needs is made warp-uniform, or the compiler moves it to uniform registers copy by copy
+      const int asked = warp_uniform(x.id), row = warp_uniform(x.key0 & (pg.page - 1)), h = warp_uniform(x.h);
+      const bool ok = asked >= 0 && asked < pg.n_pages;
+      const unsigned bit = 1u << (n % kStages);
+      bad = ok ? bad & ~bit : bad | bit;
+      const uint32_t to = ring_at + (uint32_t)(n % kStages) * kStageBytes<T, kD>, bar = bar_at + (uint32_t)(n % kStages) * 8u;
+      const int id = ok ? asked : pg.n_pages;        // behind the pool: zeros
+      if (elect_one()) {
+        if (!ok) note(pg.status, kBadPage);
+        mbar_arrive_expect_tx(bar, kStageBytes<T, kD>);
 #pragma unroll
-        for (int e = 0; e < kStep * kChunks / 32; ++e) {
-          const int r = (e * 32 + lane) / kChunks, c = (e * 32 + lane) % kChunks;
-          const int key = next.key0 + r;
-          const bool take = ok && key < next.len && (key >= lo || key < a.sinks) && c * kVec < pg.D;
-          const int64_t off_k = take ? (int64_t)r * pg.ks[2] + c * kVec : 0, off_v = take ? (int64_t)r * pg.vs[2] + c * kVec : 0;
-          cp_async16(to + chunk_at<T, kD>(r, c), kp + off_k, take);
-          cp_async16(to + kStep * kRowBytes<T, kD> + chunk_at<T, kD>(r, c), vp + off_v, take);
+        for (int c = 0; c < kSub; ++c) {
+          tma_load_4d(to + c * kSubTile, &tm_k, bar, c * (128 / (int)sizeof(T)), row, h, id);
+          tma_load_4d(to + (kSub + c) * kSubTile, &tm_v, bar, c * (128 / (int)sizeof(T)), row, h, id);
         }
       }
-      cp_async_commit();
     };
+    Asked next;
+    {
+      Asked first[kStages];
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) {
-      ask_page(i);
-      issue(i);
+      for (int k = 0; k < kStages; ++k) first[k] = ask_page(i + k);
+#pragma unroll
+      for (int k = 0; k < kStages - 1; ++k) issue(i + k, first[k]);
+      next = first[kStages - 1];
     }
-    ask_page(kStages - 1);
-
-    int i = 0;                                         // this warp's steps that are done; stage (i + kStages - 1) % kStages is free
-    for (int64_t at = begin; at < end;) {
+    for (int at = begin; at < end;) {
       const Span sp = now.sp;
       const int b = now.b, step0 = now.step, h = now.item / a.tiles, row0 = (now.item - h * a.tiles) * kRowTile;
-      const int count = (int)min((int64_t)(sp.steps - step0), end - at);
+      const int count = min(sp.steps - step0, end - at);
       const int p0 = sp.len - a.T;                               // position of the first token's queries
-      const int first = (int)((warp - (at - begin)) & (kWarps - 1));
+      const int first = (warp - (at - begin)) & (kWarps - 1);
       const int64_t score_row = ((int64_t)b * pg.Hkv + h) * a.rows;
+      const int lo = a.window > 0 && p0 >= a.window ? p0 - a.window + 1 : 0;      // the first key that the first token's window holds
+      // The step's rows are there; those that nobody sees are made zeros (scores are hidden by a select, values would be multiplied).
+      auto arrive = [&](int key0) {
+        mbar_wait(bar_at + (uint32_t)(i % kStages) * 8u, (i / kStages) & 1, pg.status, kErrRing);
+        if (key0 + kStep <= sp.len && (key0 >= lo || key0 + kStep <= a.sinks)) return;
+        const uint32_t at_v = ring_at + (uint32_t)(i % kStages) * kStageBytes<T, kD> + kSub * kSubTile;
+        for (int r = 0; r < kStep; ++r) {
+          const int key = key0 + r;
+          if (key < sp.len && (key >= lo || key < a.sinks)) continue;
+          for (int c = lane; c < kSub * 8; c += 32)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at_v + (c >> 3) * kSubTile + r * 128 + (c & 7) * 16), "r"(0) : "memory");
+        }
+        __syncwarp();
+      };
       // every row that exists sees all 16 keys (the last token's window is the one that has moved on furthest)
       auto all_see = [&](int key0, bool no_page) {
         return !no_page && p0 >= 0 && key0 + kStep - 1 <= p0 && (a.window == 0 || p0 + a.T - 1 - key0 < a.window);
@@ -378,15 +394,14 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attend_kernel(const __grid_
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int r = row0 + (lane >> 2) + 8 * e;
-          pos[e] = r < a.rows ? p0 + r % a.T : -1;
+          pos[e] = r < a.rows ? p0 + a.token(r) : -1;
         }
         for (int k = first; k < count; k += kWarps, ++i) {
-          cp_async_wait<kStages - 2>();
-          __syncwarp();
           const bool no_page = bad >> (i % kStages) & 1u;
-          issue(i + kStages - 1);
-          ask_page(i + kStages);
+          issue(i + kStages - 1, next);
+          next = ask_page(i + kStages);
           const int key0 = sp.key(step0 + k);
+          arrive(key0);
           take_step<T, kD>(w, ring + (i % kStages) * kStageBytes<T, kD>, a.scale_log2, all_see(key0, no_page),
               [&](int e, int j) {
                 const int key = key0 + j;
@@ -404,6 +419,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attend_kernel(const __grid_
                           make_float2(s[n][2 * e], s[n][2 * e + 1]);
                   }
               });
+          if (i + kStages < last) fence_proxy_async_smem();      // TMA writes the stage again
           __syncwarp();
         }
         leave_result<T, kD>(w, reinterpret_cast<float*>(ring + ((i + kStages - 1) % kStages) * kStageBytes<T, kD>), s_stat[warp]);
@@ -411,7 +427,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attend_kernel(const __grid_
         // fp32 on the FMA units.  Scores: lane = (key, half of the features); outputs: lane = kD / 32 features of every row.
         Rows32<kD> w;
         const int n_rows = min(kRowTile, a.rows - row0);
-        float* const qs = reinterpret_cast<float*>(smem + kAttendSmem<T, kD>);         // [16][kD], the CTA's query rows
+        float* const qs = reinterpret_cast<float*>(smem + kAttendSmem<T, kD, kWarps>);         // [16][kD], the CTA's query rows
         float* const ps = qs + kRowTile * kD + warp * kRowTile * kStep;                // [16][16], the warp's weights
         for (int e = tid; e < kRowTile * kD; e += kWarps * 32) {
           const int r = row0 + e / kD, c = e % kD;
@@ -427,12 +443,11 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attend_kernel(const __grid_
           for (int c = 0; c < kD / 32; ++c) w.o[r][c] = 0.f;
         }
         for (int k = first; k < count; k += kWarps, ++i) {
-          cp_async_wait<kStages - 2>();
-          __syncwarp();
           const bool no_page = bad >> (i % kStages) & 1u;
-          issue(i + kStages - 1);
-          ask_page(i + kStages);
+          issue(i + kStages - 1, next);
+          next = ask_page(i + kStages);
           const int key0 = sp.key(step0 + k);
+          arrive(key0);
           const uint8_t* stage = ring + (i % kStages) * kStageBytes<T, kD>;
           const int j = lane & 15, half = lane >> 4;
           float s[kRowTile];
@@ -440,7 +455,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attend_kernel(const __grid_
           for (int r = 0; r < kRowTile; ++r) s[r] = 0.f;
           for (int c = 0; c < kD / 8; ++c) {                   // the half's 16-byte chunks
             const int chunk = half * (kD / 8) + c;
-            const float4 x = *reinterpret_cast<const float4*>(stage + chunk_at<T, kD>(j, chunk));
+            const float4 x = *reinterpret_cast<const float4*>(stage + chunk_at(j, chunk));
 #pragma unroll
             for (int r = 0; r < kRowTile; ++r) {
               if (r >= n_rows) break;
@@ -452,7 +467,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attend_kernel(const __grid_
           for (int r = 0; r < kRowTile; ++r) {
             if (r >= n_rows) break;
             float x = (s[r] + __shfl_xor_sync(0xffffffffu, s[r], 16)) * a.scale_log2;
-            const int pos = p0 + (row0 + r) % a.T, key = key0 + j;
+            const int pos = p0 + a.token(row0 + r), key = key0 + j;
             if (no_page || key > pos || !(a.window == 0 || pos - key < a.window || key < a.sinks)) x = -INFINITY;
             if (a.weights != nullptr && half == 0) a.scores[(score_row + row0 + r) * cap + key] = x;
             float mx = x;
@@ -472,13 +487,13 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attend_kernel(const __grid_
             if (half == 0) ps[r * kStep + j] = p;
           }
           __syncwarp();
-          const uint8_t* vs = stage + kStep * kRowBytes<T, kD>;
+          const uint8_t* vs = stage + kSubTiles<T, kD> * kSubTile;
           for (int key = 0; key < kStep; ++key) {
             float v[kD / 32];
 #pragma unroll
             for (int c = 0; c < kD / 32; ++c) {
               const int f = lane * (kD / 32) + c;
-              v[c] = *reinterpret_cast<const float*>(vs + chunk_at<T, kD>(key, f / 4) + (f % 4) * 4);
+              v[c] = *reinterpret_cast<const float*>(vs + chunk_at(key, f / 4) + (f % 4) * 4);
             }
 #pragma unroll
             for (int r = 0; r < kRowTile; ++r) {
@@ -488,6 +503,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attend_kernel(const __grid_
               for (int c = 0; c < kD / 32; ++c) w.o[r][c] = fmaf(p, v[c], w.o[r][c]);
             }
           }
+          if (i + kStages < last) fence_proxy_async_smem();
           __syncwarp();
         }
         float* const result = reinterpret_cast<float*>(ring + ((i + kStages - 1) % kStages) * kStageBytes<T, kD>);
@@ -500,13 +516,13 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attend_kernel(const __grid_
         }
       }
 
-      // the four warps' results, joined, 8 threads a row, while the next item's rows are on their way
+      // the warps' results, joined, while the next item's rows are on their way
       const int free_stage = (i + kStages - 1) % kStages;
-      __shared__ int s_free[kWarps];
       if (lane == 0) s_free[warp] = free_stage;
       __syncthreads();
       {
-        const int r = tid >> 3, part = tid & 7;
+        constexpr int kPer = kWarps * 2;               // threads a row
+        const int r = tid / kPer, part = tid % kPer;
         const float* res[kWarps];
         float mx = -INFINITY, l = 0.f, f[kWarps];
 #pragma unroll
@@ -523,11 +539,11 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attend_kernel(const __grid_
         const bool exists = row0 + r < a.rows, all = count == sp.steps;
         const int64_t slot = 2 * (int64_t)blockIdx.x + (step0 > 0 ? 0 : 1);
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        T* const orow = reinterpret_cast<T*>(a.o) + (((int64_t)b * a.H + h * a.G + (row0 + r) / a.T) * a.T + (row0 + r) % a.T) * pg.D;
+        T* const orow = reinterpret_cast<T*>(a.o) + (((int64_t)b * a.H + h * a.G + a.head(row0 + r)) * a.T + a.token(row0 + r)) * pg.D;
         float* const arow = a.acc + (slot * kRowTile + r) * kD;
 #pragma unroll
-        for (int c = 0; c < kD / 32; ++c) {
-          const int col = c * 32 + part * 4;
+        for (int c = 0; c < kD / (4 * kPer); ++c) {
+          const int col = (c * kPer + part) * 4;
           float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
           for (int k = 0; k < kWarps; ++k) {
@@ -551,6 +567,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attend_kernel(const __grid_
           else if (a.weights != nullptr) a.whole[(((int64_t)b * pg.Hkv + h) * a.tiles + row0 / kRowTile) * kRowTile + r] = make_float2(mx, l);
         }
       }
+      fence_proxy_async_smem();                      // the outputs' stages belong to TMA again
       __syncthreads();
       at += count;
       now.step += count;
@@ -559,8 +576,7 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attend_kernel(const __grid_
   };
 
   for (int x = blockIdx.x;; x += gridDim.x) {
-    int b, item, step = 0;
-    int64_t begin = 0, end;
+    int b, item, step = 0, begin = 0, end;
     Span sp;
     if (a.one_piece) {
       if (x >= pg.B * per_seq) break;
@@ -569,15 +585,16 @@ __global__ void __launch_bounds__(kWarps * 32) paged_attend_kernel(const __grid_
       sp = span_of(length(b), a.T, a.window, a.sinks);
       end = sp.steps;
     } else {
-      const int64_t total = warp_total(pg.B, steps_of), piece = piece_of(a, total);
+      const int total = warp_total(pg.B, steps_of), piece = piece_of(a, total);
+      if (blockIdx.x > (unsigned)(total / piece)) break;
       begin = blockIdx.x * piece;
       end = min(begin + piece, total);
       if (begin >= end) break;
       const Found f = warp_find(pg.B, begin, steps_of);
       b = f.b;
       sp = span_of(length(b), a.T, a.window, a.sinks);
-      item = (int)((begin - f.before) / sp.steps);
-      step = (int)(begin - f.before - (int64_t)item * sp.steps);
+      item = (begin - f.before) / sp.steps;
+      step = begin - f.before - item * sp.steps;
     }
     if (begin < end) take(begin, end, {b, item, step, sp});
     if (!a.one_piece) break;
@@ -594,20 +611,20 @@ __global__ void __launch_bounds__(kJoinThreads) paged_finish_kernel(const __grid
   const Pages& pg = a.pg;
   const int tid = threadIdx.x;
   const int per_seq = pg.Hkv * a.tiles;
-  auto steps_of = [&](int i) { return (int64_t)per_seq * span_of(pg.length(i), a.T, a.window, a.sinks).steps; };
+  auto steps_of = [&](int i) { return per_seq * span_of(pg.length(i), a.T, a.window, a.sinks).steps; };
   const bool join = (int)blockIdx.x < joins;
   const int x = join ? blockIdx.x / (kD / 32) : blockIdx.x - joins, slice = blockIdx.x % (kD / 32);
   const int64_t cap = (int64_t)pg.max_pages << pg.shift;
   const int runs = (int)((cap + kRunKeys - 1) / kRunKeys);
   const int b = join ? x / per_seq : x / runs / pg.Hkv;
-  const int64_t piece = piece_of(a, warp_total(pg.B, steps_of)), before = warp_total(b, steps_of);
+  const int piece = piece_of(a, warp_total(pg.B, steps_of)), before = warp_total(b, steps_of);
   const int len = pg.length(b);
   const Span sp = span_of(len, a.T, a.window, a.sinks);
   grid_dep_wait();
   grid_dep_launch();
   if (sp.steps == 0) return;
-  auto first_cta = [&](int item) { return (int)((before + (int64_t)item * sp.steps) / piece); };
-  auto last_cta = [&](int item) { return (int)((before + (int64_t)item * sp.steps + sp.steps - 1) / piece); };
+  auto first_cta = [&](int item) { return (before + item * sp.steps) / piece; };
+  auto last_cta = [&](int item) { return (before + item * sp.steps + sp.steps - 1) / piece; };
 
   if (join) {
     const int item = x - b * per_seq, c0 = first_cta(item), c1 = last_cta(item);
@@ -641,7 +658,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_finish_kernel(const __grid
       sum.y = fmaf(f, v.y, sum.y);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    T* const to = reinterpret_cast<T*>(a.o) + (((int64_t)b * a.H + h * a.G + (row0 + r) / a.T) * a.T + (row0 + r) % a.T) * pg.D + col;
+    T* const to = reinterpret_cast<T*>(a.o) + (((int64_t)b * a.H + h * a.G + a.head(row0 + r)) * a.T + a.token(row0 + r)) * pg.D + col;
     to[0] = from_f32<T>(sum.x * inv);
     to[1] = from_f32<T>(sum.y * inv);
     return;
@@ -983,13 +1000,15 @@ int status_of(Pages& pg) {             // behind all checks of arguments
   return pg.status == nullptr ? fail(LMK_ERR_CUDA, "no device status word") : LMK_OK;
 }
 
-template <typename T, int kD> constexpr int attend_smem() {
-  return kAttendSmem<T, kD> + (std::is_same<T, float>::value ? (kRowTile * kD + kWarps * kRowTile * kStep) * 4 : 0);
+template <typename T, int kD, int kWarps> constexpr int attend_smem() {
+  return 1024 + kAttendSmem<T, kD, kWarps> + (std::is_same<T, float>::value ? (kRowTile * kD + kWarps * kRowTile * kStep) * 4 : 0);
 }
 // CTAs of the attention kernel an SM holds (by shared memory: 192 KB in 16 bits at D = 128 are two CTAs)
 int attend_per_sm(int dtype, int D) { return dtype == LMK_F32 ? (D <= 64 ? 2 : 1) : (D <= 64 ? 4 : 2); }
 constexpr int kLeastSteps = 8;         // of a CTA: two a warp
-constexpr int kWholeSteps = 32;        // tables of up to this many steps a sequence: every row is one CTA's, and nothing is to be joined
+// Tables of up to this many steps a sequence: every row is one CTA's, and nothing is to be joined (us, whole / in pieces: 32 rows of 300 keys
+// 8.8 / 14.3, of 1000 15.2 / 14.5; 512 rows of 300 23.5 / 34.1).
+constexpr int kWholeSteps = 32;
 
 struct AttendPlan {
   int grid, rows, tiles, kD;
@@ -1014,19 +1033,29 @@ bool attend_sizes_ok(int B, int H, int Hkv, int T) {
   return B >= 1 && Hkv >= 1 && H >= Hkv && H % Hkv == 0 && T >= 1 && T <= 1024 && (int64_t)H / Hkv * T <= 4096 && (int64_t)B * H * T < (1 << 30);
 }
 
-template <typename T, int kD>
-int launch_attend(const AttendArgs& a, cudaStream_t st) {
+// a step's rows of one head: 128 bytes of features x 16 rows
+int page_map(CUtensorMap* m, const Pages& pg, const void* ptr, const int64_t st[3], int dtype) {
+  return tensor_map_pages(m, ptr, dtype, pg.n_pages, pg.Hkv, pg.page, pg.D, st, kStep);
+}
+template <typename T, int kD, int kWarps>
+int launch_attend(const AttendArgs& a, int dtype, cudaStream_t st) {
+  constexpr int kSmem = attend_smem<T, kD, kWarps>();
+  static_assert(kSmem <= 230000, "shared memory of one SM");
   static std::atomic<bool> ready[64];
   int dev = 0;
   LMK_CUDA(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64) return fail(LMK_ERR_UNSUPPORTED, "device index %d out of range", dev);
   if (!ready[dev].load(std::memory_order_acquire)) {
-    LMK_CUDA(cudaFuncSetAttribute(paged_attend_kernel<T, kD>, cudaFuncAttributeMaxDynamicSharedMemorySize, attend_smem<T, kD>()));
+    LMK_CUDA(cudaFuncSetAttribute(paged_attend_kernel<T, kD, kWarps>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     ready[dev].store(true, std::memory_order_release);
   }
+  CUtensorMap tk, tv;
+  int rc = page_map(&tk, a.pg, a.pg.k, a.pg.ks, dtype);
+  if (rc == LMK_OK) rc = page_map(&tv, a.pg, a.pg.v, a.pg.vs, dtype);
+  if (rc != LMK_OK) return rc;
   const int64_t items = (int64_t)a.pg.B * a.pg.Hkv * a.tiles;
   const unsigned grid = a.one_piece && items < a.grid ? (unsigned)items : (unsigned)a.grid;
-  LMK_CUDA(launch_overlapped(paged_attend_kernel<T, kD>, dim3(grid), dim3(kWarps * 32), attend_smem<T, kD>(), st, a));
+  LMK_CUDA(launch_overlapped(paged_attend_kernel<T, kD, kWarps>, dim3(grid), dim3(kWarps * 32), kSmem, st, tk, tv, a));
   const int64_t cap = (int64_t)a.pg.max_pages << a.pg.shift;
   const int64_t joins = !a.one_piece ? items * (kD / 32) : 0;
   const int64_t runs = a.weights != nullptr ? (cap + kRunKeys - 1) / kRunKeys * a.pg.B * a.pg.Hkv : 0;
@@ -1034,6 +1063,17 @@ int launch_attend(const AttendArgs& a, cudaStream_t st) {
   if (joins + runs > 0)
     LMK_CUDA(launch_overlapped(paged_finish_kernel<T, kD>, dim3((unsigned)(joins + runs)), dim3(kJoinThreads), sizeof(float2) * a.rows, st, a, (int)joins));
   return LMK_OK;
+}
+// (8 warps of fp32 rows of 128 features would not fit an SM's shared memory)
+template <typename T>
+int dispatch_attend(const AttendArgs& a, int kD, int dtype, cudaStream_t st) {
+  constexpr int kMore = std::is_same<T, float>::value ? 4 : 8;
+  int n_sm = 0;
+  const int rc = sm_count(&n_sm);
+  if (rc != LMK_OK) return rc;
+  const bool few = a.one_piece && (int64_t)a.pg.B * a.pg.Hkv * a.tiles <= n_sm;
+  if (kD == 64) return few ? launch_attend<T, 64, 8>(a, dtype, st) : launch_attend<T, 64, 4>(a, dtype, st);
+  return few ? launch_attend<T, 128, kMore>(a, dtype, st) : launch_attend<T, 128, 4>(a, dtype, st);
 }
 
 }  // namespace
@@ -1058,6 +1098,10 @@ extern "C" int lmk_paged_attend(const void* q, const int64_t q_strides[3], const
   LMK_CHECK_ARG(H >= Hkv && H % Hkv == 0, "paged attention: %d query heads are not a multiple of %d key heads", H, Hkv);
   LMK_CHECK_ARG(attend_sizes_ok(B, H, Hkv, T), "paged attention: T=%d tokens of %d heads a key head are too many (up to 1024 tokens, 4096 rows)", T, H / Hkv);
   LMK_CHECK_ARG(window >= 0 && sinks >= 0, "paged attention: window=%d and sinks=%d must not be negative", window, sinks);
+  LMK_CHECK_ARG((int64_t)B * Hkv * ((H / Hkv * T + kRowTile - 1) / kRowTile) * ((int64_t)max_pages * page / kStep) <= INT32_MAX,
+                "paged attention: %d sequences of up to %lld tokens and %d key heads are too many for one call", B, (long long)max_pages * page, Hkv);
+  LMK_CHECK_ARG((n_pages == 1 || (k_strides[0] > 0 && v_strides[0] > 0)) && (Hkv == 1 || (k_strides[1] > 0 && v_strides[1] > 0)) &&
+                    k_strides[2] >= D && v_strides[2] >= D, "paged attention: pages must not be broadcast, nor their rows overlap");
   LMK_CHECK_ARG(isfinite(sm_scale) && isfinite(decay), "paged attention: scale and decay must be finite");
   LMK_CHECK_ARG(((uintptr_t)weights & 15) == 0, "paged attention: weights must start on a 16-byte boundary");
   const int pair = 4 / dtype_size(dtype);
@@ -1082,11 +1126,9 @@ extern "C" int lmk_paged_attend(const void* q, const int64_t q_strides[3], const
   a.one_piece = (int64_t)max_pages * page <= kWholeSteps * kStep;
   a.scale_log2 = sm_scale * kLog2e;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define LMK_ATTEND(T) return p.kD == 64 ? launch_attend<T, 64>(a, st) : launch_attend<T, 128>(a, st)
-  if (dtype == LMK_BF16) LMK_ATTEND(__nv_bfloat16);
-  if (dtype == LMK_F16) LMK_ATTEND(__half);
-  LMK_ATTEND(float);
-#undef LMK_ATTEND
+  if (dtype == LMK_BF16) return dispatch_attend<__nv_bfloat16>(a, p.kD, dtype, st);
+  if (dtype == LMK_F16) return dispatch_attend<__half>(a, p.kD, dtype, st);
+  return dispatch_attend<float>(a, p.kD, dtype, st);
 }
 
 extern "C" int lmk_paged_append(const void* k_new, const void* v_new, const int64_t k_new_strides[3], const int64_t v_new_strides[3],
