@@ -20,25 +20,28 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
-// 64 rows of D features -> [kD][kPad], rows from `valid` on and features from D on as zeros
-template <int kD>
-__device__ __forceinline__ void load_transposed(float* to, const float* from, int64_t stride, int valid, int D) {
-  for (int e = threadIdx.x; e < kTile * kD / 4; e += kThreads) {
-    const int r = e / (kD / 4), c = (e % (kD / 4)) * 4;
-    const float4 x = r < valid && c < D ? load4(from + r * stride + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-    to[c * kPad + r] = x.x;
-    to[(c + 1) * kPad + r] = x.y;
-    to[(c + 2) * kPad + r] = x.z;
-    to[(c + 3) * kPad + r] = x.w;
+// A 64-row tile on its way to shared memory: asked for while the tile in front is worked on, stored as [kD][kPad].  A warp takes 32 rows of
+// one 16-byte chunk: the stores of a feature lie next to each other (along the features they met in two banks).
+template <int kD> struct Tile {
+  float4 x[kTile * kD / 4 / kThreads];
+  __device__ __forceinline__ void ask(const float* from, int64_t stride, int valid, int D) {
+#pragma unroll
+    for (int e = 0; e < kTile * kD / 4 / kThreads; ++e) {
+      const int i = e * kThreads + threadIdx.x, r = i % kTile, c = i / kTile * 4;
+      x[e] = r < valid && c < D ? load4(from + r * stride + c) : make_float4(0.f, 0.f, 0.f, 0.f);      // (rows behind the end: zeros)
+    }
   }
-}
-template <int kD>
-__device__ __forceinline__ void load_rows(float* to, const float* from, int64_t stride, int valid, int D) {      // -> [64][kD]
-  for (int e = threadIdx.x; e < kTile * kD / 4; e += kThreads) {
-    const int r = e / (kD / 4), c = (e % (kD / 4)) * 4;
-    *reinterpret_cast<float4*>(to + r * kD + c) = r < valid && c < D ? load4(from + r * stride + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+  __device__ __forceinline__ void store(float* to) const {
+#pragma unroll
+    for (int e = 0; e < kTile * kD / 4 / kThreads; ++e) {
+      const int i = e * kThreads + threadIdx.x, r = i % kTile, c = i / kTile * 4;
+      to[c * kPad + r] = x[e].x;
+      to[(c + 1) * kPad + r] = x[e].y;
+      to[(c + 2) * kPad + r] = x[e].z;
+      to[(c + 3) * kPad + r] = x[e].w;
+    }
   }
-}
+};
 // d[4][4] = sum over n of a[n][row ..] b[n][col ..]
 template <int kN>
 __device__ __forceinline__ void product(float (&d)[4][4], const float* a, const float* b, int ty, int tx) {
@@ -57,6 +60,28 @@ __device__ __forceinline__ void product(float (&d)[4][4], const float* a, const 
       for (int j = 0; j < 4; ++j) d[i][j] = fmaf(xs[i], ys[j], d[i][j]);
   }
 }
+// d[4][kD / 16] += sum over 64 n of a[n][row ..] b[feature tx + 16 c][n], four n at a time
+template <int kD>
+__device__ __forceinline__ void accumulate(float (&d)[4][kD / 16], const float* a, const float* b, int ty, int tx) {
+#pragma unroll 2
+  for (int n = 0; n < kTile; n += 4) {
+    float4 x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = *reinterpret_cast<const float4*>(a + (n + e) * kPad + ty * 4);
+#pragma unroll
+    for (int c = 0; c < kD / 16; ++c) {
+      const float4 y = *reinterpret_cast<const float4*>(b + (c * 16 + tx) * kPad + n);
+      const float ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        d[0][c] = fmaf(x[e].x, ys[e], d[0][c]);
+        d[1][c] = fmaf(x[e].y, ys[e], d[1][c]);
+        d[2][c] = fmaf(x[e].z, ys[e], d[2][c]);
+        d[3][c] = fmaf(x[e].w, ys[e], d[3][c]);
+      }
+    }
+  }
+}
 __device__ __forceinline__ int length_of(const WindowParams& p, int b) {
   return p.lengths == nullptr ? p.Lk : min(max(ld_behind_wait(p.lengths + b), 0), p.Lk);
 }
@@ -64,7 +89,7 @@ __device__ __forceinline__ int length_of(const WindowParams& p, int b) {
 template <int kD>
 __global__ void __launch_bounds__(kThreads) window_fwd_f32_kernel(const __grid_constant__ WindowParams p, float scale_log2) {
   extern __shared__ float smem[];
-  float *qt = smem, *kt = qt + kD * kPad, *vr = kt + kD * kPad, *pt = vr + kTile * kD;      // pt [key][row]
+  float *qt = smem, *kt = qt + kD * kPad, *vt = kt + kD * kPad, *pt = vt + kD * kPad;      // pt [key][row]
   grid_dep_wait();
   grid_dep_launch();
   const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
@@ -74,7 +99,9 @@ __global__ void __launch_bounds__(kThreads) window_fwd_f32_kernel(const __grid_c
   const float* q = (const float*)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)tile * kTile * p.qs[2];
   const float* k = (const float*)p.k + b * p.ks[0] + hk * p.ks[1];
   const float* v = (const float*)p.v + b * p.vs[0] + hk * p.vs[1];
-  load_transposed<kD>(qt, q, p.qs[2], min(rows, len - p0), p.D);
+  Tile<kD> tk, tv;
+  tk.ask(q, p.qs[2], min(rows, len - p0), p.D);
+  tk.store(qt);
   float m[4], l[4], o[4][kD / 16];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -84,12 +111,20 @@ __global__ void __launch_bounds__(kThreads) window_fwd_f32_kernel(const __grid_c
     for (int c = 0; c < kD / 16; ++c) o[i][c] = 0.f;
   }
   const KeyTiles kts = keys_of_queries(tile, kTile, kTile, p.Lq, off, len, p.window, p.sinks);
-  for (int i = 0, n = kts.sink_tiles + kts.last - kts.first + 1; i < n; ++i) {
-    const int key0 = (i < kts.sink_tiles ? i : kts.first + i - kts.sink_tiles) * kTile;
+  const int n = kts.sink_tiles + kts.last - kts.first + 1;
+  auto key_of = [&](int i) { return (i < kts.sink_tiles ? i : kts.first + i - kts.sink_tiles) * kTile; };
+  auto ask = [&](int i) {
+    tk.ask(k + key_of(i) * p.ks[2], p.ks[2], len - key_of(i), p.D);
+    tv.ask(v + key_of(i) * p.vs[2], p.vs[2], len - key_of(i), p.D);
+  };
+  if (n > 0) ask(0);
+  for (int i = 0; i < n; ++i) {
+    const int key0 = key_of(i);
     __syncthreads();
-    load_transposed<kD>(kt, k + key0 * p.ks[2], p.ks[2], len - key0, p.D);
-    load_rows<kD>(vr, v + key0 * p.vs[2], p.vs[2], len - key0, p.D);
+    tk.store(kt);
+    tv.store(vt);
     __syncthreads();
+    if (i + 1 < n) ask(i + 1);
     float s[4][4];
     product<kD>(s, qt, kt, ty, tx);
 #pragma unroll
@@ -119,22 +154,7 @@ __global__ void __launch_bounds__(kThreads) window_fwd_f32_kernel(const __grid_c
       }
     }
     __syncthreads();
-#pragma unroll 4
-    for (int j = 0; j < kTile; ++j) {
-      const float4 x = *reinterpret_cast<const float4*>(pt + j * kPad + ty * 4);
-      const float xs[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int c = 0; c < kD / 64; ++c) {
-        const float4 y = *reinterpret_cast<const float4*>(vr + j * kD + c * 64 + tx * 4);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          o[r][4 * c] = fmaf(xs[r], y.x, o[r][4 * c]);
-          o[r][4 * c + 1] = fmaf(xs[r], y.y, o[r][4 * c + 1]);
-          o[r][4 * c + 2] = fmaf(xs[r], y.z, o[r][4 * c + 2]);
-          o[r][4 * c + 3] = fmaf(xs[r], y.w, o[r][4 * c + 3]);
-        }
-      }
-    }
+    accumulate<kD>(o, pt, vt, ty, tx);
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
@@ -145,10 +165,8 @@ __global__ void __launch_bounds__(kThreads) window_fwd_f32_kernel(const __grid_c
     const int64_t at = (int64_t)bh * p.Lq + tile * kTile + row;
     const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
 #pragma unroll
-    for (int c = 0; c < kD / 64; ++c)
-      if (c * 64 + tx * 4 < p.D)
-        *reinterpret_cast<float4*>((float*)p.o + at * p.D + c * 64 + tx * 4) =
-            make_float4(o[r][4 * c] * inv, o[r][4 * c + 1] * inv, o[r][4 * c + 2] * inv, o[r][4 * c + 3] * inv);
+    for (int c = 0; c < kD / 16; ++c)
+      if (c * 16 + tx < p.D) ((float*)p.o)[at * p.D + c * 16 + tx] = o[r][c] * inv;
     if (tx == 0) p.lse[at] = l[r] == 0.f ? INFINITY : m[r] + log2f(l[r]);
   }
 }
@@ -167,8 +185,11 @@ __global__ void __launch_bounds__(kThreads) window_dq_f32_kernel(const __grid_co
   const int64_t row0 = (int64_t)bh * p.Lq + tile * kTile;
   const float* k = (const float*)p.k + b * p.ks[0] + hk * p.ks[1];
   const float* v = (const float*)p.v + b * p.vs[0] + hk * p.vs[1];
-  load_transposed<kD>(qt, (const float*)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)tile * kTile * p.qs[2], p.qs[2], valid, p.D);
-  load_transposed<kD>(gt, (const float*)p.dO + b * p.dos[0] + h * p.dos[1] + (int64_t)tile * kTile * p.dos[2], p.dos[2], valid, p.D);
+  Tile<kD> tk, tv;
+  tk.ask((const float*)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)tile * kTile * p.qs[2], p.qs[2], valid, p.D);
+  tv.ask((const float*)p.dO + b * p.dos[0] + h * p.dos[1] + (int64_t)tile * kTile * p.dos[2], p.dos[2], valid, p.D);
+  tk.store(qt);
+  tv.store(gt);
   __syncthreads();
   float delta[4], lse[4], dq[4][kD / 16];
 #pragma unroll
@@ -186,12 +207,20 @@ __global__ void __launch_bounds__(kThreads) window_dq_f32_kernel(const __grid_co
     for (int c = 0; c < kD / 16; ++c) dq[r][c] = 0.f;
   }
   const KeyTiles kts = keys_of_queries(tile, kTile, kTile, p.Lq, off, len, p.window, p.sinks);
-  for (int i = 0, n = kts.sink_tiles + kts.last - kts.first + 1; i < n; ++i) {
-    const int key0 = (i < kts.sink_tiles ? i : kts.first + i - kts.sink_tiles) * kTile;
+  const int n = kts.sink_tiles + kts.last - kts.first + 1;
+  auto key_of = [&](int i) { return (i < kts.sink_tiles ? i : kts.first + i - kts.sink_tiles) * kTile; };
+  auto ask = [&](int i) {
+    tk.ask(k + key_of(i) * p.ks[2], p.ks[2], len - key_of(i), p.D);
+    tv.ask(v + key_of(i) * p.vs[2], p.vs[2], len - key_of(i), p.D);
+  };
+  if (n > 0) ask(0);
+  for (int i = 0; i < n; ++i) {
+    const int key0 = key_of(i);
     __syncthreads();
-    load_transposed<kD>(kt, k + key0 * p.ks[2], p.ks[2], len - key0, p.D);
-    load_transposed<kD>(vt, v + key0 * p.vs[2], p.vs[2], len - key0, p.D);
+    tk.store(kt);
+    tv.store(vt);
     __syncthreads();
+    if (i + 1 < n) ask(i + 1);
     float s[4][4], dp[4][4];
     product<kD>(s, qt, kt, ty, tx);
     product<kD>(dp, gt, vt, ty, tx);
@@ -206,17 +235,7 @@ __global__ void __launch_bounds__(kThreads) window_dq_f32_kernel(const __grid_co
       }
     }
     __syncthreads();
-#pragma unroll 4
-    for (int j = 0; j < kTile; ++j) {
-      const float4 x = *reinterpret_cast<const float4*>(dst + j * kPad + ty * 4);
-      const float xs[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-      for (int c = 0; c < kD / 16; ++c) {
-        const float y = kt[(c * 16 + tx) * kPad + j];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) dq[r][c] = fmaf(xs[r], y, dq[r][c]);
-      }
-    }
+    accumulate<kD>(dq, dst, kt, ty, tx);
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
@@ -250,55 +269,52 @@ __global__ void __launch_bounds__(kThreads) window_dkv_f32_kernel(const __grid_c
     if (first > last) return;
   }
   const int key0 = tile * kTile, valid_k = min(kTile, len - key0);
-  load_transposed<kD>(kt, (const float*)p.k + b * p.ks[0] + hk * p.ks[1] + key0 * p.ks[2], p.ks[2], valid_k, p.D);
-  load_transposed<kD>(vt, (const float*)p.v + b * p.vs[0] + hk * p.vs[1] + key0 * p.vs[2], p.vs[2], valid_k, p.D);
+  Tile<kD> tq, tg;
+  tq.ask((const float*)p.k + b * p.ks[0] + hk * p.ks[1] + key0 * p.ks[2], p.ks[2], valid_k, p.D);
+  tg.ask((const float*)p.v + b * p.vs[0] + hk * p.vs[1] + key0 * p.vs[2], p.vs[2], valid_k, p.D);
+  tq.store(kt);
+  tg.store(vt);
   float dk[4][kD / 16], dv[4][kD / 16];                                  // keys 4 ty .., features tx + 16 c
 #pragma unroll
   for (int r = 0; r < 4; ++r)
 #pragma unroll
     for (int c = 0; c < kD / 16; ++c) dk[r][c] = dv[r][c] = 0.f;
-  for (int g = 0; g < G; ++g) {
-    const int h = hk * G + g;
-    for (int t = first; t <= last; ++t) {
-      const int valid_q = min(min(kTile, p.Lq - t * kTile), len - off - t * kTile);
-      const int64_t row0 = ((int64_t)b * p.H + h) * p.Lq + t * kTile;
-      __syncthreads();
-      load_transposed<kD>(qt, (const float*)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)t * kTile * p.qs[2], p.qs[2], valid_q, p.D);
-      load_transposed<kD>(gt, (const float*)p.dO + b * p.dos[0] + h * p.dos[1] + (int64_t)t * kTile * p.dos[2], p.dos[2], valid_q, p.D);
-      __syncthreads();
-      float s[4][4], dp[4][4];
-      product<kD>(s, qt, kt, ty, tx);
-      product<kD>(dp, gt, vt, ty, tx);
+  const int per_head = last - first + 1, n = per_head > 0 ? per_head * G : 0;
+  auto rows_of = [&](int t) { return min(min(kTile, p.Lq - t * kTile), len - off - t * kTile); };
+  auto ask = [&](int i) {
+    const int g = i / per_head, t = first + i - g * per_head, h = hk * G + g;
+    tq.ask((const float*)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)t * kTile * p.qs[2], p.qs[2], rows_of(t), p.D);
+    tg.ask((const float*)p.dO + b * p.dos[0] + h * p.dos[1] + (int64_t)t * kTile * p.dos[2], p.dos[2], rows_of(t), p.D);
+  };
+  if (n > 0) ask(0);
+  for (int i = 0; i < n; ++i) {
+    const int g = i / per_head, t = first + i - g * per_head, valid_q = rows_of(t);
+    const int64_t row0 = ((int64_t)b * p.H + hk * G + g) * p.Lq + t * kTile;
+    __syncthreads();
+    tq.store(qt);
+    tg.store(gt);
+    __syncthreads();
+    if (i + 1 < n) ask(i + 1);
+    float s[4][4], dp[4][4];
+    product<kD>(s, qt, kt, ty, tx);
+    product<kD>(dp, gt, vt, ty, tx);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = ty * 4 + r, pos = off + t * kTile + row;
-        const float lse = row < valid_q ? ld_behind_wait(p.lse + row0 + row) : INFINITY;
-        const float delta = row < valid_q ? ld_behind_wait(p.delta + row0 + row) : 0.f;
-        float w[4], d[4];
+    for (int r = 0; r < 4; ++r) {
+      const int row = ty * 4 + r, pos = off + t * kTile + row;
+      const float lse = row < valid_q ? ld_behind_wait(p.lse + row0 + row) : INFINITY;
+      const float delta = row < valid_q ? ld_behind_wait(p.delta + row0 + row) : 0.f;
+      float w[4], d[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          w[j] = window_sees(pos, key0 + tx * 4 + j, p.window, p.sinks) ? exp2f(fmaf(s[r][j], scale_log2, -lse)) : 0.f;
-          d[j] = w[j] * (dp[r][j] - delta) * p.scale;
-        }
-        *reinterpret_cast<float4*>(pr + row * kPad + tx * 4) = make_float4(w[0], w[1], w[2], w[3]);
-        *reinterpret_cast<float4*>(dsr + row * kPad + tx * 4) = make_float4(d[0], d[1], d[2], d[3]);
+      for (int j = 0; j < 4; ++j) {
+        w[j] = window_sees(pos, key0 + tx * 4 + j, p.window, p.sinks) ? exp2f(fmaf(s[r][j], scale_log2, -lse)) : 0.f;
+        d[j] = w[j] * (dp[r][j] - delta) * p.scale;
       }
-      __syncthreads();
-#pragma unroll 4
-      for (int j = 0; j < kTile; ++j) {
-        const float4 x = *reinterpret_cast<const float4*>(pr + j * kPad + ty * 4), y = *reinterpret_cast<const float4*>(dsr + j * kPad + ty * 4);
-        const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-        for (int c = 0; c < kD / 16; ++c) {
-          const float gv = gt[(c * 16 + tx) * kPad + j], qv = qt[(c * 16 + tx) * kPad + j];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            dv[r][c] = fmaf(xs[r], gv, dv[r][c]);
-            dk[r][c] = fmaf(ys[r], qv, dk[r][c]);
-          }
-        }
-      }
+      *reinterpret_cast<float4*>(pr + row * kPad + tx * 4) = make_float4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<float4*>(dsr + row * kPad + tx * 4) = make_float4(d[0], d[1], d[2], d[3]);
     }
+    __syncthreads();
+    accumulate<kD>(dv, pr, gt, ty, tx);
+    accumulate<kD>(dk, dsr, qt, ty, tx);
   }
   float* const part = split ? p.split.part + (((int64_t)bk * p.split.tiles + tile) * (1 + p.split.runs) + 1 + run) * 2 * kTile * p.D : nullptr;
 #pragma unroll
@@ -321,7 +337,7 @@ __global__ void __launch_bounds__(kThreads) window_dkv_f32_kernel(const __grid_c
   }
 }
 
-template <int kD> constexpr size_t kSmemFwd = sizeof(float) * (2 * kD * kPad + kTile * kD + kTile * kPad);
+template <int kD> constexpr size_t kSmemFwd = sizeof(float) * (3 * kD * kPad + kTile * kPad);
 template <int kD> constexpr size_t kSmemDq = sizeof(float) * (4 * kD * kPad + kTile * kPad);
 template <int kD> constexpr size_t kSmemDkv = sizeof(float) * (4 * kD * kPad + 2 * kTile * kPad);
 
