@@ -262,8 +262,10 @@ template <int kD> struct Rows32 {
 
 // kWarps: 4, with two CTAs an SM or four for 64 features; 8 on whole rows where there are no more of them than SMs, and the latency of a
 // warp's steps counts (us: 32 rows of 300 keys 10.1 with 4, 8.8 with 8; 512 rows 23.5 / 34.6).
+// (registers are only held down where four CTAs are to fit; 128 features then leave room for the next kernel's first CTAs)
+template <typename T, int kD, int kWarps> constexpr int kAttendPerSm = kWarps == 4 && kD == 64 && sizeof(T) == 2 ? 4 : 1;
 template <typename T, int kD, int kWarps>
-__global__ void __launch_bounds__(kWarps * 32) paged_attend_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+__global__ void __launch_bounds__(kWarps * 32, kAttendPerSm<T, kD, kWarps>) paged_attend_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
                                                                    const __grid_constant__ AttendArgs a) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ float2 s_stat[kWarps][kRowTile];
