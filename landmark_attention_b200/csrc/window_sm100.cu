@@ -2,7 +2,7 @@
 // accumulators in TMEM.  Query tiles of 128 rows meet key tiles of 64 (forward, dQ) or pairs of them (dK, dV); only the tiles that
 // the window or the sinks make visible are visited (window_params.h), and only those on an edge are masked.
 //
-// Forward: one or two query tiles a CTA that share one stream of key tiles, newest first, the sinks' last.
+// Forward: unit = (query tile, head), persistent; key tiles newest first, the sinks' last.
 //   S = Q K^T -> a softmax thread owns one row (= one TMEM lane): p = 2^(s c - m), l += sum p, P written in 16 bits over the TMEM
 //   columns its S came from -> O += P V with A = P from TMEM.  m is the running maximum, but is only moved when a tile exceeds it by more
 //   than 2^8: O then has to be read, scaled and written back (TMEM), which with the first tile's maximum as m happens to a few rows of
@@ -62,24 +62,29 @@ __device__ __forceinline__ bool none_seen(int p0, int p1, int k0, int k1, int wi
 }
 
 struct WindowTensors {
-  void* o;                  // forward: output
+  void* o;
   float* lse;
   const int* lengths;
-  int H, G, Lq, Lk, D, window, sinks;
-  float scale, scale_log2;
+  int BH, H, G, Lq, Lk, D, window, sinks;
+  float scale_log2;
 };
 
 // ---------------------------------------------------------------------------------------------- forward
-template <int kTiles> constexpr int kFwdStages = kTiles == 2 ? 5 : 2;
-template <int kTiles> constexpr int kFwdThreads = (4 * kTiles + 3) * 32;
+// Persistent, two CTAs an SM whose gaps fill each other; a unit is a query tile of 128 rows of a head.  The loads run on into the next unit
+// and its first scores are there when the last one's output has been written: with a CTA a unit, setting up, fetching Q and ending took
+// 7000 of a unit's 17 000 clk (B1 H32 L2048, window 512).
+// One warp issues all products: S of item i + 2 right behind P V of item i, which reads the P that stands in its place (the tensor core works
+// through what one thread issues in order).  TMEM: 2 x 64 S / P + kD O.  Shared memory: Q, and a ring of K and V tiles.
+constexpr int kFwdThreads = (4 + 2) * 32;
+template <int kD> constexpr int kFwdSlots = kD == 128 ? 5 : 10;      // 64-row K and V tiles, in turn
 constexpr int kFwdPolyEvery = 8;         // one pair of exponentials in this many is a polynomial on the FMA pipe
 constexpr float kLazy = 8.f;             // the maximum moves when it is exceeded by this much (log2)
 
-template <int kStages> struct FwdSmem {
-  uint64_t q_full, patch;
-  uint64_t full[kStages], empty[kStages];
-  uint64_t s_full[2][2], s_free[2][2], p_ready[2][2];      // [tile][S / P buffer]
-  uint64_t o_full;
+template <int kSlots> struct FwdSmem {
+  uint64_t q_full, q_empty, patch;
+  uint64_t full[kSlots], empty[kSlots];
+  uint64_t s_full[2], p_ready[2];        // [S / P buffer]
+  uint64_t o_full, o_empty;
   uint32_t tmem_base;
 };
 
@@ -90,289 +95,296 @@ __device__ __forceinline__ float max_of_64(const float (&v)[64]) {      // NaN w
   return max3_nan(max3_nan(m[0], m[1], m[2]), m[3], m[3]);
 }
 
-template <bool kBf16, int kD, int kTiles>
-__global__ void __launch_bounds__(kFwdThreads<kTiles>, 3 - kTiles)
-window_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                        const __grid_constant__ CUtensorMap tm_v, const WindowTensors p, int* status) {
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw = smem_u32(smem_raw);
-  const uint32_t base = (raw + 1023u) & ~1023u;
-  constexpr int kStages = kFwdStages<kTiles>, kSw = 4 * kTiles;        // softmax warps; the three roles follow them
-  auto q_tile = [&](int w) { return base + (uint32_t)w * 32768u; };
-  auto k_slot = [&](int s) { return base + kTiles * 32768u + (uint32_t)s * 32768u; };
-  auto v_slot = [&](int s) { return base + kTiles * 32768u + (uint32_t)s * 32768u + 16384u; };
-  FwdSmem<kStages>* sm = reinterpret_cast<FwdSmem<kStages>*>(smem_raw + (base - raw) + (kTiles + kStages) * 32768u);
+// a query tile of 128 rows of a head, and the key tiles it meets: the newest first, the sinks' last
+struct RowUnit {
+  int t, bh, b, h, len, n_win, total;
+  KeyTiles k;
+  __device__ int tile_of(int i) const { return i < n_win ? k.last - i : k.sink_tiles - 1 - (i - n_win); }
+};
+__device__ __forceinline__ RowUnit row_unit(int w, int n_tiles, int BH, int H, const int* lengths, int Lq, int Lk, int window, int sinks) {
+  RowUnit u;
+  u.t = n_tiles - 1 - w / BH;                // longest tiles first, across all heads
+  u.bh = w % BH;
+  u.b = u.bh / H;
+  u.h = u.bh - u.b * H;
+  u.len = length_of(lengths, u.b, Lk);
+  u.k = keys_of_queries(u.t, kQTile, kBlk, Lq, Lk - Lq, u.len, window, sinks);
+  u.n_win = u.k.last - u.k.first + 1;        // 0: nothing but padding
+  u.total = u.n_win + u.k.sink_tiles;
+  return u;
+}
+// units are dealt to the CTAs in rounds, in alternating direction
+__device__ __forceinline__ int unit_at(int r) { return r * (int)gridDim.x + ((r & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x); }
 
-  const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
-  const int t_a = ((int)gridDim.y - 1 - (int)blockIdx.y) * kTiles;      // longest tiles first, across all heads
-  const int bh = blockIdx.x, b = bh / p.H, h = bh - b * p.H, hk = h / p.G;
-  const int off = p.Lk - p.Lq;
-  grid_dep_wait();
-  grid_dep_launch();
-  const int len = warp_uniform(length_of(p.lengths, b, p.Lk));
-  const int pos_a = off + t_a * kQTile;                 // key position of tile A's first row
-  if (pos_a >= len) {                                   // nothing but padding
-    const int rows = min(kTiles * kQTile, p.Lq - t_a * kQTile);
-    uint4* const o = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.o) + ((int64_t)bh * p.Lq + t_a * kQTile) * p.D);
-    for (int e = tid; e < rows * p.D / 8; e += kFwdThreads<kTiles>) o[e] = make_uint4(0u, 0u, 0u, 0u);
-    for (int r = tid; r < rows; r += kFwdThreads<kTiles>) p.lse[(int64_t)bh * p.Lq + t_a * kQTile + r] = INFINITY;
+template <bool kBf16, int kD>
+__global__ void __launch_bounds__(kFwdThreads, 2)
+window_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ WindowTensors p, int* status) {
+  constexpr int kSlots = kFwdSlots<kD>;
+  constexpr uint32_t kQBytes = (kD / 64) * kTileBytes, kKvBytes = kQBytes / 2;
+  extern __shared__ __align__(1024) uint8_t smem_aligned[];      // (a kilobyte of slack would not fit twice)
+  const uint32_t base = smem_u32(smem_aligned);
+  if ((base & 1023u) != 0) {                                     // the swizzle needs it
+    if (threadIdx.x == 0) atomicCAS(status, 0, kErrFwdProducer);
     return;
   }
-  const bool has_b = kTiles == 2 && (t_a + 1) * kQTile < p.Lq && pos_a + kQTile < len;
-  const KeyTiles ka = keys_of_queries(t_a, kQTile, kBlk, p.Lq, off, len, p.window, p.sinks);
-  const KeyTiles kb = has_b ? keys_of_queries(t_a + 1, kQTile, kBlk, p.Lq, off, len, p.window, p.sinks) : ka;
-  const int st = (p.sinks + kBlk - 1) / kBlk;
-  const int newest = kb.last, n_win = newest - ka.first + 1, total = n_win + ka.sink_tiles;
-  auto tile_of = [&](int i) { return i < n_win ? newest - i : ka.sink_tiles - 1 - (i - n_win); };
-  auto active = [&](int w, int i) {
-    const int n = tile_of(i);
-    return w == 1 ? has_b && (n < st || n >= kb.first) : n <= ka.last;
-  };
+  auto slot = [&](int m) { return base + kQBytes + (uint32_t)(m % kSlots) * kKvBytes; };
+  FwdSmem<kSlots>* sm = reinterpret_cast<FwdSmem<kSlots>*>(smem_aligned + kQBytes + kSlots * kKvBytes);
+
+  const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
+  const int off = p.Lk - p.Lq, n_tiles = (p.Lq + kQTile - 1) / kQTile, n_units = n_tiles * p.BH;
+  auto unit_of = [&](int w) { return row_unit(w, n_tiles, p.BH, p.H, p.lengths, p.Lq, p.Lk, p.window, p.sinks); };
 
   if (tid == 0) {
-    mbar_init(smem_u32(&sm->q_full), 1);
-    mbar_init(smem_u32(&sm->patch), 1);
-    for (int s = 0; s < kStages; ++s) {
+    for (uint64_t* bar : {&sm->q_full, &sm->q_empty, &sm->patch, &sm->o_full, &sm->s_full[0], &sm->s_full[1]}) mbar_init(smem_u32(bar), 1);
+    for (uint64_t* bar : {&sm->o_empty, &sm->p_ready[0], &sm->p_ready[1]}) mbar_init(smem_u32(bar), 128);
+    for (int s = 0; s < kSlots; ++s) {
       mbar_init(smem_u32(&sm->full[s]), 1);
       mbar_init(smem_u32(&sm->empty[s]), 1);
     }
-    for (int w = 0; w < 2; ++w)
-      for (int s = 0; s < 2; ++s) {
-        mbar_init(smem_u32(&sm->s_full[w][s]), 1);
-        mbar_init(smem_u32(&sm->s_free[w][s]), 1);
-        mbar_init(smem_u32(&sm->p_ready[w][s]), 128);
-      }
-    mbar_init(smem_u32(&sm->o_full), 1);
     mbar_init_fence();
   }
-  if (warp == kSw + 1) tmem_alloc(smem_u32(&sm->tmem_base), kTiles * 256);
+  if (warp == 5) tmem_alloc(smem_u32(&sm->tmem_base), 256);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = (uint32_t)warp_uniform((int)sm->tmem_base);
-  auto tmem_s = [&](int w, int sb) { return tmem + (uint32_t)(w * 128 + sb * 64); };
-  auto tmem_o = [&](int w) { return tmem + kTiles * 128u + (uint32_t)w * 128u; };
+  const uint32_t tmem_s = tmem, tmem_o = tmem + 128u;
+  grid_dep_wait();
+  grid_dep_launch();
 
-  if (warp == kSw) {
-    // ------------------------------------------------------------------ TMA producer
+  if (warp == 4) {
+    // ------------------------------------------------------------------ loads
     if (lane == 0) {
-      const uint32_t qb = smem_u32(&sm->q_full);
-      mbar_arrive_expect_tx(qb, (has_b ? 2 : 1) * (kD / 64) * kTileBytes);
-      for (int w = 0; w < (has_b ? 2 : 1); ++w)
-        for (int c = 0; c < kD / 64; ++c) tma_load_4d(q_tile(w) + c * kTileBytes, &tm_q, qb, 64 * c, (t_a + w) * kQTile, h, b);
-      for (int i = 0; i < total; ++i) {
-        const int s = i % kStages, key0 = tile_of(i) * kBlk;
-        mbar_wait(smem_u32(&sm->empty[s]), ((i / kStages) & 1) ^ 1, status, kErrFwdProducer);
-        const bool ends = key0 + kBlk > len && len < p.Lk;      // the tile the sequence ends in, once at most (the newest)
-        const uint32_t fb = smem_u32(ends ? &sm->patch : &sm->full[s]);
-        mbar_arrive_expect_tx(fb, 2 * (kD / 64) * kHalfTile);
-        for (int c = 0; c < kD / 64; ++c) {
-          tma_load_4d(k_slot(s) + c * kHalfTile, &tm_k, fb, 64 * c, key0, hk, b);
-          tma_load_4d(v_slot(s) + c * kHalfTile, &tm_v, fb, 64 * c, key0, hk, b);
-        }
-        if (ends) {
-          mbar_wait(fb, 0, status, kErrFwdProducer);
-          zero_rows(v_slot(s), kHalfTile, kD / 64, len - key0, kBlk);
-          mbar_arrive(smem_u32(&sm->full[s]));
+      int m = 0, uq = 0, patches = 0;
+      for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
+        const RowUnit u = unit_of(w);
+        if (u.total == 0) continue;
+        const int hk = u.h / p.G;
+        auto load_kv = [&](const CUtensorMap* tm, int key0, bool patch) {
+          mbar_wait(smem_u32(&sm->empty[m % kSlots]), ((m / kSlots) & 1) ^ 1, status, kErrFwdProducer);
+          const uint32_t bar = smem_u32(patch ? &sm->patch : &sm->full[m % kSlots]);
+          mbar_arrive_expect_tx(bar, kKvBytes);
+          for (int c = 0; c < kD / 64; ++c) tma_load_4d(slot(m) + c * kHalfTile, tm, bar, 64 * c, key0, hk, u.b);
+          if (patch) {
+            mbar_wait(bar, patches++ & 1, status, kErrFwdProducer);
+            zero_rows(slot(m), kHalfTile, kD / 64, u.len - key0, kBlk);
+            mbar_arrive(smem_u32(&sm->full[m % kSlots]));
+          }
+          ++m;
+        };
+        mbar_wait(smem_u32(&sm->q_empty), (uq++ & 1) ^ 1, status, kErrFwdProducer);
+        mbar_arrive_expect_tx(smem_u32(&sm->q_full), kQBytes);
+        for (int c = 0; c < kD / 64; ++c) tma_load_4d(base + c * kTileBytes, &tm_q, smem_u32(&sm->q_full), 64 * c, u.t * kQTile, u.h, u.b);
+        for (int i = 0; i < u.total; ++i) {
+          const int key0 = u.tile_of(i) * kBlk;
+          load_kv(&tm_k, key0, false);
+          load_kv(&tm_v, key0, key0 + kBlk > u.len && u.len < p.Lk);      // values of the tile the sequence ends in
         }
       }
     }
     __syncwarp();
-  } else if (warp == kSw + 1) {
-    // ------------------------------------------------------------------ MMA issuer 1: S = Q K^T
+  } else if (warp == 5) {
+    // ------------------------------------------------------------------ products
     constexpr uint32_t fmt = kBf16 ? 1u : 0u;
-    constexpr uint32_t idesc_s = instr_desc_f16(fmt, 128, 64, 0, 0);
-    mbar_wait(smem_u32(&sm->q_full), 0, status, kErrFwdMma);
-    const uint64_t dq0 = smem_desc_sw128(q_tile(0), 16, 1024);
-    const uint64_t dk0 = smem_desc_sw128(k_slot(0), 16, 1024);
-    int ks[2] = {0, 0};
-    int s = 0;
-    uint32_t ph = 0;
-    for (int j = 0; j < total; ++j) {
-      mbar_wait(smem_u32(&sm->full[s]), ph, status, kErrFwdMma);
-      const uint64_t dk = desc_advance(dk0, (uint32_t)s * 32768u);
-#pragma unroll
-      for (int w = 0; w < kTiles; ++w) {
-        if (!active(w, j)) continue;
-        const int k = ks[w]++, sb = k & 1;
-        if (k >= 2) mbar_wait(smem_u32(&sm->s_free[w][sb]), ((k >> 1) & 1) ^ 1, status, kErrFwdMma);
-        tc_fence_after();
-        const uint64_t dq = desc_advance(dq0, (uint32_t)w * 32768u);
-        if (elect_one()) {
-#pragma unroll
-          for (int kk = 0; kk < kD / 16; ++kk)
-            mma_f16_ss(tmem_s(w, sb), desc_advance(dq, kmajor_step(kk, kTileBytes)), desc_advance(dk, kmajor_step(kk, kHalfTile)), idesc_s, kk > 0);
-          mma_commit(smem_u32(&sm->s_full[w][sb]));
+    constexpr uint32_t idesc_s = instr_desc_f16(fmt, 128, 64, 0, 0), idesc_o = instr_desc_f16(fmt, 128, kD, 0, 1);
+    const uint64_t dq = smem_desc_sw128(base, 16, 1024), dk0 = smem_desc_sw128(slot(0), 16, 1024), dv0 = smem_desc_sw128(slot(0), kHalfTile, 1024);
+    int r = -1, u = -1, it = 0;                      // it: items of all units
+    auto next_unit = [&]() {                         // items of the next unit that has any, 0: no more
+      for (;;) {
+        const int w = unit_at(++r);
+        if (w >= n_units) return 0;
+        const int n = warp_uniform(unit_of(w).total);
+        if (n > 0) {
+          ++u;
+          return n;
         }
       }
-      if (++s == kStages) { s = 0; ph ^= 1; }
-    }
-    __syncwarp();
-  } else if (warp == kSw + 2) {
-    // ------------------------------------------------------------------ MMA issuer 2: O += P V
-    constexpr uint32_t fmt = kBf16 ? 1u : 0u;
-    constexpr uint32_t idesc_o = instr_desc_f16(fmt, 128, kD, 0, 1);
-    const uint64_t dv0 = smem_desc_sw128(v_slot(0), kHalfTile, 1024);
-    int kp[2] = {0, 0};
-    int s = 0;
-    for (int i = 0; i < total; ++i) {
-      const uint64_t dv = desc_advance(dv0, (uint32_t)s * 32768u);
+    };
+    auto arrived = [&](int m) {
+      mbar_wait(smem_u32(&sm->full[m % kSlots]), (m / kSlots) & 1, status, kErrFwdMma);
+      tc_fence_after();
+    };
+    auto issue_s = [&](int i, int n, int j) {        // item i of n, the j-th of all
+      if (i == 0) mbar_wait(smem_u32(&sm->q_full), u & 1, status, kErrFwdMma);
+      arrived(2 * j);
+      const uint64_t dk = desc_advance(dk0, (uint32_t)((2 * j) % kSlots) * kKvBytes);
+      if (elect_one()) {
 #pragma unroll
-      for (int w = 0; w < kTiles; ++w) {
-        if (!active(w, i)) continue;
-        const int k = kp[w]++;
-        mbar_wait(smem_u32(&sm->p_ready[w][k & 1]), (k >> 1) & 1, status, kErrFwdMma);
+        for (int kk = 0; kk < kD / 16; ++kk)
+          mma_f16_ss(tmem_s + (j & 1) * 64, desc_advance(dq, kmajor_step(kk, kTileBytes)), desc_advance(dk, kmajor_step(kk, kHalfTile)), idesc_s, kk > 0);
+        mma_commit(smem_u32(&sm->s_full[j & 1]));
+        mma_commit(smem_u32(&sm->empty[(2 * j) % kSlots]));
+        if (i == n - 1) mma_commit(smem_u32(&sm->q_empty));
+      }
+    };
+    for (int n = next_unit(); n > 0; n = next_unit()) {
+      for (int i = 0; i < min(n, 2); ++i) issue_s(i, n, it + i);
+      for (int i = 0; i < n; ++i, ++it) {
+        arrived(2 * it + 1);
+        if (i == 0) mbar_wait(smem_u32(&sm->o_empty), (u & 1) ^ 1, status, kErrFwdMma);
+        mbar_wait(smem_u32(&sm->p_ready[it & 1]), (it >> 1) & 1, status, kErrFwdMma);
         tc_fence_after();
-        const uint32_t tp = tmem_s(w, k & 1);      // P: 8 columns = 16 keys per K-step
+        const uint64_t dv = desc_advance(dv0, (uint32_t)((2 * it + 1) % kSlots) * kKvBytes);
         if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kBlk / 16; ++kk)
-            mma_f16_ts(tmem_o(w), tp + kk * 8, desc_advance(dv, kk * 2048), idesc_o, (k > 0 || kk > 0) ? 1u : 0u);
-          mma_commit(smem_u32(&sm->s_free[w][k & 1]));
+          for (int kk = 0; kk < kBlk / 16; ++kk)     // P: 8 columns = 16 keys per K-step
+            mma_f16_ts(tmem_o, tmem_s + (it & 1) * 64 + kk * 8, desc_advance(dv, kk * 2048), idesc_o, (i > 0 || kk > 0) ? 1u : 0u);
+          mma_commit(smem_u32(&sm->empty[(2 * it + 1) % kSlots]));
+          if (i == n - 1) mma_commit(smem_u32(&sm->o_full));
         }
+        if (i + 2 < n) issue_s(i + 2, n, it + 2);
       }
-      // the stage is free once both P V products are done; each of them waited for its S product to be read
-      if (elect_one()) mma_commit(smem_u32(&sm->empty[s]));
-      if (++s == kStages) s = 0;
     }
-    if (elect_one()) mma_commit(smem_u32(&sm->o_full));
     __syncwarp();
   } else {
-    // ------------------------------------------------------------------ softmax warpgroups
-    const int w = warp >> 2;                       // 0: tile A, 1: tile B
-    const int row = tid & 127;
-    const int pos = pos_a + w * kQTile + row;
-    const int warp_p0 = warp_uniform(pos_a + w * kQTile + (warp & 3) * 32), warp_p1 = warp_p0 + 31;
-    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    // ------------------------------------------------------------------ softmax
+    const int row = tid;
+    const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
     const float c = p.scale_log2;
-    float m2 = -INFINITY, l = 0.f;
-    int k = 0;
-    for (int i = 0; i < total; ++i) {
-      if (!active(w, i)) continue;
-      const int sb = k & 1, key0 = tile_of(i) * kBlk;
-      mbar_wait(smem_u32(&sm->s_full[w][sb]), (k / 2) & 1, status, kErrFwdSoftmax);
-      tc_fence_after();
-      uint32_t wgt[32];
-      if (none_seen(warp_p0, warp_p1, key0, key0 + kBlk - 1, p.window, p.sinks)) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j) wgt[j] = 0u;
-      } else {
-        float sv[64];
-        {
-          uint32_t ra[32], rb[32];
-          tmem_ld_32x32b_x32(tmem_s(w, sb) + lane_base, ra);
-          tmem_ld_32x32b_x32(tmem_s(w, sb) + 32 + lane_base, rb);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            sv[j] = __uint_as_float(ra[j]);
-            sv[32 + j] = __uint_as_float(rb[j]);
-          }
+    int it = 0, units = 0;
+    for (int r = 0, x = unit_at(0); x < n_units; x = unit_at(++r)) {
+      const RowUnit u = unit_of(x);
+      const int pos = off + u.t * kQTile + row, grow = u.t * kQTile + row;
+      const bool stored = grow < p.Lq;
+      uint4* const orow = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.o) + ((int64_t)u.bh * p.Lq + grow) * p.D);
+      if (u.total == 0) {                            // nothing but padding
+        if (stored) {
+          for (int e = 0; e < p.D / 8; ++e) orow[e] = make_uint4(0u, 0u, 0u, 0u);
+          p.lse[(int64_t)u.bh * p.Lq + grow] = INFINITY;
         }
+        __syncwarp();
+        continue;
+      }
+      const int warp_p0 = warp_uniform(off + u.t * kQTile + warp * 32), warp_p1 = warp_p0 + 31;
+      float m2 = -INFINITY, l = 0.f;
+      for (int i = 0; i < u.total; ++i, ++it) {
+        const int key0 = u.tile_of(i) * kBlk;
+        const uint32_t ts = tmem_s + (uint32_t)(it & 1) * 64u + lane_base;
+        const bool none = none_seen(warp_p0, warp_p1, key0, key0 + kBlk - 1, p.window, p.sinks);
         const bool full = all_seen(warp_p0, warp_p1, key0, key0 + kBlk - 1, p.window, p.sinks);
-        if (!full) {
-          const Columns col(pos, key0, p.window, p.sinks);
+        mbar_wait(smem_u32(&sm->s_full[it & 1]), (it >> 1) & 1, status, kErrFwdSoftmax);
+        tc_fence_after();
+        uint32_t wgt[32];
+        if (none) {
 #pragma unroll
-          for (int j = 0; j < 64; ++j) sv[j] = col.sees(j) ? sv[j] : -INFINITY;
-        }
-        const float mx = max_of_64(sv);
-        const float mc = mx * c;                                     // -inf: nothing visible
-        const bool move = mc > m2 + kLazy;                           // from -inf on too
-        if (__any_sync(0xffffffffu, move && m2 != -INFINITY)) {
-          // O is rescaled behind the product of the item before, whose end s_free of its buffer tells (this thread sees every
-          // second phase of it at the latest: S of this item was only issued behind the product two items back)
-          mbar_wait(smem_u32(&sm->s_free[w][sb ^ 1]), ((k - 1) >> 1) & 1, status, kErrFwdSoftmax);
-          tc_fence_after();
-          const float f = move ? ex2(m2 - mc) : 1.f;                 // from -inf: 0, where O is 0
-          l *= f;
-          for (int cc = 0; cc < kD / 16; ++cc) {                      // 16 columns at a time: the row's scores stay in registers
-            uint32_t r[16];
-            tmem_ld_32x32b_x16(tmem_o(w) + cc * 16 + lane_base, r);
+          for (int j = 0; j < 32; ++j) wgt[j] = 0u;
+        } else {
+          float sv[64];
+          {
+            uint32_t ra[32], rb[32];
+            tmem_ld_32x32b_x32(ts, ra);
+            tmem_ld_32x32b_x32(ts + 32, rb);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * f);
-            tmem_st_32x32b_x16(tmem_o(w) + cc * 16 + lane_base, r);
-          }
-          tmem_st_wait();
-        }
-        if (move) m2 = mc;
-        uint64_t sp[32];
-        if (!full) {
-          const float shift = m2 == -INFINITY ? 0.f : m2;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) sp[j] = pk2(ex2(fmaf(sv[2 * j], c, -shift)), ex2(fmaf(sv[2 * j + 1], c, -shift)));
-        } else {
-          // polynomials make finite numbers of NaN and infinities: a maximum that is one makes NaN of the shift of all
-          const float n = fmaf(mx, 0.f, -m2);
-          const uint64_t c2 = pk2(c, c), n2 = pk2(n, n);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const uint64_t x = fma2(pk2(sv[2 * j], sv[2 * j + 1]), c2, n2);
-            if (j % kFwdPolyEvery == 1) {
-              sp[j] = ex2_poly2<4>(x);
-            } else {
-              float x0, x1;
-              upk2(x, x0, x1);
-              sp[j] = pk2(ex2(x0), ex2(x1));
+            for (int j = 0; j < 32; ++j) {
+              sv[j] = __uint_as_float(ra[j]);
+              sv[32 + j] = __uint_as_float(rb[j]);
             }
           }
-        }
-        uint64_t s0 = sp[0], s1 = sp[1], s2 = sp[2], s3 = sp[3];
+          if (!full) {
+            const Columns col(pos, key0, p.window, p.sinks);
 #pragma unroll
-        for (int j = 4; j < 32; j += 4) {
-          s0 = add2(s0, sp[j]);
-          s1 = add2(s1, sp[j + 1]);
-          s2 = add2(s2, sp[j + 2]);
-          s3 = add2(s3, sp[j + 3]);
-        }
-        float dl, dh;
-        upk2(add2(add2(s0, s1), add2(s2, s3)), dl, dh);
-        l += dl + dh;
-        // P enters the product in 16 bits: half a step of relative error a weight; l sums the unrounded ones
+            for (int j = 0; j < 64; ++j) sv[j] = col.sees(j) ? sv[j] : -INFINITY;
+          }
+          const float mx = max_of_64(sv);
+          const float mc = mx * c;                                     // -inf: nothing visible
+          const bool move = mc > m2 + kLazy;                           // from -inf on too
+          if (__any_sync(0xffffffffu, move && m2 != -INFINITY)) {
+            // O is rescaled behind P V of the item before.  That came behind S of this one: its end is that of the item's V tile, or
+            // of the unit; the next S of its buffer would tell as well, but is not due before this item's P.
+            mbar_wait(smem_u32(&sm->empty[(2 * it - 1) % kSlots]), ((2 * it - 1) / kSlots) & 1, status, kErrFwdSoftmax);
+            tc_fence_after();
+            const float f = move ? ex2(m2 - mc) : 1.f;                 // from -inf: 0, where O is 0
+            l *= f;
+            for (int cc = 0; cc < kD / 16; ++cc) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(tmem_o + cc * 16 + lane_base, o);
+              tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) wgt[j] = pack2p<kBf16>(sp[j]);
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tmem_st_32x32b_x16(tmem_o + cc * 16 + lane_base, o);
+            }
+            tmem_st_wait();
+          }
+          if (move) m2 = mc;
+          uint64_t sp[32];
+          if (!full) {
+            const float shift = m2 == -INFINITY ? 0.f : m2;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) sp[j] = pk2(ex2(fmaf(sv[2 * j], c, -shift)), ex2(fmaf(sv[2 * j + 1], c, -shift)));
+          } else {
+            // polynomials make finite numbers of NaN and infinities: a maximum that is one makes NaN of the shift of all
+            const float n = fmaf(mx, 0.f, -m2);
+            const uint64_t c2 = pk2(c, c), n2 = pk2(n, n);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              const uint64_t e = fma2(pk2(sv[2 * j], sv[2 * j + 1]), c2, n2);
+              if (j % kFwdPolyEvery == 1) {
+                sp[j] = ex2_poly2<4>(e);
+              } else {
+                float e0, e1;
+                upk2(e, e0, e1);
+                sp[j] = pk2(ex2(e0), ex2(e1));
+              }
+            }
+          }
+          uint64_t s0 = sp[0], s1 = sp[1], s2 = sp[2], s3 = sp[3];
+#pragma unroll
+          for (int j = 4; j < 32; j += 4) {
+            s0 = add2(s0, sp[j]);
+            s1 = add2(s1, sp[j + 1]);
+            s2 = add2(s2, sp[j + 2]);
+            s3 = add2(s3, sp[j + 3]);
+          }
+          float dl, dh;
+          upk2(add2(add2(s0, s1), add2(s2, s3)), dl, dh);
+          l += dl + dh;
+          // P enters the product in 16 bits: half a step of relative error a weight; l sums the unrounded ones
+#pragma unroll
+          for (int j = 0; j < 32; ++j) wgt[j] = pack2p<kBf16>(sp[j]);
+        }
+        tmem_st_32x32b_x32(ts, wgt);                 // P replaces S in place; the P V product reads it there
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&sm->p_ready[it & 1]));
       }
-      tmem_st_32x32b_x32(tmem_s(w, sb) + lane_base, wgt);     // P replaces S in place; the P V product reads it there
-      tmem_st_wait();
-      tc_fence_before();
-      mbar_arrive(smem_u32(&sm->p_ready[w][sb]));
-      ++k;
-    }
-    // ------------------------------------------------------------------ epilogue
-    const int t = t_a + w;
-    if (w == 0 || has_b) {
-      mbar_wait(smem_u32(&sm->o_full), 0, status, kErrFwdEpilogue);
+      // epilogue
+      mbar_wait(smem_u32(&sm->o_full), units & 1, status, kErrFwdEpilogue);
+      ++units;
       tc_fence_after();
-    }
-    const int grow = t * kQTile + row;
-    const bool stored = grow < p.Lq, valid = pos < len && l != 0.f;
-    const float inv = valid ? 1.f / l : 0.f;
-    uint4* orow = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.o) + ((int64_t)bh * p.Lq + grow) * p.D);
+      const bool valid = pos < u.len && l != 0.f;
+      const float inv = valid ? 1.f / l : 0.f;
 #pragma unroll
-    for (int cc = 0; cc < kD / 32; ++cc) {
-      uint32_t r[32];
-      if (w == 0 || has_b) {
-        tmem_ld_32x32b_x32(tmem_o(w) + cc * 32 + lane_base, r);
+      for (int cc = 0; cc < kD / 32; ++cc) {
+        uint32_t o[32];
+        tmem_ld_32x32b_x32(tmem_o + cc * 32 + lane_base, o);
         tmem_ld_wait();
-      }
+        if (cc == kD / 32 - 1) {
+          tc_fence_before();
+          mbar_arrive(smem_u32(&sm->o_empty));       // the next unit may start accumulating
+        }
 #pragma unroll
-      for (int v4 = 0; v4 < 4; ++v4) {
-        uint4 pk;
-        pk.x = pack2<kBf16>(__uint_as_float(r[8 * v4 + 0]) * inv, __uint_as_float(r[8 * v4 + 1]) * inv);
-        pk.y = pack2<kBf16>(__uint_as_float(r[8 * v4 + 2]) * inv, __uint_as_float(r[8 * v4 + 3]) * inv);
-        pk.z = pack2<kBf16>(__uint_as_float(r[8 * v4 + 4]) * inv, __uint_as_float(r[8 * v4 + 5]) * inv);
-        pk.w = pack2<kBf16>(__uint_as_float(r[8 * v4 + 6]) * inv, __uint_as_float(r[8 * v4 + 7]) * inv);
-        if (!valid) pk = make_uint4(0u, 0u, 0u, 0u);          // (not 0 * whatever padding left in the accumulator)
-        if (stored && cc * 32 + v4 * 8 < p.D) orow[cc * 4 + v4] = pk;
+        for (int v4 = 0; v4 < 4; ++v4) {
+          uint4 pk;
+          pk.x = pack2<kBf16>(__uint_as_float(o[8 * v4 + 0]) * inv, __uint_as_float(o[8 * v4 + 1]) * inv);
+          pk.y = pack2<kBf16>(__uint_as_float(o[8 * v4 + 2]) * inv, __uint_as_float(o[8 * v4 + 3]) * inv);
+          pk.z = pack2<kBf16>(__uint_as_float(o[8 * v4 + 4]) * inv, __uint_as_float(o[8 * v4 + 5]) * inv);
+          pk.w = pack2<kBf16>(__uint_as_float(o[8 * v4 + 6]) * inv, __uint_as_float(o[8 * v4 + 7]) * inv);
+          if (!valid) pk = make_uint4(0u, 0u, 0u, 0u);          // (not 0 * whatever padding left in the accumulator)
+          if (stored && cc * 32 + v4 * 8 < p.D) orow[cc * 4 + v4] = pk;
+        }
+        __syncwarp();
       }
+      if (stored) p.lse[(int64_t)u.bh * p.Lq + grow] = valid ? m2 + __log2f(l) : INFINITY;
+      __syncwarp();
     }
-    if (stored) p.lse[(int64_t)bh * p.Lq + grow] = valid ? m2 + __log2f(l) : INFINITY;
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == kSw + 1) {
+  if (warp == 5) {
     tc_fence_after();
-    tmem_dealloc(tmem, kTiles * 256);
+    tmem_dealloc(tmem, 256);
   }
 }
 
@@ -511,7 +523,6 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
   const int off = p.Lk - p.Lq, heads = p.B * p.Hkv;
   const int n_runs = p.split.tiles * p.split.runs * heads, n_units = n_runs + p.n_pairs * heads;
-  auto unit_at = [&](int r) { return r * (int)gridDim.x + ((r & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x); };
   // the runs first: they are as long as the longest of the others
   auto unit_of = [&](int w) {
     DkvUnit u;
@@ -898,11 +909,6 @@ struct DqArgs {
   int H, Hkv, G, BH, Lq, Lk, D, window, sinks;
   float scale, scale_log2;
 };
-struct DqUnit {
-  int t, bh, b, h, len, total, n_win;
-  KeyTiles k;
-  __device__ int tile_of(int i) const { return i < n_win ? k.last - i : k.sink_tiles - 1 - (i - n_win); }
-};
 
 template <bool kBf16, int kD>
 __global__ void __launch_bounds__(kDqThreads, 1)
@@ -920,19 +926,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 
   const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
   const int n_tiles = (p.Lq + kQTile - 1) / kQTile, off = p.Lk - p.Lq, n_units = n_tiles * p.BH;
-  auto unit_at = [&](int r) { return r * (int)gridDim.x + ((r & 1) ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x); };
-  auto unit_of = [&](int w) {
-    DqUnit u;
-    u.t = n_tiles - 1 - w / p.BH;
-    u.bh = w % p.BH;
-    u.b = u.bh / p.H;
-    u.h = u.bh - u.b * p.H;
-    u.len = length_of(p.lengths, u.b, p.Lk);
-    u.k = keys_of_queries(u.t, kQTile, kBlk, p.Lq, off, u.len, p.window, p.sinks);
-    u.n_win = u.k.last - u.k.first + 1;
-    u.total = u.n_win + u.k.sink_tiles;
-    return u;
-  };
+  auto unit_of = [&](int w) { return row_unit(w, n_tiles, p.BH, p.H, p.lengths, p.Lq, p.Lk, p.window, p.sinks); };
 
   if (tid == 0) {
     for (uint64_t* bar : {&sm->qdo_full, &sm->patch}) mbar_init(smem_u32(bar), 1);
@@ -969,7 +963,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     if (lane == 0) {
       int it = 0, u = 0, patches = 0;
       for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
-        const DqUnit un = unit_of(w);
+        const RowUnit un = unit_of(w);
         if (un.total == 0) continue;
         const int hk = un.h / p.G;
         const uint32_t qb = smem_u32(&sm->qdo_full);
@@ -1124,7 +1118,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     };
     fetch_rows(unit_at(0));
     for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
-      const DqUnit un = unit_of(w);
+      const RowUnit un = unit_of(w);
       const int64_t grow = (int64_t)un.bh * p.Lq + un.t * kQTile + row;
       const int pos = off + un.t * kQTile + row;
       const bool stored = un.t * kQTile + row < p.Lq, valid = stored && pos < un.len;
@@ -1250,10 +1244,10 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 }
 
 // ---------------------------------------------------------------------------------------------- host side
-template <int kTiles> constexpr size_t kSmemFwd = 1024 + (kTiles + kFwdStages<kTiles>) * 32768 + sizeof(FwdSmem<kFwdStages<kTiles>>);
+template <int kD> constexpr size_t kSmemFwd = (kD / 64) * (kTileBytes + kFwdSlots<kD> * kHalfTile) + sizeof(FwdSmem<kFwdSlots<kD>>);
 template <int kD> constexpr size_t kSmemDkv = 1024 + (2 + 2 * kDkvStages) * (kD / 64) * kTileBytes + sizeof(DkvSmem);
 constexpr size_t kSmemDq = 1024 + 65536 + kDqStages * 32768 + 32768 + sizeof(DqSmem);
-static_assert(kSmemFwd<2> <= 232448 && kSmemFwd<1> <= 232448 / 2 - 1024 && kSmemDkv<128> <= 232448 && kSmemDkv<64> <= 232448 && kSmemDq <= 232448,
+static_assert(kSmemFwd<128> <= 233472 / 2 - 1024 && kSmemFwd<64> <= 233472 / 2 - 1024 && kSmemDkv<128> <= 232448 && kSmemDkv<64> <= 232448 && kSmemDq <= 232448,
               "shared memory of one SM");
 
 struct Facts {
@@ -1276,8 +1270,7 @@ int facts_of(const Facts** out) {
     if (f.status == nullptr) return fail(LMK_ERR_CUDA, "no device status word");
     const auto attr = cudaFuncAttributeMaxDynamicSharedMemorySize;
 #define LMK_ATTRS(BF, DIM)                                                                         \
-    LMK_CUDA(cudaFuncSetAttribute(window_fwd_sm100_kernel<BF, DIM, 1>, attr, (int)kSmemFwd<1>));   \
-    LMK_CUDA(cudaFuncSetAttribute(window_fwd_sm100_kernel<BF, DIM, 2>, attr, (int)kSmemFwd<2>));   \
+    LMK_CUDA(cudaFuncSetAttribute(window_fwd_sm100_kernel<BF, DIM>, attr, (int)kSmemFwd<DIM>));    \
     LMK_CUDA(cudaFuncSetAttribute(window_dq_sm100_kernel<BF, DIM>, attr, (int)kSmemDq));           \
     LMK_CUDA(cudaFuncSetAttribute(window_dkv_sm100_kernel<BF, DIM>, attr, (int)kSmemDkv<DIM>));
     LMK_ATTRS(true, 128) LMK_ATTRS(true, 64) LMK_ATTRS(false, 128) LMK_ATTRS(false, 64)
@@ -1306,17 +1299,14 @@ int window_sm100_fwd(const WindowParams& p, int dtype, cudaStream_t st) {
   CUtensorMap tq, tk, tv;
   int rc = facts_of(&f);
   if (rc != LMK_OK || (rc = maps(p, dtype, &tq, &tk, &tv)) != LMK_OK) return rc;
-  WindowTensors a = {p.o, p.lse, p.lengths, p.H, p.H / p.Hkv, p.Lq, p.Lk, p.D, p.window, p.sinks, p.scale, p.scale * kLog2e};
-  const int n_tiles = (p.Lq + kQTile - 1) / kQTile;
-  const int per_cta = n_tiles == 1 ? 2 : 1;
-  const dim3 grid(p.B * p.H, (n_tiles + per_cta - 1) / per_cta);
-#define LMK_FWD(BF, DIM)                                                                                                                \
-  do {                                                                                                                                  \
-    if (per_cta == 1)                                                                                                                   \
-      LMK_CUDA(launch_overlapped(window_fwd_sm100_kernel<BF, DIM, 1>, grid, dim3(kFwdThreads<1>), kSmemFwd<1>, st, tq, tk, tv, a, f->status)); \
-    else                                                                                                                                \
-      LMK_CUDA(launch_overlapped(window_fwd_sm100_kernel<BF, DIM, 2>, grid, dim3(kFwdThreads<2>), kSmemFwd<2>, st, tq, tk, tv, a, f->status)); \
-  } while (0)
+  const WindowTensors a = {p.o, p.lse, p.lengths, p.B * p.H, p.H, p.H / p.Hkv, p.Lq, p.Lk, p.D, p.window, p.sinks, p.scale * kLog2e};
+  const int64_t units = (int64_t)((p.Lq + kQTile - 1) / kQTile) * p.B * p.H;
+  int most = 2 * f->n_sm;
+  const int cap = attn_sm100_max_ctas();
+  if (cap >= 1 && cap < most) most = cap;
+  const dim3 grid((unsigned)(units < most ? units : most));
+#define LMK_FWD(BF, DIM) \
+  LMK_CUDA(launch_overlapped(window_fwd_sm100_kernel<BF, DIM>, grid, dim3(kFwdThreads), kSmemFwd<DIM>, st, tq, tk, tv, a, f->status))
   if (dtype == LMK_BF16) {
     if (p.D <= 64) LMK_FWD(true, 64); else LMK_FWD(true, 128);
   } else {
