@@ -47,12 +47,12 @@ __device__ __forceinline__ void zero_rows(uint32_t tile, uint32_t subtile_bytes,
   fence_proxy_async_smem();
 }
 
-// A row's visible columns of the key tile that starts at key0: j <= last and (j >= first or j < sink)
-struct Columns {
-  int last, first, sink;
-  __device__ Columns(int pos, int key0, int window, int sinks) : last(pos - key0), first(pos - window + 1 - key0), sink(sinks - key0) {}
-  __device__ bool sees(int j) const { return j <= last && (j >= first || j < sink); }
-};
+// A row's visible columns among 32 keys from key0 on, a bit each: j <= pos - key0 and (j > pos - key0 - window or j < sinks - key0).  (With
+// the comparisons at each column an item at an edge took twice the time of a full one.)
+__device__ __forceinline__ uint32_t low_bits(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u; }
+__device__ __forceinline__ uint32_t columns_seen(int pos, int key0, int window, int sinks) {
+  return low_bits(pos - key0 + 1) & (~low_bits(pos - window + 1 - key0) | low_bits(sinks - key0));
+}
 // Every one of the rows at positions p0 .. p1 sees every one of the keys k0 .. k1 / none sees one.
 __device__ __forceinline__ bool all_seen(int p0, int p1, int k0, int k1, int window, int sinks) {
   return k1 <= p0 && (p1 - k0 < window || k1 < sinks);
@@ -283,9 +283,12 @@ window_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             }
           }
           if (!full) {
-            const Columns col(pos, key0, p.window, p.sinks);
+            const uint32_t lo = columns_seen(pos, key0, p.window, p.sinks), hi = columns_seen(pos, key0 + 32, p.window, p.sinks);
 #pragma unroll
-            for (int j = 0; j < 64; ++j) sv[j] = col.sees(j) ? sv[j] : -INFINITY;
+            for (int j = 0; j < 32; ++j) {
+              sv[j] = lo & (1u << j) ? sv[j] : -INFINITY;
+              sv[32 + j] = hi & (1u << j) ? sv[32 + j] : -INFINITY;
+            }
           }
           const float mx = max_of_64(sv);
           const float mc = mx * c;                                     // -inf: nothing visible
@@ -426,17 +429,16 @@ __device__ __forceinline__ uint64_t ex2_pair(uint64_t x) {
   upk2(x, a, b);
   return pk2(ex2(a), ex2(b));
 }
-// x: scores -> weights 2^(s c + nl), nl = -lse, of pair j given by nl(j); hidden columns become 0 (kind 1)
-template <typename NegLse, typename Sees>
-__device__ __forceinline__ void weights_of(uint64_t (&x)[kCols / 2], int kind, float c, NegLse nl, Sees sees) {
+// x: scores -> weights 2^(s c + nl), nl = -lse; hidden columns become 0 (kind 1)
+__device__ __forceinline__ void weights_of(uint64_t (&x)[kCols / 2], int kind, uint32_t seen, float c, uint64_t nl) {
   const uint64_t c2 = pk2(c, c);
 #pragma unroll
   for (int j = 0; j < kCols / 2; ++j) {
-    const uint64_t e = fma2(x[j], c2, nl(j));
+    const uint64_t e = fma2(x[j], c2, nl);
     if (kind == 1) {
       float a, b;
       upk2(e, a, b);
-      x[j] = pk2(sees(2 * j) ? ex2(a) : 0.f, sees(2 * j + 1) ? ex2(b) : 0.f);
+      x[j] = pk2(seen & (1u << 2 * j) ? ex2(a) : 0.f, seen & (2u << 2 * j) ? ex2(b) : 0.f);
     } else if (j % kBwdPolyEvery == 1) {
       x[j] = ex2_poly2<3>(e);
     } else {
@@ -446,19 +448,19 @@ __device__ __forceinline__ void weights_of(uint64_t (&x)[kCols / 2], int kind, f
     }
   }
 }
-// dS = p (dP - delta) scale in 16 bits; nd(j): -delta scale of pair j.  What a hidden value or a padded row brought along is dropped by
+// dS = p (dP - delta) scale in 16 bits; nd = -delta scale.  What a hidden value or a padded row brought along is dropped by
 // a select, not multiplied by 0 (kind 1).
-template <bool kBf16, typename NegDelta, typename Sees>
+template <bool kBf16>
 __device__ __forceinline__ void dscores_of(uint32_t (&w)[kCols / 2], const uint64_t (&p)[kCols / 2], const uint64_t (&dp)[kCols / 2], int kind,
-                                           float scale, NegDelta nd, Sees sees) {
+                                           uint32_t seen, float scale, uint64_t nd) {
   const uint64_t s2 = pk2(scale, scale);
 #pragma unroll
   for (int j = 0; j < kCols / 2; ++j) {
     float a, b;
-    upk2(mul2(p[j], fma2(dp[j], s2, nd(j))), a, b);
+    upk2(mul2(p[j], fma2(dp[j], s2, nd)), a, b);
     if (kind == 1) {
-      a = sees(2 * j) ? a : 0.f;
-      b = sees(2 * j + 1) ? b : 0.f;
+      a = seen & (1u << 2 * j) ? a : 0.f;
+      b = seen & (2u << 2 * j) ? b : 0.f;
     }
     w[j] = pack2<kBf16>(a, b);
   }
@@ -891,7 +893,7 @@ constexpr int kDqThreads = (kBwdWarps + 2) * 32;
 
 struct DqSmem {
   uint64_t qdo_full, patch;
-  uint64_t ops_ready;       // the unit's Q and dO rows sit in TMEM (written by the softmax warpgroups)
+  uint64_t ops_ready;       // the unit's Q and dO rows sit in TMEM (written by the pair of warpgroups that takes its first item)
   uint64_t ops_free;        // the S / dP products of the unit have read them
   uint64_t delta_read;      // the softmax warpgroups are done with the Q, dO and O tiles in shared memory
   uint64_t full[kDqStages], empty[kDqStages];
@@ -900,6 +902,7 @@ struct DqSmem {
   uint64_t acc_full[2];     // per draining pair of warpgroups (the one that took the unit's last item)
   uint64_t acc_empty;
   uint32_t tmem_base;
+  float part[2][2][kQTile];                            // [pair][half]: shares of the sums of O dO
 };
 struct DqArgs {
   const float* lse;
@@ -915,14 +918,17 @@ __global__ void __launch_bounds__(kDqThreads, 1)
 window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
                        const __grid_constant__ CUtensorMap tm_o, const DqArgs p, int* status) {
-  extern __shared__ uint8_t smem_raw[];
-  const uint32_t raw = smem_u32(smem_raw);
-  const uint32_t base = (raw + 1023u) & ~1023u;
+  extern __shared__ __align__(1024) uint8_t smem_aligned[];
+  const uint32_t base = smem_u32(smem_aligned);
+  if ((base & 1023u) != 0) {                         // the swizzle needs it
+    if (threadIdx.x == 0) atomicCAS(status, 0, kErrDqProducer);
+    return;
+  }
   const uint32_t q_tile = base, do_tile = base + 32768u;
   auto k_slot = [&](int s) { return base + 65536u + (uint32_t)s * 32768u; };
   auto v_slot = [&](int s) { return base + 65536u + (uint32_t)s * 32768u + 16384u; };
   const uint32_t o_tile = base + 65536u + kDqStages * 32768u;                           // forward output tile, only for delta
-  DqSmem* sm = reinterpret_cast<DqSmem*>(smem_raw + (base - raw) + 65536u + kDqStages * 32768u + 32768u);
+  DqSmem* sm = reinterpret_cast<DqSmem*>(smem_aligned + 65536u + kDqStages * 32768u + 32768u);
 
   const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
   const int n_tiles = (p.Lq + kQTile - 1) / kQTile, off = p.Lk - p.Lq, n_units = n_tiles * p.BH;
@@ -930,7 +936,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 
   if (tid == 0) {
     for (uint64_t* bar : {&sm->qdo_full, &sm->patch}) mbar_init(smem_u32(bar), 1);
-    mbar_init(smem_u32(&sm->ops_ready), kBwdWarps * 32);
+    mbar_init(smem_u32(&sm->ops_ready), 256);
     mbar_init(smem_u32(&sm->ops_free), 1);
     mbar_init(smem_u32(&sm->delta_read), kBwdWarps * 32);
     for (int s = 0; s < kDqStages; ++s) {
@@ -1001,24 +1007,25 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     constexpr uint32_t idesc_s = instr_desc_f16(fmt, 128, 64, 0, 0), idesc_q = instr_desc_f16(fmt, 128, kD, 0, 1);
     const uint64_t dk0 = smem_desc_sw128(k_slot(0), 16, 1024), dv0 = smem_desc_sw128(v_slot(0), 16, 1024);
     const uint64_t dk0t = smem_desc_sw128(k_slot(0), kHalfTile, 1024);
-    int r = -1, u = -1;
-    auto next_unit = [&]() {                       // items of the next unit that has any, 0: no more
+    struct Cursor { int r, i, n, u; };             // item i of n in the u-th unit that has any; n = 0: no more
+    auto advance = [&](Cursor& c) {
+      if (++c.i < c.n) return;
+      c.i = 0;
+      c.n = 0;
+      ++c.u;
       for (;;) {
-        const int w = unit_at(++r);
-        if (w >= n_units) return 0;
-        const int n = warp_uniform(unit_of(w).total);
-        if (n > 0) {
-          ++u;
-          return n;
-        }
+        const int w = unit_at(++c.r);
+        if (w >= n_units) return;
+        c.n = warp_uniform(unit_of(w).total);
+        if (c.n > 0) return;
       }
     };
     auto slot = [&](uint64_t d, int it) { return desc_advance(d, (uint32_t)(it % kDqStages) * 32768u); };
-    auto issue_s = [&](bool first, int it) {
+    auto issue_s = [&](const Cursor& c, int it) {
       const int sb = it % kSdpBufs;
       mbar_wait(smem_u32(&sm->full[it % kDqStages]), (it / kDqStages) & 1, status, kErrDqMma);
       if (it >= kSdpBufs) mbar_wait(smem_u32(&sm->s_free[sb]), ((it / kSdpBufs) & 1) ^ 1, status, kErrDqMma);
-      if (first) mbar_wait(smem_u32(&sm->ops_ready), u & 1, status, kErrDqMma);
+      if (c.i == 0) mbar_wait(smem_u32(&sm->ops_ready), c.u & 1, status, kErrDqMma);
       tc_fence_after();
       const uint64_t db = slot(dk0, it);
       if (elect_one()) {
@@ -1028,7 +1035,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         mma_commit(smem_u32(&sm->s_full[sb]));
       }
     };
-    auto issue_dp = [&](bool last, int it) {
+    auto issue_dp = [&](const Cursor& c, int it) {
       const int sb = it % kSdpBufs;
       const uint64_t db = slot(dv0, it);
       if (elect_one()) {
@@ -1036,36 +1043,40 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         for (int kk = 0; kk < kD / 16; ++kk)
           mma_f16_ts(tmem_dp + sb * 64, tmem_do + kk * 8, desc_advance(db, kmajor_step(kk, kHalfTile)), idesc_s, kk > 0);
         mma_commit(smem_u32(&sm->dp_full[sb]));
-        if (last) mma_commit(smem_u32(&sm->ops_free));        // the next unit's Q / dO rows may be written
+        if (c.i == c.n - 1) mma_commit(smem_u32(&sm->ops_free));        // the next unit's Q / dO rows may be written
       }
     };
-    // A unit's first two items are issued behind the last dQ of the unit before: its rows come to TMEM only when the softmax warps are
-    // through with that one's items.
-    int it = 0;
-    for (int n = next_unit(); n > 0;) {
-      for (int i = 0; i < min(n, kSdpBufs); ++i) {
-        issue_s(i == 0, it + i);
-        issue_dp(i == n - 1, it + i);
-      }
-      for (int i = 0; i < n; ++i, ++it) {
-        const int sb = it % kSdpBufs;
-        const bool more = i + kSdpBufs < n;
-        if (more) issue_s(false, it + kSdpBufs);
-        if (i == 0) mbar_wait(smem_u32(&sm->acc_empty), (u & 1) ^ 1, status, kErrDqMma);
-        mbar_wait(smem_u32(&sm->ds_ready[sb]), (it / kSdpBufs) & 1, status, kErrDqMma);
-        tc_fence_after();
-        const uint64_t dkt = slot(dk0t, it);
-        if (elect_one()) {
+    Cursor now = {-1, 0, 0, -1};
+    advance(now);
+    Cursor ahead = now;
+    for (int j = 0; j < kSdpBufs && ahead.n > 0; ++j) {
+      issue_s(ahead, j);
+      issue_dp(ahead, j);
+      advance(ahead);
+    }
+    for (int it = 0; now.n > 0; ++it) {
+      const int sb = it % kSdpBufs, next = it + kSdpBufs;
+      // S goes ahead of dQ but for a unit's first item: its rows come behind this item's dS, from the same warpgroups
+      const bool early = ahead.n > 0 && ahead.i > 0;
+      if (early) issue_s(ahead, next);
+      if (now.i == 0) mbar_wait(smem_u32(&sm->acc_empty), (now.u & 1) ^ 1, status, kErrDqMma);
+      mbar_wait(smem_u32(&sm->ds_ready[sb]), (it / kSdpBufs) & 1, status, kErrDqMma);
+      tc_fence_after();
+      const uint64_t dkt = slot(dk0t, it);
+      if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kBlk / 16; ++kk)
-            mma_f16_ts(tmem_dq, tmem_dp + sb * 64 + (kk >> 1) * kCols + (kk & 1) * 8, desc_advance(dkt, kk * 2048), idesc_q,
-                       (i > 0 || kk > 0) ? 1u : 0u);
-          mma_commit(smem_u32(&sm->empty[it % kDqStages]));
-          if (i == n - 1) mma_commit(smem_u32(&sm->acc_full[it & 1]));     // drained by the pair that took the last item
-        }
-        if (more) issue_dp(i + kSdpBufs == n - 1, it + kSdpBufs);
+        for (int kk = 0; kk < kBlk / 16; ++kk)
+          mma_f16_ts(tmem_dq, tmem_dp + sb * 64 + (kk >> 1) * kCols + (kk & 1) * 8, desc_advance(dkt, kk * 2048), idesc_q,
+                     (now.i > 0 || kk > 0) ? 1u : 0u);
+        mma_commit(smem_u32(&sm->empty[it % kDqStages]));
+        if (now.i == now.n - 1) mma_commit(smem_u32(&sm->acc_full[it & 1]));     // drained by the pair that took the last item
       }
-      n = next_unit();
+      if (ahead.n > 0) {
+        if (!early) issue_s(ahead, next);
+        issue_dp(ahead, next);
+        advance(ahead);
+      }
+      advance(now);
     }
     __syncwarp();
   } else {
@@ -1075,8 +1086,8 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     const int row = tid & 127;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     int it0 = 0, u = 0, drains = 0;
-    // dQ of a unit is drained by the pair that took its last item, half of the features each, but only behind the prologue of the next
-    // unit: its last product queues behind that unit's first S / dP products
+    // dQ of a unit is drained by the pair that took its last item, half of the features each, while that item's product runs it sums up
+    // the next unit's O dO; the other pair has brought that unit's rows to TMEM meanwhile
     constexpr int kOut = kD / 2;
     int64_t drain_row = -1;
     bool drain_stored = false, drain_valid = false;
@@ -1134,22 +1145,33 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         continue;
       }
       const int warp_p0 = warp_uniform(off + un.t * kQTile + (warp & 3) * 32), warp_p1 = warp_p0 + 31;
-      // The unit's rows: a warpgroup moves half of the features of Q (pair 0) or dO (pair 1) to TMEM and sums O * dO over a quarter of
-      // them, straight from the swizzled tiles.
       mbar_wait(smem_u32(&sm->qdo_full), u & 1, status, kErrDqSoftmax);
-      constexpr int kChunks = kD / 16;             // 16-byte chunks of half a row
-      uint32_t opw[4 * kChunks];
       auto chunk_at = [&](int c) { return (uint32_t)(c >> 3) * kTileBytes + (uint32_t)row * 128u + (uint32_t)(((c & 7) ^ (row & 7)) << 4); };
+      // The pair that takes the unit's first item moves its rows to TMEM, a warpgroup Q and the other dO: row -> lane, 32-bit word j (two
+      // features) -> column j, the layout of a K-major A operand
+      if (pair == (it0 & 1)) {
+        mbar_wait(smem_u32(&sm->ops_free), (u & 1) ^ 1, status, kErrDqSoftmax);
+        tc_fence_after();
 #pragma unroll
-      for (int c = 0; c < kChunks; ++c)
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(opw[4 * c]), "=r"(opw[4 * c + 1]), "=r"(opw[4 * c + 2]), "=r"(opw[4 * c + 3])
-                     : "r"((pair == 0 ? q_tile : do_tile) + chunk_at(half * kChunks + c)));
+        for (int c0 = 0; c0 < kD / 8; c0 += 8) {
+          uint32_t x[32];
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(x[4 * c]), "=r"(x[4 * c + 1]), "=r"(x[4 * c + 2]), "=r"(x[4 * c + 3])
+                         : "r"((half == 0 ? q_tile : do_tile) + chunk_at(c0 + c)));
+          tmem_st_32x32b_x32((half == 0 ? tmem_q : tmem_do) + c0 * 4 + lane_base, x);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(smem_u32(&sm->ops_ready));
+      }
+      // delta = rowsum(O dO): each pair for itself, a warpgroup half of the features
       float sum = 0.f;
 #pragma unroll
-      for (int c = 0; c < kChunks / 2; ++c) {
+      for (int c = 0; c < kD / 16; ++c) {
         uint32_t ov[4], gv[4];
-        const uint32_t at = chunk_at(g * (kChunks / 2) + c);
+        const uint32_t at = chunk_at(half * (kD / 16) + c);
         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(ov[0]), "=r"(ov[1]), "=r"(ov[2]), "=r"(ov[3]) : "r"(o_tile + at));
         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(gv[0]), "=r"(gv[1]), "=r"(gv[2]), "=r"(gv[3]) : "r"(do_tile + at));
 #pragma unroll
@@ -1166,26 +1188,11 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           sum = fmaf(fo.y, fg.y, sum);
         }
       }
-      // the shares of the sum change hands in the O tile, which everybody has read by then
-      asm volatile("bar.sync 1, %0;" ::"n"(kBwdWarps * 32) : "memory");
-      auto share = [&](int k) { return o_tile + (uint32_t)(k * kQTile + row) * 4u; };
-      asm volatile("st.shared.f32 [%0], %1;" ::"r"(share(g)), "f"(sum) : "memory");
-      // row -> TMEM lane, 32-bit word j (two features) -> column j: the layout of a K-major A operand
-      mbar_wait(smem_u32(&sm->ops_free), (u & 1) ^ 1, status, kErrDqSoftmax);
-      tc_fence_after();
-      {
-        const uint32_t dst = (pair == 0 ? tmem_q : tmem_do) + half * (kD / 4) + lane_base;
-        if constexpr (kD == 128) tmem_st_32x32b_x32(dst, opw);
-        else tmem_st_32x32b_x16(dst, opw);
-        tmem_st_wait();
-      }
-      tc_fence_before();
-      mbar_arrive(smem_u32(&sm->ops_ready));
-      asm volatile("bar.sync 1, %0;" ::"n"(kBwdWarps * 32) : "memory");
-      float part[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(part[k]) : "r"(share(k)) : "memory");
-      const float delta = (part[0] + part[1]) + (part[2] + part[3]);
+      auto together = [&]() { asm volatile("bar.sync %0, 256;" ::"r"(1 + pair) : "memory"); };
+      together();                                  // the last unit's shares have been read
+      sm->part[pair][half][row] = sum;
+      together();
+      const float delta = sm->part[pair][0][row] + sm->part[pair][1][row];
       // TMA writes the next unit's rows through another proxy than these accesses went through
       fence_proxy_async_smem();
       mbar_arrive(smem_u32(&sm->delta_read));
@@ -1196,8 +1203,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       const uint64_t nd = pk2(nds, nds);
       for (int i = (it0 + pair) & 1; i < un.total; i += 2) {
         const int it = it0 + i, sb = it % kSdpBufs, key0 = un.tile_of(i) * kBlk + half * kCols;
-        const Columns col(pos, key0, p.window, p.sinks);
-        auto sees = [&](int j) { return col.sees(j); };
+        const uint32_t seen = columns_seen(pos, key0, p.window, p.sinks);
         // a row of padding spoils its own row of dQ alone, which is not stored
         const int kind = warp_uniform(none_seen(warp_p0, warp_p1, key0, key0 + kCols - 1, p.window, p.sinks) ? 0
                                       : all_seen(warp_p0, warp_p1, key0, key0 + kCols - 1, p.window, p.sinks) ? 2 : 1);
@@ -1208,14 +1214,14 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         if (kind != 0) load_pairs(sp, ts);
         tc_fence_before();
         mbar_arrive(smem_u32(&sm->s_free[sb]));      // S is in registers: its buffer may take the next product
-        if (kind != 0) weights_of(sp, kind, p.scale_log2, [&](int) { return nl; }, sees);
+        if (kind != 0) weights_of(sp, kind, seen, p.scale_log2, nl);
         mbar_wait(smem_u32(&sm->dp_full[sb]), (it / kSdpBufs) & 1, status, kErrDqSoftmax);
         tc_fence_after();
         uint32_t wd[kCols / 2];
         if (kind != 0) {
           uint64_t dp[kCols / 2];
           load_pairs(dp, tdp);
-          dscores_of<kBf16>(wd, sp, dp, kind, p.scale, [&](int) { return nd; }, sees);
+          dscores_of<kBf16>(wd, sp, dp, kind, seen, p.scale, nd);
         } else {
 #pragma unroll
           for (int j = 0; j < kCols / 2; ++j) wd[j] = 0u;
@@ -1246,7 +1252,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 // ---------------------------------------------------------------------------------------------- host side
 template <int kD> constexpr size_t kSmemFwd = (kD / 64) * (kTileBytes + kFwdSlots<kD> * kHalfTile) + sizeof(FwdSmem<kFwdSlots<kD>>);
 template <int kD> constexpr size_t kSmemDkv = 1024 + (2 + 2 * kDkvStages) * (kD / 64) * kTileBytes + sizeof(DkvSmem);
-constexpr size_t kSmemDq = 1024 + 65536 + kDqStages * 32768 + 32768 + sizeof(DqSmem);
+constexpr size_t kSmemDq = 65536 + kDqStages * 32768 + 32768 + sizeof(DqSmem);
 static_assert(kSmemFwd<128> <= 233472 / 2 - 1024 && kSmemFwd<64> <= 233472 / 2 - 1024 && kSmemDkv<128> <= 232448 && kSmemDkv<64> <= 232448 && kSmemDq <= 232448,
               "shared memory of one SM");
 
