@@ -6,6 +6,7 @@
 namespace lmk {
 namespace {
 
+constexpr size_t kNextBytes = 256;
 constexpr size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 int check_window(const void* q, const void* k, const void* v, const float* lse, int B, int H, int Hkv, int Lq, int Lk, int D,
@@ -78,7 +79,7 @@ __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant_
 #pragma unroll
   for (int g = 0; g < 2; ++g) {                     // dK, dV
     float4 sum = *reinterpret_cast<const float4*>(part + g * (slot / 2));
-    for (int r = 1; r <= runs; ++r) {
+    for (int r = 1; r <= runs && tile * kk + key < p.sinks; ++r) {      // (the runs' rows see no other keys)
       const float4 x = *reinterpret_cast<const float4*>(part + r * slot + g * (slot / 2));
       sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
     }
@@ -126,7 +127,7 @@ extern "C" size_t lmk_window_bwd_workspace(int B, int H, int Hkv, int Lq, int Lk
   int qt, kk;
   tile_sizes(dtype, &qt, &kk);
   if (plan_split(&s, B, Hkv, Lq, Lk, window < Lk ? window : Lk, sinks < Lk ? sinks : Lk, qt, kk) != LMK_OK) return 0;
-  return up256(sizeof(float) * (size_t)B * H * Lq) + up256(part_bytes(s, B, Hkv, D, kk));
+  return kNextBytes + up256(sizeof(float) * (size_t)B * H * Lq) + up256(part_bytes(s, B, Hkv, D, kk));
 }
 
 extern "C" int lmk_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dO, const float* lse,
@@ -151,11 +152,12 @@ extern "C" int lmk_window_bwd(const void* q, const void* k, const void* v, const
   if ((rc = plan_split(&p.split, B, Hkv, Lq, Lk, p.window, p.sinks, qt, kk)) != LMK_OK) return rc;
   LMK_CHECK_ARG((int64_t)B * Hkv * (p.split.tiles > 0 ? p.split.tiles : 1) <= 65535, "window attention backward: %d sinks of %d key heads are too many",
                 sinks, B * Hkv);
-  const size_t delta_bytes = up256(sizeof(float) * (size_t)B * H * Lq), need = delta_bytes + up256(part_bytes(p.split, B, Hkv, D, kk));
+  const size_t delta_bytes = up256(sizeof(float) * (size_t)B * H * Lq), need = kNextBytes + delta_bytes + up256(part_bytes(p.split, B, Hkv, D, kk));
   if (workspace == nullptr || workspace_bytes < need || ((uintptr_t)workspace & 255) != 0)
     return fail(LMK_ERR_WORKSPACE, "window attention backward: workspace of %zu bytes on a 256-byte boundary needed", need);
-  p.delta = static_cast<float*>(workspace);
-  p.split.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + delta_bytes);
+  p.next = static_cast<int*>(workspace);
+  p.delta = reinterpret_cast<float*>(static_cast<char*>(workspace) + kNextBytes);
+  p.split.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kNextBytes + delta_bytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return dtype == LMK_F32 ? window_f32_bwd(p, st) : window_sm100_bwd(p, dtype, st);
 }

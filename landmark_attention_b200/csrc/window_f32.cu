@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(kThreads) window_dkv_f32_kernel(const __grid_c
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const int key = ty * 4 + r;
-    if (key0 + key >= p.Lk) continue;
+    if (key0 + key >= (run >= 0 ? p.sinks : p.Lk)) continue;      // a run's rows see the sinks alone
     const int64_t at = ((int64_t)bk * p.Lk + key0 + key) * p.D;
 #pragma unroll
     for (int c = 0; c < kD / 16; ++c) {

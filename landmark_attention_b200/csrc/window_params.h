@@ -7,7 +7,7 @@ namespace lmk {
 
 // dK and dV of the key tiles that hold sinks get contributions from every later query.  Their query tiles are dealt out to several units:
 // the ones that see the tile through the window (as for every key tile), and runs of `run` tiles of the others, at most `runs` of
-// them.  Each unit leaves an fp32 sum, and a last kernel adds these up in order.
+// them.  Each unit leaves an fp32 sum, the runs of the sinks' rows alone, and a last kernel adds these up in order.
 struct SinkSplit {
   int tiles = 0;       // key tiles that hold sinks; 0: no tile is split
   int run = 0, runs = 0;
@@ -21,6 +21,7 @@ struct WindowParams {
   const int* lengths;          // [B] or null
   void *dq, *dk, *dv;
   float* delta;                // [B*H, Lq] scratch (backward)
+  int* next;                   // scratch (backward of 16-bit types): the next unit of the dK/dV kernel
   int B, H, Hkv, Lq, Lk, D, window, sinks;      // 1 <= window <= Lk, 0 <= sinks <= Lk
   int64_t qs[3], ks[3], vs[3], dos[3];          // element strides {batch, head, row}
   float scale;

@@ -61,6 +61,12 @@ __device__ __forceinline__ bool none_seen(int p0, int p1, int k0, int k1, int wi
   return k0 > p1 || (p0 - k1 >= window && k0 >= sinks);
 }
 
+// n 16-byte pieces from `to` on become zeros, by `threads` threads side by side (a row a thread took 15 000 clk for 128 rows)
+__device__ __forceinline__ void zero_fill(void* to, int n, int thread, int threads) {
+#pragma unroll 1
+  for (int i = thread; i < n; i += threads) reinterpret_cast<uint4*>(to)[i] = make_uint4(0u, 0u, 0u, 0u);
+}
+
 struct WindowTensors {
   void* o;
   float* lse;
@@ -249,10 +255,8 @@ window_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       const bool stored = grow < p.Lq;
       uint4* const orow = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.o) + ((int64_t)u.bh * p.Lq + grow) * p.D);
       if (u.total == 0) {                            // nothing but padding
-        if (stored) {
-          for (int e = 0; e < p.D / 8; ++e) orow[e] = make_uint4(0u, 0u, 0u, 0u);
-          p.lse[(int64_t)u.bh * p.Lq + grow] = INFINITY;
-        }
+        zero_fill(reinterpret_cast<uint16_t*>(p.o) + ((int64_t)u.bh * p.Lq + u.t * kQTile) * p.D, min(kQTile, p.Lq - u.t * kQTile) * p.D / 8, tid, 128);
+        if (stored) p.lse[(int64_t)u.bh * p.Lq + grow] = INFINITY;
         __syncwarp();
         continue;
       }
@@ -478,6 +482,7 @@ __device__ __forceinline__ void dscores_of(uint32_t (&w)[kCols / 2], const uint6
 constexpr int kPair = 128;                          // keys of a unit
 constexpr int kDkvThreads = (kBwdWarps + 2) * 32;
 constexpr int kDkvStages = 2;
+constexpr int kDealt = 4;                           // unit numbers on their way from the loading warp to the others
 
 struct DkvSmem {
   uint64_t k_full, k_empty, v_full, v_empty, patch;
@@ -487,6 +492,8 @@ struct DkvSmem {
   uint64_t s_full, dp_full;                               // the products' results are there
   uint64_t p_ready, ds_ready;                             // P and dS have taken their places
   uint64_t acc_full[2], acc_empty[2];                     // [0] dV, [1] dK
+  uint64_t dealt_full[kDealt], dealt_empty[kDealt];
+  int dealt[kDealt];
   uint32_t tmem_base;
   alignas(16) float nlse[kDkvStages][kQTile];             // -lse
   alignas(16) float ndelta[kDkvStages][kQTile];           // -delta scale
@@ -496,6 +503,7 @@ struct DkvArgs {
   const float *lse, *delta;
   void *dk, *dv;
   const int* lengths;
+  int* next;                                        // units given out beyond the first of each CTA; set to 0 by the dQ kernel
   int H, Hkv, G, B, Lq, Lk, D, window, sinks, n_pairs;
   float scale, scale_log2;
   SinkSplit split;
@@ -525,7 +533,8 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
   const int off = p.Lk - p.Lq, heads = p.B * p.Hkv;
   const int n_runs = p.split.tiles * p.split.runs * heads, n_units = n_runs + p.n_pairs * heads;
-  // the runs first: they are as long as the longest of the others
+  // Units differ by the number of query tiles, with ragged sequences many times over: each CTA asks for its next one (dealt out in turn, the
+  // busiest had 93 000 clk and the idlest 59 000 at the training size).  The runs come first: they are as long as the longest of the others.
   auto unit_of = [&](int w) {
     DkvUnit u;
     int bk;
@@ -568,6 +577,10 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       mbar_init(smem_u32(&sm->acc_full[g]), 1);
       mbar_init(smem_u32(&sm->acc_empty[g]), kBwdWarps * 16);
     }
+    for (int s = 0; s < kDealt; ++s) {
+      mbar_init(smem_u32(&sm->dealt_full[s]), 1);
+      mbar_init(smem_u32(&sm->dealt_empty[s]), kBwdWarps + 1);
+    }
     mbar_init_fence();
   }
   if (warp == kBwdWarps + 1) tmem_alloc(smem_u32(&sm->tmem_base), 512);
@@ -576,6 +589,13 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   tc_fence_after();
   const uint32_t tmem = (uint32_t)warp_uniform((int)sm->tmem_base);
   const uint32_t tmem_s = tmem, tmem_dp = tmem + 128u, tmem_dv = tmem + 256u, tmem_dk = tmem + 256u + kD;
+  auto dealt = [&](int r, int where) {             // number of the CTA's r-th unit
+    mbar_wait(smem_u32(&sm->dealt_full[r % kDealt]), (r / kDealt) & 1, status, where);
+    const int w = warp_uniform(sm->dealt[r % kDealt]);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&sm->dealt_empty[r % kDealt]));
+    return w;
+  };
   // A operand of K-step kk (16 queries) of P^T / dS^T: a warpgroup's 32 queries sit in the first 16 of their 32 columns
   auto a_step = [](int kk) { return (uint32_t)((kk >> 1) * kCols + (kk & 1) * 8); };
 
@@ -583,10 +603,45 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     // ------------------------------------------------------------------ loads: lane 0 issues TMA, all lanes bring the statistics
     int it = 0, u = 0, patches = 0;
     bool behind = false;                           // behind the dQ kernel, which writes delta
-    for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
+    auto deal = [&](int r, int w) {
+      mbar_wait(smem_u32(&sm->dealt_empty[r % kDealt]), ((r / kDealt) & 1) ^ 1, status, kErrDkvProducer);
+      if (lane == 0) {
+        sm->dealt[r % kDealt] = w;
+        mbar_arrive(smem_u32(&sm->dealt_full[r % kDealt]));
+      }
+      __syncwarp();
+    };
+    auto ask_unit = [&]() {
+      if (!behind) grid_dep_wait();
+      behind = true;
+      int w = 0;
+      if (lane == 0) w = gridDim.x + atomicAdd(p.next, 1);
+      return __shfl_sync(0xffffffffu, w, 0);
+    };
+    // The others get no unit without items: whoever issues the products looks one unit ahead, and the softmax warps would have to clear a
+    // row of such units first.  Gradients of keys that nobody sees are written here.
+    auto with_items = [&](int w) {
+      for (; w < n_units; w = ask_unit()) {
+        const DkvUnit un = unit_of(w);
+        if (un.n_q > 0) break;
+        if (!un.base()) continue;
+        const int bk = un.b * p.Hkv + un.hk;
+        if (un.pair < p.split.tiles) {
+          zero_fill(p.split.part + ((int64_t)bk * p.split.tiles + un.pair) * (1 + p.split.runs) * 2 * kPair * p.D, 2 * kPair * p.D / 4, lane, 32);
+        } else {
+          const int64_t at = ((int64_t)bk * p.Lk + un.pair * kPair) * p.D;
+          const int n = min(kPair, p.Lk - un.pair * kPair) * p.D / 8;
+          zero_fill(reinterpret_cast<uint16_t*>(p.dk) + at, n, lane, 32);
+          zero_fill(reinterpret_cast<uint16_t*>(p.dv) + at, n, lane, 32);
+        }
+      }
+      return w;
+    };
+    int w_next = with_items(blockIdx.x);
+    deal(0, w_next);
+    for (int r = 0, w = w_next; w < n_units; w = w_next, ++r) {
       const DkvUnit un = unit_of(w);
       const int n_items = un.n_q * p.G;
-      if (n_items == 0) continue;
       auto load_pair = [&](uint32_t dst, const CUtensorMap* tm, uint64_t* full, uint64_t* empty) {
         const uint32_t fb = smem_u32(full);
         mbar_wait(smem_u32(empty), (u & 1) ^ 1, status, kErrDkvProducer);
@@ -634,11 +689,11 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         const int s = it % kStages, g = i / un.n_q, h = un.hk * p.G + g, tile = un.first + i - g * un.n_q;
         load_rows(q_slot(s), &tm_q, &sm->q_full[s], &sm->q_empty[s], h, tile);
         if (i == 0) load_pair(v_pair, &tm_v, &sm->v_full, &sm->v_empty);
-        if (!behind) {
-          grid_dep_wait();
-          behind = true;
+        if (i == 0) {
+          w_next = with_items(ask_unit());
+          deal(r + 1, w_next);
+          ask(0);
         }
-        if (i == 0) ask(0);
         *reinterpret_cast<float4*>(&sm->nlse[s][lane * 4]) = nl;
         *reinterpret_cast<float4*>(&sm->ndelta[s][lane * 4]) = nd;
         mbar_arrive(smem_u32(&sm->stat_full[s]));
@@ -658,18 +713,12 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     const uint64_t dk0 = smem_desc_sw128(k_pair, 16, 1024), dv0 = smem_desc_sw128(v_pair, 16, 1024);
     const uint64_t dq0 = smem_desc_sw128(q_slot(0), 16, 1024), ddo0 = smem_desc_sw128(do_slot(0), 16, 1024);
     const uint64_t dq0t = smem_desc_sw128(q_slot(0), kTileBytes, 1024), ddo0t = smem_desc_sw128(do_slot(0), kTileBytes, 1024);
-    struct Cursor { int r, i, n, u; };             // item i of n in the u-th unit that has any; n = 0: no more
+    struct Cursor { int i, n, u; };                // item i of n in the u-th unit; n = 0: no more
     auto advance = [&](Cursor& c) {
       if (++c.i < c.n) return;
       c.i = 0;
-      c.n = 0;
-      ++c.u;
-      for (;;) {
-        const int w = unit_at(++c.r);
-        if (w >= n_units) return;
-        c.n = warp_uniform(unit_of(w).n_q) * p.G;
-        if (c.n > 0) return;
-      }
+      const int w = dealt(++c.u, kErrDkvMma);
+      c.n = w < n_units ? warp_uniform(unit_of(w).n_q) * p.G : 0;
     };
     auto slot = [&](uint64_t d, int it) { return desc_advance(d, (uint32_t)(it % kStages) * 2 * kOperand); };
     auto issue_s = [&](const Cursor& c, int it) {
@@ -698,7 +747,7 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         if (c.i == c.n - 1) mma_commit(smem_u32(&sm->v_empty));
       }
     };
-    Cursor now = {-1, 0, 0, -1};
+    Cursor now = {0, 0, -1};
     advance(now);
     if (now.n > 0) {
       issue_s(now, 0);
@@ -741,7 +790,7 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t ts = tmem_s + (uint32_t)g * kCols + lane_base, tdp = tmem_dp + (uint32_t)g * kCols + lane_base;
     int it = 0, u = 0;
-    for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
+    for (int w = dealt(0, kErrDkvSoftmax); w < n_units; w = dealt(++u, kErrDkvSoftmax)) {
       const DkvUnit un = unit_of(w);
       const int n_items = un.n_q * p.G, bk = un.b * p.Hkv + un.hk, key = un.pair * kPair + row;
       const bool split = un.pair < p.split.tiles;
@@ -750,19 +799,6 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       constexpr int kOut = kD / 2;
       const bool is_dv = g < 2;
       const int col0 = (g & 1) * kOut;
-      if (n_items == 0) {                          // keys that nobody sees
-        if (un.base() && key < p.Lk) {
-          if (split) {
-            float* to = part + ((is_dv ? kPair : 0) + row) * p.D;
-            for (int e = col0; e < min(col0 + kOut, p.D); e += 4) *reinterpret_cast<float4*>(to + e) = make_float4(0.f, 0.f, 0.f, 0.f);
-          } else {
-            uint16_t* to = reinterpret_cast<uint16_t*>(is_dv ? p.dv : p.dk) + ((int64_t)bk * p.Lk + key) * p.D;
-            for (int e = col0; e < min(col0 + kOut, p.D); e += 2) *reinterpret_cast<uint32_t*>(to + e) = 0u;
-          }
-        }
-        __syncwarp();
-        continue;
-      }
       const int kmin = warp_uniform(un.pair * kPair + (warp & 3) * 32), kmax = kmin + 31;
       const int frow = kmin + (lane >> 2), fcol = 2 * (lane & 3);      // fragments: keys frow + 8 e, queries fcol + 8 j and the next
       for (int i = 0, tq = un.first; i < n_items; ++i, ++it) {
@@ -855,6 +891,7 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       tc_fence_after();
       const uint32_t t_acc = (is_dv ? tmem_dv : tmem_dk) + col0 + lane_base;
       float* const prow = split ? part + ((is_dv ? kPair : 0) + row) * p.D : nullptr;
+      const bool kept = un.base() || key < p.sinks;      // (a run's rows see the sinks alone)
 #pragma unroll
       for (int c = 0; c < kOut / 32; ++c) {
         uint32_t ra[32];
@@ -867,14 +904,13 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         if (split) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (col0 + c * 32 + e * 4 < p.D)
+            if (kept && col0 + c * 32 + e * 4 < p.D)
               *reinterpret_cast<uint4*>(prow + col0 + c * 32 + e * 4) = make_uint4(ra[4 * e], ra[4 * e + 1], ra[4 * e + 2], ra[4 * e + 3]);
         } else {
           store_acc_cols<kBf16>(is_dv ? p.dv : p.dk, row_off, ra, col0 + c * 32, p.D, lane);
         }
         __syncwarp();
       }
-      ++u;
     }
     grid_dep_wait();                               // a CTA without units, too, ends behind the kernel in front
     tc_fence_before();
@@ -907,6 +943,7 @@ struct DqSmem {
 struct DqArgs {
   const float* lse;
   float* delta;
+  int* next;                // set to 0 for the dK/dV kernel
   void* dq;
   const int* lengths;
   int H, Hkv, G, BH, Lq, Lk, D, window, sinks;
@@ -963,6 +1000,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   const uint32_t tmem_s = tmem, tmem_dp = tmem + 128, tmem_dq = tmem + 256, tmem_q = tmem + 384, tmem_do = tmem + 448;
   grid_dep_wait();
   grid_dep_launch();
+  if (blockIdx.x == 0 && tid == 0) *p.next = 0;
 
   if (warp == kBwdWarps) {
     // ------------------------------------------------------------------ TMA producer
@@ -1136,11 +1174,9 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       const float lse = n_lse;
       fetch_rows(unit_at(r + 1));
       if (un.total == 0) {                         // nothing but padding
-        if (g == 0 && stored) {
-          uint4* orow = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.dq) + grow * p.D);
-          for (int e = 0; e < p.D / 8; ++e) orow[e] = make_uint4(0u, 0u, 0u, 0u);
-          p.delta[grow] = 0.f;
-        }
+        zero_fill(reinterpret_cast<uint16_t*>(p.dq) + ((int64_t)un.bh * p.Lq + un.t * kQTile) * p.D, min(kQTile, p.Lq - un.t * kQTile) * p.D / 8, tid,
+                  kBwdWarps * 32);
+        if (g == 0 && stored) p.delta[grow] = 0.f;
         __syncwarp();
         continue;
       }
@@ -1336,8 +1372,8 @@ int window_sm100_bwd(const WindowParams& p, int dtype, cudaStream_t st) {
   const int n_pairs = (p.Lk + kPair - 1) / kPair, G = p.H / p.Hkv;
   const int64_t dq_units = (int64_t)((p.Lq + kQTile - 1) / kQTile) * p.B * p.H;
   const int64_t dkv_units = ((int64_t)n_pairs + (int64_t)p.split.tiles * p.split.runs) * p.B * p.Hkv;
-  const DqArgs aq = {p.lse, p.delta, p.dq, p.lengths, p.H, p.Hkv, G, p.B * p.H, p.Lq, p.Lk, p.D, p.window, p.sinks, p.scale, p.scale * kLog2e};
-  const DkvArgs ak = {p.lse, p.delta, p.dk, p.dv, p.lengths, p.H, p.Hkv, G, p.B, p.Lq, p.Lk, p.D, p.window, p.sinks, n_pairs, p.scale, p.scale * kLog2e,
+  const DqArgs aq = {p.lse, p.delta, p.next, p.dq, p.lengths, p.H, p.Hkv, G, p.B * p.H, p.Lq, p.Lk, p.D, p.window, p.sinks, p.scale, p.scale * kLog2e};
+  const DkvArgs ak = {p.lse, p.delta, p.dk, p.dv, p.lengths, p.next, p.H, p.Hkv, G, p.B, p.Lq, p.Lk, p.D, p.window, p.sinks, n_pairs, p.scale, p.scale * kLog2e,
                       p.split};
   const dim3 grid_q((unsigned)(dq_units < n_sm ? dq_units : n_sm)), grid_k((unsigned)(dkv_units < n_sm ? dkv_units : n_sm));
   // The dK/dV kernel may start on every SM that the dQ kernel has left: it reads q, k, v, dO, lse and lengths, which were complete before
