@@ -39,12 +39,14 @@ enum { kErrFwdProducer = 711, kErrFwdMma = 712, kErrFwdSoftmax = 713, kErrFwdEpi
 __device__ __forceinline__ int length_of(const int* lengths, int b, int Lk) {
   return lengths == nullptr ? Lk : min(max(ld_behind_wait(lengths + b), 0), Lk);
 }
-// rows [from, rows) of a tile of 64-feature sub-tiles become zeros; one thread, ahead of products that read the tile
-__device__ __forceinline__ void zero_rows(uint32_t tile, uint32_t subtile_bytes, int subtiles, int from, int rows) {
+// rows [from, rows) of a tile of 64-feature sub-tiles become zeros, ahead of products that read the tile; one warp (one thread took 6000 clk)
+__device__ __forceinline__ void zero_rows(uint32_t tile, uint32_t subtile_bytes, int subtiles, int from, int rows, int lane) {
+  from = max(from, 0);
   for (int c = 0; c < subtiles; ++c)
-    for (uint32_t a = tile + c * subtile_bytes + from * 128u; a < tile + c * subtile_bytes + rows * 128u; a += 16)
+    for (uint32_t a = tile + c * subtile_bytes + from * 128u + lane * 16u; a < tile + c * subtile_bytes + rows * 128u; a += 512)
       asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(a), "r"(0) : "memory");
   fence_proxy_async_smem();
+  __syncwarp();
 }
 
 // A row's visible columns among 32 keys from key0 on, a bit each: j <= pos - key0 and (j > pos - key0 - window or j < sinks - key0).  (With
@@ -161,35 +163,38 @@ window_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
 
   if (warp == 4) {
     // ------------------------------------------------------------------ loads
-    if (lane == 0) {
-      int m = 0, uq = 0, patches = 0;
-      for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
-        const RowUnit u = unit_of(w);
-        if (u.total == 0) continue;
-        const int hk = u.h / p.G;
-        auto load_kv = [&](const CUtensorMap* tm, int key0, bool patch) {
-          mbar_wait(smem_u32(&sm->empty[m % kSlots]), ((m / kSlots) & 1) ^ 1, status, kErrFwdProducer);
-          const uint32_t bar = smem_u32(patch ? &sm->patch : &sm->full[m % kSlots]);
+    int m = 0, uq = 0, patches = 0;
+    for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
+      const RowUnit u = unit_of(w);
+      if (u.total == 0) continue;
+      const int hk = u.h / p.G;
+      auto load_kv = [&](const CUtensorMap* tm, int key0, bool patch) {
+        mbar_wait(smem_u32(&sm->empty[m % kSlots]), ((m / kSlots) & 1) ^ 1, status, kErrFwdProducer);
+        const uint32_t bar = smem_u32(patch ? &sm->patch : &sm->full[m % kSlots]);
+        if (lane == 0) {
           mbar_arrive_expect_tx(bar, kKvBytes);
           for (int c = 0; c < kD / 64; ++c) tma_load_4d(slot(m) + c * kHalfTile, tm, bar, 64 * c, key0, hk, u.b);
-          if (patch) {
-            mbar_wait(bar, patches++ & 1, status, kErrFwdProducer);
-            zero_rows(slot(m), kHalfTile, kD / 64, u.len - key0, kBlk);
-            mbar_arrive(smem_u32(&sm->full[m % kSlots]));
-          }
-          ++m;
-        };
-        mbar_wait(smem_u32(&sm->q_empty), (uq++ & 1) ^ 1, status, kErrFwdProducer);
+        }
+        __syncwarp();
+        if (patch) {
+          mbar_wait(bar, patches++ & 1, status, kErrFwdProducer);
+          zero_rows(slot(m), kHalfTile, kD / 64, u.len - key0, kBlk, lane);
+          if (lane == 0) mbar_arrive(smem_u32(&sm->full[m % kSlots]));
+        }
+        ++m;
+      };
+      mbar_wait(smem_u32(&sm->q_empty), (uq++ & 1) ^ 1, status, kErrFwdProducer);
+      if (lane == 0) {
         mbar_arrive_expect_tx(smem_u32(&sm->q_full), kQBytes);
         for (int c = 0; c < kD / 64; ++c) tma_load_4d(base + c * kTileBytes, &tm_q, smem_u32(&sm->q_full), 64 * c, u.t * kQTile, u.h, u.b);
-        for (int i = 0; i < u.total; ++i) {
-          const int key0 = u.tile_of(i) * kBlk;
-          load_kv(&tm_k, key0, false);
-          load_kv(&tm_v, key0, key0 + kBlk > u.len && u.len < p.Lk);      // values of the tile the sequence ends in
-        }
+      }
+      __syncwarp();
+      for (int i = 0; i < u.total; ++i) {
+        const int key0 = u.tile_of(i) * kBlk;
+        load_kv(&tm_k, key0, false);
+        load_kv(&tm_v, key0, key0 + kBlk > u.len && u.len < p.Lk);      // values of the tile the sequence ends in
       }
     }
-    __syncwarp();
   } else if (warp == 5) {
     // ------------------------------------------------------------------ products
     constexpr uint32_t fmt = kBf16 ? 1u : 0u;
@@ -618,23 +623,9 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       if (lane == 0) w = gridDim.x + atomicAdd(p.next, 1);
       return __shfl_sync(0xffffffffu, w, 0);
     };
-    // The others get no unit without items: whoever issues the products looks one unit ahead, and the softmax warps would have to clear a
-    // row of such units first.  Gradients of keys that nobody sees are written here.
+    // the others get no unit without items: their keys' gradients, zeros, come from the dQ kernel
     auto with_items = [&](int w) {
-      for (; w < n_units; w = ask_unit()) {
-        const DkvUnit un = unit_of(w);
-        if (un.n_q > 0) break;
-        if (!un.base()) continue;
-        const int bk = un.b * p.Hkv + un.hk;
-        if (un.pair < p.split.tiles) {
-          zero_fill(p.split.part + ((int64_t)bk * p.split.tiles + un.pair) * (1 + p.split.runs) * 2 * kPair * p.D, 2 * kPair * p.D / 4, lane, 32);
-        } else {
-          const int64_t at = ((int64_t)bk * p.Lk + un.pair * kPair) * p.D;
-          const int n = min(kPair, p.Lk - un.pair * kPair) * p.D / 8;
-          zero_fill(reinterpret_cast<uint16_t*>(p.dk) + at, n, lane, 32);
-          zero_fill(reinterpret_cast<uint16_t*>(p.dv) + at, n, lane, 32);
-        }
-      }
+      while (w < n_units && unit_of(w).n_q == 0) w = ask_unit();
       return w;
     };
     int w_next = with_items(blockIdx.x);
@@ -661,14 +652,13 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         if (lane == 0) {
           mbar_arrive_expect_tx(fb, kOperand);
           for (int c = 0; c < kD / 64; ++c) tma_load_4d(dst + c * kTileBytes, tm, fb, 64 * c, tile * kQTile, h, un.b);
-          if (ends) {
-            mbar_wait(fb, patches & 1, status, kErrDkvProducer);
-            zero_rows(dst, kTileBytes, kD / 64, rows, kQTile);
-            mbar_arrive(smem_u32(full));
-          }
         }
-        if (ends) ++patches;
         __syncwarp();
+        if (ends) {
+          mbar_wait(fb, patches++ & 1, status, kErrDkvProducer);
+          zero_rows(dst, kTileBytes, kD / 64, rows, kQTile, lane);
+          if (lane == 0) mbar_arrive(smem_u32(full));
+        }
       };
       float4 nl, nd;
       auto ask = [&](int i) {                      // statistics of an item's rows 4 lane .. 4 lane + 3, one item ahead
@@ -944,17 +934,18 @@ struct DqArgs {
   const float* lse;
   float* delta;
   int* next;                // set to 0 for the dK/dV kernel
-  void* dq;
+  void *dq, *dk, *dv;       // dk, dv: rows that no query sees
   const int* lengths;
-  int H, Hkv, G, BH, Lq, Lk, D, window, sinks;
+  int H, Hkv, G, BH, Lq, Lk, D, window, sinks, n_pairs;
   float scale, scale_log2;
+  SinkSplit split;
 };
 
 template <bool kBf16, int kD>
 __global__ void __launch_bounds__(kDqThreads, 1)
 window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
-                       const __grid_constant__ CUtensorMap tm_o, const DqArgs p, int* status) {
+                       const __grid_constant__ CUtensorMap tm_o, const __grid_constant__ DqArgs p, int* status) {
   extern __shared__ __align__(1024) uint8_t smem_aligned[];
   const uint32_t base = smem_u32(smem_aligned);
   if ((base & 1023u) != 0) {                         // the swizzle needs it
@@ -1004,38 +995,42 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 
   if (warp == kBwdWarps) {
     // ------------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      int it = 0, u = 0, patches = 0;
-      for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
-        const RowUnit un = unit_of(w);
-        if (un.total == 0) continue;
-        const int hk = un.h / p.G;
-        const uint32_t qb = smem_u32(&sm->qdo_full);
-        mbar_wait(smem_u32(&sm->delta_read), (u & 1) ^ 1, status, kErrDqProducer);
+    int it = 0, u = 0, patches = 0;
+    for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
+      const RowUnit un = unit_of(w);
+      if (un.total == 0) continue;
+      const int hk = un.h / p.G;
+      const uint32_t qb = smem_u32(&sm->qdo_full);
+      mbar_wait(smem_u32(&sm->delta_read), (u & 1) ^ 1, status, kErrDqProducer);
+      if (lane == 0) {
         mbar_arrive_expect_tx(qb, 3 * (kD / 64) * kTileBytes);
         for (int c = 0; c < kD / 64; ++c) {
           tma_load_4d(o_tile + c * kTileBytes, &tm_o, qb, 64 * c, un.t * kQTile, un.h, un.b);
           tma_load_4d(q_tile + c * kTileBytes, &tm_q, qb, 64 * c, un.t * kQTile, un.h, un.b);
           tma_load_4d(do_tile + c * kTileBytes, &tm_do, qb, 64 * c, un.t * kQTile, un.h, un.b);
         }
-        for (int i = 0; i < un.total; ++i, ++it) {
-          const int s = it % kDqStages, key0 = un.tile_of(i) * kBlk;
-          mbar_wait(smem_u32(&sm->empty[s]), ((it / kDqStages) & 1) ^ 1, status, kErrDqProducer);
-          const bool ends = key0 + kBlk > un.len && un.len < p.Lk;
-          const uint32_t fb = smem_u32(ends ? &sm->patch : &sm->full[s]);
+      }
+      __syncwarp();
+      for (int i = 0; i < un.total; ++i, ++it) {
+        const int s = it % kDqStages, key0 = un.tile_of(i) * kBlk;
+        mbar_wait(smem_u32(&sm->empty[s]), ((it / kDqStages) & 1) ^ 1, status, kErrDqProducer);
+        const bool ends = key0 + kBlk > un.len && un.len < p.Lk;
+        const uint32_t fb = smem_u32(ends ? &sm->patch : &sm->full[s]);
+        if (lane == 0) {
           mbar_arrive_expect_tx(fb, 2 * (kD / 64) * kHalfTile);
           for (int c = 0; c < kD / 64; ++c) {
             tma_load_4d(k_slot(s) + c * kHalfTile, &tm_k, fb, 64 * c, key0, hk, un.b);
             tma_load_4d(v_slot(s) + c * kHalfTile, &tm_v, fb, 64 * c, key0, hk, un.b);
           }
-          if (ends) {                              // dS is 0 there, and dQ += dS K
-            mbar_wait(fb, patches++ & 1, status, kErrDqProducer);
-            zero_rows(k_slot(s), kHalfTile, kD / 64, un.len - key0, kBlk);
-            mbar_arrive(smem_u32(&sm->full[s]));
-          }
         }
-        ++u;
+        __syncwarp();
+        if (ends) {                                // dS is 0 there, and dQ += dS K
+          mbar_wait(fb, patches++ & 1, status, kErrDqProducer);
+          zero_rows(k_slot(s), kHalfTile, kD / 64, un.len - key0, kBlk, lane);
+          if (lane == 0) mbar_arrive(smem_u32(&sm->full[s]));
+        }
       }
+      ++u;
     }
     __syncwarp();
   } else if (warp == kBwdWarps + 1) {
@@ -1276,6 +1271,21 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       ++u;
     }
     if (warp_uniform(drain_row >= 0)) drain();
+    // Gradients of keys that nobody sees, in the time in which other CTAs have a unit more.  (In the dK/dV kernel the softmax warps reach such
+    // a unit only when the one before is done, and the loading warp alone took 7000 clk for each.)
+    for (int w = blockIdx.x; w < p.n_pairs * (p.BH / p.G); w += gridDim.x) {
+      const int bk = w / p.n_pairs, tile = w - bk * p.n_pairs;
+      const QueryTiles q = queries_of_keys(tile, kQTile, kPair, p.Lq, off, length_of(p.lengths, bk / p.Hkv, p.Lk), p.window, p.sinks);
+      if ((tile < p.split.tiles ? q.last : q.end) >= q.first) continue;
+      if (tile < p.split.tiles) {
+        zero_fill(p.split.part + ((int64_t)bk * p.split.tiles + tile) * (1 + p.split.runs) * 2 * kPair * p.D, 2 * kPair * p.D / 4, tid, kBwdWarps * 32);
+      } else {
+        const int64_t at = ((int64_t)bk * p.Lk + tile * kPair) * p.D;
+        const int n = min(kPair, p.Lk - tile * kPair) * p.D / 8;
+        zero_fill(reinterpret_cast<uint16_t*>(p.dk) + at, n, tid, kBwdWarps * 32);
+        zero_fill(reinterpret_cast<uint16_t*>(p.dv) + at, n, tid, kBwdWarps * 32);
+      }
+    }
     tc_fence_before();
   }
   __syncthreads();
@@ -1372,7 +1382,8 @@ int window_sm100_bwd(const WindowParams& p, int dtype, cudaStream_t st) {
   const int n_pairs = (p.Lk + kPair - 1) / kPair, G = p.H / p.Hkv;
   const int64_t dq_units = (int64_t)((p.Lq + kQTile - 1) / kQTile) * p.B * p.H;
   const int64_t dkv_units = ((int64_t)n_pairs + (int64_t)p.split.tiles * p.split.runs) * p.B * p.Hkv;
-  const DqArgs aq = {p.lse, p.delta, p.next, p.dq, p.lengths, p.H, p.Hkv, G, p.B * p.H, p.Lq, p.Lk, p.D, p.window, p.sinks, p.scale, p.scale * kLog2e};
+  const DqArgs aq = {p.lse, p.delta, p.next, p.dq, p.dk, p.dv, p.lengths, p.H, p.Hkv, G, p.B * p.H, p.Lq, p.Lk, p.D, p.window, p.sinks, n_pairs, p.scale,
+                     p.scale * kLog2e, p.split};
   const DkvArgs ak = {p.lse, p.delta, p.dk, p.dv, p.lengths, p.next, p.H, p.Hkv, G, p.B, p.Lq, p.Lk, p.D, p.window, p.sinks, n_pairs, p.scale, p.scale * kLog2e,
                       p.split};
   const dim3 grid_q((unsigned)(dq_units < n_sm ? dq_units : n_sm)), grid_k((unsigned)(dkv_units < n_sm ? dkv_units : n_sm));
