@@ -1,11 +1,12 @@
-// Sliding-window attention with sinks in fp32, on the CUDA cores: 64 x 64 tiles of scores, 4 x 4 results a thread.
+// Sliding-window attention with sinks in fp32, on the CUDA cores: 64 x 64 tiles of scores, 8 rows a warp, 8 x 2 results a thread.
 //
 //   S = scale Q K^T over the visible keys, P = e^{S - lse}, O = P V (running maximum and sum, one pass over the keys)
 //   dV = P^T dO,  dP = dO V^T,  delta = rowsum(O dO),  dS = scale P (dP - delta),  dQ = dS K,  dK = dS^T Q
 // Only the key tiles that a query tile sees are visited (window_params.h).  dK and dV of heads that share keys are summed in the
 // unit that owns the keys; no atomics.  Rows behind a sequence's end are read as zeros, whatever they hold.
-// Operands of the products lie in shared memory with the contracted index outermost, so that a thread reads its four rows and its four
-// columns as one 16-byte vector each: two reads for 16 multiply-adds, which keeps the FMA units the bound and not the shared memory.
+// Shared memory bounds the products (a 16-byte read of 32 different places takes 4 cycles, of one place 1): a warp's eight rows are the same
+// for all its lanes, which hold the columns, so 64 multiply-adds cost 8 + 2 reads of 16 cycles in all.  The tiles lie as in memory, and P
+// and dS go to the second product through a buffer of the warp's own.
 #include "common.cuh"
 #include "window_params.h"
 #include "sm100_ptx.cuh"
@@ -15,247 +16,264 @@ namespace {
 
 using namespace ptx;
 
-constexpr int kTile = 64, kPad = 68, kThreads = 256;
+constexpr int kTile = 64, kThreads = 256, kRows = 8;      // kRows: rows of a warp
 constexpr float kLog2e = 1.4426950408889634f;
+template <int kD> constexpr int kStride = kD + 4;          // of a row in shared memory: eight rows' 16 bytes meet in no bank
+template <int kD> constexpr int kTileFloats = kTile * kStride<kD>;
 
-__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
-
-// A 64-row tile on its way to shared memory: asked for while the tile in front is worked on, stored as [kD][kPad].  A warp takes 32 rows of
-// one 16-byte chunk: the stores of a feature lie next to each other (along the features they met in two banks).
-template <int kD> struct Tile {
-  float4 x[kTile * kD / 4 / kThreads];
-  __device__ __forceinline__ void ask(const float* from, int64_t stride, int valid, int D) {
+// a 64-row tile on its way to shared memory; rows from `valid` on and features from D on become zeros
+template <int kD>
+__device__ __forceinline__ void copy_tile(float* to, const float* from, int64_t stride, int valid, int D) {
 #pragma unroll
-    for (int e = 0; e < kTile * kD / 4 / kThreads; ++e) {
-      const int i = e * kThreads + threadIdx.x, r = i % kTile, c = i / kTile * 4;
-      x[e] = r < valid && c < D ? load4(from + r * stride + c) : make_float4(0.f, 0.f, 0.f, 0.f);      // (rows behind the end: zeros)
-    }
-  }
-  __device__ __forceinline__ void store(float* to) const {
-#pragma unroll
-    for (int e = 0; e < kTile * kD / 4 / kThreads; ++e) {
-      const int i = e * kThreads + threadIdx.x, r = i % kTile, c = i / kTile * 4;
-      to[c * kPad + r] = x[e].x;
-      to[(c + 1) * kPad + r] = x[e].y;
-      to[(c + 2) * kPad + r] = x[e].z;
-      to[(c + 3) * kPad + r] = x[e].w;
-    }
-  }
-};
-// d[4][4] = sum over n of a[n][row ..] b[n][col ..]
-template <int kN>
-__device__ __forceinline__ void product(float (&d)[4][4], const float* a, const float* b, int ty, int tx) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) d[i][j] = 0.f;
-#pragma unroll 8
-  for (int n = 0; n < kN; ++n) {
-    const float4 x = *reinterpret_cast<const float4*>(a + n * kPad + ty * 4);
-    const float4 y = *reinterpret_cast<const float4*>(b + n * kPad + tx * 4);
-    const float xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) d[i][j] = fmaf(xs[i], ys[j], d[i][j]);
+  for (int e = 0; e < kTile * kD / 4 / kThreads; ++e) {
+    const int i = e * kThreads + threadIdx.x, r = i / (kD / 4), c = i % (kD / 4) * 4;
+    const bool is = r < valid && c < D;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to + r * kStride<kD> + c)), "l"(is ? from + r * stride + c : from),
+                 "r"(is ? 16 : 0) : "memory");
   }
 }
-// d[4][kD / 16] += sum over 64 n of a[n][row ..] b[feature tx + 16 c][n], four n at a time
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+
+__device__ __forceinline__ void read4(float (&x)[4], const float* from) {
+  const float4 t = *reinterpret_cast<const float4*>(from);
+  x[0] = t.x;
+  x[1] = t.y;
+  x[2] = t.z;
+  x[3] = t.w;
+}
+// d[r][j] = a's row r times b's row lane + 32 j; a: the warp's rows
 template <int kD>
-__device__ __forceinline__ void accumulate(float (&d)[4][kD / 16], const float* a, const float* b, int ty, int tx) {
+__device__ __forceinline__ void product(float (&d)[kRows][2], const float* a, const float* b, int lane) {
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) d[r][0] = d[r][1] = 0.f;
+#pragma unroll 2
+  for (int c = 0; c < kD; c += 4) {
+    float x[kRows][4], y[2][4];
+    read4(y[0], b + lane * kStride<kD> + c);
+    read4(y[1], b + (lane + 32) * kStride<kD> + c);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) read4(x[r], a + r * kStride<kD> + c);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        d[r][0] = fmaf(x[r][e], y[0][e], d[r][0]);
+        d[r][1] = fmaf(x[r][e], y[1][e], d[r][1]);
+      }
+  }
+}
+// d[r][f] += sum over 64 n of w[r][n] b[n][lane kF + f]; w [kRows][64]: the warp's weights
+template <int kD>
+__device__ __forceinline__ void accumulate(float (&d)[kRows][kD / 32], const float* w, const float* b, int lane) {
+  constexpr int kF = kD / 32;
 #pragma unroll 2
   for (int n = 0; n < kTile; n += 4) {
-    float4 x[4];
+    float x[kRows][4], y[4][kF];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = *reinterpret_cast<const float4*>(a + (n + e) * kPad + ty * 4);
-#pragma unroll
-    for (int c = 0; c < kD / 16; ++c) {
-      const float4 y = *reinterpret_cast<const float4*>(b + (c * 16 + tx) * kPad + n);
-      const float ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        d[0][c] = fmaf(x[e].x, ys[e], d[0][c]);
-        d[1][c] = fmaf(x[e].y, ys[e], d[1][c]);
-        d[2][c] = fmaf(x[e].z, ys[e], d[2][c]);
-        d[3][c] = fmaf(x[e].w, ys[e], d[3][c]);
+    for (int e = 0; e < 4; ++e) {
+      const float* const from = b + (n + e) * kStride<kD> + lane * kF;
+      if constexpr (kF == 2) {
+        const float2 t = *reinterpret_cast<const float2*>(from);
+        y[e][0] = t.x;
+        y[e][1] = t.y;
+      } else {
+        read4(y[e], from);
       }
     }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) read4(x[r], w + r * kTile + n);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+      for (int r = 0; r < kRows; ++r)
+#pragma unroll
+        for (int f = 0; f < kF; ++f) d[r][f] = fmaf(x[r][e], y[e][f], d[r][f]);
   }
+}
+// the warp's weights take the places that the last product has read
+__device__ __forceinline__ void share(float* w, const float (&x)[kRows][2], int lane) {
+  __syncwarp();
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    w[r * kTile + lane] = x[r][0];
+    w[r * kTile + lane + 32] = x[r][1];
+  }
+  __syncwarp();
+}
+template <int kF> __device__ __forceinline__ void write_row(float* to, const float (&x)[kF], bool nonzero) {
+  if constexpr (kF == 2) *reinterpret_cast<float2*>(to) = nonzero ? make_float2(x[0], x[1]) : make_float2(0.f, 0.f);
+  else *reinterpret_cast<float4*>(to) = nonzero ? make_float4(x[0], x[1], x[2], x[3]) : make_float4(0.f, 0.f, 0.f, 0.f);
+}
+__device__ __forceinline__ float warp_sum(float x) {
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) x += __shfl_xor_sync(0xffffffffu, x, w);
+  return x;
+}
+__device__ __forceinline__ float warp_max_nan(float x) {      // NaN where a lane has one
+#pragma unroll
+  for (int w = 16; w > 0; w >>= 1) {
+    const float y = __shfl_xor_sync(0xffffffffu, x, w);
+    x = max3_nan(x, y, y);
+  }
+  return x;
 }
 __device__ __forceinline__ int length_of(const WindowParams& p, int b) {
   return p.lengths == nullptr ? p.Lk : min(max(ld_behind_wait(p.lengths + b), 0), p.Lk);
 }
 
 template <int kD>
-__global__ void __launch_bounds__(kThreads) window_fwd_f32_kernel(const __grid_constant__ WindowParams p, float scale_log2) {
-  extern __shared__ float smem[];
-  float *qt = smem, *kt = qt + kD * kPad, *vt = kt + kD * kPad, *pt = vt + kD * kPad;      // pt [key][row]
+__global__ void __launch_bounds__(kThreads, 1) window_fwd_f32_kernel(const __grid_constant__ WindowParams p, float scale_log2) {
+  constexpr int kF = kD / 32, kT = kTileFloats<kD>;
+  extern __shared__ __align__(16) float smem[];
+  float *const qt = smem, *const kv = qt + kT, *const wts = kv + 4 * kT + threadIdx.x / 32 * (kRows * kTile);      // kv: 2 x (K, V)
   grid_dep_wait();
   grid_dep_launch();
-  const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
+  const int lane = threadIdx.x % 32, r0 = threadIdx.x / 32 * kRows;
   const int tiles = gridDim.x, tile = tiles - 1 - (int)blockIdx.x, bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H;
   const int hk = h / (p.H / p.Hkv), off = p.Lk - p.Lq, len = length_of(p, b);
   const int rows = min(kTile, p.Lq - tile * kTile), p0 = off + tile * kTile;
-  const float* q = (const float*)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)tile * kTile * p.qs[2];
   const float* k = (const float*)p.k + b * p.ks[0] + hk * p.ks[1];
   const float* v = (const float*)p.v + b * p.vs[0] + hk * p.vs[1];
-  Tile<kD> tk, tv;
-  tk.ask(q, p.qs[2], min(rows, len - p0), p.D);
-  tk.store(qt);
-  float m[4], l[4], o[4][kD / 16];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    m[i] = -INFINITY;
-    l[i] = 0.f;
-#pragma unroll
-    for (int c = 0; c < kD / 16; ++c) o[i][c] = 0.f;
-  }
   const KeyTiles kts = keys_of_queries(tile, kTile, kTile, p.Lq, off, len, p.window, p.sinks);
   const int n = kts.sink_tiles + kts.last - kts.first + 1;
   auto key_of = [&](int i) { return (i < kts.sink_tiles ? i : kts.first + i - kts.sink_tiles) * kTile; };
   auto ask = [&](int i) {
-    tk.ask(k + key_of(i) * p.ks[2], p.ks[2], len - key_of(i), p.D);
-    tv.ask(v + key_of(i) * p.vs[2], p.vs[2], len - key_of(i), p.D);
+    float* const to = kv + (i & 1) * 2 * kT;
+    copy_tile<kD>(to, k + key_of(i) * p.ks[2], p.ks[2], len - key_of(i), p.D);
+    copy_tile<kD>(to + kT, v + key_of(i) * p.vs[2], p.vs[2], len - key_of(i), p.D);
+    copy_commit();
   };
-  if (n > 0) ask(0);
+  if (n > 0) {
+    copy_tile<kD>(qt, (const float*)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)tile * kTile * p.qs[2], p.qs[2], min(rows, len - p0), p.D);
+    ask(0);
+  }
+  float m[kRows], l[kRows], o[kRows][kF];      // l: the lane's share
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int f = 0; f < kF; ++f) o[r][f] = 0.f;
+  }
   for (int i = 0; i < n; ++i) {
-    const int key0 = key_of(i);
-    __syncthreads();
-    tk.store(kt);
-    tv.store(vt);
-    __syncthreads();
+    const float* const kt = kv + (i & 1) * 2 * kT;
+    const int key0 = key_of(i) + lane;
+    copy_wait();
+    __syncthreads();                           // tile i is there, and nobody reads tile i - 1 any more
     if (i + 1 < n) ask(i + 1);
-    float s[4][4];
-    product<kD>(s, qt, kt, ty, tx);
+    float s[kRows][2];
+    product<kD>(s, qt + r0 * kStride<kD>, kt, lane);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int pos = p0 + ty * 4 + r;
-      float mx = m[r];
+    for (int r = 0; r < kRows; ++r) {
+      const int pos = p0 + r0 + r;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[r][j] = pos < len && window_sees(pos, key0 + tx * 4 + j, p.window, p.sinks) ? s[r][j] * scale_log2 : -INFINITY;
-        mx = max3_nan(mx, s[r][j], s[r][j]);
-      }
-#pragma unroll
-      for (int w = 8; w > 0; w >>= 1) {
-        const float y = __shfl_xor_sync(0xffffffffu, mx, w);
-        mx = max3_nan(mx, y, y);
-      }
+      for (int j = 0; j < 2; ++j) s[r][j] = pos < len && window_sees(pos, key0 + 32 * j, p.window, p.sinks) ? s[r][j] * scale_log2 : -INFINITY;
+      const float mx = warp_max_nan(max3_nan(m[r], s[r][0], s[r][1]));
       const float shift = mx == -INFINITY ? 0.f : mx, f = exp2f(m[r] - shift);
       m[r] = mx;
-      l[r] *= f;
 #pragma unroll
-      for (int c = 0; c < kD / 16; ++c) o[r][c] *= f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        s[r][j] = exp2f(s[r][j] - shift);
-        l[r] += s[r][j];
-        pt[(tx * 4 + j) * kPad + ty * 4 + r] = s[r][j];
-      }
+      for (int c = 0; c < kF; ++c) o[r][c] *= f;
+      s[r][0] = exp2f(s[r][0] - shift);
+      s[r][1] = exp2f(s[r][1] - shift);
+      l[r] = fmaf(l[r], f, s[r][0] + s[r][1]);
     }
-    __syncthreads();
-    accumulate<kD>(o, pt, vt, ty, tx);
+    share(wts, s, lane);
+    accumulate<kD>(o, wts, kt + kT, lane);
   }
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
+  for (int r = 0; r < kRows; ++r) {
+    const float sum = warp_sum(l[r]);
+    if (r0 + r >= rows) continue;
+    const int64_t at = (int64_t)bh * p.Lq + tile * kTile + r0 + r;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
-    for (int w = 8; w > 0; w >>= 1) l[r] += __shfl_xor_sync(0xffffffffu, l[r], w);
-    const int row = ty * 4 + r;
-    if (row >= rows) continue;
-    const int64_t at = (int64_t)bh * p.Lq + tile * kTile + row;
-    const float inv = l[r] == 0.f ? 0.f : 1.f / l[r];
-#pragma unroll
-    for (int c = 0; c < kD / 16; ++c)
-      if (c * 16 + tx < p.D) ((float*)p.o)[at * p.D + c * 16 + tx] = o[r][c] * inv;
-    if (tx == 0) p.lse[at] = l[r] == 0.f ? INFINITY : m[r] + log2f(l[r]);
+    for (int c = 0; c < kF; ++c) o[r][c] *= inv;
+    if (lane * kF < p.D) write_row<kF>((float*)p.o + at * p.D + lane * kF, o[r], sum != 0.f);
+    if (lane == 0) p.lse[at] = sum == 0.f ? INFINITY : m[r] + log2f(sum);
   }
 }
 
 // dQ of a tile of 64 query rows, and delta for the dK/dV kernel
 template <int kD>
-__global__ void __launch_bounds__(kThreads) window_dq_f32_kernel(const __grid_constant__ WindowParams p, float scale_log2) {
-  extern __shared__ float smem[];
-  float *qt = smem, *gt = qt + kD * kPad, *kt = gt + kD * kPad, *vt = kt + kD * kPad, *dst = vt + kD * kPad;      // dst [key][row]
+__global__ void __launch_bounds__(kThreads, 1) window_dq_f32_kernel(const __grid_constant__ WindowParams p, float scale_log2) {
+  constexpr int kF = kD / 32, kT = kTileFloats<kD>;
+  extern __shared__ __align__(16) float smem[];
+  float *const qt = smem, *const gt = qt + kT, *const kv = gt + kT, *const wts = kv + 4 * kT + threadIdx.x / 32 * (kRows * kTile);
   grid_dep_wait();
   grid_dep_launch();
-  const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
+  const int lane = threadIdx.x % 32, r0 = threadIdx.x / 32 * kRows;
   const int tiles = gridDim.x, tile = tiles - 1 - (int)blockIdx.x, bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H;
   const int hk = h / (p.H / p.Hkv), off = p.Lk - p.Lq, len = length_of(p, b);
   const int rows = min(kTile, p.Lq - tile * kTile), p0 = off + tile * kTile, valid = min(rows, len - p0);
   const int64_t row0 = (int64_t)bh * p.Lq + tile * kTile;
   const float* k = (const float*)p.k + b * p.ks[0] + hk * p.ks[1];
   const float* v = (const float*)p.v + b * p.vs[0] + hk * p.vs[1];
-  Tile<kD> tk, tv;
-  tk.ask((const float*)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)tile * kTile * p.qs[2], p.qs[2], valid, p.D);
-  tv.ask((const float*)p.dO + b * p.dos[0] + h * p.dos[1] + (int64_t)tile * kTile * p.dos[2], p.dos[2], valid, p.D);
-  tk.store(qt);
-  tv.store(gt);
-  __syncthreads();
-  float delta[4], lse[4], dq[4][kD / 16];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int row = ty * 4 + r;
-    float sum = 0.f;
-    if (row < valid)
-      for (int c = tx; c < p.D; c += 16) sum = fmaf(((const float*)p.o)[(row0 + row) * p.D + c], gt[c * kPad + row], sum);
-#pragma unroll
-    for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
-    delta[r] = sum;
-    lse[r] = row < valid ? ld_behind_wait(p.lse + row0 + row) : INFINITY;
-    if (row < rows && tx == 0) p.delta[row0 + row] = sum;
-#pragma unroll
-    for (int c = 0; c < kD / 16; ++c) dq[r][c] = 0.f;
-  }
   const KeyTiles kts = keys_of_queries(tile, kTile, kTile, p.Lq, off, len, p.window, p.sinks);
   const int n = kts.sink_tiles + kts.last - kts.first + 1;
   auto key_of = [&](int i) { return (i < kts.sink_tiles ? i : kts.first + i - kts.sink_tiles) * kTile; };
   auto ask = [&](int i) {
-    tk.ask(k + key_of(i) * p.ks[2], p.ks[2], len - key_of(i), p.D);
-    tv.ask(v + key_of(i) * p.vs[2], p.vs[2], len - key_of(i), p.D);
+    float* const to = kv + (i & 1) * 2 * kT;
+    copy_tile<kD>(to, k + key_of(i) * p.ks[2], p.ks[2], len - key_of(i), p.D);
+    copy_tile<kD>(to + kT, v + key_of(i) * p.vs[2], p.vs[2], len - key_of(i), p.D);
+    copy_commit();
   };
-  if (n > 0) ask(0);
-  for (int i = 0; i < n; ++i) {
-    const int key0 = key_of(i);
+  if (n > 0) {
+    copy_tile<kD>(qt, (const float*)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)tile * kTile * p.qs[2], p.qs[2], valid, p.D);
+    copy_tile<kD>(gt, (const float*)p.dO + b * p.dos[0] + h * p.dos[1] + (int64_t)tile * kTile * p.dos[2], p.dos[2], valid, p.D);
+    ask(0);
+    copy_wait();
     __syncthreads();
-    tk.store(kt);
-    tv.store(vt);
+  }
+  float delta[kRows], lse[kRows], dq[kRows][kF];
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    const bool is = r0 + r < valid;
+    float sum = 0.f;
+    if (is && lane * kF < p.D) {
+#pragma unroll
+      for (int f = 0; f < kF; ++f)
+        sum = fmaf(ld_behind_wait((const float*)p.o + (row0 + r0 + r) * p.D + lane * kF + f), gt[(r0 + r) * kStride<kD> + lane * kF + f], sum);
+    }
+    delta[r] = warp_sum(sum);
+    lse[r] = is ? ld_behind_wait(p.lse + row0 + r0 + r) : INFINITY;
+    if (r0 + r < rows && lane == 0) p.delta[row0 + r0 + r] = delta[r];
+#pragma unroll
+    for (int f = 0; f < kF; ++f) dq[r][f] = 0.f;
+  }
+  for (int i = 0; i < n; ++i) {
+    const float* const kt = kv + (i & 1) * 2 * kT;
+    const int key0 = key_of(i) + lane;
+    copy_wait();
     __syncthreads();
     if (i + 1 < n) ask(i + 1);
-    float s[4][4], dp[4][4];
-    product<kD>(s, qt, kt, ty, tx);
-    product<kD>(dp, gt, vt, ty, tx);
+    float s[kRows][2], dp[kRows][2];
+    product<kD>(s, qt + r0 * kStride<kD>, kt, lane);
+    product<kD>(dp, gt + r0 * kStride<kD>, kt + kT, lane);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int pos = p0 + ty * 4 + r;
+    for (int r = 0; r < kRows; ++r)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool seen = window_sees(pos, key0 + tx * 4 + j, p.window, p.sinks);
-        const float w = seen ? exp2f(fmaf(s[r][j], scale_log2, -lse[r])) : 0.f;
-        dst[(tx * 4 + j) * kPad + ty * 4 + r] = w * (dp[r][j] - delta[r]) * p.scale;
+      for (int j = 0; j < 2; ++j) {
+        const float w = window_sees(p0 + r0 + r, key0 + 32 * j, p.window, p.sinks) ? exp2f(fmaf(s[r][j], scale_log2, -lse[r])) : 0.f;
+        s[r][j] = w * (dp[r][j] - delta[r]) * p.scale;
       }
-    }
-    __syncthreads();
-    accumulate<kD>(dq, dst, kt, ty, tx);
+    share(wts, s, lane);
+    accumulate<kD>(dq, wts, kt, lane);
   }
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int row = ty * 4 + r;
-    if (row >= rows) continue;
-#pragma unroll
-    for (int c = 0; c < kD / 16; ++c)
-      if (c * 16 + tx < p.D) ((float*)p.dq)[(row0 + row) * p.D + c * 16 + tx] = row < valid ? dq[r][c] : 0.f;
-  }
+  for (int r = 0; r < kRows; ++r)
+    if (r0 + r < rows && lane * kF < p.D) write_row<kF>((float*)p.dq + (row0 + r0 + r) * p.D + lane * kF, dq[r], r0 + r < valid);
 }
 
-// dK and dV of a tile of 64 keys of one key head from a run of query tiles of all heads that share it
+// dK and dV of a tile of 64 keys of one key head from a run of query tiles of all heads that share it; a warp has eight keys
 template <int kD>
-__global__ void __launch_bounds__(kThreads) window_dkv_f32_kernel(const __grid_constant__ WindowParams p, float scale_log2) {
-  extern __shared__ float smem[];
-  float *kt = smem, *vt = kt + kD * kPad, *qt = vt + kD * kPad, *gt = qt + kD * kPad;
-  float *pr = gt + kD * kPad, *dsr = pr + kTile * kPad;                  // [query][key]
+__global__ void __launch_bounds__(kThreads, 1) window_dkv_f32_kernel(const __grid_constant__ WindowParams p, float scale_log2) {
+  constexpr int kF = kD / 32, kT = kTileFloats<kD>;
+  extern __shared__ __align__(16) float smem[];
+  float *const kt = smem, *const vt = kt + kT, *const qg = vt + kT, *const wts = qg + 4 * kT + threadIdx.x / 32 * (kRows * kTile);
   grid_dep_wait();
   grid_dep_launch();
-  const int tid = threadIdx.x, ty = tid / 16, tx = tid % 16;
+  const int lane = threadIdx.x % 32, r0 = threadIdx.x / 32 * kRows;
   const int key_tiles = (p.Lk + kTile - 1) / kTile, bk = blockIdx.y, b = bk / p.Hkv, hk = bk - b * p.Hkv, G = p.H / p.Hkv;
   const int off = p.Lk - p.Lq, len = length_of(p, b);
   const int extra = (int)blockIdx.x - key_tiles;                         // >= 0: a run of a split tile
@@ -268,78 +286,73 @@ __global__ void __launch_bounds__(kThreads) window_dkv_f32_kernel(const __grid_c
     last = min(qts.end, first + p.split.run - 1);
     if (first > last) return;
   }
-  const int key0 = tile * kTile, valid_k = min(kTile, len - key0);
-  Tile<kD> tq, tg;
-  tq.ask((const float*)p.k + b * p.ks[0] + hk * p.ks[1] + key0 * p.ks[2], p.ks[2], valid_k, p.D);
-  tg.ask((const float*)p.v + b * p.vs[0] + hk * p.vs[1] + key0 * p.vs[2], p.vs[2], valid_k, p.D);
-  tq.store(kt);
-  tg.store(vt);
-  float dk[4][kD / 16], dv[4][kD / 16];                                  // keys 4 ty .., features tx + 16 c
+  const int key0 = tile * kTile + r0, valid_k = min(kTile, len - tile * kTile);
+  float dk[kRows][kF], dv[kRows][kF];
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
+  for (int r = 0; r < kRows; ++r)
 #pragma unroll
-    for (int c = 0; c < kD / 16; ++c) dk[r][c] = dv[r][c] = 0.f;
+    for (int f = 0; f < kF; ++f) dk[r][f] = dv[r][f] = 0.f;
   const int per_head = last - first + 1, n = per_head > 0 ? per_head * G : 0;
   auto rows_of = [&](int t) { return min(min(kTile, p.Lq - t * kTile), len - off - t * kTile); };
   auto ask = [&](int i) {
     const int g = i / per_head, t = first + i - g * per_head, h = hk * G + g;
-    tq.ask((const float*)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)t * kTile * p.qs[2], p.qs[2], rows_of(t), p.D);
-    tg.ask((const float*)p.dO + b * p.dos[0] + h * p.dos[1] + (int64_t)t * kTile * p.dos[2], p.dos[2], rows_of(t), p.D);
+    float* const to = qg + (i & 1) * 2 * kT;
+    copy_tile<kD>(to, (const float*)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)t * kTile * p.qs[2], p.qs[2], rows_of(t), p.D);
+    copy_tile<kD>(to + kT, (const float*)p.dO + b * p.dos[0] + h * p.dos[1] + (int64_t)t * kTile * p.dos[2], p.dos[2], rows_of(t), p.D);
+    copy_commit();
   };
-  if (n > 0) ask(0);
+  if (n > 0) {
+    copy_tile<kD>(kt, (const float*)p.k + b * p.ks[0] + hk * p.ks[1] + (int64_t)tile * kTile * p.ks[2], p.ks[2], valid_k, p.D);
+    copy_tile<kD>(vt, (const float*)p.v + b * p.vs[0] + hk * p.vs[1] + (int64_t)tile * kTile * p.vs[2], p.vs[2], valid_k, p.D);
+    ask(0);
+  }
   for (int i = 0; i < n; ++i) {
+    const float* const qt = qg + (i & 1) * 2 * kT;
     const int g = i / per_head, t = first + i - g * per_head, valid_q = rows_of(t);
-    const int64_t row0 = ((int64_t)b * p.H + hk * G + g) * p.Lq + t * kTile;
-    __syncthreads();
-    tq.store(qt);
-    tg.store(gt);
+    const int64_t row0 = ((int64_t)b * p.H + hk * G + g) * p.Lq + t * kTile + lane;
+    float lse[2], delta[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const bool is = lane + 32 * j < valid_q;
+      lse[j] = is ? ld_behind_wait(p.lse + row0 + 32 * j) : INFINITY;
+      delta[j] = is ? ld_behind_wait(p.delta + row0 + 32 * j) : 0.f;
+    }
+    copy_wait();
     __syncthreads();
     if (i + 1 < n) ask(i + 1);
-    float s[4][4], dp[4][4];
-    product<kD>(s, qt, kt, ty, tx);
-    product<kD>(dp, gt, vt, ty, tx);
+    float s[kRows][2];                         // [key][query lane + 32 j]
+    product<kD>(s, kt + r0 * kStride<kD>, qt, lane);
+    const int pos = off + t * kTile + lane;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int row = ty * 4 + r, pos = off + t * kTile + row;
-      const float lse = row < valid_q ? ld_behind_wait(p.lse + row0 + row) : INFINITY;
-      const float delta = row < valid_q ? ld_behind_wait(p.delta + row0 + row) : 0.f;
-      float w[4], d[4];
+    for (int r = 0; r < kRows; ++r)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        w[j] = window_sees(pos, key0 + tx * 4 + j, p.window, p.sinks) ? exp2f(fmaf(s[r][j], scale_log2, -lse)) : 0.f;
-        d[j] = w[j] * (dp[r][j] - delta) * p.scale;
-      }
-      *reinterpret_cast<float4*>(pr + row * kPad + tx * 4) = make_float4(w[0], w[1], w[2], w[3]);
-      *reinterpret_cast<float4*>(dsr + row * kPad + tx * 4) = make_float4(d[0], d[1], d[2], d[3]);
-    }
-    __syncthreads();
-    accumulate<kD>(dv, pr, gt, ty, tx);
-    accumulate<kD>(dk, dsr, qt, ty, tx);
+      for (int j = 0; j < 2; ++j)
+        s[r][j] = window_sees(pos + 32 * j, key0 + r, p.window, p.sinks) ? exp2f(fmaf(s[r][j], scale_log2, -lse[j])) : 0.f;
+    share(wts, s, lane);
+    accumulate<kD>(dv, wts, qt + kT, lane);
+    float dp[kRows][2];
+    product<kD>(dp, vt + r0 * kStride<kD>, qt + kT, lane);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) dp[r][j] = s[r][j] * (dp[r][j] - delta[j]) * p.scale;
+    share(wts, dp, lane);
+    accumulate<kD>(dk, wts, qt, lane);
   }
+  if (lane * kF >= p.D) return;
   float* const part = split ? p.split.part + (((int64_t)bk * p.split.tiles + tile) * (1 + p.split.runs) + 1 + run) * 2 * kTile * p.D : nullptr;
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int key = ty * 4 + r;
-    if (key0 + key >= (run >= 0 ? p.sinks : p.Lk)) continue;      // a run's rows see the sinks alone
-    const int64_t at = ((int64_t)bk * p.Lk + key0 + key) * p.D;
-#pragma unroll
-    for (int c = 0; c < kD / 16; ++c) {
-      const int f = c * 16 + tx;
-      if (f >= p.D) continue;
-      if (split) {
-        part[key * p.D + f] = dk[r][c];
-        part[(kTile + key) * p.D + f] = dv[r][c];
-      } else {
-        ((float*)p.dk)[at + f] = dk[r][c];
-        ((float*)p.dv)[at + f] = dv[r][c];
-      }
-    }
+  for (int r = 0; r < kRows; ++r) {
+    if (key0 + r >= (run >= 0 ? p.sinks : p.Lk)) continue;               // a run's rows see the sinks alone
+    const int64_t at = split ? (int64_t)(r0 + r) * p.D : ((int64_t)bk * p.Lk + key0 + r) * p.D;
+    write_row<kF>((split ? part : (float*)p.dk) + at + lane * kF, dk[r], true);
+    write_row<kF>((split ? part + kTile * p.D : (float*)p.dv) + at + lane * kF, dv[r], true);
   }
 }
 
-template <int kD> constexpr size_t kSmemFwd = sizeof(float) * (3 * kD * kPad + kTile * kPad);
-template <int kD> constexpr size_t kSmemDq = sizeof(float) * (4 * kD * kPad + kTile * kPad);
-template <int kD> constexpr size_t kSmemDkv = sizeof(float) * (4 * kD * kPad + 2 * kTile * kPad);
+template <int kD> constexpr size_t kSmemFwd = sizeof(float) * (5 * kTileFloats<kD> + kTile * kTile);
+template <int kD> constexpr size_t kSmemBwd = sizeof(float) * (6 * kTileFloats<kD> + kTile * kTile);
+static_assert(kSmemBwd<128> <= 232448, "shared memory of one SM");
 
 template <typename F> int allow(F* kernel, size_t smem) {
   LMK_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
@@ -353,13 +366,13 @@ template <int kD> int fwd(const WindowParams& p, cudaStream_t st) {
   return LMK_OK;
 }
 template <int kD> int bwd(const WindowParams& p, cudaStream_t st) {
-  int rc = allow(window_dq_f32_kernel<kD>, kSmemDq<kD>);
-  if (rc == LMK_OK) rc = allow(window_dkv_f32_kernel<kD>, kSmemDkv<kD>);
+  int rc = allow(window_dq_f32_kernel<kD>, kSmemBwd<kD>);
+  if (rc == LMK_OK) rc = allow(window_dkv_f32_kernel<kD>, kSmemBwd<kD>);
   if (rc != LMK_OK) return rc;
   const dim3 grid_q((p.Lq + kTile - 1) / kTile, p.B * p.H);
   const dim3 grid_k((p.Lk + kTile - 1) / kTile + p.split.tiles * p.split.runs, p.B * p.Hkv);
-  LMK_CUDA(launch_overlapped(window_dq_f32_kernel<kD>, grid_q, dim3(kThreads), kSmemDq<kD>, st, p, p.scale * kLog2e));
-  LMK_CUDA(launch_overlapped(window_dkv_f32_kernel<kD>, grid_k, dim3(kThreads), kSmemDkv<kD>, st, p, p.scale * kLog2e));
+  LMK_CUDA(launch_overlapped(window_dq_f32_kernel<kD>, grid_q, dim3(kThreads), kSmemBwd<kD>, st, p, p.scale * kLog2e));
+  LMK_CUDA(launch_overlapped(window_dkv_f32_kernel<kD>, grid_k, dim3(kThreads), kSmemBwd<kD>, st, p, p.scale * kLog2e));
   return p.split.tiles > 0 ? window_join_parts(p, kTile, kTile, LMK_F32, st) : LMK_OK;
 }
 
