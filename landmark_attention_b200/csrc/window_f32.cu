@@ -4,9 +4,11 @@
 //   dV = P^T dO,  dP = dO V^T,  delta = rowsum(O dO),  dS = scale P (dP - delta),  dQ = dS K,  dK = dS^T Q
 // Only the key tiles that a query tile sees are visited (window_params.h).  dK and dV of heads that share keys are summed in the
 // unit that owns the keys; no atomics.  Rows behind a sequence's end are read as zeros, whatever they hold.
-// Shared memory bounds the products (a 16-byte read of 32 different places takes 4 cycles, of one place 1): a warp's eight rows are the same
-// for all its lanes, which hold the columns, so 64 multiply-adds cost 8 + 2 reads of 16 cycles in all.  The tiles lie as in memory, and P
-// and dS go to the second product through a buffer of the warp's own.
+// A 16-byte read of 32 different places takes the shared memory 4 cycles, of one place 1.  A warp's eight rows are the same for all its lanes,
+// which hold the columns: 64 multiply-adds a lane, issued as 32 pairs, cost 16 cycles of reads (with 4 x 4 results a thread 32, and
+// the reads were the bound: B2 H16 Hkv8 L2048 D128, window 512, forward and backward 3040 -> 2360 us, 22 of 74 TFLOP/s).  The tiles lie as
+// in memory, two of each on their way; P and dS go to the second product through a buffer of the warp's own.  What is left is latency: two
+// to four warps a scheduler, with a third of the cycles issuing (sixteen warps of four rows: 2650 us).
 #include "common.cuh"
 #include "window_params.h"
 #include "sm100_ptx.cuh"
@@ -35,71 +37,97 @@ __device__ __forceinline__ void copy_tile(float* to, const float* from, int64_t 
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
 
-__device__ __forceinline__ void read4(float (&x)[4], const float* from) {
-  const float4 t = *reinterpret_cast<const float4*>(from);
+__device__ __forceinline__ void read4(uint64_t (&x)[2], const float* from) {      // two pairs
+  const ulonglong2 t = *reinterpret_cast<const ulonglong2*>(from);
   x[0] = t.x;
   x[1] = t.y;
-  x[2] = t.z;
-  x[3] = t.w;
 }
-// d[r][j] = a's row r times b's row lane + 32 j; a: the warp's rows
+// d[r][j] = a's row r times b's row lane + 32 j; a: the warp's rows.  Multiply-adds in pairs: even and odd features.
 template <int kD>
 __device__ __forceinline__ void product(float (&d)[kRows][2], const float* a, const float* b, int lane) {
+  uint64_t sum[kRows][2];
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) d[r][0] = d[r][1] = 0.f;
+  for (int r = 0; r < kRows; ++r) sum[r][0] = sum[r][1] = 0ull;
 #pragma unroll 2
   for (int c = 0; c < kD; c += 4) {
-    float x[kRows][4], y[2][4];
+    uint64_t x[kRows][2], y[2][2];
     read4(y[0], b + lane * kStride<kD> + c);
     read4(y[1], b + (lane + 32) * kStride<kD> + c);
 #pragma unroll
     for (int r = 0; r < kRows; ++r) read4(x[r], a + r * kStride<kD> + c);
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < 2; ++e)
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
-        d[r][0] = fmaf(x[r][e], y[0][e], d[r][0]);
-        d[r][1] = fmaf(x[r][e], y[1][e], d[r][1]);
+        sum[r][0] = fma2(x[r][e], y[0][e], sum[r][0]);
+        sum[r][1] = fma2(x[r][e], y[1][e], sum[r][1]);
       }
   }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float even, odd;
+      upk2(sum[r][j], even, odd);
+      d[r][j] = even + odd;
+    }
 }
-// d[r][f] += sum over 64 n of w[r][n] b[n][lane kF + f]; w [kRows][64]: the warp's weights
+// d[r][f] += sum over 64 n of w[n][2 r ..] b[n][lane kF + f], r a pair of rows; w [64][kRows]: the warp's weights
 template <int kD>
-__device__ __forceinline__ void accumulate(float (&d)[kRows][kD / 32], const float* w, const float* b, int lane) {
+__device__ __forceinline__ void accumulate(uint64_t (&d)[kRows / 2][kD / 32], const float* w, const float* b, int lane) {
   constexpr int kF = kD / 32;
 #pragma unroll 2
-  for (int n = 0; n < kTile; n += 4) {
-    float x[kRows][4], y[4][kF];
+  for (int n = 0; n < kTile; n += 2) {
+    uint64_t x[2][kRows / 2];
+    float y[2][kF];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < 2; ++e) {
       const float* const from = b + (n + e) * kStride<kD> + lane * kF;
       if constexpr (kF == 2) {
         const float2 t = *reinterpret_cast<const float2*>(from);
         y[e][0] = t.x;
         y[e][1] = t.y;
       } else {
-        read4(y[e], from);
+        const float4 t = *reinterpret_cast<const float4*>(from);
+        y[e][0] = t.x;
+        y[e][1] = t.y;
+        y[e][2] = t.z;
+        y[e][3] = t.w;
       }
+      const ulonglong2 lo = *reinterpret_cast<const ulonglong2*>(w + (n + e) * kRows), hi = *reinterpret_cast<const ulonglong2*>(w + (n + e) * kRows + 4);
+      x[e][0] = lo.x;
+      x[e][1] = lo.y;
+      x[e][2] = hi.x;
+      x[e][3] = hi.y;
     }
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) read4(x[r], w + r * kTile + n);
+    for (int e = 0; e < 2; ++e)
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+      for (int f = 0; f < kF; ++f) {
+        const uint64_t y2 = pk2(y[e][f], y[e][f]);
 #pragma unroll
-      for (int r = 0; r < kRows; ++r)
-#pragma unroll
-        for (int f = 0; f < kF; ++f) d[r][f] = fmaf(x[r][e], y[e][f], d[r][f]);
+        for (int r = 0; r < kRows / 2; ++r) d[r][f] = fma2(x[e][r], y2, d[r][f]);
+      }
   }
 }
 // the warp's weights take the places that the last product has read
 __device__ __forceinline__ void share(float* w, const float (&x)[kRows][2], int lane) {
   __syncwarp();
 #pragma unroll
-  for (int r = 0; r < kRows; ++r) {
-    w[r * kTile + lane] = x[r][0];
-    w[r * kTile + lane + 32] = x[r][1];
-  }
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int r = 0; r < kRows; r += 4)
+      *reinterpret_cast<float4*>(w + (lane + 32 * j) * kRows + r) = make_float4(x[r][j], x[r + 1][j], x[r + 2][j], x[r + 3][j]);
   __syncwarp();
+}
+// row r of a pair-wise sum
+template <int kF> __device__ __forceinline__ void row_of(float (&x)[kF], const uint64_t (&d)[kRows / 2][kF], int r) {
+#pragma unroll
+  for (int f = 0; f < kF; ++f) {
+    float a, b;
+    upk2(d[r / 2][f], a, b);
+    x[f] = r & 1 ? b : a;
+  }
 }
 template <int kF> __device__ __forceinline__ void write_row(float* to, const float (&x)[kF], bool nonzero) {
   if constexpr (kF == 2) *reinterpret_cast<float2*>(to) = nonzero ? make_float2(x[0], x[1]) : make_float2(0.f, 0.f);
@@ -123,7 +151,7 @@ __device__ __forceinline__ int length_of(const WindowParams& p, int b) {
 }
 
 template <int kD>
-__global__ void __launch_bounds__(kThreads, 1) window_fwd_f32_kernel(const __grid_constant__ WindowParams p, float scale_log2) {
+__global__ void __launch_bounds__(kThreads, kD == 64 ? 2 : 1) window_fwd_f32_kernel(const __grid_constant__ WindowParams p, float scale_log2) {
   constexpr int kF = kD / 32, kT = kTileFloats<kD>;
   extern __shared__ __align__(16) float smem[];
   float *const qt = smem, *const kv = qt + kT, *const wts = kv + 4 * kT + threadIdx.x / 32 * (kRows * kTile);      // kv: 2 x (K, V)
@@ -148,13 +176,12 @@ __global__ void __launch_bounds__(kThreads, 1) window_fwd_f32_kernel(const __gri
     copy_tile<kD>(qt, (const float*)p.q + b * p.qs[0] + h * p.qs[1] + (int64_t)tile * kTile * p.qs[2], p.qs[2], min(rows, len - p0), p.D);
     ask(0);
   }
-  float m[kRows], l[kRows], o[kRows][kF];      // l: the lane's share
+  float m[kRows], l[kRows];                    // l: the lane's share
+  uint64_t o[kRows / 2][kF] = {};
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     m[r] = -INFINITY;
     l[r] = 0.f;
-#pragma unroll
-    for (int f = 0; f < kF; ++f) o[r][f] = 0.f;
   }
   for (int i = 0; i < n; ++i) {
     const float* const kt = kv + (i & 1) * 2 * kT;
@@ -162,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_fwd_f32_kernel(const __gri
     copy_wait();
     __syncthreads();                           // tile i is there, and nobody reads tile i - 1 any more
     if (i + 1 < n) ask(i + 1);
-    float s[kRows][2];
+    float s[kRows][2], turn[kRows];
     product<kD>(s, qt + r0 * kStride<kD>, kt, lane);
 #pragma unroll
     for (int r = 0; r < kRows; ++r) {
@@ -170,14 +197,17 @@ __global__ void __launch_bounds__(kThreads, 1) window_fwd_f32_kernel(const __gri
 #pragma unroll
       for (int j = 0; j < 2; ++j) s[r][j] = pos < len && window_sees(pos, key0 + 32 * j, p.window, p.sinks) ? s[r][j] * scale_log2 : -INFINITY;
       const float mx = warp_max_nan(max3_nan(m[r], s[r][0], s[r][1]));
-      const float shift = mx == -INFINITY ? 0.f : mx, f = exp2f(m[r] - shift);
+      const float shift = mx == -INFINITY ? 0.f : mx;
+      turn[r] = exp2f(m[r] - shift);
       m[r] = mx;
-#pragma unroll
-      for (int c = 0; c < kF; ++c) o[r][c] *= f;
       s[r][0] = exp2f(s[r][0] - shift);
       s[r][1] = exp2f(s[r][1] - shift);
-      l[r] = fmaf(l[r], f, s[r][0] + s[r][1]);
+      l[r] = fmaf(l[r], turn[r], s[r][0] + s[r][1]);
     }
+#pragma unroll
+    for (int r = 0; r < kRows / 2; ++r)
+#pragma unroll
+      for (int f = 0; f < kF; ++f) o[r][f] = mul2(o[r][f], pk2(turn[2 * r], turn[2 * r + 1]));
     share(wts, s, lane);
     accumulate<kD>(o, wts, kt + kT, lane);
   }
@@ -187,9 +217,11 @@ __global__ void __launch_bounds__(kThreads, 1) window_fwd_f32_kernel(const __gri
     if (r0 + r >= rows) continue;
     const int64_t at = (int64_t)bh * p.Lq + tile * kTile + r0 + r;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    float x[kF];
+    row_of<kF>(x, o, r);
 #pragma unroll
-    for (int c = 0; c < kF; ++c) o[r][c] *= inv;
-    if (lane * kF < p.D) write_row<kF>((float*)p.o + at * p.D + lane * kF, o[r], sum != 0.f);
+    for (int f = 0; f < kF; ++f) x[f] *= inv;
+    if (lane * kF < p.D) write_row<kF>((float*)p.o + at * p.D + lane * kF, x, sum != 0.f);
     if (lane == 0) p.lse[at] = sum == 0.f ? INFINITY : m[r] + log2f(sum);
   }
 }
@@ -225,7 +257,8 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_f32_kernel(const __grid
     copy_wait();
     __syncthreads();
   }
-  float delta[kRows], lse[kRows], dq[kRows][kF];
+  float delta[kRows], lse[kRows];
+  uint64_t dq[kRows / 2][kF] = {};
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     const bool is = r0 + r < valid;
@@ -238,8 +271,6 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_f32_kernel(const __grid
     delta[r] = warp_sum(sum);
     lse[r] = is ? ld_behind_wait(p.lse + row0 + r0 + r) : INFINITY;
     if (r0 + r < rows && lane == 0) p.delta[row0 + r0 + r] = delta[r];
-#pragma unroll
-    for (int f = 0; f < kF; ++f) dq[r][f] = 0.f;
   }
   for (int i = 0; i < n; ++i) {
     const float* const kt = kv + (i & 1) * 2 * kT;
@@ -261,8 +292,11 @@ __global__ void __launch_bounds__(kThreads, 1) window_dq_f32_kernel(const __grid
     accumulate<kD>(dq, wts, kt, lane);
   }
 #pragma unroll
-  for (int r = 0; r < kRows; ++r)
-    if (r0 + r < rows && lane * kF < p.D) write_row<kF>((float*)p.dq + (row0 + r0 + r) * p.D + lane * kF, dq[r], r0 + r < valid);
+  for (int r = 0; r < kRows; ++r) {
+    float x[kF];
+    row_of<kF>(x, dq, r);
+    if (r0 + r < rows && lane * kF < p.D) write_row<kF>((float*)p.dq + (row0 + r0 + r) * p.D + lane * kF, x, r0 + r < valid);
+  }
 }
 
 // dK and dV of a tile of 64 keys of one key head from a run of query tiles of all heads that share it; a warp has eight keys
@@ -287,11 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkv_f32_kernel(const __gri
     if (first > last) return;
   }
   const int key0 = tile * kTile + r0, valid_k = min(kTile, len - tile * kTile);
-  float dk[kRows][kF], dv[kRows][kF];
-#pragma unroll
-  for (int r = 0; r < kRows; ++r)
-#pragma unroll
-    for (int f = 0; f < kF; ++f) dk[r][f] = dv[r][f] = 0.f;
+  uint64_t dk[kRows / 2][kF] = {}, dv[kRows / 2][kF] = {};
   const int per_head = last - first + 1, n = per_head > 0 ? per_head * G : 0;
   auto rows_of = [&](int t) { return min(min(kTile, p.Lq - t * kTile), len - off - t * kTile); };
   auto ask = [&](int i) {
@@ -345,8 +375,11 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkv_f32_kernel(const __gri
   for (int r = 0; r < kRows; ++r) {
     if (key0 + r >= (run >= 0 ? p.sinks : p.Lk)) continue;               // a run's rows see the sinks alone
     const int64_t at = split ? (int64_t)(r0 + r) * p.D : ((int64_t)bk * p.Lk + key0 + r) * p.D;
-    write_row<kF>((split ? part : (float*)p.dk) + at + lane * kF, dk[r], true);
-    write_row<kF>((split ? part + kTile * p.D : (float*)p.dv) + at + lane * kF, dv[r], true);
+    float x[kF];
+    row_of<kF>(x, dk, r);
+    write_row<kF>((split ? part : (float*)p.dk) + at + lane * kF, x, true);
+    row_of<kF>(x, dv, r);
+    write_row<kF>((split ? part + kTile * p.D : (float*)p.dv) + at + lane * kF, x, true);
   }
 }
 
