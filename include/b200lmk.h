@@ -491,15 +491,17 @@ int lmk_cached_rows(const void* q, const void* k, const void* v, const int64_t q
  * sequence's end give zeros and take no part in any gradient, whatever they hold.
  *   q [B,H,Lq,D], k, v [B,Hkv,Lk,D] with H a multiple of Hkv (head h reads key head h / (H / Hkv)), strided; o [B,H,Lq,D] dense; lse
  *   [B*H, Lq] fp32: log2 of the row's normaliser (+inf where a row sees nothing).  D a multiple of 8 up to 128, Lk >= Lq, sm_scale > 0.
- *   Backward: o, dQ [B,H,Lq,D], dK, dV [B,Hkv,Lk,D] dense, dO strided; workspace of lmk_window_bwd_workspace(...) bytes, 256-byte
- *   aligned, contents irrelevant.  dK and dV are sums over the heads that share them; no atomics, bit-reproducible.
+ *   o_rest (16-bit types, nullable; null in fp32): what the rounding of o left, a byte a number, for the backward pass.
+ *   Backward: o, o_rest (16-bit types), dQ [B,H,Lq,D], dK, dV [B,Hkv,Lk,D] dense, dO strided; workspace of
+ *   lmk_window_bwd_workspace(...) bytes, 256-byte aligned, contents irrelevant.  dK and dV are sums over the heads that share them;
+ *   bit-reproducible.
  */
-int lmk_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* lengths, int B, int H, int Hkv,
-                   int Lq, int Lk, int D, const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
+int lmk_window_fwd(const void* q, const void* k, const void* v, void* o, void* o_rest, float* lse, const int32_t* lengths, int B, int H,
+                   int Hkv, int Lq, int Lk, int D, const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
                    int window, int sinks, float sm_scale, int dtype, void* stream);
 size_t lmk_window_bwd_workspace(int B, int H, int Hkv, int Lq, int Lk, int D, int window, int sinks, int dtype);
-int lmk_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dO, const float* lse, const int32_t* lengths,
-                   void* dQ, void* dK, void* dV, void* workspace, size_t workspace_bytes, int B, int H, int Hkv, int Lq, int Lk, int D,
+int lmk_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const void* dO, const float* lse,
+                   const int32_t* lengths, void* dQ, void* dK, void* dV, void* workspace, size_t workspace_bytes, int B, int H, int Hkv, int Lq, int Lk, int D,
                    const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3], const int64_t do_strides[3],
                    int window, int sinks, float sm_scale, int dtype, void* stream);
 

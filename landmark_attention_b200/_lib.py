@@ -122,9 +122,9 @@ PROTOTYPES = {
                               c_int, c_void_p]),
     "lmk_selected_pv": (c_int, [c_void_p, c_int64, c_int64, c_void_p, POINTER(CacheDesc), c_void_p, c_void_p, c_int,
                                 c_int, c_int, c_int, c_int, c_void_p]),
-    "lmk_window_fwd": (c_int, [c_void_p] * 6 + [c_int] * 6 + [POINTER(c_int64)] * 3 + [c_int, c_int, c_float, c_int, c_void_p]),
+    "lmk_window_fwd": (c_int, [c_void_p] * 7 + [c_int] * 6 + [POINTER(c_int64)] * 3 + [c_int, c_int, c_float, c_int, c_void_p]),
     "lmk_window_bwd_workspace": (c_size_t, [c_int] * 9),
-    "lmk_window_bwd": (c_int, [c_void_p] * 11 + [c_size_t] + [c_int] * 6 + [POINTER(c_int64)] * 4 +
+    "lmk_window_bwd": (c_int, [c_void_p] * 12 + [c_size_t] + [c_int] * 6 + [POINTER(c_int64)] * 4 +
                        [c_int, c_int, c_float, c_int, c_void_p]),
     "lmk_paged_append": (c_int, [c_void_p] * 2 + [POINTER(c_int64)] * 2 + [c_void_p] * 2 + [POINTER(c_int64)] * 2 + [c_void_p] * 4 +
                          [c_int] * 8 + [c_void_p]),

@@ -915,12 +915,14 @@ bool window_rows(const Tensor& t) {
 }
 
 Tensor window_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths, int64_t window, int64_t sinks, double scale,
-                  Tensor* lse) {
+                  Tensor* lse, Tensor* rest) {
   const auto B = q.size(0), H = q.size(1), Lq = q.size(2), D = q.size(3), Hkv = k.size(1), Lk = k.size(2);
   Tensor o = empty_like_dtype({B, H, Lq, D}, q);
+  if (rest != nullptr && q.scalar_type() != at::kFloat) *rest = at::empty({B, H, Lq, D}, q.options().requires_grad(false).dtype(at::kByte));
   *lse = empty_f32({B * H, Lq}, q);
-  check(lib.lmk_window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse->data_ptr<float>(), i32_ptr(lengths), B, H, Hkv, Lq,
-                           Lk, D, S3(q).v, S3(k).v, S3(v).v, window, sinks, (float)scale, dtype_code(q), stream_of(q)),
+  check(lib.lmk_window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
+                           rest != nullptr && rest->defined() ? rest->data_ptr() : nullptr, lse->data_ptr<float>(), i32_ptr(lengths), B, H, Hkv, Lq, Lk, D,
+                           S3(q).v, S3(k).v, S3(v).v, window, sinks, (float)scale, dtype_code(q), stream_of(q)),
         "lmk_window_fwd");
   return o;
 }
@@ -930,8 +932,8 @@ struct WindowAttention : public torch::autograd::Function<WindowAttention> {
                         int64_t window, int64_t sinks, double scale) {
     at::AutoDispatchBelowADInplaceOrView below;
     const Tensor lengths = lengths_.value_or(Tensor());
-    Tensor lse, o = window_fwd(q, k, v, lengths, window, sinks, scale, &lse);
-    ctx->save_for_backward({q, k, v, o, lse, lengths});
+    Tensor lse, rest, o = window_fwd(q, k, v, lengths, window, sinks, scale, &lse, &rest);
+    ctx->save_for_backward({q, k, v, o, lse, lengths, rest});
     ctx->saved_data["window"] = window;
     ctx->saved_data["sinks"] = sinks;
     ctx->saved_data["scale"] = scale;
@@ -941,7 +943,7 @@ struct WindowAttention : public torch::autograd::Function<WindowAttention> {
     if (at::GradMode::is_enabled())
       C10_THROW_ERROR(NotImplementedError, "window_attention has first derivatives only (create_graph is not supported)");
     auto saved = ctx->get_saved_variables();
-    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &lse = saved[4], &lengths = saved[5];
+    const Tensor &q = saved[0], &k = saved[1], &v = saved[2], &o = saved[3], &lse = saved[4], &lengths = saved[5], &rest = saved[6];
     const int64_t window = ctx->saved_data["window"].toInt(), sinks = ctx->saved_data["sinks"].toInt();
     const auto B = q.size(0), H = q.size(1), Lq = q.size(2), D = q.size(3), Hkv = k.size(1), Lk = k.size(2);
     c10::cuda::OptionalCUDAGuard guard(q.device());
@@ -950,8 +952,8 @@ struct WindowAttention : public torch::autograd::Function<WindowAttention> {
     const int code = dtype_code(q);
     const size_t need = std::max<size_t>(lib.lmk_window_bwd_workspace(B, H, Hkv, Lq, Lk, D, window, sinks, code), 256);
     Tensor ws = at::empty({(int64_t)need}, q.options().requires_grad(false).dtype(at::kByte));
-    check(lib.lmk_window_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dO.data_ptr(), lse.data_ptr<float>(), i32_ptr(lengths),
-                             dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), need, B, H, Hkv, Lq, Lk, D, S3(q).v, S3(k).v,
+    check(lib.lmk_window_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), rest.defined() ? rest.data_ptr() : nullptr, dO.data_ptr(),
+                             lse.data_ptr<float>(), i32_ptr(lengths), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), need, B, H, Hkv, Lq, Lk, D, S3(q).v, S3(k).v,
                              S3(v).v, S3(dO).v, window, sinks, (float)ctx->saved_data["scale"].toDouble(), code, stream_of(q)),
           "lmk_window_bwd");
     return {dq, dk, dv, Tensor(), Tensor(), Tensor(), Tensor()};
@@ -991,7 +993,7 @@ Tensor window_attention(const Tensor& q_, const Tensor& k_, const Tensor& v_, co
     if (!window_rows(*t)) *t = t->clone(at::MemoryFormat::Contiguous);        // part of the graph where a gradient is wanted
   if (!needs_grad({q, k, v})) {
     Tensor lse;
-    return window_fwd(q, k, v, lengths, window, sinks, scale, &lse);
+    return window_fwd(q, k, v, lengths, window, sinks, scale, &lse, nullptr);
   }
   if (at::GradMode::is_enabled() && c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
     for (const Tensor* t : {&q_, &k_, &v_}) check_capture(*t);

@@ -105,15 +105,18 @@ int window_join_parts(const WindowParams& p, int qt, int kk, int dtype, cudaStre
 
 using namespace lmk;
 
-extern "C" int lmk_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, const int32_t* lengths, int B, int H,
-                              int Hkv, int Lq, int Lk, int D, const int64_t q_strides[3], const int64_t k_strides[3],
+extern "C" int lmk_window_fwd(const void* q, const void* k, const void* v, void* o, void* o_rest, float* lse, const int32_t* lengths, int B,
+                              int H, int Hkv, int Lq, int Lk, int D, const int64_t q_strides[3], const int64_t k_strides[3],
                               const int64_t v_strides[3], int window, int sinks, float sm_scale, int dtype, void* stream) {
   int rc = check_window(q, k, v, lse, B, H, Hkv, Lq, Lk, D, q_strides, k_strides, v_strides, window, sinks, sm_scale, dtype);
   if (rc != LMK_OK) return rc;
   LMK_CHECK_ARG(o != nullptr, "window attention: o is null");
+  LMK_CHECK_ARG(o_rest == nullptr || dtype != LMK_F32, "window attention: o_rest is for 16-bit types");
+  LMK_CHECK_ARG((((uintptr_t)o | (uintptr_t)o_rest) & 15) == 0, "window attention: o and o_rest must start on 16-byte boundaries");
   WindowParams p = {};
   fill(p, q, k, v, lengths, B, H, Hkv, Lq, Lk, D, q_strides, k_strides, v_strides, window, sinks, sm_scale);
   p.o = o;
+  p.rest = o_rest;
   p.lse = lse;
   LMK_CHECK_ARG(rows_ok(q, q_strides, D, dtype) && rows_ok(k, k_strides, D, dtype) && rows_ok(v, v_strides, D, dtype),
                 "window attention: tensors must start on 16-byte boundaries, strides be multiples of 16 bytes (16-bit types: positive, rows not overlapping)");
@@ -130,7 +133,7 @@ extern "C" size_t lmk_window_bwd_workspace(int B, int H, int Hkv, int Lq, int Lk
   return kNextBytes + up256(sizeof(float) * (size_t)B * H * Lq) + up256(part_bytes(s, B, Hkv, D, kk));
 }
 
-extern "C" int lmk_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* dO, const float* lse,
+extern "C" int lmk_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const void* dO, const float* lse,
                               const int32_t* lengths, void* dQ, void* dK, void* dV, void* workspace, size_t workspace_bytes, int B, int H,
                               int Hkv, int Lq, int Lk, int D, const int64_t q_strides[3], const int64_t k_strides[3],
                               const int64_t v_strides[3], const int64_t do_strides[3], int window, int sinks, float sm_scale, int dtype,
@@ -138,9 +141,13 @@ extern "C" int lmk_window_bwd(const void* q, const void* k, const void* v, const
   int rc = check_window(q, k, v, lse, B, H, Hkv, Lq, Lk, D, q_strides, k_strides, v_strides, window, sinks, sm_scale, dtype);
   if (rc != LMK_OK) return rc;
   LMK_CHECK_ARG(o && dO && dQ && dK && dV && do_strides, "window attention backward: o, dO or a gradient is null");
+  LMK_CHECK_ARG((o_rest != nullptr) == (dtype != LMK_F32), "window attention backward: 16-bit types need o_rest, fp32 has none");
+  LMK_CHECK_ARG((((uintptr_t)o | (uintptr_t)o_rest | (uintptr_t)dQ | (uintptr_t)dK | (uintptr_t)dV) & 15) == 0,
+                "window attention backward: o, o_rest and the gradients must start on 16-byte boundaries");
   WindowParams p = {};
   fill(p, q, k, v, lengths, B, H, Hkv, Lq, Lk, D, q_strides, k_strides, v_strides, window, sinks, sm_scale);
   p.o = const_cast<void*>(o);
+  p.rest = const_cast<void*>(o_rest);
   p.dO = dO;
   p.lse = const_cast<float*>(lse);
   p.dq = dQ; p.dk = dK; p.dv = dV;

@@ -17,6 +17,7 @@ struct SinkSplit {
 struct WindowParams {
   const void *q, *k, *v, *dO;
   void* o;                     // forward output / backward input
+  void* rest;                  // what the rounding of o left, a byte a number (16-bit types; null: not wanted)
   float* lse;                  // [B*H, Lq]: log2 of the row's normaliser, +inf for a row that sees nothing
   const int* lengths;          // [B] or null
   void *dq, *dk, *dv;

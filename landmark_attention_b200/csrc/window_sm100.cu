@@ -17,6 +17,7 @@
 // shared memory by the loading thread, so that NaN there stays there.
 // All waits are bounded (sm100_ptx.cuh).
 #include <mutex>
+#include <cuda_fp8.h>
 #include "common.cuh"
 #include "attn_params.h"
 #include "window_params.h"
@@ -69,8 +70,34 @@ __device__ __forceinline__ void zero_fill(void* to, int n, int thread, int threa
   for (int i = thread; i < n; i += threads) reinterpret_cast<uint4*>(to)[i] = make_uint4(0u, 0u, 0u, 0u);
 }
 
+// two numbers in the 16-bit type, as fp32
+template <bool kBf16> __device__ __forceinline__ float2 unpack2(uint32_t x) {
+  if (kBf16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
+  return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
+
+// What rounding x to 16 bits left, four numbers in a word: e5m2, times 2^11 (fp16) or 2^8 (bf16), so that it has about the size of x.  Two
+// bits are enough: delta, which it goes into, then is off by an eighth of what the rounding of O alone would do.
+template <bool kBf16> constexpr float kRestScale = kBf16 ? 256.f : 2048.f;
+template <bool kBf16> __device__ __forceinline__ uint32_t rest4(const float (&x)[4]) {
+  uint32_t r = 0;
+#pragma unroll
+  for (int e = 0; e < 4; e += 2) {
+    const float2 back = unpack2<kBf16>(pack2<kBf16>(x[e], x[e + 1]));
+    const float2 left = make_float2((x[e] - back.x) * kRestScale<kBf16>, (x[e + 1] - back.y) * kRestScale<kBf16>);
+    r |= (uint32_t)__nv_cvt_float2_to_fp8x2(left, __NV_SATFINITE, __NV_E5M2) << (8 * e);
+  }
+  return r;
+}
+template <bool kBf16> __device__ __forceinline__ float2 rest_of(uint32_t pair) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)pair, __NV_E5M2);
+  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  return make_float2(x.x * (1.f / kRestScale<kBf16>), x.y * (1.f / kRestScale<kBf16>));
+}
+
 struct WindowTensors {
   void* o;
+  uint8_t* rest;
   float* lse;
   const int* lengths;
   int BH, H, G, Lq, Lk, D, window, sinks;
@@ -258,9 +285,11 @@ window_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       const RowUnit u = unit_of(x);
       const int pos = off + u.t * kQTile + row, grow = u.t * kQTile + row;
       const bool stored = grow < p.Lq;
-      uint4* const orow = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.o) + ((int64_t)u.bh * p.Lq + grow) * p.D);
       if (u.total == 0) {                            // nothing but padding
-        zero_fill(reinterpret_cast<uint16_t*>(p.o) + ((int64_t)u.bh * p.Lq + u.t * kQTile) * p.D, min(kQTile, p.Lq - u.t * kQTile) * p.D / 8, tid, 128);
+        const int64_t at = ((int64_t)u.bh * p.Lq + u.t * kQTile) * p.D;
+        const int n = min(kQTile, p.Lq - u.t * kQTile) * p.D / 8;
+        zero_fill(reinterpret_cast<uint16_t*>(p.o) + at, n, tid, 128);
+        // (what stands in rest is not read behind a sequence's end)
         if (stored) p.lse[(int64_t)u.bh * p.Lq + grow] = INFINITY;
         __syncwarp();
         continue;
@@ -367,6 +396,12 @@ window_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       tc_fence_after();
       const bool valid = pos < u.len && l != 0.f;
       const float inv = valid ? 1.f / l : 0.f;
+      int64_t row_off[4];                            // of the four rows that four lanes write together
+      {
+        const int64_t at = stored ? ((int64_t)u.bh * p.Lq + grow) * p.D : -1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) row_off[j] = __shfl_sync(0xffffffffu, at, (lane & ~3) + j);
+      }
 #pragma unroll
       for (int cc = 0; cc < kD / 32; ++cc) {
         uint32_t o[32];
@@ -377,14 +412,16 @@ window_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
           mbar_arrive(smem_u32(&sm->o_empty));       // the next unit may start accumulating
         }
 #pragma unroll
-        for (int v4 = 0; v4 < 4; ++v4) {
-          uint4 pk;
-          pk.x = pack2<kBf16>(__uint_as_float(o[8 * v4 + 0]) * inv, __uint_as_float(o[8 * v4 + 1]) * inv);
-          pk.y = pack2<kBf16>(__uint_as_float(o[8 * v4 + 2]) * inv, __uint_as_float(o[8 * v4 + 3]) * inv);
-          pk.z = pack2<kBf16>(__uint_as_float(o[8 * v4 + 4]) * inv, __uint_as_float(o[8 * v4 + 5]) * inv);
-          pk.w = pack2<kBf16>(__uint_as_float(o[8 * v4 + 6]) * inv, __uint_as_float(o[8 * v4 + 7]) * inv);
-          if (!valid) pk = make_uint4(0u, 0u, 0u, 0u);          // (not 0 * whatever padding left in the accumulator)
-          if (stored && cc * 32 + v4 * 8 < p.D) orow[cc * 4 + v4] = pk;
+        for (int e = 0; e < 32; ++e) o[e] = valid ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;      // (not 0 * what padding left there)
+        store_acc_cols<kBf16>(p.o, row_off, o, cc * 32, p.D, lane);
+        if (p.rest != nullptr && valid) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            const float x[4] = {__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])};
+            const float y[4] = {__uint_as_float(o[e + 4]), __uint_as_float(o[e + 5]), __uint_as_float(o[e + 6]), __uint_as_float(o[e + 7])};
+            if (cc * 32 + e < p.D)
+              *reinterpret_cast<uint2*>(p.rest + ((int64_t)u.bh * p.Lq + grow) * p.D + cc * 32 + e) = make_uint2(rest4<kBf16>(x), rest4<kBf16>(y));
+          }
         }
         __syncwarp();
       }
@@ -508,7 +545,7 @@ struct DkvArgs {
   const float *lse, *delta;
   void *dk, *dv;
   const int* lengths;
-  int* next;                                        // units given out beyond the first of each CTA; set to 0 by the dQ kernel
+  int* next;                                        // units given out beyond the first of each CTA; set to 0 by the delta kernel
   int H, Hkv, G, B, Lq, Lk, D, window, sinks, n_pairs;
   float scale, scale_log2;
   SinkSplit split;
@@ -607,7 +644,6 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   if (warp == kBwdWarps) {
     // ------------------------------------------------------------------ loads: lane 0 issues TMA, all lanes bring the statistics
     int it = 0, u = 0, patches = 0;
-    bool behind = false;                           // behind the dQ kernel, which writes delta
     auto deal = [&](int r, int w) {
       mbar_wait(smem_u32(&sm->dealt_empty[r % kDealt]), ((r / kDealt) & 1) ^ 1, status, kErrDkvProducer);
       if (lane == 0) {
@@ -617,8 +653,6 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       __syncwarp();
     };
     auto ask_unit = [&]() {
-      if (!behind) grid_dep_wait();
-      behind = true;
       int w = 0;
       if (lane == 0) w = gridDim.x + atomicAdd(p.next, 1);
       return __shfl_sync(0xffffffffu, w, 0);
@@ -912,8 +946,64 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   }
 }
 
+// ---------------------------------------------------------------------------------------------- backward: delta = rowsum(O dO)
+// with what the rounding of O left: without it a row of dS would miss its sum of 0 by as much as dS's own rounding is off, and dQ and dK
+// had 1.53 instead of 1.41 times the error of their own rounding.  Bound by memory; in the dQ kernel the tiles of O and of the rest took
+// the places of key tiles on their way (training size 46 -> 53 us), and the dK/dV kernel had to wait for the last of its CTAs.
+struct DeltaArgs {
+  const void *o, *dO;
+  const uint8_t* rest;
+  float* delta;
+  int* next;                // set to 0 for the dK/dV kernel
+  const int* lengths;
+  int BH, H, Lq, Lk, D;
+  int64_t dos[3];
+};
+constexpr int kDeltaThreads = 256, kDeltaSteps = 4;
+
+template <bool kBf16, int kD>
+__global__ void __launch_bounds__(kDeltaThreads, 4) window_delta_kernel(const __grid_constant__ DeltaArgs p) {
+  constexpr int kLanes = kD / 8, kRows = kDeltaThreads / kLanes;      // lanes of a row, rows a step
+  grid_dep_wait();
+  grid_dep_launch();
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *p.next = 0;
+  const int bh = blockIdx.y, b = bh / p.H, h = bh - b * p.H, f = threadIdx.x % kLanes * 8;
+  const int len = length_of(p.lengths, b, p.Lk) - (p.Lk - p.Lq);      // rows that are some
+  const int row0 = blockIdx.x * kRows * kDeltaSteps + threadIdx.x / kLanes;
+  const uint16_t* const dO = reinterpret_cast<const uint16_t*>(p.dO) + b * p.dos[0] + h * p.dos[1] + f;
+  uint4 x[kDeltaSteps], g[kDeltaSteps];
+  uint2 y[kDeltaSteps];
+#pragma unroll
+  for (int e = 0; e < kDeltaSteps; ++e) {
+    const int row = row0 + e * kRows;
+    x[e] = g[e] = make_uint4(0u, 0u, 0u, 0u);
+    y[e] = make_uint2(0u, 0u);
+    if (row < min(len, p.Lq) && f < p.D) {
+      const int64_t at = ((int64_t)bh * p.Lq + row) * p.D + f;
+      x[e] = ld_behind_wait(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(p.o) + at));
+      y[e] = ld_behind_wait(reinterpret_cast<const uint2*>(p.rest + at));
+      g[e] = ld_behind_wait(reinterpret_cast<const uint4*>(dO + row * p.dos[2]));
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < kDeltaSteps; ++e) {
+    const uint32_t xs[4] = {x[e].x, x[e].y, x[e].z, x[e].w}, ys[2] = {y[e].x, y[e].y}, gs[4] = {g[e].x, g[e].y, g[e].z, g[e].w};
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float2 fx = unpack2<kBf16>(xs[w]), fy = rest_of<kBf16>(ys[w / 2] >> (16 * (w & 1)) & 0xffffu), fg = unpack2<kBf16>(gs[w]);
+      sum = fmaf(fx.x + fy.x, fg.x, sum);
+      sum = fmaf(fx.y + fy.y, fg.y, sum);
+    }
+#pragma unroll
+    for (int d = kLanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    const int row = row0 + e * kRows;
+    if (f == 0 && row < p.Lq) p.delta[(int64_t)bh * p.Lq + row] = sum;
+  }
+}
+
 // ---------------------------------------------------------------------------------------------- backward: dQ
-constexpr int kDqStages = 4;
+constexpr int kDqK = 6, kDqV = 4;                   // tiles of keys (kept until dQ has been formed) and of values (until dP has)
 constexpr int kSdpBufs = 2;                         // S / dP buffers in TMEM
 constexpr int kDqThreads = (kBwdWarps + 2) * 32;
 
@@ -921,19 +1011,16 @@ struct DqSmem {
   uint64_t qdo_full, patch;
   uint64_t ops_ready;       // the unit's Q and dO rows sit in TMEM (written by the pair of warpgroups that takes its first item)
   uint64_t ops_free;        // the S / dP products of the unit have read them
-  uint64_t delta_read;      // the softmax warpgroups are done with the Q, dO and O tiles in shared memory
-  uint64_t full[kDqStages], empty[kDqStages];
+  uint64_t rows_read;       // and are no longer needed in shared memory
+  uint64_t k_full[kDqK], k_empty[kDqK], v_full[kDqV], v_empty[kDqV];
   uint64_t s_full[kSdpBufs], s_free[kSdpBufs], dp_full[kSdpBufs];
   uint64_t ds_ready[kSdpBufs];                         // dS has taken dP's place
   uint64_t acc_full[2];     // per draining pair of warpgroups (the one that took the unit's last item)
   uint64_t acc_empty;
   uint32_t tmem_base;
-  float part[2][2][kQTile];                            // [pair][half]: shares of the sums of O dO
 };
 struct DqArgs {
-  const float* lse;
-  float* delta;
-  int* next;                // set to 0 for the dK/dV kernel
+  const float *lse, *delta;
   void *dq, *dk, *dv;       // dk, dv: rows that no query sees
   const int* lengths;
   int H, Hkv, G, BH, Lq, Lk, D, window, sinks, n_pairs;
@@ -945,7 +1032,7 @@ template <bool kBf16, int kD>
 __global__ void __launch_bounds__(kDqThreads, 1)
 window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
-                       const __grid_constant__ CUtensorMap tm_o, const __grid_constant__ DqArgs p, int* status) {
+                       const __grid_constant__ DqArgs p, int* status) {
   extern __shared__ __align__(1024) uint8_t smem_aligned[];
   const uint32_t base = smem_u32(smem_aligned);
   if ((base & 1023u) != 0) {                         // the swizzle needs it
@@ -953,10 +1040,9 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     return;
   }
   const uint32_t q_tile = base, do_tile = base + 32768u;
-  auto k_slot = [&](int s) { return base + 65536u + (uint32_t)s * 32768u; };
-  auto v_slot = [&](int s) { return base + 65536u + (uint32_t)s * 32768u + 16384u; };
-  const uint32_t o_tile = base + 65536u + kDqStages * 32768u;                           // forward output tile, only for delta
-  DqSmem* sm = reinterpret_cast<DqSmem*>(smem_aligned + 65536u + kDqStages * 32768u + 32768u);
+  auto k_slot = [&](int s) { return base + 65536u + (uint32_t)s * 16384u; };
+  auto v_slot = [&](int s) { return base + 65536u + (uint32_t)(kDqK + s) * 16384u; };
+  DqSmem* sm = reinterpret_cast<DqSmem*>(smem_aligned + 65536u + (kDqK + kDqV) * 16384u);
 
   const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
   const int n_tiles = (p.Lq + kQTile - 1) / kQTile, off = p.Lk - p.Lq, n_units = n_tiles * p.BH;
@@ -966,10 +1052,14 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     for (uint64_t* bar : {&sm->qdo_full, &sm->patch}) mbar_init(smem_u32(bar), 1);
     mbar_init(smem_u32(&sm->ops_ready), 256);
     mbar_init(smem_u32(&sm->ops_free), 1);
-    mbar_init(smem_u32(&sm->delta_read), kBwdWarps * 32);
-    for (int s = 0; s < kDqStages; ++s) {
-      mbar_init(smem_u32(&sm->full[s]), 1);
-      mbar_init(smem_u32(&sm->empty[s]), 1);
+    mbar_init(smem_u32(&sm->rows_read), 256);
+    for (int s = 0; s < kDqK; ++s) {
+      mbar_init(smem_u32(&sm->k_full[s]), 1);
+      mbar_init(smem_u32(&sm->k_empty[s]), 1);
+    }
+    for (int s = 0; s < kDqV; ++s) {
+      mbar_init(smem_u32(&sm->v_full[s]), 1);
+      mbar_init(smem_u32(&sm->v_empty[s]), 1);
     }
     for (int s = 0; s < kSdpBufs; ++s) {
       mbar_init(smem_u32(&sm->ds_ready[s]), 256);
@@ -991,7 +1081,6 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   const uint32_t tmem_s = tmem, tmem_dp = tmem + 128, tmem_dq = tmem + 256, tmem_q = tmem + 384, tmem_do = tmem + 448;
   grid_dep_wait();
   grid_dep_launch();
-  if (blockIdx.x == 0 && tid == 0) *p.next = 0;
 
   if (warp == kBwdWarps) {
     // ------------------------------------------------------------------ TMA producer
@@ -1001,34 +1090,36 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       if (un.total == 0) continue;
       const int hk = un.h / p.G;
       const uint32_t qb = smem_u32(&sm->qdo_full);
-      mbar_wait(smem_u32(&sm->delta_read), (u & 1) ^ 1, status, kErrDqProducer);
+      mbar_wait(smem_u32(&sm->rows_read), (u & 1) ^ 1, status, kErrDqProducer);
       if (lane == 0) {
-        mbar_arrive_expect_tx(qb, 3 * (kD / 64) * kTileBytes);
+        mbar_arrive_expect_tx(qb, 2 * (kD / 64) * kTileBytes);
         for (int c = 0; c < kD / 64; ++c) {
-          tma_load_4d(o_tile + c * kTileBytes, &tm_o, qb, 64 * c, un.t * kQTile, un.h, un.b);
           tma_load_4d(q_tile + c * kTileBytes, &tm_q, qb, 64 * c, un.t * kQTile, un.h, un.b);
           tma_load_4d(do_tile + c * kTileBytes, &tm_do, qb, 64 * c, un.t * kQTile, un.h, un.b);
         }
       }
       __syncwarp();
       for (int i = 0; i < un.total; ++i, ++it) {
-        const int s = it % kDqStages, key0 = un.tile_of(i) * kBlk;
-        mbar_wait(smem_u32(&sm->empty[s]), ((it / kDqStages) & 1) ^ 1, status, kErrDqProducer);
+        const int sk = it % kDqK, sv = it % kDqV, key0 = un.tile_of(i) * kBlk;
         const bool ends = key0 + kBlk > un.len && un.len < p.Lk;
-        const uint32_t fb = smem_u32(ends ? &sm->patch : &sm->full[s]);
+        const uint32_t kb = smem_u32(ends ? &sm->patch : &sm->k_full[sk]), vb = smem_u32(&sm->v_full[sv]);
+        mbar_wait(smem_u32(&sm->k_empty[sk]), ((it / kDqK) & 1) ^ 1, status, kErrDqProducer);
         if (lane == 0) {
-          mbar_arrive_expect_tx(fb, 2 * (kD / 64) * kHalfTile);
-          for (int c = 0; c < kD / 64; ++c) {
-            tma_load_4d(k_slot(s) + c * kHalfTile, &tm_k, fb, 64 * c, key0, hk, un.b);
-            tma_load_4d(v_slot(s) + c * kHalfTile, &tm_v, fb, 64 * c, key0, hk, un.b);
-          }
+          mbar_arrive_expect_tx(kb, (kD / 64) * kHalfTile);
+          for (int c = 0; c < kD / 64; ++c) tma_load_4d(k_slot(sk) + c * kHalfTile, &tm_k, kb, 64 * c, key0, hk, un.b);
         }
         __syncwarp();
         if (ends) {                                // dS is 0 there, and dQ += dS K
-          mbar_wait(fb, patches++ & 1, status, kErrDqProducer);
-          zero_rows(k_slot(s), kHalfTile, kD / 64, un.len - key0, kBlk, lane);
-          if (lane == 0) mbar_arrive(smem_u32(&sm->full[s]));
+          mbar_wait(kb, patches++ & 1, status, kErrDqProducer);
+          zero_rows(k_slot(sk), kHalfTile, kD / 64, un.len - key0, kBlk, lane);
+          if (lane == 0) mbar_arrive(smem_u32(&sm->k_full[sk]));
         }
+        mbar_wait(smem_u32(&sm->v_empty[sv]), ((it / kDqV) & 1) ^ 1, status, kErrDqProducer);
+        if (lane == 0) {
+          mbar_arrive_expect_tx(vb, (kD / 64) * kHalfTile);
+          for (int c = 0; c < kD / 64; ++c) tma_load_4d(v_slot(sv) + c * kHalfTile, &tm_v, vb, 64 * c, key0, hk, un.b);
+        }
+        __syncwarp();
       }
       ++u;
     }
@@ -1053,14 +1144,14 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         if (c.n > 0) return;
       }
     };
-    auto slot = [&](uint64_t d, int it) { return desc_advance(d, (uint32_t)(it % kDqStages) * 32768u); };
+    auto k_of = [&](uint64_t d, int it) { return desc_advance(d, (uint32_t)(it % kDqK) * 16384u); };
     auto issue_s = [&](const Cursor& c, int it) {
       const int sb = it % kSdpBufs;
-      mbar_wait(smem_u32(&sm->full[it % kDqStages]), (it / kDqStages) & 1, status, kErrDqMma);
+      mbar_wait(smem_u32(&sm->k_full[it % kDqK]), (it / kDqK) & 1, status, kErrDqMma);
       if (it >= kSdpBufs) mbar_wait(smem_u32(&sm->s_free[sb]), ((it / kSdpBufs) & 1) ^ 1, status, kErrDqMma);
       if (c.i == 0) mbar_wait(smem_u32(&sm->ops_ready), c.u & 1, status, kErrDqMma);
       tc_fence_after();
-      const uint64_t db = slot(dk0, it);
+      const uint64_t db = k_of(dk0, it);
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kD / 16; ++kk)      // A from TMEM: 8 columns = 16 features per K-step
@@ -1070,12 +1161,15 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     };
     auto issue_dp = [&](const Cursor& c, int it) {
       const int sb = it % kSdpBufs;
-      const uint64_t db = slot(dv0, it);
+      mbar_wait(smem_u32(&sm->v_full[it % kDqV]), (it / kDqV) & 1, status, kErrDqMma);
+      tc_fence_after();
+      const uint64_t db = desc_advance(dv0, (uint32_t)(it % kDqV) * 16384u);
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kD / 16; ++kk)
           mma_f16_ts(tmem_dp + sb * 64, tmem_do + kk * 8, desc_advance(db, kmajor_step(kk, kHalfTile)), idesc_s, kk > 0);
         mma_commit(smem_u32(&sm->dp_full[sb]));
+        mma_commit(smem_u32(&sm->v_empty[it % kDqV]));
         if (c.i == c.n - 1) mma_commit(smem_u32(&sm->ops_free));        // the next unit's Q / dO rows may be written
       }
     };
@@ -1095,13 +1189,13 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       if (now.i == 0) mbar_wait(smem_u32(&sm->acc_empty), (now.u & 1) ^ 1, status, kErrDqMma);
       mbar_wait(smem_u32(&sm->ds_ready[sb]), (it / kSdpBufs) & 1, status, kErrDqMma);
       tc_fence_after();
-      const uint64_t dkt = slot(dk0t, it);
+      const uint64_t dkt = k_of(dk0t, it);
       if (elect_one()) {
 #pragma unroll
         for (int kk = 0; kk < kBlk / 16; ++kk)
           mma_f16_ts(tmem_dq, tmem_dp + sb * 64 + (kk >> 1) * kCols + (kk & 1) * 8, desc_advance(dkt, kk * 2048), idesc_q,
                      (now.i > 0 || kk > 0) ? 1u : 0u);
-        mma_commit(smem_u32(&sm->empty[it % kDqStages]));
+        mma_commit(smem_u32(&sm->k_empty[it % kDqK]));
         if (now.i == now.n - 1) mma_commit(smem_u32(&sm->acc_full[it & 1]));     // drained by the pair that took the last item
       }
       if (ahead.n > 0) {
@@ -1119,8 +1213,8 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
     const int row = tid & 127;
     const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
     int it0 = 0, u = 0, drains = 0;
-    // dQ of a unit is drained by the pair that took its last item, half of the features each, while that item's product runs it sums up
-    // the next unit's O dO; the other pair has brought that unit's rows to TMEM meanwhile
+    // dQ of a unit is drained by the pair that took its last item, half of the features each; the other pair has brought the next unit's
+    // rows to TMEM meanwhile
     constexpr int kOut = kD / 2;
     int64_t drain_row = -1;
     bool drain_stored = false, drain_valid = false;
@@ -1128,7 +1222,12 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       mbar_wait(smem_u32(&sm->acc_full[pair]), drains & 1, status, kErrDqEpilogue);
       ++drains;
       tc_fence_after();
-      uint4* orow = reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.dq) + drain_row * p.D);
+      int64_t row_off[4];
+      {
+        const int64_t at = drain_stored ? drain_row * p.D : -1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) row_off[j] = __shfl_sync(0xffffffffu, at, (lane & ~3) + j);
+      }
 #pragma unroll
       for (int c = 0; c < kOut / 32; ++c) {
         const int col = half * kOut + c * 32;
@@ -1140,25 +1239,19 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           mbar_arrive(smem_u32(&sm->acc_empty));     // the next unit may start accumulating
         }
 #pragma unroll
-        for (int v4 = 0; v4 < 4; ++v4) {
-          uint4 pk;
-          pk.x = pack2<kBf16>(__uint_as_float(r[8 * v4 + 0]), __uint_as_float(r[8 * v4 + 1]));
-          pk.y = pack2<kBf16>(__uint_as_float(r[8 * v4 + 2]), __uint_as_float(r[8 * v4 + 3]));
-          pk.z = pack2<kBf16>(__uint_as_float(r[8 * v4 + 4]), __uint_as_float(r[8 * v4 + 5]));
-          pk.w = pack2<kBf16>(__uint_as_float(r[8 * v4 + 6]), __uint_as_float(r[8 * v4 + 7]));
-          if (!drain_valid) pk = make_uint4(0u, 0u, 0u, 0u);
-          if (drain_stored && col + v4 * 8 < p.D) orow[col / 8 + v4] = pk;
-        }
+        for (int e = 0; e < 32; ++e) r[e] = drain_valid ? r[e] : 0u;
+        store_acc_cols<kBf16>(p.dq, row_off, r, col, p.D, lane);
         __syncwarp();
       }
       drain_row = -1;
     };
     // row statistics of the next unit are asked for while the current one runs
-    float n_lse = 0.f;
+    float n_lse = 0.f, n_delta = 0.f;
     auto fetch_rows = [&](int w) {
       if (w >= n_units) return;
       const int rr = min((n_tiles - 1 - w / p.BH) * kQTile + row, p.Lq - 1);
       n_lse = ld_behind_wait(p.lse + (int64_t)(w % p.BH) * p.Lq + rr);
+      n_delta = ld_behind_wait(p.delta + (int64_t)(w % p.BH) * p.Lq + rr);
     };
     fetch_rows(unit_at(0));
     for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
@@ -1166,24 +1259,23 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       const int64_t grow = (int64_t)un.bh * p.Lq + un.t * kQTile + row;
       const int pos = off + un.t * kQTile + row;
       const bool stored = un.t * kQTile + row < p.Lq, valid = stored && pos < un.len;
-      const float lse = n_lse;
+      const float lse = n_lse, delta = n_delta;
       fetch_rows(unit_at(r + 1));
       if (un.total == 0) {                         // nothing but padding
         zero_fill(reinterpret_cast<uint16_t*>(p.dq) + ((int64_t)un.bh * p.Lq + un.t * kQTile) * p.D, min(kQTile, p.Lq - un.t * kQTile) * p.D / 8, tid,
                   kBwdWarps * 32);
-        if (g == 0 && stored) p.delta[grow] = 0.f;
         __syncwarp();
         continue;
       }
       const int warp_p0 = warp_uniform(off + un.t * kQTile + (warp & 3) * 32), warp_p1 = warp_p0 + 31;
-      mbar_wait(smem_u32(&sm->qdo_full), u & 1, status, kErrDqSoftmax);
       auto chunk_at = [&](int c) { return (uint32_t)(c >> 3) * kTileBytes + (uint32_t)row * 128u + (uint32_t)(((c & 7) ^ (row & 7)) << 4); };
       // The pair that takes the unit's first item moves its rows to TMEM, a warpgroup Q and the other dO: row -> lane, 32-bit word j (two
       // features) -> column j, the layout of a K-major A operand
       if (pair == (it0 & 1)) {
+        mbar_wait(smem_u32(&sm->qdo_full), u & 1, status, kErrDqSoftmax);
         mbar_wait(smem_u32(&sm->ops_free), (u & 1) ^ 1, status, kErrDqSoftmax);
         tc_fence_after();
-#pragma unroll
+#pragma unroll 1
         for (int c0 = 0; c0 < kD / 8; c0 += 8) {
           uint32_t x[32];
 #pragma unroll
@@ -1196,38 +1288,9 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(smem_u32(&sm->ops_ready));
+        fence_proxy_async_smem();                  // TMA writes the next unit's rows through another proxy than these reads went through
+        mbar_arrive(smem_u32(&sm->rows_read));
       }
-      // delta = rowsum(O dO): each pair for itself, a warpgroup half of the features
-      float sum = 0.f;
-#pragma unroll
-      for (int c = 0; c < kD / 16; ++c) {
-        uint32_t ov[4], gv[4];
-        const uint32_t at = chunk_at(half * (kD / 16) + c);
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(ov[0]), "=r"(ov[1]), "=r"(ov[2]), "=r"(ov[3]) : "r"(o_tile + at));
-        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(gv[0]), "=r"(gv[1]), "=r"(gv[2]), "=r"(gv[3]) : "r"(do_tile + at));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float2 fo, fg;
-          if (kBf16) {
-            fo = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&ov[e]));
-            fg = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&gv[e]));
-          } else {
-            fo = __half22float2(*reinterpret_cast<const __half2*>(&ov[e]));
-            fg = __half22float2(*reinterpret_cast<const __half2*>(&gv[e]));
-          }
-          sum = fmaf(fo.x, fg.x, sum);
-          sum = fmaf(fo.y, fg.y, sum);
-        }
-      }
-      auto together = [&]() { asm volatile("bar.sync %0, 256;" ::"r"(1 + pair) : "memory"); };
-      together();                                  // the last unit's shares have been read
-      sm->part[pair][half][row] = sum;
-      together();
-      const float delta = sm->part[pair][0][row] + sm->part[pair][1][row];
-      // TMA writes the next unit's rows through another proxy than these accesses went through
-      fence_proxy_async_smem();
-      mbar_arrive(smem_u32(&sm->delta_read));
-      if (g == 0 && stored) p.delta[grow] = valid ? delta : 0.f;
       if (warp_uniform(drain_row >= 0)) drain();
       const uint64_t nl = pk2(-lse, -lse);
       const float nds = -delta * p.scale;
@@ -1298,7 +1361,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 // ---------------------------------------------------------------------------------------------- host side
 template <int kD> constexpr size_t kSmemFwd = (kD / 64) * (kTileBytes + kFwdSlots<kD> * kHalfTile) + sizeof(FwdSmem<kFwdSlots<kD>>);
 template <int kD> constexpr size_t kSmemDkv = 1024 + (2 + 2 * kDkvStages) * (kD / 64) * kTileBytes + sizeof(DkvSmem);
-constexpr size_t kSmemDq = 65536 + kDqStages * 32768 + 32768 + sizeof(DqSmem);
+constexpr size_t kSmemDq = 65536 + (kDqK + kDqV) * 16384 + sizeof(DqSmem);
 static_assert(kSmemFwd<128> <= 233472 / 2 - 1024 && kSmemFwd<64> <= 233472 / 2 - 1024 && kSmemDkv<128> <= 232448 && kSmemDkv<64> <= 232448 && kSmemDq <= 232448,
               "shared memory of one SM");
 
@@ -1351,7 +1414,7 @@ int window_sm100_fwd(const WindowParams& p, int dtype, cudaStream_t st) {
   CUtensorMap tq, tk, tv;
   int rc = facts_of(&f);
   if (rc != LMK_OK || (rc = maps(p, dtype, &tq, &tk, &tv)) != LMK_OK) return rc;
-  const WindowTensors a = {p.o, p.lse, p.lengths, p.B * p.H, p.H, p.H / p.Hkv, p.Lq, p.Lk, p.D, p.window, p.sinks, p.scale * kLog2e};
+  const WindowTensors a = {p.o, static_cast<uint8_t*>(p.rest), p.lse, p.lengths, p.B * p.H, p.H, p.H / p.Hkv, p.Lq, p.Lk, p.D, p.window, p.sinks, p.scale * kLog2e};
   const int64_t units = (int64_t)((p.Lq + kQTile - 1) / kQTile) * p.B * p.H;
   int most = 2 * f->n_sm;
   const int cap = attn_sm100_max_ctas();
@@ -1370,28 +1433,30 @@ int window_sm100_fwd(const WindowParams& p, int dtype, cudaStream_t st) {
 
 int window_sm100_bwd(const WindowParams& p, int dtype, cudaStream_t st) {
   const Facts* f;
-  CUtensorMap tq, tk, tv, tdo, to;
-  const int64_t dense[3] = {(int64_t)p.H * p.Lq * p.D, (int64_t)p.Lq * p.D, (int64_t)p.D};
+  CUtensorMap tq, tk, tv, tdo;
   int rc = facts_of(&f);
   if (rc != LMK_OK || (rc = maps(p, dtype, &tq, &tk, &tv)) != LMK_OK) return rc;
   if ((rc = tensor_map_4d_now(&tdo, p.dO, dtype, p.B, p.H, p.Lq, p.D, p.dos, kQTile)) != LMK_OK) return rc;
-  if ((rc = tensor_map_4d_now(&to, p.o, dtype, p.B, p.H, p.Lq, p.D, dense, kQTile)) != LMK_OK) return rc;
   int n_sm = f->n_sm;
   const int cap = attn_sm100_max_ctas();
   if (cap >= 1 && cap < n_sm) n_sm = cap;
   const int n_pairs = (p.Lk + kPair - 1) / kPair, G = p.H / p.Hkv;
   const int64_t dq_units = (int64_t)((p.Lq + kQTile - 1) / kQTile) * p.B * p.H;
   const int64_t dkv_units = ((int64_t)n_pairs + (int64_t)p.split.tiles * p.split.runs) * p.B * p.Hkv;
-  const DqArgs aq = {p.lse, p.delta, p.next, p.dq, p.dk, p.dv, p.lengths, p.H, p.Hkv, G, p.B * p.H, p.Lq, p.Lk, p.D, p.window, p.sinks, n_pairs, p.scale,
+  const DqArgs aq = {p.lse, p.delta, p.dq, p.dk, p.dv, p.lengths, p.H, p.Hkv, G, p.B * p.H, p.Lq, p.Lk, p.D, p.window, p.sinks, n_pairs, p.scale,
                      p.scale * kLog2e, p.split};
   const DkvArgs ak = {p.lse, p.delta, p.dk, p.dv, p.lengths, p.next, p.H, p.Hkv, G, p.B, p.Lq, p.Lk, p.D, p.window, p.sinks, n_pairs, p.scale, p.scale * kLog2e,
                       p.split};
   const dim3 grid_q((unsigned)(dq_units < n_sm ? dq_units : n_sm)), grid_k((unsigned)(dkv_units < n_sm ? dkv_units : n_sm));
-  // The dK/dV kernel may start on every SM that the dQ kernel has left: it reads q, k, v, dO, lse and lengths, which were complete before
-  // any CTA of the dQ kernel was behind its wait, and delta, for which its loading warp waits.
+  const DeltaArgs ad = {p.o, p.dO, static_cast<const uint8_t*>(p.rest), p.delta, p.next, p.lengths, p.B * p.H, p.H, p.Lq, p.Lk, p.D, {p.dos[0], p.dos[1], p.dos[2]}};
+  const int delta_rows = kDeltaSteps * kDeltaThreads / ((p.D <= 64 ? 64 : 128) / 8);
+  const dim3 grid_d((p.Lq + delta_rows - 1) / delta_rows, p.B * p.H);
+  // The dK/dV kernel starts on every SM that the dQ kernel has left and waits for nothing: what it reads, delta included, was complete before
+  // any CTA of the dQ kernel was behind its wait.  It ends behind the dQ kernel.
 #define LMK_BWD(BF, DIM)                                                                                                                    \
   do {                                                                                                                                      \
-    LMK_CUDA(launch_overlapped(window_dq_sm100_kernel<BF, DIM>, grid_q, dim3(kDqThreads), kSmemDq, st, tq, tk, tv, tdo, to, aq, f->status)); \
+    LMK_CUDA(launch_overlapped(window_delta_kernel<BF, DIM>, grid_d, dim3(kDeltaThreads), 0, st, ad));                                      \
+    LMK_CUDA(launch_overlapped(window_dq_sm100_kernel<BF, DIM>, grid_q, dim3(kDqThreads), kSmemDq, st, tq, tk, tv, tdo, aq, f->status));     \
     LMK_CUDA(launch_overlapped(window_dkv_sm100_kernel<BF, DIM>, grid_k, dim3(kDkvThreads), kSmemDkv<DIM>, st, tq, tk, tv, tdo, ak, f->status)); \
   } while (0)
   if (dtype == LMK_BF16) {

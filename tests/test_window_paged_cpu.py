@@ -28,7 +28,7 @@ def test_window_argument_checks_return_codes():
     def fwd(**kw):
         a = dict(q=one, H=4, Hkv=2, Lq=64, Lk=64, D=64, w=8, s=0, scale=0.1, dt=L.LMK_BF16)
         a.update(kw)
-        return lib.lmk_window_fwd(a["q"], one, one, one, one, None, 1, a["H"], a["Hkv"], a["Lq"], a["Lk"], a["D"], s, s, s, a["w"], a["s"],
+        return lib.lmk_window_fwd(a["q"], one, one, one, None, one, None, 1, a["H"], a["Hkv"], a["Lq"], a["Lk"], a["D"], s, s, s, a["w"], a["s"],
                                   a["scale"], a["dt"], None)
     for bad in (dict(q=None), dict(H=3), dict(Lq=65), dict(D=12), dict(D=136), dict(w=0), dict(s=-1), dict(scale=0.0), dict(dt=5), dict(Lq=0)):
         assert fwd(**bad) == L.LMK_ERR_INVALID, bad
