@@ -112,7 +112,7 @@ struct WindowTensors {
 // through what one thread issues in order).  TMEM: 2 x 64 S / P + kD O.  Shared memory: Q, and a ring of K and V tiles.
 constexpr int kFwdThreads = (4 + 2) * 32;
 template <int kD> constexpr int kFwdSlots = kD == 128 ? 5 : 10;      // 64-row K and V tiles, in turn
-constexpr int kFwdPolyEvery = 8;         // one pair of exponentials in this many is a polynomial on the FMA pipe
+constexpr int kFwdPolyEvery = 4;         // one pair of exponentials in this many is a polynomial on the FMA pipe
 constexpr float kLazy = 8.f;             // the maximum moves when it is exceeded by this much (log2)
 
 template <int kSlots> struct FwdSmem {
@@ -288,8 +288,7 @@ window_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       if (u.total == 0) {                            // nothing but padding
         const int64_t at = ((int64_t)u.bh * p.Lq + u.t * kQTile) * p.D;
         const int n = min(kQTile, p.Lq - u.t * kQTile) * p.D / 8;
-        zero_fill(reinterpret_cast<uint16_t*>(p.o) + at, n, tid, 128);
-        // (what stands in rest is not read behind a sequence's end)
+        zero_fill(reinterpret_cast<uint16_t*>(p.o) + at, n, tid, 128);      // (its rest is not read)
         if (stored) p.lse[(int64_t)u.bh * p.Lq + grow] = INFINITY;
         __syncwarp();
         continue;
@@ -414,7 +413,7 @@ window_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[e] = valid ? __float_as_uint(__uint_as_float(o[e]) * inv) : 0u;      // (not 0 * what padding left there)
         store_acc_cols<kBf16>(p.o, row_off, o, cc * 32, p.D, lane);
-        if (p.rest != nullptr && valid) {
+        if (p.rest != nullptr && stored) {
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             const float x[4] = {__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]), __uint_as_float(o[e + 3])};

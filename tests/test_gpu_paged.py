@@ -416,3 +416,38 @@ def test_two_streams_at_once():
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(x, want[i]) for x in outs[i])
+
+
+def test_many_sequences_of_all_lengths():
+    """More sequences than a warp has lanes, most of them short or empty."""
+    lengths = [0, 1, 16, 17, 0, 2500] + [(37 * i) % 211 for i in range(40)] + [0, 900, 0]
+    H, Hkv, T, D, page = 8, 2, 2, 64, 32
+    k, v, table, n, _ = pool(torch.bfloat16, lengths, Hkv, D, page, seed=30, extra=1)
+    q = torch.randn((len(lengths), H, T, D), generator=gen(31), device="cuda").to(torch.bfloat16)
+    for window, sinks in ((None, 0), (100, 5)):
+        want, bound, sums = plain_attend(q, k, v, table, n, window, sinks, D ** -0.5)
+        w = torch.zeros((len(lengths), Hkv, table.shape[1] * page), device="cuda")
+        o = P.paged_attention(q, k, v, table, n, window=window, sinks=sinks, weights=w)
+        assert ((o.double() - want).abs() <= bound).all()
+        for b, m in enumerate(lengths):
+            if m:
+                s, sb = sums[b]
+                assert ((w[b, :, :m].double() - s).abs() <= sb + s * 2.0 ** -23).all()
+    assert L.device_status() == 0
+
+
+def test_eviction_from_a_very_long_sequence():
+    """More weights than a CTA keeps at hand."""
+    lengths, Hkv, D, page, budget, recent, sinks = [70001, 69999], 1, 8, 1024, 20000, 500, 4
+    need = -(-budget // page)
+    k, v, table, n, free = pool(torch.float16, lengths, Hkv, D, page, seed=32, spare=2 * need)
+    fresh = free.reshape(2, need).contiguous()
+    w = (torch.rand((2, Hkv, table.shape[1] * page), generator=gen(33), device="cuda") * 5000).floor()      # many equal ones
+    stay = plain_evict(w.cpu(), lengths, budget, recent, sinks)
+    t2, n2, w2, kept = P.paged_evict(k, v, table, n, w, fresh, budget, recent=recent, sinks=sinks)
+    for b, m in enumerate(lengths):
+        at = torch.tensor(stay[b][0], device="cuda")
+        assert torch.equal(kept[b, 0].long(), at) and torch.equal(w2[b, 0, :budget], w[b, 0, at])
+        for pages in (k, v):
+            assert torch.equal(rows_of(pages, t2, b, budget)[0], rows_of(pages, table, b, m)[0, at])
+    assert L.device_status() == 0

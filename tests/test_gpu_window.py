@@ -3,7 +3,8 @@
 Tolerances are bounds, per element.  With u half a step of the type (bf16 2^-8, fp16 2^-11, fp32 2^-24) and all sums in fp32:
   o   = sum p v:    p is rounded where it enters the product, o where it is stored: u (sum p |v| + |o|)
   dv  = sum p g:    the same with g = dO
-  dq  = sum ds k:   ds is rounded, and delta = rowsum(o g) comes from the rounded o: sum (u |ds| + scale p u sum|o||g|) |k| + u |dq|
+  dq  = sum ds k:   ds is rounded, and delta = rowsum(o g) comes from an o that is off by less than u: sum (u |ds| + scale p u sum|o||g|) |k|
+                    + u |dq|
   dk  likewise with q for k
 Each p carries the errors of its score besides: D products summed in fp32 and the exponent's argument, e = (2 D + 64) 2^-24 (1 + X),
 where X is the largest scaled sum of |q||k|, and the polynomial exponentials of the 16-bit kernels, 7.5e-5 (below half a step of either
@@ -290,3 +291,82 @@ def test_lengths_out_of_range_are_held():
     held = torch.tensor([100, 0], dtype=torch.int32, device="cuda")
     for a, b in zip(run(q, k, v, g, 30, 2, lengths=far), run(q, k, v, g, 30, 2, lengths=held)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("cap", [1, 3])
+def test_many_units_per_cta(D, cap):
+    """A few CTAs walk all units, and meet long rows of key tiles that nobody sees."""
+    lengths = torch.tensor([1100, 0, 0, 0, 3, 0, 0, 0, 129, 1], dtype=torch.int32, device="cuda")
+    q, k, v, g = inputs(torch.bfloat16, 10, 2, 1, 1100, 1100, D, 13)
+    want = run(q, k, v, g, 130, 3, lengths=lengths)
+    L.lib().lmk_debug_set_max_ctas(cap)
+    try:
+        got = run(q, k, v, g, 130, 3, lengths=lengths)
+        torch.cuda.synchronize()
+    finally:
+        L.lib().lmk_debug_set_max_ctas(0)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    check(got, *plain(q, k, v, g, 130, 3, D ** -0.5, lengths))
+    assert L.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_no_sequence_has_a_row(dtype):
+    q, k, v, g = inputs(dtype, 3, 4, 2, 300, 420, 64, 14)
+    for n in ([0, 0, 0], [120, 100, 7]):               # every query stands behind its sequence's end
+        lengths = torch.tensor(n, dtype=torch.int32, device="cuda")
+        assert not any(t.any() for t in run(q * float("nan"), k, v, g, 60, 5, lengths=lengths))
+    assert L.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_error_of_the_gradients(dtype):
+    """dQ and dK are rounded twice, as dS and as themselves: by independent errors of the same relative size, sqrt(2) of one rounding's.  What
+    else there is (exponentials, O in 16 bits plus the byte kept of its rest) adds squares below a tenth of that: 1.5 in all."""
+    q, k, v, g = inputs(dtype, 2, 4, 4, 700, 700, 64, 15)
+    want, _ = plain(q, k, v, g, 333, 3, 64 ** -0.5)
+    for i, a in enumerate(run(q, k, v, g, 333, 3)):
+        once = (want[i].to(dtype).double() - want[i]).norm()
+        assert (a.detach().double() - want[i]).norm() <= 1.5 * once, i
+
+
+def test_a_step_replayed_with_other_numbers():
+    sets = [inputs(torch.float16, 2, 4, 2, 600, 600, 64, seed) for seed in (16, 17, 18)]
+    lengths = [torch.tensor(n, dtype=torch.int32, device="cuda") for n in ([600, 600], [0, 77], [599, 300])]
+    want = [[t.detach().clone() for t in run(*x, 100, 9, lengths=n)] for x, n in zip(sets, lengths)]
+    leaves, g, n = [t.clone().requires_grad_(True) for t in sets[0][:3]], sets[0][3].clone(), lengths[0].clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = P.window_attention(*leaves, 100, sinks=9, lengths=n)
+        grads = torch.autograd.grad(o, leaves, g)
+    for i in (0, 1, 2, 1, 0):
+        with torch.no_grad():
+            for to, x in zip((*leaves, g, n), (*sets[i], lengths[i])):
+                to.copy_(x)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip((o, *grads), want[i])), i
+
+
+def test_two_streams_at_once():
+    sets = [inputs(torch.bfloat16, 1, 8, 2, 1500, 1500, 128, seed) for seed in (19, 20)]
+    want = [[t.detach().clone() for t in run(*x, 200, 130)] for x in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(run(*sets[i], 200, 130))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for i in range(2) for r in got[i] for a, b in zip(r, want[i]))
+    assert L.device_status() == 0
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs a second device")
+def test_a_device_that_is_not_current():
+    q, k, v, g = inputs(torch.bfloat16, 1, 4, 2, 300, 300, 64, 21)
+    want = run(q, k, v, g, 100, 3)
+    got = run(*[t.to("cuda:1") for t in (q, k, v, g)], 100, 3)
+    assert all(torch.equal(a, b.to(a.device)) for a, b in zip(want, got))
