@@ -62,7 +62,7 @@ size_t part_bytes(const SinkSplit& s, int B, int Hkv, int D, int kk) {
 }
 void tile_sizes(int dtype, int* qt, int* kk) { *qt = *kk = dtype == LMK_F32 ? 64 : 128; }      // of the dK/dV kernels
 
-// The parts of the split key tiles, added up in the order of their runs.
+// The parts of the sinks, added up in the order of their runs.
 template <typename T>
 __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ WindowParams p, int qt, int kk) {
   ptx::grid_dep_wait();
@@ -72,14 +72,14 @@ __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant_
   const QueryTiles qts = queries_of_keys(tile, qt, kk, p.Lq, p.Lk - p.Lq, len, p.window, p.sinks);
   const int runs = (qts.end - qts.last + p.split.run - 1) / p.split.run;
   const int e = (blockIdx.x * 256 + threadIdx.x) * 4, key = e / p.D, f = e - key * p.D;
-  if (key >= kk || tile * kk + key >= p.Lk) return;
+  if (key >= kk || tile * kk + key >= p.sinks) return;
   const int64_t slot = 2ll * kk * p.D;
   const float* part = p.split.part + ((int64_t)bk * p.split.tiles + tile) * (1 + p.split.runs) * slot + e;
   const int64_t at = ((int64_t)bk * p.Lk + tile * kk + key) * p.D + f;
 #pragma unroll
   for (int g = 0; g < 2; ++g) {                     // dK, dV
     float4 sum = *reinterpret_cast<const float4*>(part + g * (slot / 2));
-    for (int r = 1; r <= runs && tile * kk + key < p.sinks; ++r) {      // (the runs' rows see no other keys)
+    for (int r = 1; r <= runs; ++r) {
       const float4 x = *reinterpret_cast<const float4*>(part + r * slot + g * (slot / 2));
       sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
     }
@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant_
 }  // namespace
 
 int window_join_parts(const WindowParams& p, int qt, int kk, int dtype, cudaStream_t st) {
-  const dim3 grid((kk * p.D / 4 + 255) / 256, p.B * p.Hkv * p.split.tiles);
+  const dim3 grid(((p.sinks < kk ? p.sinks : kk) * p.D / 4 + 255) / 256, p.B * p.Hkv * p.split.tiles);
   if (dtype == LMK_F32) LMK_CUDA(launch_overlapped(window_join_kernel<float>, grid, dim3(256), 0, st, p, qt, kk));
   else if (dtype == LMK_F16) LMK_CUDA(launch_overlapped(window_join_kernel<__half>, grid, dim3(256), 0, st, p, qt, kk));
   else LMK_CUDA(launch_overlapped(window_join_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p, qt, kk));

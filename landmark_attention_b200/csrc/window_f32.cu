@@ -374,12 +374,13 @@ __global__ void __launch_bounds__(kThreads, 1) window_dkv_f32_kernel(const __gri
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
     if (key0 + r >= (run >= 0 ? p.sinks : p.Lk)) continue;               // a run's rows see the sinks alone
-    const int64_t at = split ? (int64_t)(r0 + r) * p.D : ((int64_t)bk * p.Lk + key0 + r) * p.D;
+    const bool sink = split && key0 + r < p.sinks;
+    const int64_t at = sink ? (int64_t)(r0 + r) * p.D : ((int64_t)bk * p.Lk + key0 + r) * p.D;
     float x[kF];
     row_of<kF>(x, dk, r);
-    write_row<kF>((split ? part : (float*)p.dk) + at + lane * kF, x, true);
+    write_row<kF>((sink ? part : (float*)p.dk) + at + lane * kF, x, true);
     row_of<kF>(x, dv, r);
-    write_row<kF>((split ? part + kTile * p.D : (float*)p.dv) + at + lane * kF, x, true);
+    write_row<kF>((sink ? part + kTile * p.D : (float*)p.dv) + at + lane * kF, x, true);
   }
 }
 

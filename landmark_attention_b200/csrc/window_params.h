@@ -7,7 +7,7 @@ namespace lmk {
 
 // dK and dV of the key tiles that hold sinks get contributions from every later query.  Their query tiles are dealt out to several units:
 // the ones that see the tile through the window (as for every key tile), and runs of `run` tiles of the others, at most `runs` of
-// them.  Each unit leaves an fp32 sum, the runs of the sinks' rows alone, and a last kernel adds these up in order.
+// them.  Each unit leaves an fp32 sum for the sinks, and a last kernel adds these up in order; the tile's other keys are the first unit's alone.
 struct SinkSplit {
   int tiles = 0;       // key tiles that hold sinks; 0: no tile is split
   int run = 0, runs = 0;
@@ -84,7 +84,7 @@ int window_f32_bwd(const WindowParams& p, cudaStream_t st);
 int window_sm100_fwd(const WindowParams& p, int dtype, cudaStream_t st);
 int window_sm100_bwd(const WindowParams& p, int dtype, cudaStream_t st);
 bool window_sm100_operand_ok(const void* p, const int64_t st[3], int D);
-// adds up the parts of the split key tiles (kk keys each) into dk and dv
+// adds up the parts of the sinks, in tiles of kk keys, into dk and dv
 int window_join_parts(const WindowParams& p, int qt, int kk, int dtype, cudaStream_t st);
 
 }  // namespace lmk

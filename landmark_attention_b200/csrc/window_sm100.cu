@@ -905,7 +905,9 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         mbar_arrive(smem_u32(&sm->ds_ready));
       }
       // epilogue
-      const int64_t off_r = key < p.Lk ? ((int64_t)bk * p.Lk + key) * p.D : -1;
+      // a run's rows see the sinks alone, and the sinks' sums are joined later
+      const bool sink = split && key < p.sinks;
+      const int64_t off_r = key < p.Lk && !sink ? ((int64_t)bk * p.Lk + key) * p.D : -1;
       int64_t row_off[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) row_off[j] = __shfl_sync(0xffffffffu, off_r, (lane & ~3) + j);
@@ -914,7 +916,6 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       tc_fence_after();
       const uint32_t t_acc = (is_dv ? tmem_dv : tmem_dk) + col0 + lane_base;
       float* const prow = split ? part + ((is_dv ? kPair : 0) + row) * p.D : nullptr;
-      const bool kept = un.base() || key < p.sinks;      // (a run's rows see the sinks alone)
 #pragma unroll
       for (int c = 0; c < kOut / 32; ++c) {
         uint32_t ra[32];
@@ -924,14 +925,14 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
           tc_fence_before();
           mbar_arrive(smem_u32(&sm->acc_empty[acc]));     // the next unit may start accumulating
         }
-        if (split) {
+        if (sink) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
-            if (kept && col0 + c * 32 + e * 4 < p.D)
+            if (col0 + c * 32 + e * 4 < p.D)
               *reinterpret_cast<uint4*>(prow + col0 + c * 32 + e * 4) = make_uint4(ra[4 * e], ra[4 * e + 1], ra[4 * e + 2], ra[4 * e + 3]);
-        } else {
-          store_acc_cols<kBf16>(is_dv ? p.dv : p.dk, row_off, ra, col0 + c * 32, p.D, lane);
         }
+        __syncwarp();
+        if (un.base()) store_acc_cols<kBf16>(is_dv ? p.dv : p.dk, row_off, ra, col0 + c * 32, p.D, lane);
         __syncwarp();
       }
     }
@@ -1339,13 +1340,13 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       const int bk = w / p.n_pairs, tile = w - bk * p.n_pairs;
       const QueryTiles q = queries_of_keys(tile, kQTile, kPair, p.Lq, off, length_of(p.lengths, bk / p.Hkv, p.Lk), p.window, p.sinks);
       if ((tile < p.split.tiles ? q.last : q.end) >= q.first) continue;
-      if (tile < p.split.tiles) {
-        zero_fill(p.split.part + ((int64_t)bk * p.split.tiles + tile) * (1 + p.split.runs) * 2 * kPair * p.D, 2 * kPair * p.D / 4, tid, kBwdWarps * 32);
-      } else {
-        const int64_t at = ((int64_t)bk * p.Lk + tile * kPair) * p.D;
-        const int n = min(kPair, p.Lk - tile * kPair) * p.D / 8;
-        zero_fill(reinterpret_cast<uint16_t*>(p.dk) + at, n, tid, kBwdWarps * 32);
-        zero_fill(reinterpret_cast<uint16_t*>(p.dv) + at, n, tid, kBwdWarps * 32);
+      const int64_t at = ((int64_t)bk * p.Lk + tile * kPair) * p.D;
+      const int n = min(kPair, p.Lk - tile * kPair) * p.D / 8;
+      zero_fill(reinterpret_cast<uint16_t*>(p.dk) + at, n, tid, kBwdWarps * 32);
+      zero_fill(reinterpret_cast<uint16_t*>(p.dv) + at, n, tid, kBwdWarps * 32);
+      if (tile < p.split.tiles) {                    // (whose sinks' sums are joined over these rows)
+        float* const part = p.split.part + ((int64_t)bk * p.split.tiles + tile) * (1 + p.split.runs) * 2 * kPair * p.D;
+        zero_fill(part, 2 * kPair * p.D / 4, tid, kBwdWarps * 32);
       }
     }
     tc_fence_before();
