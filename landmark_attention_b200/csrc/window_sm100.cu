@@ -171,6 +171,7 @@ window_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   auto unit_of = [&](int w) { return row_unit(w, n_tiles, p.BH, p.H, p.lengths, p.Lq, p.Lk, p.window, p.sinks); };
 
   if (tid == 0) {
+    for (const CUtensorMap* tm : {&tm_q, &tm_k, &tm_v}) prefetch_tensormap(tm);
     for (uint64_t* bar : {&sm->q_full, &sm->q_empty, &sm->patch, &sm->o_full, &sm->s_full[0], &sm->s_full[1]}) mbar_init(smem_u32(bar), 1);
     for (uint64_t* bar : {&sm->o_empty, &sm->p_ready[0], &sm->p_ready[1]}) mbar_init(smem_u32(bar), 128);
     for (int s = 0; s < kSlots; ++s) {
@@ -604,6 +605,7 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   };
 
   if (tid == 0) {
+    for (const CUtensorMap* tm : {&tm_q, &tm_k, &tm_v, &tm_do}) prefetch_tensormap(tm);
     for (uint64_t* bar : {&sm->k_full, &sm->k_empty, &sm->v_full, &sm->v_empty, &sm->patch, &sm->s_full, &sm->dp_full})
       mbar_init(smem_u32(bar), 1);
     for (int s = 0; s < kStages; ++s) {
@@ -1049,6 +1051,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   auto unit_of = [&](int w) { return row_unit(w, n_tiles, p.BH, p.H, p.lengths, p.Lq, p.Lk, p.window, p.sinks); };
 
   if (tid == 0) {
+    for (const CUtensorMap* tm : {&tm_q, &tm_k, &tm_v, &tm_do}) prefetch_tensormap(tm);
     for (uint64_t* bar : {&sm->qdo_full, &sm->patch}) mbar_init(smem_u32(bar), 1);
     mbar_init(smem_u32(&sm->ops_ready), 256);
     mbar_init(smem_u32(&sm->ops_free), 1);
@@ -1079,8 +1082,6 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
   const uint32_t tmem = (uint32_t)warp_uniform((int)sm->tmem_base);
   // TMEM: S buffers [0,128), dP buffers [128,256), dQ [256,384), Q rows [384,448), dO rows [448,512)
   const uint32_t tmem_s = tmem, tmem_dp = tmem + 128, tmem_dq = tmem + 256, tmem_q = tmem + 384, tmem_do = tmem + 448;
-  grid_dep_wait();
-  grid_dep_launch();
 
   if (warp == kBwdWarps) {
     // ------------------------------------------------------------------ TMA producer
@@ -1253,6 +1254,9 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       n_lse = ld_behind_wait(p.lse + (int64_t)(w % p.BH) * p.Lq + rr);
       n_delta = ld_behind_wait(p.delta + (int64_t)(w % p.BH) * p.Lq + rr);
     };
+    // delta comes from the kernel in front, what else is read was complete before that one's first CTA was behind its wait
+    grid_dep_wait();
+    grid_dep_launch();
     fetch_rows(unit_at(0));
     for (int r = 0, w = unit_at(0); w < n_units; w = unit_at(++r)) {
       const RowUnit un = unit_of(w);
