@@ -6,9 +6,10 @@
 // unit that owns the keys; no atomics.  Rows behind a sequence's end are read as zeros, whatever they hold.
 // A 16-byte read of 32 different places takes the shared memory 4 cycles, of one place 1.  A warp's eight rows are the same for all its lanes,
 // which hold the columns: 64 multiply-adds a lane, issued as 32 pairs, cost 16 cycles of reads (with 4 x 4 results a thread 32, and
-// the reads were the bound: B2 H16 Hkv8 L2048 D128, window 512, forward and backward 3040 -> 2360 us, 22 of 74 TFLOP/s).  The tiles lie as
-// in memory, two of each on their way; P and dS go to the second product through a buffer of the warp's own.  What is left is latency: two
-// to four warps a scheduler, with a third of the cycles issuing (sixteen warps of four rows: 2650 us).
+// the reads were the bound: B2 H16 Hkv8 L2048 D128, window 512, forward and backward 3040 -> 2195 us, 24 of 74 TFLOP/s).  The tiles lie as
+// in memory, two of each on their way; P and dS go to the second product through a buffer of the warp's own.  The products are unrolled
+// whole (by two: 2360 us), so that reads run ahead of their multiply-adds.  What is left is latency: two to four warps a scheduler, with
+// two fifths of the cycles issuing.  (Sixteen warps of four rows 2650 us; tiles that need no mask told apart: no difference.)
 #include "common.cuh"
 #include "window_params.h"
 #include "sm100_ptx.cuh"
@@ -48,7 +49,7 @@ __device__ __forceinline__ void product(float (&d)[kRows][2], const float* a, co
   uint64_t sum[kRows][2];
 #pragma unroll
   for (int r = 0; r < kRows; ++r) sum[r][0] = sum[r][1] = 0ull;
-#pragma unroll 2
+#pragma unroll 16
   for (int c = 0; c < kD; c += 4) {
     uint64_t x[kRows][2], y[2][2];
     read4(y[0], b + lane * kStride<kD> + c);
@@ -76,7 +77,7 @@ __device__ __forceinline__ void product(float (&d)[kRows][2], const float* a, co
 template <int kD>
 __device__ __forceinline__ void accumulate(uint64_t (&d)[kRows / 2][kD / 32], const float* w, const float* b, int lane) {
   constexpr int kF = kD / 32;
-#pragma unroll 2
+#pragma unroll
   for (int n = 0; n < kTile; n += 2) {
     uint64_t x[2][kRows / 2];
     float y[2][kF];
@@ -139,11 +140,7 @@ __device__ __forceinline__ float warp_sum(float x) {
   return x;
 }
 __device__ __forceinline__ float warp_max_nan(float x) {      // NaN where a lane has one
-#pragma unroll
-  for (int w = 16; w > 0; w >>= 1) {
-    const float y = __shfl_xor_sync(0xffffffffu, x, w);
-    x = max3_nan(x, y, y);
-  }
+  asm volatile("redux.sync.max.NaN.f32 %0, %0, 0xffffffff;" : "+f"(x));
   return x;
 }
 __device__ __forceinline__ int length_of(const WindowParams& p, int b) {
