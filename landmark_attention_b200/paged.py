@@ -86,7 +86,11 @@ class PagedKVCache:
 
     def append(self, k, v, counts=None):
         """Store k, v [B,Hkv,T,D] behind the cached tokens; counts: how many of the T rows each sequence has (a list), for ragged prompts."""
+        if counts is not None and self.table.is_cuda and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("append with counts cannot be captured: paged_append takes them from the device")
         n = [k.shape[2]] * len(self._tokens) if counts is None else [min(max(int(c), 0), k.shape[2]) for c in counts]
+        if len(n) != len(self._tokens):
+            raise ValueError(f"expected one count for each of {len(self._tokens)} sequences")
         self.reserve(n)
         on_device = None if counts is None else torch.tensor(n, dtype=torch.int32, device=self.table.device)
         paged_append(k, v, self.k_pages, self.v_pages, self.table, self.lengths, on_device, self.weights)

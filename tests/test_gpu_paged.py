@@ -451,3 +451,19 @@ def test_eviction_from_a_very_long_sequence():
         for pages in (k, v):
             assert torch.equal(rows_of(pages, t2, b, budget)[0], rows_of(pages, table, b, m)[0, at])
     assert L.device_status() == 0
+
+
+def test_what_a_captured_step_cannot_do_is_refused():
+    cache = P.PagedKVCache(2, 2, 64, torch.float16, "cuda", max_tokens=64, page=16, track_weights=True)
+    k = torch.randn((2, 2, 5, 64), generator=gen(34), device="cuda").half()
+    cache.append(k, k, [5, 2])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x = torch.zeros(1, device="cuda") + 1
+        for refused in (lambda: cache.append(k, k, [1, 1]), lambda: cache.reserve(40), lambda: cache.evict(3)):
+            with pytest.raises(RuntimeError):
+                refused()
+    graph.replay()
+    assert x.item() == 1 and cache.refresh() == [5, 2]
+    with pytest.raises(ValueError):
+        cache.append(k, k, [1])
