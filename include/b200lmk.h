@@ -490,7 +490,7 @@ int lmk_cached_rows(const void* q, const void* k, const void* v, const int64_t q
  * (p - j < window or j < sinks), and, with lengths [B] (int32, nullable), p < lengths[b]: a right-padded batch, whose rows behind a
  * sequence's end give zeros and take no part in any gradient, whatever they hold.
  *   q [B,H,Lq,D], k, v [B,Hkv,Lk,D] with H a multiple of Hkv (head h reads key head h / (H / Hkv)), strided; o [B,H,Lq,D] dense; lse
- *   [B*H, Lq] fp32: log2 of the row's normaliser (+inf where a row sees nothing).  D a multiple of 8 up to 128, Lk >= Lq, sm_scale > 0.
+ *   [B*H, Lq] fp32 (nullable forward): log2 of the row's normaliser (+inf where a row sees nothing).  D a multiple of 8 up to 128, Lk >= Lq, sm_scale > 0.
  *   o_rest (16-bit types, nullable; null in fp32): what the rounding of o left, a byte a number, for the backward pass.
  *   Backward: o, o_rest (16-bit types), dQ [B,H,Lq,D], dK, dV [B,Hkv,Lk,D] dense, dO strided; workspace of
  *   lmk_window_bwd_workspace(...) bytes, 256-byte aligned, contents irrelevant.  dK and dV are sums over the heads that share them;
@@ -519,6 +519,7 @@ int lmk_window_bwd(const void* q, const void* k, const void* v, const void* o, c
  * or p - j < window or j < sinks); o [B,H,T,D] dense, zeros where nothing is visible.  weights (nullable) [B, Hkv, max_pages *
  * page] fp32: weights = decay * weights + the sum of the key's attention weights over the T queries of the heads that share it, for
  * every j < lengths[b]; decay 0 does not read what stood there.
+ * workspace: lmk_paged_attend_workspace(...) bytes, 256-byte aligned (null where that is 0), contents irrelevant.
  *
  * lmk_paged_evict: sequences of more than `budget` tokens keep the first `sinks`, the last `recent` and the budget - sinks - recent of
  * the rest with the largest weights (the lower index first where they are equal; NaN is the largest), per key head, in order, copied to

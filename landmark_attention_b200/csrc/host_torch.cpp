@@ -919,9 +919,10 @@ Tensor window_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
   const auto B = q.size(0), H = q.size(1), Lq = q.size(2), D = q.size(3), Hkv = k.size(1), Lk = k.size(2);
   Tensor o = empty_like_dtype({B, H, Lq, D}, q);
   if (rest != nullptr && q.scalar_type() != at::kFloat) *rest = at::empty({B, H, Lq, D}, q.options().requires_grad(false).dtype(at::kByte));
-  *lse = empty_f32({B * H, Lq}, q);
+  if (lse != nullptr) *lse = empty_f32({B * H, Lq}, q);
   check(lib.lmk_window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(),
-                           rest != nullptr && rest->defined() ? rest->data_ptr() : nullptr, lse->data_ptr<float>(), i32_ptr(lengths), B, H, Hkv, Lq, Lk, D,
+                           rest != nullptr && rest->defined() ? rest->data_ptr() : nullptr, lse != nullptr ? lse->data_ptr<float>() : nullptr,
+                           i32_ptr(lengths), B, H, Hkv, Lq, Lk, D,
                            S3(q).v, S3(k).v, S3(v).v, window, sinks, (float)scale, dtype_code(q), stream_of(q)),
         "lmk_window_fwd");
   return o;
@@ -991,10 +992,7 @@ Tensor window_attention(const Tensor& q_, const Tensor& k_, const Tensor& v_, co
   Tensor q = q_, k = k_, v = v_;
   for (Tensor* t : {&q, &k, &v})
     if (!window_rows(*t)) *t = t->clone(at::MemoryFormat::Contiguous);        // part of the graph where a gradient is wanted
-  if (!needs_grad({q, k, v})) {
-    Tensor lse;
-    return window_fwd(q, k, v, lengths, window, sinks, scale, &lse, nullptr);
-  }
+  if (!needs_grad({q, k, v})) return window_fwd(q, k, v, lengths, window, sinks, scale, nullptr, nullptr);
   if (at::GradMode::is_enabled() && c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None)
     for (const Tensor* t : {&q_, &k_, &v_}) check_capture(*t);
   return WindowAttention::apply(q, k, v, lengths.defined() ? std::optional<Tensor>(lengths) : std::nullopt, window, sinks, scale);
@@ -1046,10 +1044,11 @@ Tensor paged_attention(const Tensor& q_, const Tensor& k, const Tensor& v, const
   const auto H = q.size(1), T = q.size(2);
   LMK_ASSERT(p.Hkv > 0 && H % p.Hkv == 0, "query heads must be a multiple of the cache's heads");
   Tensor o = empty_like_dtype({p.B, H, T, p.D}, q);
-  const size_t need = std::max<size_t>(lib.lmk_paged_attend_workspace(p.B, H, p.Hkv, fits_int(T, "T"), p.D, p.page, p.max_pages, w != nullptr, p.code), 256);
-  Tensor ws = at::empty({(int64_t)need}, q.options().requires_grad(false).dtype(at::kByte));
+  const size_t need = lib.lmk_paged_attend_workspace(p.B, H, p.Hkv, fits_int(T, "T"), p.D, p.page, p.max_pages, w != nullptr, p.code);
+  Tensor ws;                                             // short tables without weights need none
+  if (need > 0) ws = at::empty({(int64_t)need}, q.options().requires_grad(false).dtype(at::kByte));
   check(lib.lmk_paged_attend(q.data_ptr(), S3(q).v, k.data_ptr(), v.data_ptr(), p.ks.v, p.vs.v, i32_ptr(table), i32_ptr(lengths), o.data_ptr(),
-                             w, (float)decay, ws.data_ptr(), need, p.B, H, p.Hkv, T, p.D, p.page, p.n_pages, p.max_pages,
+                             w, (float)decay, need > 0 ? ws.data_ptr() : nullptr, need, p.B, H, p.Hkv, T, p.D, p.page, p.n_pages, p.max_pages,
                              fits_int(window, "window"), fits_int(sinks, "sinks"), (float)scale, p.code, stream_of(q)),
         "lmk_paged_attend");
   return o;

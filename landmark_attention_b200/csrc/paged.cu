@@ -1014,6 +1014,7 @@ constexpr int kWholeSteps = 32;
 
 struct AttendPlan {
   int grid, rows, tiles, kD;
+  bool one_piece;
   size_t acc, stat, whole, scores, bytes;
 };
 int attend_plan(AttendPlan* p, int B, int H, int Hkv, int T, int D, int page, int max_pages, bool weights, int dtype) {
@@ -1024,9 +1025,11 @@ int attend_plan(AttendPlan* p, int B, int H, int Hkv, int T, int D, int page, in
   p->tiles = (p->rows + kRowTile - 1) / kRowTile;
   p->kD = D <= 64 ? 64 : 128;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  p->one_piece = (int64_t)max_pages * page <= kWholeSteps * kStep;
+  const size_t pieces = p->one_piece ? 0 : (size_t)2 * p->grid * kRowTile;
   p->acc = 0;
-  p->stat = up(p->acc + sizeof(float) * 2 * p->grid * kRowTile * p->kD);
-  p->whole = up(p->stat + sizeof(float2) * 2 * p->grid * kRowTile);
+  p->stat = up(p->acc + sizeof(float) * pieces * p->kD);
+  p->whole = up(p->stat + sizeof(float2) * pieces);
   p->scores = up(p->whole + (weights ? sizeof(float2) * B * Hkv * (size_t)p->tiles * kRowTile : 0));
   p->bytes = up(p->scores + (weights ? sizeof(float) * (size_t)B * Hkv * p->rows * max_pages * page : 0));
   return LMK_OK;
@@ -1112,7 +1115,7 @@ extern "C" int lmk_paged_attend(const void* q, const int64_t q_strides[3], const
   LMK_CHECK_ARG(((uintptr_t)o & 15) == 0, "paged attention: o must start on a 16-byte boundary");
   AttendPlan p;
   if ((rc = attend_plan(&p, B, H, Hkv, T, D, page, max_pages, weights != nullptr, dtype)) != LMK_OK) return rc;
-  if (workspace == nullptr || workspace_bytes < p.bytes || ((uintptr_t)workspace & 255) != 0)
+  if (p.bytes > 0 && (workspace == nullptr || workspace_bytes < p.bytes || ((uintptr_t)workspace & 255) != 0))
     return fail(LMK_ERR_WORKSPACE, "paged attention: workspace of %zu bytes on a 256-byte boundary needed", p.bytes);
   if ((rc = status_of(a.pg)) != LMK_OK) return rc;
   a.q = q; a.o = o;
@@ -1125,7 +1128,7 @@ extern "C" int lmk_paged_attend(const void* q, const int64_t q_strides[3], const
   a.scores = reinterpret_cast<float*>(ws + p.scores);
   a.H = H; a.T = T; a.G = H / Hkv; a.rows = p.rows; a.tiles = p.tiles; a.window = window; a.sinks = window > 0 ? sinks : 0; a.grid = p.grid;
   a.least = kLeastSteps;
-  a.one_piece = (int64_t)max_pages * page <= kWholeSteps * kStep;
+  a.one_piece = p.one_piece;
   a.scale_log2 = sm_scale * kLog2e;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == LMK_BF16) return dispatch_attend<__nv_bfloat16>(a, p.kD, dtype, st);

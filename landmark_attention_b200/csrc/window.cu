@@ -9,9 +9,9 @@ namespace {
 constexpr size_t kNextBytes = 256;
 constexpr size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-int check_window(const void* q, const void* k, const void* v, const float* lse, int B, int H, int Hkv, int Lq, int Lk, int D,
+int check_window(const void* q, const void* k, const void* v, int B, int H, int Hkv, int Lq, int Lk, int D,
                  const int64_t* qs, const int64_t* ks, const int64_t* vs, int window, int sinks, float scale, int dtype) {
-  LMK_CHECK_ARG(q && k && v && lse, "window attention: q, k, v or lse is null");
+  LMK_CHECK_ARG(q && k && v, "window attention: q, k or v is null");
   LMK_CHECK_ARG(qs && ks && vs, "window attention: stride arrays are required");
   LMK_CHECK_ARG(B >= 1 && H >= 1 && Hkv >= 1 && Lq >= 1 && Lk >= 1, "window attention: empty problem (B=%d H=%d Hkv=%d Lq=%d Lk=%d)", B, H, Hkv, Lq, Lk);
   LMK_CHECK_ARG(H % Hkv == 0, "window attention: %d query heads are not a multiple of %d key heads", H, Hkv);
@@ -108,10 +108,10 @@ using namespace lmk;
 extern "C" int lmk_window_fwd(const void* q, const void* k, const void* v, void* o, void* o_rest, float* lse, const int32_t* lengths, int B,
                               int H, int Hkv, int Lq, int Lk, int D, const int64_t q_strides[3], const int64_t k_strides[3],
                               const int64_t v_strides[3], int window, int sinks, float sm_scale, int dtype, void* stream) {
-  int rc = check_window(q, k, v, lse, B, H, Hkv, Lq, Lk, D, q_strides, k_strides, v_strides, window, sinks, sm_scale, dtype);
+  int rc = check_window(q, k, v, B, H, Hkv, Lq, Lk, D, q_strides, k_strides, v_strides, window, sinks, sm_scale, dtype);
   if (rc != LMK_OK) return rc;
   LMK_CHECK_ARG(o != nullptr, "window attention: o is null");
-  LMK_CHECK_ARG(o_rest == nullptr || dtype != LMK_F32, "window attention: o_rest is for 16-bit types");
+  LMK_CHECK_ARG(o_rest == nullptr || (dtype != LMK_F32 && lse != nullptr), "window attention: o_rest is for 16-bit types, beside lse");
   LMK_CHECK_ARG((((uintptr_t)o | (uintptr_t)o_rest) & 15) == 0, "window attention: o and o_rest must start on 16-byte boundaries");
   WindowParams p = {};
   fill(p, q, k, v, lengths, B, H, Hkv, Lq, Lk, D, q_strides, k_strides, v_strides, window, sinks, sm_scale);
@@ -138,9 +138,9 @@ extern "C" int lmk_window_bwd(const void* q, const void* k, const void* v, const
                               int Hkv, int Lq, int Lk, int D, const int64_t q_strides[3], const int64_t k_strides[3],
                               const int64_t v_strides[3], const int64_t do_strides[3], int window, int sinks, float sm_scale, int dtype,
                               void* stream) {
-  int rc = check_window(q, k, v, lse, B, H, Hkv, Lq, Lk, D, q_strides, k_strides, v_strides, window, sinks, sm_scale, dtype);
+  int rc = check_window(q, k, v, B, H, Hkv, Lq, Lk, D, q_strides, k_strides, v_strides, window, sinks, sm_scale, dtype);
   if (rc != LMK_OK) return rc;
-  LMK_CHECK_ARG(o && dO && dQ && dK && dV && do_strides, "window attention backward: o, dO or a gradient is null");
+  LMK_CHECK_ARG(o && lse && dO && dQ && dK && dV && do_strides, "window attention backward: o, lse, dO or a gradient is null");
   LMK_CHECK_ARG((o_rest != nullptr) == (dtype != LMK_F32), "window attention backward: 16-bit types need o_rest, fp32 has none");
   LMK_CHECK_ARG((((uintptr_t)o | (uintptr_t)o_rest | (uintptr_t)dQ | (uintptr_t)dK | (uintptr_t)dV) & 15) == 0,
                 "window attention backward: o, o_rest and the gradients must start on 16-byte boundaries");

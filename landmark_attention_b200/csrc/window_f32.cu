@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, kD == 64 ? 2 : 1) window_fwd_f32_ker
 #pragma unroll
     for (int f = 0; f < kF; ++f) x[f] *= inv;
     if (lane * kF < p.D) write_row<kF>((float*)p.o + at * p.D + lane * kF, x, sum != 0.f);
-    if (lane == 0) p.lse[at] = sum == 0.f ? INFINITY : m[r] + log2f(sum);
+    if (lane == 0 && p.lse != nullptr) p.lse[at] = sum == 0.f ? INFINITY : m[r] + log2f(sum);
   }
 }
 

@@ -18,7 +18,7 @@ struct WindowParams {
   const void *q, *k, *v, *dO;
   void* o;                     // forward output / backward input
   void* rest;                  // what the rounding of o left, a byte a number (16-bit types; null: not wanted)
-  float* lse;                  // [B*H, Lq]: log2 of the row's normaliser, +inf for a row that sees nothing
+  float* lse;                  // [B*H, Lq]: log2 of the row's normaliser, +inf for a row that sees nothing (null: not wanted)
   const int* lengths;          // [B] or null
   void *dq, *dk, *dv;
   float* delta;                // [B*H, Lq] scratch (backward)

@@ -294,7 +294,7 @@ window_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         const int64_t at = ((int64_t)u.bh * p.Lq + u.t * kQTile) * p.D;
         const int n = min(kQTile, p.Lq - u.t * kQTile) * p.D / 8;
         zero_fill(reinterpret_cast<uint16_t*>(p.o) + at, n, tid, 128);      // (its rest is not read)
-        if (stored) p.lse[(int64_t)u.bh * p.Lq + grow] = INFINITY;
+        if (stored && p.lse != nullptr) p.lse[(int64_t)u.bh * p.Lq + grow] = INFINITY;
         __syncwarp();
         continue;
       }
@@ -429,7 +429,7 @@ window_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         }
         __syncwarp();
       }
-      if (stored) p.lse[(int64_t)u.bh * p.Lq + grow] = valid ? m2 + __log2f(l) : INFINITY;
+      if (stored && p.lse != nullptr) p.lse[(int64_t)u.bh * p.Lq + grow] = valid ? m2 + __log2f(l) : INFINITY;
       __syncwarp();
     }
     tc_fence_before();
