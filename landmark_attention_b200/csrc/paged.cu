@@ -265,8 +265,8 @@ template <int kD> struct Rows32 {
 // (registers are only held down where four CTAs are to fit; 128 features then leave room for the next kernel's first CTAs)
 template <typename T, int kD, int kWarps> constexpr int kAttendPerSm = kWarps == 4 && kD == 64 && sizeof(T) == 2 ? 4 : 1;
 template <typename T, int kD, int kWarps>
-__global__ void __launch_bounds__(kWarps * 32, kAttendPerSm<T, kD, kWarps>) paged_attend_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                                                                   const __grid_constant__ AttendArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, kAttendPerSm<T, kD, kWarps>)
+paged_attend_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ AttendArgs a) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ float2 s_stat[kWarps][kRowTile];
   __shared__ int s_free[kWarps];
