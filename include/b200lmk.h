@@ -4,7 +4,7 @@
  * Conventions
  *   - Every pointer is a DEVICE pointer owned by the caller unless stated otherwise; the library
  *     never allocates or frees device memory.  What it keeps between calls: a per-thread error string,
- *     a per-device status word (lmk_device_status), a host-side table of encoded TMA descriptors keyed
+ *     two per-device status words (lmk_device_status), a host-side table of encoded TMA descriptors keyed
  *     by (pointer, shape, strides), and the fixed scratch array of lmk_attn_bwd_static.
  *   - Calls are asynchronous: they return once the kernels are queued on `stream`.
  *   - Tensors are row-major with a contiguous last dimension.  q/k/v take explicit element strides
@@ -37,7 +37,7 @@ enum {
   LMK_ERR_UNSUPPORTED = -2, /* valid request that no kernel in this build covers */
   LMK_ERR_CUDA = -3,        /* a CUDA runtime or driver call failed */
   LMK_ERR_WORKSPACE = -4,   /* workspace missing or too small */
-  LMK_ERR_DEVICE = -5       /* returned by lmk_device_status only: a bounded wait expired inside an earlier kernel */
+  LMK_ERR_DEVICE = -5       /* returned by lmk_device_status only: it has a code to report */
 };
 
 /* Kernel family selection for the fused attention entry points. */
@@ -51,11 +51,14 @@ int lmk_version(void);
 const char* lmk_last_error(void);
 
 /*
- * Device-side status word of the current device.  Every wait inside the tcgen05 kernels is bounded; a wait that
- * expires records a site code (> 0) here instead of hanging, and the kernel runs to its end with undefined results.
+ * Device-side status of the current device, in two words.  Every wait inside the tcgen05 kernels is bounded; a wait that
+ * expires records a site code (> 0) instead of hanging, and the kernel runs to its end with undefined results.  Conditions that a
+ * kernel meets in its arguments on the device (431 and 501: rows with too many landmarks, 601 and 602: the paged cache) are noted
+ * apart from these and concern the noting call alone.  Each word keeps the first code until it is cleared.
  * The compute entry points cannot see this (they return before their kernels run), so a caller that wants to know
- * polls this function after the work: it synchronises the device, writes the code (0 = healthy) to *status (nullable),
- * clears it when `clear` != 0, and returns LMK_ERR_DEVICE when the code is non-zero.  No counterpart in the reference.
+ * polls this function after the work: it synchronises the device, writes the code (0 = healthy; an expired wait before a
+ * condition, which then is reported by the next call) to *status (nullable), clears what it reports when `clear` != 0, and returns
+ * LMK_ERR_DEVICE when the code is non-zero.  No counterpart in the reference.
  */
 int lmk_device_status(int* status, int clear);
 
@@ -158,7 +161,7 @@ int lmk_attn_bwd_static(const void* q, const void* k, const void* v, const void*
  *     outer softmax and of every closed landmark group).
  *   max_groups: upper bound on the number of landmarks before any query (the reference's max_mem_cnt - 1,
  *     landmark.py:88-119); lmk_attn_mask_supported returns the largest value this build accepts (0: shape not
- *     supported).  A row with more landmarks sets the device status word (lmk_device_status) and gets undefined output.
+ *     supported).  A row with more landmarks notes condition 431 (lmk_device_status) and gets undefined output.
  *   Shape contract: bf16/fp16, D = 128, Lq a multiple of 128, Lk and Lk - Lq multiples of 64, Lk <= 32768.
  */
 int lmk_attn_mask_supported(int B, int H, int Lq, int Lk, int D, int dtype);
@@ -200,7 +203,7 @@ int lmk_attn_mask_bwd_strided(const void* q, const void* k, const void* v, const
  *     (slot g = probability of the landmark closing group g, last slot = total last-section probability).
  *   guards != 0 selects the lm_benchmark flavour (all -inf group -> 0 instead of NaN).
  *   max_groups: upper bound on 1 + number of landmarks in any row (<= 2048); a row with max_groups or more
- *     landmarks records 501 in the device status word (lmk_device_status) and its surplus groups get probability 0.
+ *     landmarks notes condition 501 (lmk_device_status) and its surplus groups get probability 0.
  */
 int lmk_grouped_softmax_fwd(const void* x, const int64_t x_strides[3],
                             const uint8_t* is_mem, const int64_t is_mem_strides[4],

@@ -187,7 +187,8 @@ def on_host_load(fn):
 
 
 def device_status(clear: bool = True) -> int:
-    """Status word of the current device (0 = healthy); a non-zero value names the bounded wait that expired."""
+    """Status of the current device (0 = healthy): the bounded wait that expired or, if none did, the condition (431, 501, 601, 602) that a
+    kernel noted.  Waits for the device; with `clear`, what is reported is cleared."""
     v = c_int(0)
     rc = lib().lmk_device_status(ctypes.byref(v), int(clear))
     if rc != LMK_ERR_DEVICE:          # LMK_ERR_DEVICE only says that the word is non-zero; the caller gets the value

@@ -122,10 +122,11 @@ extern "C" const char* lmk_last_error(void) { return error_buffer(); }
 
 extern "C" int lmk_device_status(int* status, int clear) {
   int v = 0;
-  const int rc = device_status(&v, clear);
+  bool expired = false;
+  const int rc = device_status(&v, &expired, clear);
   if (status) *status = v;
   if (rc != LMK_OK) return rc;
-  if (v != 0) return fail(LMK_ERR_DEVICE, "a bounded wait expired inside a kernel (site %d)", v);
+  if (v != 0) return fail(LMK_ERR_DEVICE, expired ? "a bounded wait expired inside a kernel (site %d)" : "a kernel met condition %d in its arguments", v);
   return LMK_OK;
 }
 

@@ -278,7 +278,7 @@ __device__ __forceinline__ void mask_fwd_tile(const CUtensorMap& tm_q, const CUt
     const int kd = pos / kKT, jl_own = pos % kKT;
     // landmarks strictly before the row's own position = number of closed groups the row sees
     const int c_row = gbase[kd] + __popcll(kmask[kd] & ((1ull << jl_own) - 1ull));
-    if (c_row > G) atomicCAS(status, 0, kErrMaskGroups);
+    if (c_row > G) note_condition(status, kErrMaskGroups);
     const uint32_t lane_base = (uint32_t)(warp * 32) << 16;
     Online grp, outer;
     grp.reset();

@@ -48,7 +48,7 @@ int attn_sm100_flags_bwd(const AttnParams& p, const uint8_t* flags, int64_t stri
                          cudaStream_t st);
 size_t attn_sm100_plan_bytes(int B);
 int attn_sm100_plan_stride();
-int device_status(int* out, int clear);
+int device_status(int* out, bool* expired, int clear);
 int* device_status_word();
 
 // TMA descriptor of a [B, H, L, 128] 16-bit tensor with element strides {batch, head, row}: box = 64 features x

@@ -39,7 +39,7 @@
 
 namespace lmk {
 
-__device__ int g_lmk_status = 0;   // first bounded wait that expired (0 = none); see lmk_device_status()
+__device__ int g_lmk_status[2];   // the status words, see common.cuh and lmk_device_status()
 
 
 namespace {
@@ -343,7 +343,7 @@ sm100_fwd2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
           tma_load_4d(q_tile(w) + c * kTileBytes, &tm_q, qb, 64 * c, (t_a + w) * kQTile, h, b);
       for (int i = 0; i < total; ++i) {
         const int s = i % kStages;
-        mbar_wait(smem_u32(&sm->empty[s]), ((i / kStages) & 1) ^ 1, &g_lmk_status, kErrFwd2Producer);
+        mbar_wait(smem_u32(&sm->empty[s]), ((i / kStages) & 1) ^ 1, g_lmk_status, kErrFwd2Producer);
         const uint32_t fb = smem_u32(&sm->full[s]);
         if (kIrr && i < n_lm_tiles) continue;           // the softmax warps gather the landmark keys themselves
         if (i < n_lm_tiles) {
@@ -368,20 +368,20 @@ sm100_fwd2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     // softmax of the current one.
     constexpr uint32_t fmt = kBf16 ? 1u : 0u;
     constexpr uint32_t idesc_s = instr_desc_f16(fmt, 128, 64, 0, 0);
-    mbar_wait(smem_u32(&sm->q_full), 0, &g_lmk_status, kErrFwd2Mma);
+    mbar_wait(smem_u32(&sm->q_full), 0, g_lmk_status, kErrFwd2Mma);
     const uint64_t dq0 = smem_desc_sw128(q_tile(0), 16, 1024);
     const uint64_t dk0 = smem_desc_sw128(k_slot(0), 16, 1024);
     int ks[2] = {0, 0};
     int s = 0;
     uint32_t ph = 0;
     for (int j = 0; j < total; ++j) {
-      mbar_wait(smem_u32(&sm->full[s]), ph, &g_lmk_status, kErrFwd2Mma);
+      mbar_wait(smem_u32(&sm->full[s]), ph, g_lmk_status, kErrFwd2Mma);
       const uint64_t dk = desc_advance(dk0, (uint32_t)s * 32768u);
 #pragma unroll
       for (int w = 0; w < kTiles; ++w) {
         if (!active(w, j)) continue;
         const int k = ks[w]++, sb = k & 1;
-        if (k >= 2) mbar_wait(smem_u32(&sm->s_free[w][sb]), ((k >> 1) & 1) ^ 1, &g_lmk_status, kErrFwd2Mma);
+        if (k >= 2) mbar_wait(smem_u32(&sm->s_free[w][sb]), ((k >> 1) & 1) ^ 1, g_lmk_status, kErrFwd2Mma);
         tc_fence_after();
         const uint64_t dq = desc_advance(dq0, (uint32_t)w * 32768u);
         if (elect_one()) {
@@ -409,7 +409,7 @@ sm100_fwd2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       for (int w = 0; w < kTiles; ++w) {
         if (!active(w, i)) continue;
         const int k = kp[w]++;
-        mbar_wait(smem_u32(&sm->p_ready[w][k & 1]), (k >> 1) & 1, &g_lmk_status, kErrFwd2Mma);
+        mbar_wait(smem_u32(&sm->p_ready[w][k & 1]), (k >> 1) & 1, g_lmk_status, kErrFwd2Mma);
         tc_fence_after();
         if (i >= n_lm_tiles) {
           // A = P straight from TMEM: the softmax threads wrote it over the first 32 columns of the S buffer it was
@@ -468,7 +468,7 @@ sm100_fwd2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
     for (int i = 0; i < total; ++i) {
       if (!active(w, i)) continue;
       const int sb = k & 1;
-      mbar_wait(smem_u32(&sm->s_full[w][sb]), (k / 2) & 1, &g_lmk_status, kErrFwd2Softmax);
+      mbar_wait(smem_u32(&sm->s_full[w][sb]), (k / 2) & 1, g_lmk_status, kErrFwd2Softmax);
       tc_fence_after();
       if (kIrr) __syncwarp();
       float sv[64];
@@ -575,7 +575,7 @@ sm100_fwd2_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constan
       ++k;
     }
     // ------------------------------------------------------------------ epilogue
-    mbar_wait(smem_u32(&sm->o_full), 0, &g_lmk_status, kErrFwd2Epilogue);
+    mbar_wait(smem_u32(&sm->o_full), 0, g_lmk_status, kErrFwd2Epilogue);
     tc_fence_after();
     const float inv = kIrr && l == 0.f ? 0.f : 1.f / l;
     const int grow = (t_a + w) * kQTile + row;
@@ -913,7 +913,7 @@ sm100_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         }
         auto load_pair = [&](uint32_t dst, const CUtensorMap* tm, uint64_t* full, uint64_t* empty) {
           const uint32_t fb = smem_u32(full);
-          mbar_wait(smem_u32(empty), (u & 1) ^ 1, &g_lmk_status, kErrDkvProducer);
+          mbar_wait(smem_u32(empty), (u & 1) ^ 1, g_lmk_status, kErrDkvProducer);
           mbar_arrive_expect_tx(fb, kOperand);
           for (int g = 0; g < 2; ++g)
             for (int c = 0; c < kD / 64; ++c)
@@ -921,7 +921,7 @@ sm100_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         };
         auto load_rows = [&](uint32_t dst, const CUtensorMap* tm, uint64_t* full, uint64_t* empty, int tile) {
           const uint32_t fb = smem_u32(full);
-          mbar_wait(smem_u32(empty), ((it / kStages) & 1) ^ 1, &g_lmk_status, kErrDkvProducer);
+          mbar_wait(smem_u32(empty), ((it / kStages) & 1) ^ 1, g_lmk_status, kErrDkvProducer);
           mbar_arrive_expect_tx(fb, kOperand);
           for (int c = 0; c < kD / 64; ++c) tma_load_4d(dst + c * kTileBytes, tm, fb, 64 * c, tile * kQTile, h, b);
         };
@@ -947,12 +947,12 @@ sm100_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     for (int r = 0, w = unit_of(0); w < n_units; w = unit_of(++r)) {
       if (warp_uniform(skipped(w))) continue;
       const int n_items = n_tiles - warp_uniform(unit_tq0(w));
-      mbar_wait(smem_u32(&sm->k_full), u & 1, &g_lmk_status, kErrDkvMma);
+      mbar_wait(smem_u32(&sm->k_full), u & 1, g_lmk_status, kErrDkvMma);
       for (int i = 0; i < n_items; ++i, ++it) {
         const int s = it % kStages;
         const uint64_t dq = desc_advance(dq0, (uint32_t)s * 2 * kOperand), ddo = desc_advance(ddo0, (uint32_t)s * 2 * kOperand);
-        mbar_wait(smem_u32(&sm->q_full[s]), (it / kStages) & 1, &g_lmk_status, kErrDkvMma);
-        if (it >= 1) mbar_wait(smem_u32(&sm->s_free), (it & 1) ^ 1, &g_lmk_status, kErrDkvMma);
+        mbar_wait(smem_u32(&sm->q_full[s]), (it / kStages) & 1, g_lmk_status, kErrDkvMma);
+        if (it >= 1) mbar_wait(smem_u32(&sm->s_free), (it & 1) ^ 1, g_lmk_status, kErrDkvMma);
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
@@ -962,9 +962,9 @@ sm100_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           mma_commit(smem_u32(&sm->s_full));
           if (i == n_items - 1) mma_commit(smem_u32(&sm->k_empty));
         }
-        if (i == 0) mbar_wait(smem_u32(&sm->v_full), u & 1, &g_lmk_status, kErrDkvMma);
-        mbar_wait(smem_u32(&sm->do_full[s]), (it / kStages) & 1, &g_lmk_status, kErrDkvMma);
-        if (it >= 1) mbar_wait(smem_u32(&sm->dp_free), (it & 1) ^ 1, &g_lmk_status, kErrDkvMma);
+        if (i == 0) mbar_wait(smem_u32(&sm->v_full), u & 1, g_lmk_status, kErrDkvMma);
+        mbar_wait(smem_u32(&sm->do_full[s]), (it / kStages) & 1, g_lmk_status, kErrDkvMma);
+        if (it >= 1) mbar_wait(smem_u32(&sm->dp_free), (it & 1) ^ 1, g_lmk_status, kErrDkvMma);
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
@@ -993,9 +993,9 @@ sm100_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       for (int i = 0; i < n_items; ++i, ++it) {
         const int s = it % kStages;
         const uint64_t ddot = desc_advance(ddo0t, (uint32_t)s * 2 * kOperand), dqt = desc_advance(dq0t, (uint32_t)s * 2 * kOperand);
-        mbar_wait(smem_u32(&sm->do_full[s]), (it / kStages) & 1, &g_lmk_status, kErrDkvMma);
-        if (i == 0) mbar_wait(smem_u32(&sm->acc_empty[0]), (u & 1) ^ 1, &g_lmk_status, kErrDkvMma);
-        mbar_wait(smem_u32(&sm->p_ready), it & 1, &g_lmk_status, kErrDkvMma);
+        mbar_wait(smem_u32(&sm->do_full[s]), (it / kStages) & 1, g_lmk_status, kErrDkvMma);
+        if (i == 0) mbar_wait(smem_u32(&sm->acc_empty[0]), (u & 1) ^ 1, g_lmk_status, kErrDkvMma);
+        mbar_wait(smem_u32(&sm->p_ready), it & 1, g_lmk_status, kErrDkvMma);
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
@@ -1005,8 +1005,8 @@ sm100_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           mma_commit(smem_u32(&sm->do_empty[s]));
           if (i == n_items - 1) mma_commit(smem_u32(&sm->acc_full[0]));
         }
-        if (i == 0) mbar_wait(smem_u32(&sm->acc_empty[1]), (u & 1) ^ 1, &g_lmk_status, kErrDkvMma);
-        mbar_wait(smem_u32(&sm->ds_ready), it & 1, &g_lmk_status, kErrDkvMma);
+        if (i == 0) mbar_wait(smem_u32(&sm->acc_empty[1]), (u & 1) ^ 1, g_lmk_status, kErrDkvMma);
+        mbar_wait(smem_u32(&sm->ds_ready), it & 1, g_lmk_status, kErrDkvMma);
         tc_fence_after();
         if (elect_one()) {
 #pragma unroll
@@ -1079,7 +1079,7 @@ sm100_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         const float delta = row_valid ? nDelta : 0.f;
         if (i + 1 < n_items) fetch_rows(tq + 1);      // one item ahead, so that their latency is never exposed
         const int kind = n > own ? 0 : (n == own ? 1 : 2);
-        mbar_wait(smem_u32(&sm->s_full), it & 1, &g_lmk_status, kErrDkvSoftmax);
+        mbar_wait(smem_u32(&sm->s_full), it & 1, g_lmk_status, kErrDkvSoftmax);
         tc_fence_after();
         uint64_t sp[32];
         const RowFactors f = bwd_weights<kIrr>(sp, c0, tmem_s + (uint32_t)g * 64u + lane_base, kind, vis, scale_log2, M2L, [&]() {
@@ -1092,14 +1092,14 @@ sm100_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 #pragma unroll
           for (int j = 0; j < 32; ++j) wd[j] = pack2p<kBf16>(mul2(sp[j], w2));
         }
-        if (it >= 1) mbar_wait(smem_u32(&sm->ds_free), (it & 1) ^ 1, &g_lmk_status, kErrDkvSoftmax);
+        if (it >= 1) mbar_wait(smem_u32(&sm->ds_free), (it & 1) ^ 1, g_lmk_status, kErrDkvSoftmax);
         store_row_sw128(my_tile, row, wd);
         fence_proxy_async_smem();
         mbar_arrive(smem_u32(&sm->p_ready));
-        mbar_wait(smem_u32(&sm->dp_full), it & 1, &g_lmk_status, kErrDkvSoftmax);
+        mbar_wait(smem_u32(&sm->dp_full), it & 1, g_lmk_status, kErrDkvSoftmax);
         tc_fence_after();
         bwd_dscores<kBf16, kIrr>(wd, sp, f, tmem_dp + (uint32_t)g * 64u + lane_base, smem_u32(&sm->dp_free), kind, scale, delta);
-        mbar_wait(smem_u32(&sm->p_free), it & 1, &g_lmk_status, kErrDkvSoftmax);
+        mbar_wait(smem_u32(&sm->p_free), it & 1, g_lmk_status, kErrDkvSoftmax);
         store_row_sw128(my_tile, row, wd);
         fence_proxy_async_smem();
         mbar_arrive(smem_u32(&sm->ds_ready));
@@ -1120,7 +1120,7 @@ sm100_bwd_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 #pragma unroll
       for (int j = 0; j < 4; ++j) row_off[j] = __shfl_sync(0xffffffffu, off, (lane & ~3) + j);
       if constexpr (kIrr) fetch_unit();
-      mbar_wait(smem_u32(&sm->acc_full[g]), u & 1, &g_lmk_status, kErrDkvEpilogue);
+      mbar_wait(smem_u32(&sm->acc_full[g]), u & 1, g_lmk_status, kErrDkvEpilogue);
       tc_fence_after();
       if (kIrr) __syncwarp();
       const uint32_t t_acc = (g == 0 ? tmem_dv : tmem_dk) + lane_base;
@@ -1279,7 +1279,7 @@ sm100_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         const int t = unit_tile(w), bh = w % BH, b = bh / H, h = bh - b * H;
         const int total = unit_items(w), n_last = total - 1;
         const uint32_t qb = smem_u32(&sm->qdo_full);
-        mbar_wait(smem_u32(&sm->delta_read), (u & 1) ^ 1, &g_lmk_status, kErrDqProducer);
+        mbar_wait(smem_u32(&sm->delta_read), (u & 1) ^ 1, g_lmk_status, kErrDqProducer);
         mbar_arrive_expect_tx(qb, 3 * (kD / 64) * kTileBytes);
         for (int c = 0; c < kD / 64; ++c) {
           tma_load_4d(o_tile + c * kTileBytes, &tm_o, qb, 64 * c, t * kQTile, h, b);
@@ -1291,7 +1291,7 @@ sm100_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           const int s = it % kDqStages;
           const int n = n_last - i, r0 = kIrr ? next_end - 63 : n * kBlk;
           if (kIrr && n > 0) next_end = end_of(b, n - 1);
-          mbar_wait(smem_u32(&sm->empty[s]), ((it / kDqStages) & 1) ^ 1, &g_lmk_status, kErrDqProducer);
+          mbar_wait(smem_u32(&sm->empty[s]), ((it / kDqStages) & 1) ^ 1, g_lmk_status, kErrDqProducer);
           const uint32_t fb = smem_u32(&sm->full[s]);
           mbar_arrive_expect_tx(fb, 2 * (kD / 64) * kHalfTile);
           for (int c = 0; c < kD / 64; ++c) {
@@ -1317,11 +1317,11 @@ sm100_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       const int total = warp_uniform(unit_items(w));
       for (int i = 0; i < total; ++i, ++it) {
         const int s = it % kDqStages, sb = it % kSdpBufs;
-        mbar_wait(smem_u32(&sm->full[s]), (it / kDqStages) & 1, &g_lmk_status, kErrDqMma);
+        mbar_wait(smem_u32(&sm->full[s]), (it / kDqStages) & 1, g_lmk_status, kErrDqMma);
         if (it >= kSdpBufs)
-          mbar_wait(smem_u32(is_s ? &sm->s_free[sb] : &sm->dp_free[sb]), ((it / kSdpBufs) & 1) ^ 1, &g_lmk_status, kErrDqMma);
+          mbar_wait(smem_u32(is_s ? &sm->s_free[sb] : &sm->dp_free[sb]), ((it / kSdpBufs) & 1) ^ 1, g_lmk_status, kErrDqMma);
         // the unit's rows come last: waited for in front of the other two they cost the unit another 1000 clk
-        if (i == 0) mbar_wait(smem_u32(&sm->ops_ready), u & 1, &g_lmk_status, kErrDqMma);
+        if (i == 0) mbar_wait(smem_u32(&sm->ops_ready), u & 1, g_lmk_status, kErrDqMma);
         tc_fence_after();
         const uint64_t db = desc_advance(db0, (uint32_t)s * 32768u);
         if (elect_one()) {
@@ -1346,8 +1346,8 @@ sm100_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       const int total = warp_uniform(unit_items(w));
       for (int i = 0; i < total; ++i, ++it) {
         const int s = it % kDqStages;
-        if (i == 0) mbar_wait(smem_u32(&sm->acc_empty), (u & 1) ^ 1, &g_lmk_status, kErrDqMma);
-        mbar_wait(smem_u32(&sm->ds_ready[s]), (it / kDqStages) & 1, &g_lmk_status, kErrDqMma);
+        if (i == 0) mbar_wait(smem_u32(&sm->acc_empty), (u & 1) ^ 1, g_lmk_status, kErrDqMma);
+        mbar_wait(smem_u32(&sm->ds_ready[s]), (it / kDqStages) & 1, g_lmk_status, kErrDqMma);
         tc_fence_after();
         const uint64_t dds = desc_advance(dv0, (uint32_t)s * 32768u), dkt = desc_advance(dk0t, (uint32_t)s * 32768u);
         if (elect_one()) {
@@ -1374,7 +1374,7 @@ sm100_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
     int64_t drain_row = -1;
     bool drain_valid = false;                      // rows past the end of the sequence are computed and dropped
     auto drain = [&]() {
-      mbar_wait(smem_u32(&sm->acc_full[g]), drains & 1, &g_lmk_status, kErrDqEpilogue);
+      mbar_wait(smem_u32(&sm->acc_full[g]), drains & 1, g_lmk_status, kErrDqEpilogue);
       ++drains;
       tc_fence_after();
       if (kIrr) __syncwarp();
@@ -1432,7 +1432,7 @@ sm100_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       const int vis = min(kIrr ? 63 - (end_own - pos) : row & 63, kBlk - 2);
       // delta = rowsum(O * dO), straight from the swizzled tiles (one row per thread, 16-byte chunks); warpgroup 0
       // also publishes it for the dK/dV kernel, which runs after this one
-      mbar_wait(smem_u32(&sm->qdo_full), u & 1, &g_lmk_status, kErrDqSoftmax);
+      mbar_wait(smem_u32(&sm->qdo_full), u & 1, g_lmk_status, kErrDqSoftmax);
       float delta = 0.f;
       uint32_t opw[kD / 64][32];      // this thread's row of the operand its warpgroup moves to TMEM (0: Q, 1: dO)
 #pragma unroll
@@ -1474,7 +1474,7 @@ sm100_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
       fence_proxy_async_smem();
       mbar_arrive(smem_u32(&sm->delta_read));
       // row -> TMEM lane, 32-bit word j (two features) -> column j: the layout of a K-major A operand
-      mbar_wait(smem_u32(&sm->ops_free), (u & 1) ^ 1, &g_lmk_status, kErrDqSoftmax);
+      mbar_wait(smem_u32(&sm->ops_free), (u & 1) ^ 1, g_lmk_status, kErrDqSoftmax);
       tc_fence_after();
       if (kIrr) __syncwarp();
       {
@@ -1491,7 +1491,7 @@ sm100_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
         const int it = it0 + i;
         const int s = it % kDqStages, sb = it % kSdpBufs;
         const int n = n_last - i;
-        mbar_wait(smem_u32(&sm->s_full[sb]), (it / kSdpBufs) & 1, &g_lmk_status, kErrDqSoftmax);
+        mbar_wait(smem_u32(&sm->s_full[sb]), (it / kSdpBufs) & 1, g_lmk_status, kErrDqSoftmax);
         tc_fence_after();
         const int kind = n > own ? 0 : (n == own ? 1 : 2);
         const int c_now = c0;
@@ -1501,7 +1501,7 @@ sm100_bwd_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_const
           tc_fence_before();
           mbar_arrive(smem_u32(&sm->s_free[sb]));
         });
-        mbar_wait(smem_u32(&sm->dp_full[sb]), (it / kSdpBufs) & 1, &g_lmk_status, kErrDqSoftmax);
+        mbar_wait(smem_u32(&sm->dp_full[sb]), (it / kSdpBufs) & 1, g_lmk_status, kErrDqSoftmax);
         tc_fence_after();
         uint32_t wd[32];
         bwd_dscores<kBf16, kIrr>(wd, sp, f, tmem_dp + sb * 64 + lane_base, smem_u32(&sm->dp_free[sb]), kind, scale, delta);
@@ -1957,22 +1957,24 @@ int attn_sm100_plan_stride() { return kIrrPlanInts; }
 
 size_t attn_sm100_bwd_workspace(int B, int H, int Lq, int, int) { return sizeof(float) * (size_t)B * H * Lq; }
 
-// Device address of the status word on the current device, for kernels compiled in other translation units.
+// Device address of the status words on the current device, for kernels compiled in other translation units.
 int* device_status_word() {
   int* ptr = nullptr;
   if (cudaGetSymbolAddress(reinterpret_cast<void**>(&ptr), g_lmk_status) != cudaSuccess) return nullptr;
   return ptr;
 }
 
-int device_status(int* out, int clear) {
-  int v = 0;
+int device_status(int* out, bool* expired, int clear) {
+  int v[2] = {0, 0};
   LMK_CUDA(cudaDeviceSynchronize());
-  LMK_CUDA(cudaMemcpyFromSymbol(&v, g_lmk_status, sizeof(int)));
-  if (clear && v != 0) {
-    int z = 0;
-    LMK_CUDA(cudaMemcpyToSymbol(g_lmk_status, &z, sizeof(int)));
+  LMK_CUDA(cudaMemcpyFromSymbol(v, g_lmk_status, sizeof(v)));
+  const int which = v[0] != 0 ? 0 : 1;      // an expired wait first; a condition beside it stays for the next call
+  if (clear && v[which] != 0) {
+    const int z = 0;
+    LMK_CUDA(cudaMemcpyToSymbol(g_lmk_status, &z, sizeof(int), which * sizeof(int)));
   }
-  if (out) *out = v;
+  *expired = which == 0;
+  *out = v[which];
   return LMK_OK;
 }
 

@@ -15,6 +15,11 @@ namespace lmk {
 char* error_buffer();
 int fail(int code, const char* fmt, ...);
 
+// The device's two status words.  [0]: site of the first bounded wait that expired; long waits give up once it is set (ptx::mbar_wait), so
+// nothing but an expired wait may be recorded there.  [1]: the first condition that a kernel met in its arguments and dealt with (a row
+// with too many landmarks, a page that is none, a full table): kernels that run beside or after it are not concerned.
+__device__ __forceinline__ void note_condition(int* status, int what) { atomicCAS(status + 1, 0, what); }
+
 // Multiprocessors of the current device (asked for once per device); a status code.
 int sm_count(int* n);
 

@@ -36,7 +36,7 @@ struct GsParams {
   // "query i sees keys 0 .. i + Lk - Lq" (mask block of lm_benchmark/models/landmark.py:210-224); hidden scores count
   // as -inf whatever x holds there
   const uint8_t* row_flags; int64_t row_flags_stride; int causal;
-  int* status;          // device status word: set to kErrSoftmaxGroups when a row holds max_groups or more landmarks
+  int* status;          // device status words: kErrSoftmaxGroups is noted when a row holds max_groups or more landmarks
 };
 
 enum { kErrSoftmaxGroups = 501 };
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kGsWarps * 32) grouped_softmax_kernel(GsParams
     if (seg_tail(e.c, lane) && e.c < G) gmax[e.c] = fmaxf(gmax[e.c], v);
     __syncwarp();
   }
-  if (lane == 0 && rd.base >= G && p.status != nullptr) atomicCAS(p.status, 0, kErrSoftmaxGroups);
+  if (lane == 0 && rd.base >= G && p.status != nullptr) note_condition(p.status, kErrSoftmaxGroups);
   bmax = warp_max(bmax);
   if (guards && isinf(bmax)) bmax = 0.f;
 
@@ -620,7 +620,7 @@ __device__ __forceinline__ void grouped_softmax_chunked_row(const GsParams& p, i
       fold_chunk<true>(nlm ? head : run, run, nlm, c0, flags, gmax, G, lane);
       raw = nraw;
     }
-    if (lane == 0 && base >= G && p.status != nullptr) atomicCAS(p.status, 0, kErrSoftmaxGroups);
+    if (lane == 0 && base >= G && p.status != nullptr) note_condition(p.status, kErrSoftmaxGroups);
   }
   bmax = warp_max(bmax);
   if (guards && isinf(bmax)) bmax = 0.f;
@@ -1265,7 +1265,7 @@ __global__ void __launch_bounds__(kGsWarps * 32, K == 32 ? 8 : 6)
       ca = inc - nlm;
       n_groups = __shfl_sync(0xffffffffu, inc, 31);
     }
-    if (lane == 0 && n_groups >= G && p.status != nullptr) atomicCAS(p.status, 0, kErrSoftmaxGroups);
+    if (lane == 0 && n_groups >= G && p.status != nullptr) note_condition(p.status, kErrSoftmaxGroups);
 
     const LaneWeights lw = lane_weights<T, K, kTwo ? kOne : kNone>(xr, c0, n4, lm_slot, ga, gb, bk, lg, ca, G, guards, gm, lm2_slot, nlm);
     const float binv = lw.binv, ia = lw.ia, ib = lw.ib, wa = lw.wa, elm = lw.elm;
@@ -1532,7 +1532,7 @@ __global__ void __launch_bounds__(kCrThreads, K == 32 ? 4 : 2) cached_rows_kerne
     const int nlm = mem.count();
     const unsigned owners = __ballot_sync(0xffffffffu, nlm != 0);
     const int n_groups = __reduce_add_sync(0xffffffffu, nlm);
-    if (lane == 0 && n_groups >= p.G && p.status != nullptr) atomicCAS(p.status, 0, kErrSoftmaxGroups);
+    if (lane == 0 && n_groups >= p.G && p.status != nullptr) note_condition(p.status, kErrSoftmaxGroups);
     if (__any_sync(0xffffffffu, nlm > 1)) {
       crowded_smem_row<K>(xr, c0, n4, mem, last, bk, owners, p.G);
     } else {

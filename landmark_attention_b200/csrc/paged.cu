@@ -2,7 +2,7 @@
 //
 // Pages are [n_pages, Hkv, page, D] (any page, head and row strides); table [B, max_pages] names a sequence's pages in order, lengths [B]
 // say how many of their rows are tokens.  Nothing here trusts either: lengths are held between 0 and the table's capacity, a table
-// entry outside of the pool is never followed (its keys count as hidden, and the device status word says 601).
+// entry outside of the pool is never followed (its keys count as hidden, and the device status says 601).
 //
 // Attention.  Query t of T stands at position p = length - T + t and sees key j if j <= p and (no window, p - j < window or j < sinks).
 //   o = sum_j e^{s_j - m} v_j / sum_j e^{s_j - m}, m = max_j s_j, s_j = scale q . k_j  over the visible j; 0 where nothing is visible.
@@ -47,8 +47,6 @@ struct Pages {
   __device__ int length(int b) const { return min(max(ld_behind_wait(lengths + b), 0), max_pages << shift); }
   __device__ int id(int b, int page_no) const { return ld_behind_wait(table + (int64_t)b * max_pages + page_no); }
 };
-
-__device__ __forceinline__ void note(int* status, int what) { atomicCAS(status, 0, what); }
 
 // The steps of one sequence: `first` of them cover the sinks that lie in front of the window, the rest run from key `lo` (a multiple
 // of 16) to the end.
@@ -345,7 +343,7 @@ paged_attend_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_const
       const uint32_t to = ring_at + (uint32_t)(n % kStages) * kStageBytes<T, kD>, bar = bar_at + (uint32_t)(n % kStages) * 8u;
       const int id = ok ? asked : pg.n_pages;        // behind the pool: zeros
       if (elect_one()) {
-        if (!ok) note(pg.status, kBadPage);
+        if (!ok) note_condition(pg.status, kBadPage);
         mbar_arrive_expect_tx(bar, kStageBytes<T, kD>);
 #pragma unroll
         for (int c = 0; c < kSub; ++c) {
@@ -732,7 +730,7 @@ struct AppendArgs {
 __device__ __forceinline__ int append_count(const AppendArgs& a, int b, int len) {
   const int want = a.counts != nullptr ? min(max(ld_behind_wait(a.counts + b), 0), a.T) : a.T;
   const int room = (a.pg.max_pages << a.pg.shift) - len;
-  if (want > room && threadIdx.x == 0) note(a.pg.status, kFull);
+  if (want > room && threadIdx.x == 0) note_condition(a.pg.status, kFull);
   return min(want, room);
 }
 template <typename V>                  // 16-byte vectors
@@ -749,7 +747,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant
     const int r = r0 + (int)(e / per_row), x = (int)(e % per_row), h = x / vecs, c = x - h * vecs;
     const int at = len + r, id = pg.id(b, at >> pg.shift);
     if (id < 0 || id >= pg.n_pages) {
-      note(pg.status, kBadPage);
+      note_condition(pg.status, kBadPage);
       continue;
     }
     const int64_t row = at & (pg.page - 1);
@@ -953,7 +951,7 @@ __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const __grid_c
 #pragma unroll
   for (int e = 0; e < kMoveRounds; ++e) {
     const bool ok = src[e] >= 0 && src[e] < pg.n_pages && dst[e] >= 0 && dst[e] < pg.n_pages;
-    if (j[e] >= 0 && !ok) note(pg.status, kBadPage);
+    if (j[e] >= 0 && !ok) note_condition(pg.status, kBadPage);
     if (!ok) j[e] = -1;
     if (j[e] < 0) continue;
     const int64_t from = j[e] & (pg.page - 1);

@@ -40,7 +40,7 @@ __device__ __forceinline__ uint32_t mbar_try_wait(uint32_t bar, uint32_t parity)
 }
 
 // Every wait is bounded (about one second of polling).  When the limit is hit the kernel records where it gave up in
-// *status (first writer wins) and carries on as if the barrier had completed, so the grid always drains, TMEM is
+// status[0] (first writer wins) and carries on as if the barrier had completed, so the grid always drains, TMEM is
 // always released, and the host can read the status word afterwards.  Once a status is recorded, other long waits
 // give up early as well, so a grid with a lost signal finishes quickly.
 constexpr uint32_t kWaitPollLimit = 1u << 24;

@@ -41,7 +41,7 @@ def landmark_grouped_softmax(x, dim, is_mem, last_section_mask, max_groups=None)
     """llama flavour (llama/llama_mem.py:222-243).  The reference hard-codes room for 63 landmarks per row
     (max_mem_cnt = 64, :228); here `max_groups` bounds 1 + the number of landmarks in a row.  Default: the row length + 1,
     capped at 256 so that rows of up to 4096 keys stay on the fast kernel; a row with more landmarks than that sets
-    the device status word (501, see `_lib.device_status`) instead of passing unnoticed -- give `max_groups` then."""
+    the device status (501, see `_lib.device_status`) instead of passing unnoticed -- give `max_groups` then."""
     _check_dim(x, dim)
     if max_groups is None:
         max_groups = min(256, x.shape[-1] + 1)
