@@ -625,6 +625,7 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       mbar_init(smem_u32(&sm->acc_empty[g]), kBwdWarps * 16);
     }
     for (int s = 0; s < kDealt; ++s) {
+      sm->dealt[s] = INT32_MAX;                    // no unit: what a reader finds whose wait ran out before a number came
       mbar_init(smem_u32(&sm->dealt_full[s]), 1);
       mbar_init(smem_u32(&sm->dealt_empty[s]), kBwdWarps + 1);
     }
