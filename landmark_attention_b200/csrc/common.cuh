@@ -60,8 +60,12 @@ static inline int dtype_size(int dtype) { return dtype == LMK_F32 ? 4 : 2; }
 
 // Launch with the programmatic-stream-serialization attribute: the kernel's CTAs may start, and its launch be processed, while the
 // kernel in front of it in the stream drains.  Such a kernel executes griddepcontrol.wait (ptx::grid_dep_wait) before it
-// touches global memory, has no __restrict__ pointer among its parameters and uses no __ldg: both promise memory that no other
-// kernel writes meanwhile, and allow the compiler to read it in front of the wait.
+// touches global memory, lets the next kernel start (ptx::grid_dep_launch) only behind that wait, has no __restrict__ pointer among
+// its parameters and uses no __ldg: both promise memory that no other kernel writes meanwhile, and allow the compiler to read it in front
+// of the wait.  Since every trigger stands behind a wait, all kernels but the one directly in front are complete when a kernel starts.  A few
+// kernels use that and read ahead of their wait what the one in front does not write: the dK/dV kernels of both attention families, the
+// loading warps of the window's dQ kernel, and the lengths in paged_finish_kernel.  They write only what the one in front does not touch
+// until they are behind the wait, and end behind it.
 template <typename... P, typename... A>
 cudaError_t launch_overlapped(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, A&&... args) {
   cudaLaunchAttribute attr[1];
