@@ -101,30 +101,67 @@ class PagedKVCache:
         return paged_attention(q, self.k_pages, self.v_pages, self.table, self.lengths, window, sinks, sm_scale, self.weights, decay)
 
     def evict(self, budget, recent=0, sinks=0):
-        """paged_evict with pages of this cache; returns `kept`.  Reads the lengths back, so the host waits; not for captured steps."""
+        """paged_evict with pages of this cache; returns `kept`.  Reads the lengths back, so the host waits; not for captured steps.
+
+        All sequences go at once where ceil(budget / page) pages for each that is over the budget are free, otherwise as many at a time as
+        there is room for; with room for none, one goes through a copy of its pages."""
         if self.weights is None:
             raise ValueError("evict goes by attention weights: make the cache with track_weights=True")
         if self.table.is_cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("evict cannot be captured")
+        if budget < 1:
+            raise ValueError("the budget must be at least 1 token")
         n = -(-budget // self.page)
         over = [b for b, t in enumerate(self.refresh()) if t > budget]
-        if n * len(over) > len(self._free):
-            raise ValueError(f"evict needs {n * len(over)} free pages for {len(over)} sequences, {len(self._free)} are free")
-        taken = {b: [self._free.pop() for _ in range(n)] for b in over}
-        fresh = torch.tensor([taken.get(b, [-1] * n) for b in range(len(self._tokens))], dtype=torch.int32, device=self.table.device)
-        try:
-            table, lengths, weights, kept = paged_evict(self.k_pages, self.v_pages, self.table, self.lengths, self.weights, fresh, budget,
-                                                        recent, sinks)
-        except BaseException:
-            for pages in taken.values():
-                self._free.extend(pages)
-            raise
-        for mine, new in ((self.table, table), (self.lengths, lengths), (self.weights, weights)):
-            mine.copy_(new)                       # in place: captured steps read these tensors
+        if n * len(over) <= len(self._free):
+            return self._evict(None, over, n, budget, recent, sinks)
+        kept = torch.empty((len(self._tokens), self.k_pages.shape[1], budget), dtype=torch.int32, device=self.table.device)
+        rest = [b for b, t in enumerate(self._tokens) if t <= budget]
+        if rest:
+            kept[rest] = self._evict(rest, [], n, budget, recent, sinks)
+        while over:                               # a sequence gives back at least as many pages as it takes
+            room = len(self._free) // n
+            some, over = over[:max(room, 1)], over[max(room, 1):]
+            kept[some] = (self._evict if room else self._evict_through_copy)(some, some, n, budget, recent, sinks)
+        return kept
+
+    def _evict(self, rows, over, n, budget, recent, sinks):
+        """Evict from the sequences `rows` (None: all), of which `over` are beyond the budget: n free pages for each of these."""
+        count = len(self._tokens) if rows is None else len(rows)
+        taken = dict(zip(over, (self._free[i * n:(i + 1) * n] for i in range(len(over)))))
+        fresh = torch.tensor([taken.get(b, [-1] * n) for b in (range(count) if rows is None else rows)], dtype=torch.int32,
+                             device=self.table.device).view(count, n)
+        mine = (self.table, self.lengths, self.weights)
+        if rows is not None:
+            at = torch.tensor(rows, device=self.table.device)
+            mine = tuple(t.index_select(0, at) for t in mine)
+        *new, kept = paged_evict(self.k_pages, self.v_pages, *mine, fresh, budget, recent, sinks)
+        for to, x in zip((self.table, self.lengths, self.weights), new):      # in place: captured steps read these tensors
+            to.copy_(x) if rows is None else to.index_copy_(0, at, x)
+        del self._free[:n * len(over)]
         for b in over:
             self._free.extend(self._owned[b])
             self._owned[b] = taken[b]
             self._tokens[b] = budget
+        return kept
+
+    def _evict_through_copy(self, rows, over, n, budget, recent, sinks):
+        """The same for one sequence and no free pages: out of a copy of its pages, back into the first n of them."""
+        (b,) = rows
+        own = torch.tensor(self._owned[b], device=self.table.device)
+        m = own.numel()
+        pools = [torch.cat((p.index_select(0, own), p.new_empty((n, *p.shape[1:])))) for p in (self.k_pages, self.v_pages)]
+        table = torch.full_like(self.table[:1], -1)
+        table[0, :m] = torch.arange(m, device=own.device)
+        fresh = torch.arange(m, m + n, dtype=torch.int32, device=own.device).view(1, n)
+        _, lengths, weights, kept = paged_evict(*pools, table, self.lengths[b:b + 1], self.weights[b:b + 1], fresh, budget, recent, sinks)
+        for p, copy in zip((self.k_pages, self.v_pages), pools):
+            p.index_copy_(0, own[:n], copy[m:])
+        self.table[b, n:] = -1
+        self.lengths[b:b + 1] = lengths
+        self.weights[b:b + 1] = weights
+        self._free.extend(self._owned[b][n:])
+        self._owned[b], self._tokens[b] = self._owned[b][:n], budget
         return kept
 
     def drop(self, sequence):
