@@ -18,6 +18,7 @@ int check_window(const void* q, const void* k, const void* v, int B, int H, int 
   LMK_CHECK_ARG((int64_t)B * H <= 65535, "window attention: B*H = %lld exceeds 65535", (long long)B * H);
   LMK_CHECK_ARG(Lk >= Lq, "window attention: %d queries are more than %d keys", Lq, Lk);
   LMK_CHECK_ARG(Lk <= (1 << 22), "window attention: %d keys exceed 2^22", Lk);
+  LMK_CHECK_ARG((int64_t)B * H * ((Lk + 63) / 64) <= INT32_MAX / 4, "window attention: %d heads of %d keys are too many", B * H, Lk);
   LMK_CHECK_ARG(D >= 8 && D <= 128 && D % 8 == 0, "window attention: head dim %d must be a multiple of 8 up to 128", D);
   LMK_CHECK_ARG(dtype == LMK_F32 || dtype == LMK_F16 || dtype == LMK_BF16, "window attention: bad dtype %d", dtype);
   LMK_CHECK_ARG(window >= 1, "window attention: window %d must be at least 1", window);
@@ -67,11 +68,11 @@ template <typename T>
 __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant__ WindowParams p, int qt, int kk) {
   ptx::grid_dep_wait();
   ptx::grid_dep_launch();
-  const int tile = blockIdx.y % p.split.tiles, bk = blockIdx.y / p.split.tiles, b = bk / p.Hkv;
+  const int tile = blockIdx.x % p.split.tiles, bk = blockIdx.x / p.split.tiles, b = bk / p.Hkv;
   const int len = p.lengths == nullptr ? p.Lk : min(max(ptx::ld_behind_wait(p.lengths + b), 0), p.Lk);
   const QueryTiles qts = queries_of_keys(tile, qt, kk, p.Lq, p.Lk - p.Lq, len, p.window, p.sinks);
   const int runs = (qts.end - qts.last + p.split.run - 1) / p.split.run;
-  const int e = (blockIdx.x * 256 + threadIdx.x) * 4, key = e / p.D, f = e - key * p.D;
+  const int e = (blockIdx.y * 256 + threadIdx.x) * 4, key = e / p.D, f = e - key * p.D;
   if (key >= kk || tile * kk + key >= p.sinks) return;
   const int64_t slot = 2ll * kk * p.D;
   const float* part = p.split.part + ((int64_t)bk * p.split.tiles + tile) * (1 + p.split.runs) * slot + e;
@@ -94,7 +95,8 @@ __global__ void __launch_bounds__(256) window_join_kernel(const __grid_constant_
 }  // namespace
 
 int window_join_parts(const WindowParams& p, int qt, int kk, int dtype, cudaStream_t st) {
-  const dim3 grid(((p.sinks < kk ? p.sinks : kk) * p.D / 4 + 255) / 256, p.B * p.Hkv * p.split.tiles);
+  // the tiles in x: there may be more of them than y has room for
+  const dim3 grid((unsigned)(p.B * p.Hkv * p.split.tiles), ((p.sinks < kk ? p.sinks : kk) * p.D / 4 + 255) / 256);
   if (dtype == LMK_F32) LMK_CUDA(launch_overlapped(window_join_kernel<float>, grid, dim3(256), 0, st, p, qt, kk));
   else if (dtype == LMK_F16) LMK_CUDA(launch_overlapped(window_join_kernel<__half>, grid, dim3(256), 0, st, p, qt, kk));
   else LMK_CUDA(launch_overlapped(window_join_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, p, qt, kk));
@@ -157,8 +159,6 @@ extern "C" int lmk_window_bwd(const void* q, const void* k, const void* v, const
   int qt, kk;
   tile_sizes(dtype, &qt, &kk);
   if ((rc = plan_split(&p.split, B, Hkv, Lq, Lk, p.window, p.sinks, qt, kk)) != LMK_OK) return rc;
-  LMK_CHECK_ARG((int64_t)B * Hkv * (p.split.tiles > 0 ? p.split.tiles : 1) <= 65535, "window attention backward: %d sinks of %d key heads are too many",
-                sinks, B * Hkv);
   const size_t delta_bytes = up256(sizeof(float) * (size_t)B * H * Lq), need = kNextBytes + delta_bytes + up256(part_bytes(p.split, B, Hkv, D, kk));
   if (workspace == nullptr || workspace_bytes < need || ((uintptr_t)workspace & 255) != 0)
     return fail(LMK_ERR_WORKSPACE, "window attention backward: workspace of %zu bytes on a 256-byte boundary needed", need);
