@@ -21,7 +21,6 @@
 // products in the three that have some (S and dP are formed twice in the backward pass).
 // All waits are bounded (sm100_ptx.cuh).
 #include <mutex>
-#include <cuda_fp8.h>
 #include "common.cuh"
 #include "attn_params.h"
 #include "window_params.h"
@@ -80,23 +79,36 @@ template <bool kBf16> __device__ __forceinline__ float2 unpack2(uint32_t x) {
   return __half22float2(*reinterpret_cast<const __half2*>(&x));
 }
 
-// What rounding x to 16 bits left, four numbers in a word: e5m2, times 2^11 (fp16) or 2^8 (bf16), so that it has about the size of x.  Two
-// bits are enough: delta, which it goes into, then is off by an eighth of what the rounding of O alone would do.
-template <bool kBf16> constexpr float kRestScale = kBf16 ? 256.f : 2048.f;
-template <bool kBf16> __device__ __forceinline__ uint32_t rest4(const float (&x)[4]) {
-  uint32_t r = 0;
-#pragma unroll
-  for (int e = 0; e < 4; e += 2) {
-    const float2 back = unpack2<kBf16>(pack2<kBf16>(x[e], x[e + 1]));
-    const float2 left = make_float2((x[e] - back.x) * kRestScale<kBf16>, (x[e + 1] - back.y) * kRestScale<kBf16>);
-    r |= (uint32_t)__nv_cvt_float2_to_fp8x2(left, __NV_SATFINITE, __NV_E5M2) << (8 * e);
-  }
-  return r;
+// What rounding x to 16 bits left, a byte a number: in steps of 1 / 128 of the rounded number's last place, so at most 64 of them either way,
+// whatever the number's size, and 64 added.  (Below 2^-112 in bf16 the step stays that of 2^-112: 2^-126.)
+constexpr uint32_t kRestZero = 64;
+// two exponent fields of rounded numbers, in bf16's place, and not below the least one a step is made from
+template <bool kBf16> __device__ __forceinline__ uint32_t exponents2(uint32_t rounded) {
+  return kBf16 ? __vmaxu2(rounded & 0x7f807f80u, 0x07800780u) : __vmaxu2((rounded & 0x7c007c00u) >> 3, 0x00800080u);
 }
-template <bool kBf16> __device__ __forceinline__ float2 rest_of(uint32_t pair) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)pair, __NV_E5M2);
-  const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h));
-  return make_float2(x.x * (1.f / kRestScale<kBf16>), x.y * (1.f / kRestScale<kBf16>));
+template <bool kBf16> __device__ __forceinline__ uint32_t rest4(const float (&x)[4]) {
+  uint32_t r[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const uint32_t rounded = pack2<kBf16>(x[2 * e], x[2 * e + 1]);
+    const float2 back = unpack2<kBf16>(rounded);
+    const __nv_bfloat162 left = __floats2bfloat162_rn(x[2 * e] - back.x, x[2 * e + 1] - back.y);
+    // 1 / step = 2^(134 - field + 7) or 2^(25 - field + 7), by its exponent field
+    const uint32_t per_step = (kBf16 ? 0x86008600u : 0x4f804f80u) - exponents2<kBf16>(rounded);
+    // bf16 numbers between 128 and 256 are whole: 192 + steps, rounded, whose low byte is 64 + steps
+    const __nv_bfloat162 n = __hfma2(left, *reinterpret_cast<const __nv_bfloat162*>(&per_step), __floats2bfloat162_rn(192.f, 192.f));
+    r[e] = *reinterpret_cast<const uint32_t*>(&n);
+  }
+  return __byte_perm(r[0], r[1], 0x6420);
+}
+// the two numbers, as they were, of a pair of rounded ones and bytes first, first + 1 of the rest
+template <bool kBf16> __device__ __forceinline__ float2 restored2(uint32_t rounded, uint32_t rest, int first) {
+  const float2 x = unpack2<kBf16>(rounded);
+  const uint32_t step = exponents2<kBf16>(rounded) + (kBf16 ? 0u - 0x07000700u : 0x2f802f80u);      // 14 fields down; fp16: 112 up, 17 down
+  const float2 s = unpack2<true>(step);
+  const float a = __uint_as_float(__byte_perm(rest, 0x4b000000u, 0x7440u + first)) - (8388608.f + kRestZero);      // 2^23 + byte
+  const float b = __uint_as_float(__byte_perm(rest, 0x4b000000u, 0x7441u + first)) - (8388608.f + kRestZero);
+  return make_float2(fmaf(a, s.x, x.x), fmaf(b, s.y, x.y));
 }
 
 struct WindowTensors {
@@ -955,7 +967,7 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
 
 // ---------------------------------------------------------------------------------------------- backward: delta = rowsum(O dO)
 // with what the rounding of O left: without it a row of dS would miss its sum of 0 by as much as dS's own rounding is off, and dQ and dK
-// had 1.53 instead of 1.41 times the error of their own rounding.  Bound by memory; in the dQ kernel the tiles of O and of the rest took
+// had 1.46 to 1.53 instead of 1.43 to 1.46 times the error of their own rounding (lengths of 700 and 2048, both types).  Bound by memory; in the dQ kernel the tiles of O and of the rest took
 // the places of key tiles on their way (training size 46 -> 53 us), and the dK/dV kernel had to wait for the last of its CTAs.
 struct DeltaArgs {
   const void *o, *dO;
@@ -998,9 +1010,9 @@ __global__ void __launch_bounds__(kDeltaThreads, 4) window_delta_kernel(const __
     float sum = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float2 fx = unpack2<kBf16>(xs[w]), fy = rest_of<kBf16>(ys[w / 2] >> (16 * (w & 1)) & 0xffffu), fg = unpack2<kBf16>(gs[w]);
-      sum = fmaf(fx.x + fy.x, fg.x, sum);
-      sum = fmaf(fx.y + fy.y, fg.y, sum);
+      const float2 fx = restored2<kBf16>(xs[w], ys[w / 2], 2 * (w & 1)), fg = unpack2<kBf16>(gs[w]);
+      sum = fmaf(fx.x, fg.x, sum);
+      sum = fmaf(fx.y, fg.y, sum);
     }
 #pragma unroll
     for (int d = kLanes / 2; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
