@@ -866,10 +866,13 @@ window_dkv_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
 #pragma unroll
             for (int k = 0; k < 8; ++k) sp[h][k] = fma2(sp[h][k], c2, l2[k >> 1]);
           if (kind == 2) {
+            // polynomials make finite numbers of NaN: a row that has one has it in its lse too, from where it reaches the weight
+            const uint64_t zero = pk2(0.f, 0.f);
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-              for (int k = 0; k < 8; ++k) sp[h][k] = k % kBwdPolyEvery == 1 ? ex2_poly2<3>(sp[h][k]) : ex2_pair(sp[h][k]);
+              for (int k = 0; k < 8; ++k)
+                sp[h][k] = k % kBwdPolyEvery == 1 ? fma2(l2[k >> 1], zero, ex2_poly2<3>(sp[h][k])) : ex2_pair(sp[h][k]);
           } else {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
