@@ -213,13 +213,14 @@ __global__ void __launch_bounds__(kThreads, kD == 64 ? 2 : 1) window_fwd_f32_ker
     const float sum = warp_sum(l[r]);
     if (r0 + r >= rows) continue;
     const int64_t at = (int64_t)bh * p.Lq + tile * kTile + r0 + r;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const bool is = p0 + r0 + r < len;           // sees its own key at least; the sum is 0 where every score is -inf: NaN, as by the formula
+    const float inv = is ? 1.f / sum : 0.f;
     float x[kF];
     row_of<kF>(x, o, r);
 #pragma unroll
     for (int f = 0; f < kF; ++f) x[f] *= inv;
-    if (lane * kF < p.D) write_row<kF>((float*)p.o + at * p.D + lane * kF, x, sum != 0.f);
-    if (lane == 0 && p.lse != nullptr) p.lse[at] = sum == 0.f ? INFINITY : m[r] + log2f(sum);
+    if (lane * kF < p.D) write_row<kF>((float*)p.o + at * p.D + lane * kF, x, is);
+    if (lane == 0 && p.lse != nullptr) p.lse[at] = is ? m[r] + log2f(sum) : INFINITY;
   }
 }
 

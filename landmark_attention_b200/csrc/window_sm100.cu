@@ -410,7 +410,7 @@ window_fwd_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
       mbar_wait(smem_u32(&sm->o_full), units & 1, status, kErrFwdEpilogue);
       ++units;
       tc_fence_after();
-      const bool valid = pos < u.len && l != 0.f;
+      const bool valid = pos < u.len;                // sees its own key at least; l = 0 where every score is -inf: NaN, as by the formula
       const float inv = valid ? 1.f / l : 0.f;
       int64_t row_off[4];                            // of the four rows that four lanes write together
       {

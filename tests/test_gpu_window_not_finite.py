@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("D", [64, 128])
-@pytest.mark.parametrize("what", ["nan", "infinite"])
+@pytest.mark.parametrize("what", ["nan", "infinite", "all scores infinitely low"])
 def test_rows_that_are_not_finite(what, D, dtype):
     n, window, sinks = 900, 300, 3
     q, k, v, g = inputs(dtype, 1, 2, 1, n, n, D, 33)
