@@ -1064,6 +1064,8 @@ void paged_append(const Tensor& k_, const Tensor& v_, const Tensor& kp, const Te
   same_device(k_, kp, "k");
   same_device(v_, kp, "v");
   LMK_ASSERT(!needs_grad({kp, vp}), "the cache's pages take no gradients");
+  for (const Tensor* t : {&k_, &v_})
+    LMK_ASSERT(!t->_fw_grad(0).defined(), "paged_append stores numbers alone: a tangent would be dropped");
   float* w = cache_weights(weights, kp, p);
   if (k_.size(2) == 0) return;
   c10::cuda::OptionalCUDAGuard guard(kp.device());
