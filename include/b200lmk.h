@@ -515,8 +515,8 @@ int lmk_window_bwd(const void* q, const void* k, const void* v, const void* o, c
  * keys count as hidden, and lmk_device_status says 601.  Sequences may share pages for reading.
  *
  * lmk_paged_append: rows 0 .. n_b - 1 of k_new, v_new [B,Hkv,T,D] (strided) behind the tokens of sequence b, whose length moves on by n_b
- * = counts[b] (int32, nullable: T).  weights (nullable) [B, Hkv, max_pages * page] fp32 are set to 0 for them.  Rows that do not
- * fit are left out (status 602).
+ * = counts[b] (int32, nullable: T).  weights (nullable) [B, Hkv, max_pages * page] fp32 are set to 0 for them.  Rows that have
+ * no page are not stored (status 601: their keys count and are hidden), rows that the table has no room for do not count (status 602).
  *
  * lmk_paged_attend: query t of q [B,H,T,D] (strided) stands at position p = lengths[b] - T + t and sees key j if j <= p and (window == 0
  * or p - j < window or j < sinks); o [B,H,T,D] dense, zeros where nothing is visible.  weights (nullable) [B, Hkv, max_pages *

@@ -746,6 +746,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant
   for (int64_t e = threadIdx.x; e < (int64_t)(r1 - r0) * per_row; e += blockDim.x) {
     const int r = r0 + (int)(e / per_row), x = (int)(e % per_row), h = x / vecs, c = x - h * vecs;
     const int at = len + r, id = pg.id(b, at >> pg.shift);
+    if (a.weights != nullptr && c == 0) a.weights[((int64_t)b * pg.Hkv + h) * cap + at] = 0.f;      // (a key without a page counts too)
     if (id < 0 || id >= pg.n_pages) {
       note_condition(pg.status, kBadPage);
       continue;
@@ -756,7 +757,6 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant
     const V xv = *reinterpret_cast<const V*>((const char*)a.v_new + bytes(b * a.vns[0] + h * a.vns[1] + r * a.vns[2]) + c * 16ll);
     *reinterpret_cast<V*>((char*)a.k + bytes((int64_t)id * pg.ks[0] + h * pg.ks[1] + row * pg.ks[2]) + c * 16ll) = xk;
     *reinterpret_cast<V*>((char*)a.v + bytes((int64_t)id * pg.vs[0] + h * pg.vs[1] + row * pg.vs[2]) + c * 16ll) = xv;
-    if (a.weights != nullptr && c == 0) a.weights[((int64_t)b * pg.Hkv + h) * cap + at] = 0.f;
   }
   if (a.chunks == 1) {
     __syncthreads();                   // all threads have read the length

@@ -12,8 +12,8 @@ from . import _lib as L
 
 def paged_append(k, v, k_pages, v_pages, table, lengths, counts=None, weights=None):
     """Store rows 0 .. counts[b] - 1 (all T without counts) of k, v [B,Hkv,T,D] behind the tokens of every sequence and move `lengths`
-    on, in place.  The pages must be in the table already; rows that have none, or no room in the table, are left out, and
-    `_lib.device_status()` says 601 or 602.  weights [B, Hkv, max_pages * page] (fp32) are set to 0 for the new keys.
+    on, in place.  The pages must be in the table already.  Rows that have none are not stored (their keys count, and stay hidden), rows
+    without room in the table do not count; `_lib.device_status()` says 601 or 602.  weights [B, Hkv, max_pages * page] (fp32) are set to 0 for the new keys.
     The numbers of k and v alone are stored: no gradients go through the cache, and tangents are refused."""
     L.host().paged_append(k, v, k_pages, v_pages, table, lengths, counts, weights)
 
