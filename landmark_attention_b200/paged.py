@@ -64,11 +64,18 @@ class PagedKVCache:
         self._tokens = self.lengths.tolist()
         return self._tokens
 
+    def _all_stored(self):
+        # Replays that went on behind the reserved pages stored nothing there (status 601); pages given now would show whatever they hold.
+        for b, t in enumerate(self._tokens):
+            if t > len(self._owned[b]) * self.page:
+                raise ValueError(f"sequence {b} has {t} tokens in pages for {len(self._owned[b]) * self.page}: the others were not stored; drop it")
+
     def reserve(self, tokens):
         """Give every sequence pages for `tokens` more tokens (a number, or one per sequence), e.g. before a step is captured."""
         more = [tokens] * len(self._tokens) if isinstance(tokens, int) else list(tokens)
         if len(more) != len(self._tokens):
             raise ValueError(f"expected one number of tokens for each of {len(self._tokens)} sequences")
+        self._all_stored()
         need = [-(-(n + m) // self.page) for n, m in zip(self._tokens, more)]
         if max(need) > self.max_pages:
             raise ValueError(f"a sequence would exceed the cache's {self.max_pages * self.page} tokens")
@@ -114,6 +121,7 @@ class PagedKVCache:
             raise ValueError("the budget must be at least 1 token")
         n = -(-budget // self.page)
         over = [b for b, t in enumerate(self.refresh()) if t > budget]
+        self._all_stored()
         if n * len(over) <= len(self._free):
             return self._evict(None, over, n, budget, recent, sinks)
         kept = torch.empty((len(self._tokens), self.k_pages.shape[1], budget), dtype=torch.int32, device=self.table.device)
