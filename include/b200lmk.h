@@ -528,7 +528,7 @@ int lmk_window_bwd(const void* q, const void* k, const void* v, const void* o, c
  * the rest with the largest weights (the lower index first where they are equal; NaN is the largest), per key head, in order, copied to
  * the pages fresh [B, n_fresh] names, which must be nobody's; the others stay as they are.  Writes table_out [B, max_pages] (-1: no page),
  * lengths_out [B], weights_out [B, Hkv, max_pages * page] (0 behind the tokens) and kept [B, Hkv, budget] int32 (the survivors'
- * former positions, -1 behind them).  The pages of `table` are not written.
+ * former positions, -1 behind them).  The pages of `table` are not written.  Survivors whose page is none become rows of zeros (status 601).
  */
 int lmk_paged_append(const void* k_new, const void* v_new, const int64_t k_new_strides[3], const int64_t v_new_strides[3], void* k_pages,
                      void* v_pages, const int64_t k_strides[3], const int64_t v_strides[3], const int32_t* table, int32_t* lengths,

@@ -950,10 +950,11 @@ __global__ void __launch_bounds__(kMoveThreads) paged_move_kernel(const __grid_c
   uint4 xk[kMoveRounds], xv[kMoveRounds];
 #pragma unroll
   for (int e = 0; e < kMoveRounds; ++e) {
-    const bool ok = src[e] >= 0 && src[e] < pg.n_pages && dst[e] >= 0 && dst[e] < pg.n_pages;
-    if (j[e] >= 0 && !ok) note_condition(pg.status, kBadPage);
-    if (!ok) j[e] = -1;
-    if (j[e] < 0) continue;
+    const bool from_ok = src[e] >= 0 && src[e] < pg.n_pages, to_ok = dst[e] >= 0 && dst[e] < pg.n_pages;
+    if (j[e] >= 0 && !(from_ok && to_ok)) note_condition(pg.status, kBadPage);
+    if (!to_ok) j[e] = -1;
+    xk[e] = xv[e] = make_uint4(0u, 0u, 0u, 0u);      // a survivor that has no page: zeros, not what the fresh page held
+    if (j[e] < 0 || !from_ok) continue;
     const int64_t from = j[e] & (pg.page - 1);
     xk[e] = *reinterpret_cast<const uint4*>((const char*)a.k + at(pg.ks, src[e], from));
     xv[e] = *reinterpret_cast<const uint4*>((const char*)a.v + at(pg.vs, src[e], from));

@@ -34,6 +34,7 @@ def paged_evict(k_pages, v_pages, table, lengths, weights, fresh, budget, recent
     budget - sinks - recent keys with the largest weights stay (the lower position first where weights are equal; NaN counts as the
     largest), chosen per key head, in order.  They are copied to the pages fresh [B, n] (n * page >= budget), which must belong to
     nobody; the pages in `table` are not written, and sequences within the budget keep theirs.
+    Survivors that have no page become rows of zeros (`_lib.device_status()` says 601).
     Returns (table, lengths, weights, kept), new tensors; kept [B, Hkv, budget] are the survivors' former positions, -1 behind them."""
     return L.host().paged_evict(k_pages, v_pages, table, lengths, weights, fresh, budget, recent, sinks)
 
