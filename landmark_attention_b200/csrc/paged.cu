@@ -1102,7 +1102,8 @@ extern "C" int lmk_paged_attend(const void* q, const int64_t q_strides[3], const
   LMK_CHECK_ARG(H >= Hkv && H % Hkv == 0, "paged attention: %d query heads are not a multiple of %d key heads", H, Hkv);
   LMK_CHECK_ARG(attend_sizes_ok(B, H, Hkv, T), "paged attention: T=%d tokens of %d heads a key head are too many (up to 1024 tokens, 4096 rows)", T, H / Hkv);
   LMK_CHECK_ARG(window >= 0 && sinks >= 0, "paged attention: window=%d and sinks=%d must not be negative", window, sinks);
-  LMK_CHECK_ARG((int64_t)B * Hkv * ((H / Hkv * T + kRowTile - 1) / kRowTile) * ((int64_t)max_pages * page / kStep) <= INT32_MAX,
+  // the last piece may end behind the line, by less than one step a CTA
+  LMK_CHECK_ARG((int64_t)B * Hkv * ((H / Hkv * T + kRowTile - 1) / kRowTile) * ((int64_t)max_pages * page / kStep) <= INT32_MAX - 65536,
                 "paged attention: %d sequences of up to %lld tokens and %d key heads are too many for one call", B, (long long)max_pages * page, Hkv);
   LMK_CHECK_ARG((n_pages == 1 || (k_strides[0] > 0 && v_strides[0] > 0)) && (Hkv == 1 || (k_strides[1] > 0 && v_strides[1] > 0)) &&
                     k_strides[2] >= D && v_strides[2] >= D, "paged attention: pages must not be broadcast, nor their rows overlap");
