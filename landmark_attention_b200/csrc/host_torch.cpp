@@ -962,8 +962,10 @@ struct WindowAttention : public torch::autograd::Function<WindowAttention> {
 };
 
 // A leaf's gradient belongs to the stream on which a graph of it was built first, for as long as that graph lives.  A captured backward
-// pass would make that stream wait for the capturing one, which breaks the capture: refused here, in front of it.
-void check_capture(const Tensor& t) {
+// pass would make that stream wait for the capturing one, which breaks the capture: refused here, in front of it.  Views (heads of a
+// projection's [B, L, H, D]) are looked at through.
+void check_capture(const Tensor& t_) {
+  const Tensor t = t_.is_view() ? Tensor(t_._base()) : t_;
   if (!t.requires_grad() || !t.is_leaf()) return;
   const auto acc = torch::autograd::impl::try_get_grad_accumulator(t);
   if (!acc) return;
