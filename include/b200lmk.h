@@ -522,7 +522,9 @@ int lmk_window_bwd(const void* q, const void* k, const void* v, const void* o, c
  * or p - j < window or j < sinks); o [B,H,T,D] dense, zeros where nothing is visible.  weights (nullable) [B, Hkv, max_pages *
  * page] fp32: weights = decay * weights + the sum of the key's attention weights over the T queries of the heads that share it, for
  * every j < lengths[b]; decay 0 does not read what stood there.
- * workspace: lmk_paged_attend_workspace(...) bytes, 256-byte aligned (null where that is 0), contents irrelevant.
+ * T up to 1024, H / Hkv * T up to 4096.  Values that some of the T tokens see are expected to be finite.
+ * workspace: lmk_paged_attend_workspace(...) bytes (with weights 4 bytes per query row and key of the table's capacity), 256-byte aligned
+ * (null where that is 0), contents irrelevant.
  *
  * lmk_paged_evict: sequences of more than `budget` tokens keep the first `sinks`, the last `recent` and the budget - sinks - recent of
  * the rest with the largest weights (the lower index first where they are equal; NaN is the largest), per key head, in order, copied to

@@ -6,8 +6,9 @@
 //
 // Attention.  Query t of T stands at position p = length - T + t and sees key j if j <= p and (no window, p - j < window or j < sinks).
 //   o = sum_j e^{s_j - m} v_j / sum_j e^{s_j - m}, m = max_j s_j, s_j = scale q . k_j  over the visible j; 0 where nothing is visible.
-// Every visible row of K and V is read once, 512 bytes a key and head at D = 128 in 16 bits against 4 D multiply-adds a query row: bound
-// by HBM.  What decides is how evenly the rows are dealt out and how many loads are in flight.
+// Every visible row of K and V is read once for up to 16 query rows of its key head, 512 bytes a key and head at D = 128 in 16 bits against
+// 4 D multiply-adds a query row: bound by HBM (5.8 TB/s with one row, 5.5 with 16).  What decides is how evenly the rows are dealt out and
+// how many loads are in flight.
 //   - The work of all sequences is one line of steps of 16 keys (sequence, key head, tile of 16 query rows, step).  Every CTA takes the same
 //     length of it, so neither short sequences nor a large capacity leave SMs idle, whatever the lengths are; they are read on the
 //     device, so a captured graph serves them as they grow.  A piece that holds all of its keys is written out at once; pieces of a
@@ -16,9 +17,14 @@
 //     lane asks TMA for a step's rows (with 16-byte cp.async the addresses alone took 1200 clk a step, as long as the arithmetic, and
 //     the warps could not keep up with the memory).  Rows that nobody sees are overwritten with zeros before the values are used, so
 //     what they hold does not matter.
-//   - The G T query rows of a key head are the 16 rows of an mma.sync tile (fp32: FMAs), so K and V are read once for all of them.
-// Weights (for eviction): the scores are kept, 4 bytes a key and query row, and the second kernel, which knows every row's maximum and
-// sum, adds e^{s - m} / l of a group's rows to the key's weight.  One thread adds up one key: no atomics, bit-reproducible.
+//   - Up to 16 of the G T query rows of a key head are the rows of an mma.sync tile (fp32: FMAs), and K and V are read once for them.  More rows
+//     are further tiles, items of the line of their own that stream the history again: B8 Hkv8 D128, 16384 keys, 16 rows a key head 97 us,
+//     20 or 32 rows 180, 64 rows 343.
+//   - fp32 does the products of a row on the FMA units, a run-time number of rows a warp: 284 us with one row (3.8 TB/s), 1790 with 16.  Its
+//     exponentials for rescaling and for the sums of weights are ex2.approx, off by 2^-22 of the value at most.
+// Weights (for eviction): the scores are kept, 4 bytes a key and query row of the table's whole capacity, and the second kernel, which knows
+// every row's maximum and sum, adds e^{s - m} / l of a group's rows to the key's weight.  One thread adds up one key: no atomics,
+// bit-reproducible.
 #include <atomic>
 #include <type_traits>
 #include "common.cuh"
@@ -1008,7 +1014,8 @@ template <typename T, int kD, int kWarps> constexpr int attend_smem() {
 int attend_per_sm(int dtype, int D) { return dtype == LMK_F32 ? (D <= 64 ? 2 : 1) : (D <= 64 ? 4 : 2); }
 constexpr int kLeastSteps = 8;         // of a CTA: two a warp
 // Tables of up to this many steps a sequence: every row is one CTA's, and nothing is to be joined (us, whole / in pieces: 32 rows of 300 keys
-// 8.8 / 14.3, of 1000 15.2 / 14.5; 512 rows of 300 23.5 / 34.1).
+// 8.8 / 14.3, of 1000 15.2 / 14.5; 512 rows of 300 23.5 / 34.1).  The host knows the table's width and not the lengths: a short history in a
+// wide table takes the pieces (300 keys: 8.0 us in a table of 512, 12.8 in wider ones).
 constexpr int kWholeSteps = 32;
 
 struct AttendPlan {

@@ -16,7 +16,7 @@
 //   units (SinkSplit): one unit would be as long as the sequence.
 // Rows behind a sequence's end (lengths) are hidden by selects and, where a product would multiply them with a zero, overwritten with zeros in
 // shared memory by the loading warp, so that NaN there stays there.
-// B1 H32 L2048 D128, window 512, sinks 4, bf16: forward 34 us (37 with the rest for the backward pass), delta 5 to 9, dQ 43, dK/dV 54, join 4.
+// B1 H32 L2048 D128, window 512, sinks 4, bf16: forward 34 us (37 with the rest for the backward pass), delta 6 to 10, dQ 43, dK/dV 54, join 4.
 // L32768 on 8 key heads, window 4096, where starts and boundaries do not count: 1850, 95, 2950, 3370, at 69, 65 and 75 % of the measured rate of
 // products in the three that have some (S and dP are formed twice in the backward pass).
 // All waits are bounded (sm100_ptx.cuh).

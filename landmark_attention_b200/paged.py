@@ -25,7 +25,10 @@ def paged_attention(q, k_pages, v_pages, table, lengths, window=None, sinks=0, s
     (p - j < window or j < sinks).  H is a multiple of Hkv.  Rows that see nothing (an empty sequence) give zeros.
     weights: fp32 [B, Hkv, max_pages * page], updated in place for every j < lengths[b]:
       weights = decay * weights + sum of the key's attention weights over the T queries of the heads that share it;
-    decay=0 overwrites them.  `paged_evict` goes by them.  bf16, fp16 or fp32, D a multiple of 8 up to 128; no gradients."""
+    decay=0 overwrites them.  `paged_evict` goes by them.  bf16, fp16 or fp32, D a multiple of 8 up to 128; no gradients.
+    T up to 1024, and up to 4096 query rows a key head (H / Hkv * T).  Values that some of the T tokens see are expected to be finite: one
+    that is not can reach the other tokens of its sequence and key head.  A row whose scores are all -inf gives zeros, as one that sees nothing.
+    Weights take a workspace of 4 bytes per query row and key of the table's capacity (B * H * T * max_pages * page), whatever the lengths."""
     return L.host().paged_attention(q, k_pages, v_pages, table, lengths, window, sinks, sm_scale, weights, decay)
 
 
