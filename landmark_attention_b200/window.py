@@ -15,7 +15,7 @@ def window_attention(q, k, v, window, sinks=0, sm_scale=None, lengths=None):
     lengths: int32 [B], a right-padded batch.  Sequence b has lengths[b] keys; rows at positions from there on give zeros, take no part
     in any gradient, and may hold anything.  Read on the device: the host does not wait.
     bf16 and fp16 (fp32 accumulation, attention weights rounded to the type where they enter a product) or fp32; D a multiple of 8 up to
-    128; sm_scale > 0, 1 / sqrt(D) if None; any strides.  First derivatives in q, k and v (a byte per number of
+    128; sm_scale > 0, 1 / sqrt(D) if None; any strides; B * H up to 65535, Lk up to 2^22.  First derivatives in q, k and v (a byte per number of
     the output is kept for them beside the usual tensors); results do not change from run to run.  Keys
     and values that a sequence has are expected to be finite: one that is not can reach rows that do not see it.  A query row that is not
     finite makes NaN of its own output and dQ row and of dV of the keys it sees; dK becomes NaN there too, and can in between."""
