@@ -1035,9 +1035,11 @@ constexpr int kSdpBufs = 2;                         // S / dP buffers in TMEM
 constexpr int kDqThreads = (kBwdWarps + 2) * 32;
 
 struct DqSmem {
-  uint64_t qdo_full, patch;
+  // [2]: units in turn.  A pair of warpgroups that has no item of a unit sees nothing of it, and a parity tells only neighbouring phases
+  // apart: with one barrier the pair took rows for its next unit's that had not arrived.  Of the unit two before, it always had a part.
+  uint64_t qdo_full[2], patch;
   uint64_t ops_ready;       // the unit's Q and dO rows sit in TMEM (written by the pair of warpgroups that takes its first item)
-  uint64_t ops_free;        // the S / dP products of the unit have read them
+  uint64_t ops_free[2];     // the S / dP products of the unit have read them
   uint64_t rows_read;       // and are no longer needed in shared memory
   uint64_t k_full[kDqK], k_empty[kDqK], v_full[kDqV], v_empty[kDqV];
   uint64_t s_full[kSdpBufs], s_free[kSdpBufs], dp_full[kSdpBufs];
@@ -1077,9 +1079,8 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
 
   if (tid == 0) {
     for (const CUtensorMap* tm : {&tm_q, &tm_k, &tm_v, &tm_do}) prefetch_tensormap(tm);
-    for (uint64_t* bar : {&sm->qdo_full, &sm->patch}) mbar_init(smem_u32(bar), 1);
+    for (uint64_t* bar : {&sm->qdo_full[0], &sm->qdo_full[1], &sm->ops_free[0], &sm->ops_free[1], &sm->patch}) mbar_init(smem_u32(bar), 1);
     mbar_init(smem_u32(&sm->ops_ready), 256);
-    mbar_init(smem_u32(&sm->ops_free), 1);
     mbar_init(smem_u32(&sm->rows_read), 256);
     for (int s = 0; s < kDqK; ++s) {
       mbar_init(smem_u32(&sm->k_full[s]), 1);
@@ -1115,7 +1116,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       const RowUnit un = unit_of(w);
       if (un.total == 0) continue;
       const int hk = un.h / p.G;
-      const uint32_t qb = smem_u32(&sm->qdo_full);
+      const uint32_t qb = smem_u32(&sm->qdo_full[u & 1]);
       mbar_wait(smem_u32(&sm->rows_read), (u & 1) ^ 1, status, kErrDqProducer);
       if (lane == 0) {
         mbar_arrive_expect_tx(qb, 2 * (kD / 64) * kTileBytes);
@@ -1196,7 +1197,7 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
           mma_f16_ts(tmem_dp + sb * 64, tmem_do + kk * 8, desc_advance(db, kmajor_step(kk, kHalfTile)), idesc_s, kk > 0);
         mma_commit(smem_u32(&sm->dp_full[sb]));
         mma_commit(smem_u32(&sm->v_empty[it % kDqV]));
-        if (c.i == c.n - 1) mma_commit(smem_u32(&sm->ops_free));        // the next unit's Q / dO rows may be written
+        if (c.i == c.n - 1) mma_commit(smem_u32(&sm->ops_free[c.u & 1]));        // the next unit's Q / dO rows may be written
       }
     };
     Cursor now = {-1, 0, 0, -1};
@@ -1301,8 +1302,8 @@ window_dq_sm100_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_co
       // The pair that takes the unit's first item moves its rows to TMEM, a warpgroup Q and the other dO: row -> lane, 32-bit word j (two
       // features) -> column j, the layout of a K-major A operand
       if (pair == (it0 & 1)) {
-        mbar_wait(smem_u32(&sm->qdo_full), u & 1, status, kErrDqSoftmax);
-        mbar_wait(smem_u32(&sm->ops_free), (u & 1) ^ 1, status, kErrDqSoftmax);
+        mbar_wait(smem_u32(&sm->qdo_full[u & 1]), (u >> 1) & 1, status, kErrDqSoftmax);
+        if (u > 0) mbar_wait(smem_u32(&sm->ops_free[(u - 1) & 1]), ((u - 1) >> 1) & 1, status, kErrDqSoftmax);
         tc_fence_after();
 #pragma unroll 1
         for (int c0 = 0; c0 < kD / 8; c0 += 8) {
